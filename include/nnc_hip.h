@@ -327,6 +327,81 @@ void nnc_hip_attention(Tensor* qkv, Tensor* div, Tensor* out, int batch, int seq
 void nnc_hip_conv_packed_noalloc(Tensor* in, Tensor* w, Tensor* b, Tensor* res, Tensor* out, int kh, int kw,
                                  int sh, int sw, int ph, int pw, int act);
 
+/* ---- 8-bit serving operators ----------------------------------------------
+ * What a decoder layer does with 8-bit activations, weights and cache. No
+ * counterpart in the reference ABI. Activations are float32 or float16, all
+ * tensors of a call that hold activations of one type; 8-bit values are int8
+ * whole numbers -127 .. 127 with float32 scales, value = whole number * scale.
+ * Sums, statistics and scales are float32 or wider. Rows, heads, dims and
+ * batches are any size (0: nothing happens) where no limit is named.
+ *
+ * To 8 bits: u = the largest absolute value / 127, rounded once; each whole
+ * number is the nearest to x / u, ties to even. Largest value below 2^-100:
+ * zeros, scale 0. A NaN or an infinity among the values: scale NaN, whole
+ * numbers 0, so all of them read back as NaN.
+ *
+ * nnc_hip_rms_norm: s = in (+ res), rounded to the activations' type;
+ * y = s * w / sqrt(mean(s^2) + eps) over the last extent. `res` may be NULL;
+ * `sum`, if not NULL, receives s (it may be the same buffer as `res` or
+ * `in`, and `out` the same as `in`). weight: one row. out of in's type: y, scale NULL. out int8:
+ * the product s * w, rounded to float32, is quantised row by row and `scale`
+ * (one for each row) is its step u times 1 / sqrt(...), so the whole numbers
+ * do not depend on the order of the sum of squares.
+ *
+ * nnc_hip_quantize_rows / nnc_hip_dequantize_rows: rows (of the last extent)
+ * to 8 bits with a scale each, and back: activations between an attention or
+ * an element-wise op and the next product, weights [N][K] once.
+ *
+ * nnc_hip_matmul_i8: out[m][n] = (sum_k a[m][k] w[n][k]) * (a_scale[m] *
+ * w_scale[n]) + bias[n]: a [M][K] int8 (leading extents count as rows), w
+ * [N][K] int8, bias float32 or NULL. The sum is exact; K up to 131071. */
+void nnc_hip_rms_norm(Tensor* in, Tensor* res, Tensor* weight, Tensor* sum, Tensor* out, Tensor* scale, float eps);
+void nnc_hip_quantize_rows(Tensor* in, Tensor* out, Tensor* scale);
+void nnc_hip_dequantize_rows(Tensor* in, Tensor* scale, Tensor* out);
+void nnc_hip_matmul_i8(Tensor* a, Tensor* a_scale, Tensor* w, Tensor* w_scale, Tensor* bias, Tensor* out);
+
+/* A paged cache: k_cache int8 [pages][kv_heads][page][dim], v_cache int8
+ * [pages][kv_heads][dim][page], k_scale and v_scale float32 [pages][kv_heads];
+ * page a multiple of 16 up to 256, dim 32, 64, 128 or 256, 16-byte aligned.
+ * table int32 [batch][width]: position t of sequence b is in page
+ * table[b][t / page]. starts int32 [batch + 1], lengths int32 [batch]:
+ * sequence b's rows of the activations are starts[b] .. starts[b + 1] (never
+ * decreasing), and they are its last positions, lengths[b] being its length
+ * with them. table, starts and lengths are device memory, read when the call
+ * runs; starts and lengths outside what there is are clamped, a page number
+ * outside [0, pages) is a page that cannot be read or written. Rows of no
+ * sequence (padding behind the last) are neither read nor written.
+ *
+ * nnc_hip_kv_write: row r's keys are k's columns k_col .. k_col + kv_heads *
+ * dim, its values v's from v_col (k and v may be one tensor: the rows of a
+ * fused projection). A page that keeps positions from before the call gets
+ * the larger of its old scale and the new rows'; if that is larger than the
+ * old one, the kept whole numbers become the nearest to their value under it.
+ * A page that the new rows begin in gets theirs. Positions behind the length
+ * stay as they were. No page may belong to two sequences that write to it in
+ * one call; pages of a common prefix that no row touches may be shared.
+ *
+ * nnc_hip_kv_read: the opposite: rows starts[b] .. starts[b + 1] of k and v
+ * receive sequence b's last positions.
+ *
+ * nnc_hip_kv_attention: for every row and head, out = softmax over the
+ * sequence's positions j of scale * q . k_j, times v_j; row i of n at
+ * position p = length - n + i sees j <= p, and with window > 0 j > p -
+ * window. q's columns from q_col: heads * dim, heads a multiple of kv_heads,
+ * head h reading cached head h / (heads / kv_heads). out [rows][heads * dim],
+ * 16-byte aligned. A row that sees nothing (no length, more rows than
+ * positions, only pages that cannot be read) gets zeros; what is in the cache
+ * at positions that a row does not see does not reach its result. max_length:
+ * the longest sequence if the caller knows it, 0 otherwise (then the
+ * table's width); it decides how the work is divided, not the result. */
+void nnc_hip_kv_write(Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale,
+                      Tensor* table, Tensor* starts, Tensor* lengths, int k_col, int v_col);
+void nnc_hip_kv_read(Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table, Tensor* starts,
+                     Tensor* lengths, Tensor* k, Tensor* v, int k_col, int v_col);
+void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table,
+                          Tensor* starts, Tensor* lengths, Tensor* out, int q_col, int heads, float scale, int window,
+                          int max_length);
+
 #ifdef __cplusplus
 }
 #endif

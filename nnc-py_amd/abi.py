@@ -130,6 +130,13 @@ TARGET_SIGNATURES = {
     "nnc_hip_scaled_softmax": [TP, TP, TP, c_int],
     "nnc_hip_attention": [TP, TP, TP, c_int, c_int, c_int, c_int, c_int, c_int, c_int],
     "nnc_hip_transpose_slice": [TP, TP, I64P, c_int, c_int, c_int],
+    "nnc_hip_rms_norm": [TP, TP, TP, TP, TP, TP, c_float],
+    "nnc_hip_quantize_rows": [TP, TP, TP],
+    "nnc_hip_dequantize_rows": [TP, TP, TP],
+    "nnc_hip_matmul_i8": [TP] * 6,
+    "nnc_hip_kv_write": [TP] * 9 + [c_int, c_int],
+    "nnc_hip_kv_read": [TP] * 9 + [c_int, c_int],
+    "nnc_hip_kv_attention": [TP] * 9 + [c_int, c_int, c_float, c_int, c_int],
 }
 
 # nnc_hip_fused_eltwise's op codes (include/nnc_hip.h NNC_EW_*)

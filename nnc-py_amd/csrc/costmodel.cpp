@@ -766,6 +766,56 @@ void nnc_hip_attention(Tensor* qkv, Tensor* div, Tensor* out, int batch, int seq
            kLaunchUs + kAttnBodyUs * ceil_div(blocks, kCUs), flops,
            nbytes(qkv) + nbytes(out));
 }
+// the 8-bit serving operators: their bytes once, or their products at the
+// 8-bit matrix rate, whichever is longer
+constexpr double kMfmaI8 = 2.0e15;
+void nnc_hip_rms_norm(Tensor* in, Tensor* res, Tensor* w, Tensor* sum, Tensor* out, Tensor* scale, float eps) {
+    (void)eps;
+    if (in && out && numel(out) > 0)
+        stream_kernel("nnc_hip_rms_norm", "nnc_hip_rms_norm",
+                      nbytes(in) + nbytes(res) + nbytes(w) + nbytes(sum) + nbytes(out) + nbytes(scale));
+}
+void nnc_hip_quantize_rows(Tensor* in, Tensor* out, Tensor* scale) {
+    if (in && out && numel(out) > 0)
+        stream_kernel("nnc_hip_quantize_rows", "nnc_hip_quantize_rows", nbytes(in) + nbytes(out) + nbytes(scale));
+}
+void nnc_hip_dequantize_rows(Tensor* in, Tensor* scale, Tensor* out) {
+    if (in && out && numel(out) > 0)
+        stream_kernel("nnc_hip_dequantize_rows", "nnc_hip_dequantize_rows", nbytes(in) + nbytes(out) + nbytes(scale));
+}
+void nnc_hip_matmul_i8(Tensor* a, Tensor* as, Tensor* w, Tensor* ws, Tensor* bias, Tensor* out) {
+    (void)as, (void)ws;
+    if (!a || !w || !out || !a->shape || a->ndim < 1 || numel(out) <= 0) return;
+    const double bytes = nbytes(a) + nbytes(w) + nbytes(bias) + nbytes(out);
+    const double flops = 2.0 * (double)numel(out) * (double)a->shape[a->ndim - 1];
+    record("nnc_hip_matmul_i8", "nnc_hip_matmul_i8", kLaunchUs + fmax(flops / kMfmaI8, bytes / (kHbm * kStreamEff)) * 1e6,
+           flops, bytes);
+}
+static void cache_kernel(const char* name, Tensor* k, Tensor* v) {
+    if (k && v && numel(k) > 0) stream_kernel(name, name, 1.25 * (nbytes(k) + nbytes(v)));
+}
+void nnc_hip_kv_write(Tensor* k, Tensor* v, Tensor* kc, Tensor* vc, Tensor* ks, Tensor* vs, Tensor* table, Tensor* starts,
+                      Tensor* lengths, int k_col, int v_col) {
+    (void)kc, (void)vc, (void)ks, (void)vs, (void)table, (void)starts, (void)lengths, (void)k_col, (void)v_col;
+    cache_kernel("nnc_hip_kv_write", k, v);
+}
+void nnc_hip_kv_read(Tensor* kc, Tensor* vc, Tensor* ks, Tensor* vs, Tensor* table, Tensor* starts, Tensor* lengths,
+                     Tensor* k, Tensor* v, int k_col, int v_col) {
+    (void)kc, (void)vc, (void)ks, (void)vs, (void)table, (void)starts, (void)lengths, (void)k_col, (void)v_col;
+    cache_kernel("nnc_hip_kv_read", k, v);
+}
+// the lengths are on the device: every sequence taken as max_length (or the
+// table's width) long
+void nnc_hip_kv_attention(Tensor* q, Tensor* kc, Tensor* vc, Tensor* ks, Tensor* vs, Tensor* table, Tensor* starts,
+                          Tensor* lengths, Tensor* out, int q_col, int heads, float scale, int window, int max_length) {
+    (void)vc, (void)ks, (void)vs, (void)starts, (void)lengths, (void)q_col, (void)heads, (void)scale, (void)window;
+    if (!q || !kc || !table || !out || !kc->shape || !table->shape || kc->ndim != 4 || table->ndim != 2) return;
+    const double length = max_length > 0 ? max_length : (double)table->shape[1] * (double)kc->shape[2];
+    const double bytes = 2.0 * (double)table->shape[0] * length * (double)(kc->shape[1] * kc->shape[3]) + 2.0 * nbytes(out);
+    const double flops = 4.0 * (double)numel(out) * length;
+    record("nnc_hip_kv_attention", "nnc_hip_kv_attention",
+           kLaunchUs + fmax(flops / (kMfmaI8 / 4), bytes / (kHbm * kStreamEff)) * 1e6, flops, bytes);
+}
 // eltwise.hip nnc_hip_fused_eltwise: one streaming pass, each input read and
 // the output written once
 void nnc_hip_fused_eltwise(Tensor** ins, int n_in, const int* prog, int n_steps, const float* consts, Tensor* out) {

@@ -76,6 +76,13 @@ _HIP_SIGNATURES = {
     "nnc_hip_scaled_softmax": (abi.TARGET_SIGNATURES["nnc_hip_scaled_softmax"], None),
     "nnc_hip_transpose_slice": (abi.TARGET_SIGNATURES["nnc_hip_transpose_slice"], None),
     "nnc_hip_attention": (abi.TARGET_SIGNATURES["nnc_hip_attention"], None),
+    "nnc_hip_rms_norm": (abi.TARGET_SIGNATURES["nnc_hip_rms_norm"], None),
+    "nnc_hip_quantize_rows": (abi.TARGET_SIGNATURES["nnc_hip_quantize_rows"], None),
+    "nnc_hip_dequantize_rows": (abi.TARGET_SIGNATURES["nnc_hip_dequantize_rows"], None),
+    "nnc_hip_matmul_i8": (abi.TARGET_SIGNATURES["nnc_hip_matmul_i8"], None),
+    "nnc_hip_kv_write": (abi.TARGET_SIGNATURES["nnc_hip_kv_write"], None),
+    "nnc_hip_kv_read": (abi.TARGET_SIGNATURES["nnc_hip_kv_read"], None),
+    "nnc_hip_kv_attention": (abi.TARGET_SIGNATURES["nnc_hip_kv_attention"], None),
     "nnc_hip_ew_chain_specialized": ([ctypes.c_int, abi.I32P, ctypes.c_int], ctypes.c_int),
 }
 
