@@ -7,9 +7,9 @@
 #include <stdint.h>
 
 #ifdef __HIPCC__
-#define NNC_HD __host__ __device__ __forceinline__
+#define RAGGED_HD __host__ __device__ __forceinline__
 #else
-#define NNC_HD inline
+#define RAGGED_HD inline
 #endif
 
 namespace nnc {
@@ -25,8 +25,8 @@ struct Ragged {
     int64_t pages;
 };
 
-NNC_HD int imin(int a, int b) { return a < b ? a : b; }
-NNC_HD int imax(int a, int b) { return a > b ? a : b; }
+RAGGED_HD int imin(int a, int b) { return a < b ? a : b; }
+RAGGED_HD int imax(int a, int b) { return a > b ? a : b; }
 
 struct Span {
     int end;     // one past the sequence's last row
@@ -34,11 +34,11 @@ struct Span {
     int rows;    // rows; those with no position (more rows than length) included
     // the row at a position, and the first row's position: negative if there
     // are more rows than positions
-    NNC_HD int row(int pos) const { return end - length + pos; }
-    NNC_HD int first() const { return length - rows; }
+    RAGGED_HD int row(int pos) const { return end - length + pos; }
+    RAGGED_HD int first() const { return length - rows; }
 };
 
-NNC_HD Span span_of(const Ragged& g, int b) {
+RAGGED_HD Span span_of(const Ragged& g, int b) {
     Span s;
     const int r0 = imin(imax(g.starts[b], 0), g.rows);
     s.end = imin(imax(g.starts[b + 1], r0), g.rows);
@@ -50,18 +50,18 @@ NNC_HD Span span_of(const Ragged& g, int b) {
 // pages that a sequence's rows touch, and the most that `rows` rows of
 // `batch` sequences can: each has one row at least, and a run of n rows
 // touches n / page + 2 at most
-NNC_HD int touched_pages(const Ragged& g, int b) {
+RAGGED_HD int touched_pages(const Ragged& g, int b) {
     const Span s = span_of(g, b);
     if (s.rows <= 0 || s.length <= 0) return 0;
     return (s.length - 1) / g.page - imax(s.first(), 0) / g.page + 1;
 }
-NNC_HD int64_t touched_bound(int64_t rows, int64_t batch, int page) {
+RAGGED_HD int64_t touched_bound(int64_t rows, int64_t batch, int page) {
     const int64_t some = rows / page + 2 * batch;
     return rows < some ? rows : some;
 }
 
 // the page number of a table slot, or -1 if it is none of the cache's
-NNC_HD int page_at(const Ragged& g, int b, int slot) {
+RAGGED_HD int page_at(const Ragged& g, int b, int slot) {
     const int p = g.table[(int64_t)b * g.width + slot];
     return p >= 0 && p < g.pages ? p : -1;
 }
@@ -71,7 +71,7 @@ NNC_HD int page_at(const Ragged& g, int b, int slot) {
 struct PageShare {
     Span span;
     int begin, fresh, stop, page_no;
-    NNC_HD PageShare(const Ragged& g, int b, int share) {
+    RAGGED_HD PageShare(const Ragged& g, int b, int share) {
         span = span_of(g, b);
         const int slot = imax(span.first(), 0) / g.page + share;
         begin = slot * g.page;
@@ -83,10 +83,10 @@ struct PageShare {
 
 // Attention: the rows of one cached head's `group` query heads, tokens
 // outermost, in tiles of `tile` rows.
-NNC_HD int query_tiles(const Span& s, int group, int tile) {
+RAGGED_HD int query_tiles(const Span& s, int group, int tile) {
     return (int)(((int64_t)s.rows * group + tile - 1) / tile);
 }
-NNC_HD int64_t query_tiles_bound(int64_t rows, int64_t batch, int group, int tile) {
+RAGGED_HD int64_t query_tiles_bound(int64_t rows, int64_t batch, int group, int tile) {
     return rows * group / tile + (rows < batch ? rows : batch);
 }
 
@@ -95,13 +95,13 @@ NNC_HD int64_t query_tiles_bound(int64_t rows, int64_t batch, int group, int til
 // [lo + s * chunk, ...).
 struct KeyRange {
     int lo, hi, chunk;
-    NNC_HD KeyRange(int first, int last, int window, int splits, int least, int step) {
+    RAGGED_HD KeyRange(int first, int last, int window, int splits, int least, int step) {
         hi = imax(last + 1, 0);
         lo = window > 0 ? imax(first - window + 1, 0) & ~63 : 0;
         const int each = (imax(hi - lo, 0) + splits - 1) / splits;
         chunk = imax(least, (each + step - 1) / step * step);
     }
-    NNC_HD int shares() const { return imax(1, (int)(((int64_t)imax(hi - lo, 0) + chunk - 1) / chunk)); }
+    RAGGED_HD int shares() const { return imax(1, (int)(((int64_t)imax(hi - lo, 0) + chunk - 1) / chunk)); }
 };
 
 }  // namespace nnc
