@@ -44,93 +44,97 @@ __device__ __forceinline__ ix4 row_chunk(const int8_t* row, int k, int K) {
 }
 
 // ---------------------------------------------------------------------------
-// Tiles: BM x BN outputs per workgroup, WM x WN waves, 128 k at a time, two LDS
-// stages: the loads of slice t + 1 are in flight while slice t is used. DMA:
-// straight from global memory into LDS, 16 bytes per lane. That needs K % 16
-// == 0 and 16-byte aligned operands: a chunk is wholly inside or outside the
-// matrix, and one outside gets an offset past the buffer (zeros). Without it
-// the chunks go through registers (row_chunk).
+// Tiles: BM x BN outputs per workgroup, WM x WN waves, 128 k at a time.
+//
+// Slices go straight from global memory into NS LDS stages, 16 bytes per lane,
+// NS - 1 of them in flight. That needs K % 16 == 0 and 16-byte aligned
+// operands: a chunk is wholly inside or outside the matrix, and one outside
+// gets an offset past the buffer (zeros). Other operands are laid out so
+// first (pack8_k): chunks through registers instead took 107 us for
+// [2048,4001]x[4096,4001], 96 with 128 x 128 tiles, unaligned loads being
+// split up; with the layout 59.
+//
 // An LDS row is 128 k of one row of a or w, its 16-byte chunk c at position
-// c ^ (row % 8), so that eight lanes reading a chunk of eight rows hit all
-// banks. w's rows are the MFMA's first operand: a lane then holds four
-// consecutive columns of one output row.
+// c ^ (row / 2 % 8): LDS has 64 banks, and 16 lanes reading a chunk of 16 rows
+// hit all of them (c ^ (row % 8) has two rows on the same banks: half of all
+// LDS cycles were conflicts). w's rows are the MFMA's first operand: a lane then holds four
+// consecutive columns of one output row. The operands of a slice's four steps
+// are read one step ahead of their MFMAs; the barrier between two slices
+// comes before the last step's MFMAs, which cover the next slice's first read.
+//
+// splits > 1: the k of a tile are divided over so many workgroups, and the
+// last to finish adds the others' sums (whole numbers: in any order).
 // ---------------------------------------------------------------------------
 typedef int ix16 __attribute__((ext_vector_type(16)));
 
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int NS_, int PF_>
 struct Tile8 {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NW = WM * WN, THREADS = 64 * NW;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, PF = PF_, NW = WM * WN, THREADS = 64 * NW;
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 blocks per wave
     static constexpr int STAGE = (BM + BN) * 128;
     static constexpr int LOADS_A = BM / (8 * NW), LOADS_W = BN / (8 * NW);  // instructions per wave and slice
+    static constexpr int LOADS = LOADS_A + LOADS_W;
     static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && TM >= 1 && TN >= 1, "rows split evenly over the waves");
-    // the epilogue's 32 rows of a wave, padded to 16 bytes off a multiple of 128
+    static_assert(NW % 2 == 0, "a lane's chunk is the same in all its loads");
+    // the epilogue's 32 rows of a wave, 16 bytes off a multiple of 128
     static constexpr int WAVE_N = 32 * TN;
     template <typename T>
     static constexpr int out_ld() { return WAVE_N * (int)sizeof(T) + 16; }
-    static constexpr int LDS = 2 * STAGE > NW * 32 * out_ld<float>() ? 2 * STAGE : NW * 32 * out_ld<float>();
+    static constexpr int OUT = NW * 32 * out_ld<float>();
+    static constexpr int LDS = NS * STAGE > OUT ? NS * STAGE : OUT;
 };
 
-// the tile of a workgroup: bands of 8 tile rows, column by column, eight
-// consecutive workgroups' worth of them on one XCD, so that the operands'
-// slices are shared through its L2
-__device__ __forceinline__ void tile8_pos(int wg, int tiles_m, int tiles_n, int& mt, int& nt) {
-    const int t = xcd_remap(wg, tiles_m * tiles_n);
-    const int band = t / (8 * tiles_n), in = t - band * 8 * tiles_n, rows = min(8, tiles_m - band * 8);
+struct Split8 {
+    int tiles_m, tiles_n, splits, each;  // each: k of a split, a multiple of 128
+    int* sums;                           // [tile][split][BM * BN]
+    int* counters;                       // [tile], zero
+};
+
+// The tile of a workgroup: bands of 8 tile rows, column by column, so that the
+// workgroups of one XCD share slices of both operands through its L2.
+__device__ __forceinline__ void tile8_pos(int t, const Split8& s, int& mt, int& nt) {
+    const int band = t / (8 * s.tiles_n), in = t - band * 8 * s.tiles_n, rows = min(8, s.tiles_m - band * 8);
     nt = in / rows;
     mt = band * 8 + in - nt * rows;
 }
 
-template <class L, typename T, bool DMA>
-__global__ void __launch_bounds__(L::THREADS) gemm8_tile_k(Gemm8Args p, int tiles_m, int tiles_n) {
+template <class L, typename T>
+__global__ void __launch_bounds__(L::THREADS) gemm8_tile_k(Gemm8Args p, Split8 sp) {
     extern __shared__ __align__(16) char lds[];
+    constexpr int NS = L::NS, PF = L::PF;
     const int lane = threadIdx.x & 63, l32 = lane & 31, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / L::WN, wn = wave % L::WN;
+    const int tiles = sp.tiles_m * sp.tiles_n, wg = xcd_remap(blockIdx.x, tiles * sp.splits);
+    const int split = wg / tiles, tile = wg - split * tiles;
     int mt, nt;
-    tile8_pos(blockIdx.x, tiles_m, tiles_n, mt, nt);
+    tile8_pos(tile, sp, mt, nt);
     const int64_t m0 = (int64_t)mt * L::BM, n0 = (int64_t)nt * L::BN;
+    const int kfrom = split * sp.each, kto = min(p.k, kfrom + sp.each), slices = (kto - kfrom + 127) / 128;
     const __amdgpu_buffer_rsrc_t ra = make_rsrc((const float*)(p.a + m0 * p.k)), rw = make_rsrc((const float*)(p.w + n0 * p.k));
     // this lane's rows and chunk of the loads
-    const int kc = ((lane & 7) ^ (lane >> 3)) * 16;
+    const int kc = ((lane & 7) ^ ((4 * wave + (lane >> 4)) & 7)) * 16;  // rows 8 wave + lane / 8 (mod 16)
     uint32_t va[L::LOADS_A], vw[L::LOADS_W];
 #pragma unroll
     for (int i = 0; i < L::LOADS_A; ++i) {
         const int r = (wave + L::NW * i) * 8 + (lane >> 3);
-        va[i] = DMA ? keep_or_oob((uint32_t)(r * p.k + kc), m0 + r < p.m) : (uint32_t)(m0 + r < p.m ? r : (int)(p.m - 1 - m0)) * p.k;
+        va[i] = keep_or_oob((uint32_t)(r * p.k + kc), m0 + r < p.m);
     }
 #pragma unroll
     for (int i = 0; i < L::LOADS_W; ++i) {
         const int r = (wave + L::NW * i) * 8 + (lane >> 3);
-        vw[i] = DMA ? keep_or_oob((uint32_t)(r * p.k + kc), n0 + r < p.n) : (uint32_t)(n0 + r < p.n ? r : (int)(p.n - 1 - n0)) * p.k;
+        vw[i] = keep_or_oob((uint32_t)(r * p.k + kc), n0 + r < p.n);
     }
-    ix4 staged[DMA ? 1 : L::LOADS_A + L::LOADS_W];
-    auto issue = [&](int stage, int k0) {
-        if constexpr (DMA) {
-            char* s = lds + stage * L::STAGE;
-            const bool in = k0 + kc < p.k;
+    // slice t's loads: as many in every call, so that they can be counted
+    auto issue = [&](int t) {
+        const int k0 = kfrom + t * 128;
+        char* s = lds + t % NS * L::STAGE;
+        const bool in = k0 + kc < kto;
 #pragma unroll
-            for (int i = 0; i < L::LOADS_A; ++i)
-                dma_load16(ra, (float*)(s + (wave + L::NW * i) * 1024), in ? va[i] : kOutOfRange, (uint32_t)k0);
+        for (int i = 0; i < L::LOADS_A; ++i)
+            dma_load16(ra, (float*)(s + (wave + L::NW * i) * 1024), in ? va[i] : kOutOfRange, (uint32_t)k0);
 #pragma unroll
-            for (int i = 0; i < L::LOADS_W; ++i)
-                dma_load16(rw, (float*)(s + L::BM * 128 + (wave + L::NW * i) * 1024), in ? vw[i] : kOutOfRange, (uint32_t)k0);
-        } else {
-            (void)stage;
-#pragma unroll
-            for (int i = 0; i < L::LOADS_A; ++i) staged[i] = row_chunk(p.a + m0 * p.k + va[i], k0 + kc, p.k);
-#pragma unroll
-            for (int i = 0; i < L::LOADS_W; ++i) staged[L::LOADS_A + i] = row_chunk(p.w + n0 * p.k + vw[i], k0 + kc, p.k);
-        }
-    };
-    auto land = [&](int stage) {
-        if constexpr (!DMA) {
-            char* s = lds + stage * L::STAGE;
-#pragma unroll
-            for (int i = 0; i < L::LOADS_A; ++i) *reinterpret_cast<ix4*>(s + (wave + L::NW * i) * 1024 + lane * 16) = staged[i];
-#pragma unroll
-            for (int i = 0; i < L::LOADS_W; ++i)
-                *reinterpret_cast<ix4*>(s + L::BM * 128 + (wave + L::NW * i) * 1024 + lane * 16) = staged[L::LOADS_A + i];
-        }
+        for (int i = 0; i < L::LOADS_W; ++i)
+            dma_load16(rw, (float*)(s + L::BM * 128 + (wave + L::NW * i) * 1024), in ? vw[i] : kOutOfRange, (uint32_t)k0);
     };
     ix16 acc[L::TM][L::TN];
 #pragma unroll
@@ -140,30 +144,94 @@ __global__ void __launch_bounds__(L::THREADS) gemm8_tile_k(Gemm8Args p, int tile
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
     const int ra0 = (wm * 32 * L::TM + l32) * 128, rw0 = L::BM * 128 + (wn * L::WAVE_N + l32) * 128;
-    issue(0, 0);
-    land(0);
-    int stage = 0;
-    for (int k0 = 0; k0 < p.k; k0 += 128, stage ^= 1) {
-        if constexpr (DMA)
-            dma_barrier<0>();  // this slice has landed, the other stage is no longer read
-        else
-            __syncthreads();
-        if (k0 + 128 < p.k) issue(stage ^ 1, k0 + 128);
-        const char* s = lds + stage * L::STAGE;
+    ix4 x[2][PF][L::TM], y[2][PF][L::TN];
+    // steps st .. st + PF of slice t into register set `set`
+    auto read = [&](int t, int st, int set) {
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            const int c = ((2 * st + half) ^ (lane & 7)) * 16;
-            ix4 x[L::TM], y[L::TN];
+        for (int u = 0; u < PF; ++u) {
+            const char* s = lds + t % NS * L::STAGE + ((2 * (st + u) + half) ^ ((l32 >> 1) & 7)) * 16;
 #pragma unroll
-            for (int j = 0; j < L::TN; ++j) y[j] = *reinterpret_cast<const ix4*>(s + rw0 + j * 4096 + c);
+            for (int j = 0; j < L::TN; ++j) y[set][u][j] = *reinterpret_cast<const ix4*>(s + rw0 + j * 4096);
 #pragma unroll
-            for (int i = 0; i < L::TM; ++i) x[i] = *reinterpret_cast<const ix4*>(s + ra0 + i * 4096 + c);
+            for (int i = 0; i < L::TM; ++i) x[set][u][i] = *reinterpret_cast<const ix4*>(s + ra0 + i * 4096);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // before the MFMAs that cover it
+    };
+    auto multiply = [&](int set) {
+#pragma unroll
+        for (int u = 0; u < PF; ++u)
 #pragma unroll
             for (int i = 0; i < L::TM; ++i)
 #pragma unroll
-                for (int j = 0; j < L::TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(y[j], x[i], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < L::TN; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(y[set][u][j], x[set][u][i], acc[i][j], 0, 0, 0);
+    };
+    constexpr int READS = 4 / PF;  // of a slice
+    auto slice = [&](int t, int par) {
+#pragma unroll
+        for (int n = 0; n + 1 < READS; ++n) {
+            read(t, (n + 1) * PF, (par * READS + n + 1) & 1);
+            multiply((par * READS + n) & 1);
         }
-        if (k0 + 128 < p.k) land(stage ^ 1);
+        if (t + 1 < slices) {
+            dma_barrier<(NS - 2) * L::LOADS>();  // slice t + 1 has landed, slice t's stage is no longer read
+            issue(t + NS);
+            read(t + 1, 0, (par * READS + READS) & 1);
+        }
+        multiply((par * READS + READS - 1) & 1);
+    };
+#pragma unroll
+    for (int t = 0; t < NS - 1; ++t) issue(t);
+    dma_barrier<(NS - 2) * L::LOADS>();
+    issue(NS - 1);
+    read(0, 0, 0);
+    int t = 0;
+    for (; t + 1 < slices; t += 2) {
+        slice(t, 0);
+        slice(t + 1, 1);
+    }
+    if (t < slices) slice(t, 0);
+
+    if (sp.splits > 1) {
+        int* mine = sp.sums + (int64_t)tile * sp.splits * (L::BM * L::BN);
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc((const float*)mine);
+        const uint32_t at = (uint32_t)((wave * L::TM * L::TN * 4 * 64 + lane) * 16);
+        constexpr uint32_t SLOT = L::BM * L::BN * 4;
+#pragma unroll
+        for (int i = 0; i < L::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < L::TN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int v0 = acc[i][j][4 * q], v1 = acc[i][j][4 * q + 1], v2 = acc[i][j][4 * q + 2], v3 = acc[i][j][4 * q + 3];
+                    typedef unsigned ux4 __attribute__((ext_vector_type(4)));
+                    __builtin_amdgcn_raw_buffer_store_b128(ux4{(unsigned)v0, (unsigned)v1, (unsigned)v2, (unsigned)v3}, rs,
+                                                           (int)(at + split * SLOT + ((i * L::TN + j) * 4 + q) * 1024), 0, kDeviceScope);
+                }
+        if (!finish_arrive(sp.counters + tile, sp.splits - 1)) return;
+        // all splits' sums, this one's too: their loads go out together
+#pragma unroll
+        for (int i = 0; i < L::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < L::TN; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+#pragma unroll 4
+        for (int o = 0; o < sp.splits; ++o) {
+#pragma unroll
+            for (int i = 0; i < L::TM; ++i)
+#pragma unroll
+                for (int j = 0; j < L::TN; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const ix4 v = __builtin_bit_cast(ix4, load_partial4(rs, at + o * SLOT + ((i * L::TN + j) * 4 + q) * 1024));
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int e = v[r];
+                            acc[i][j][4 * q + r] += e;
+                        }
+                    }
+        }
     }
     dma_barrier<0>();  // every wave is done with the stages
     // scaled and rounded 32 rows at a time through this wave's part of LDS, to
@@ -208,13 +276,53 @@ __global__ void __launch_bounds__(L::THREADS) gemm8_tile_k(Gemm8Args p, int tile
     }
 }
 
-template <class L, typename T, bool DMA>
-static void launch_tile8(const char* name, const Gemm8Args& p) {
-    auto kernel = gemm8_tile_k<L, T, DMA>;
+// One operand or both with rows of k16 = K rounded up to 16, zeros behind K.
+struct Pack8Args {
+    const int8_t* from[2];
+    int8_t* to[2];
+    int64_t rows[2];
+    int k, k16;
+};
+__global__ void __launch_bounds__(256) pack8_k(Pack8Args p) {
+    const int chunks = p.k16 / 16;
+    const int64_t first = p.rows[0] * chunks, all = first + p.rows[1] * chunks;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < all; e += (int64_t)gridDim.x * 256) {
+        const int which = e >= first;
+        const int64_t at = which ? e - first : e, row = at / chunks;
+        const int c = (int)(at - row * chunks) * 16;
+        const ix4 v = row_chunk(p.from[which] + row * p.k, c, p.k);
+        *reinterpret_cast<ix4*>(p.to[which] + row * p.k16 + c) = v;
+    }
+}
+
+template <class L, typename T>
+static void launch_tile8(const char* name, Gemm8Args p, int splits) {
+    auto kernel = gemm8_tile_k<L, T>;
     static const bool ok = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, L::LDS) == hipSuccess;
     if (!ok) return fail(NNC_HIP_EDEVICE, name, "hipFuncSetAttribute failed");
     const int64_t tm = ceil_div(p.m, L::BM), tn = ceil_div(p.n, L::BN);
-    launch(name, kernel, dim3((unsigned)(tm * tn)), dim3(L::THREADS), L::LDS, p, (int)tm, (int)tn);
+    const int slices = (int)ceil_div(p.k, 128), each = (int)ceil_div(slices, splits);
+    Split8 sp{(int)tm, (int)tn, (int)ceil_div(slices, each), each * 128, nullptr, nullptr};
+    // workspace: operands laid out again, partial sums
+    const int k16 = (int)ceil_div(p.k, 16) * 16;
+    const bool pack_a = p.k != k16 || !aligned16(p.a), pack_w = p.k != k16 || !aligned16(p.w);
+    const size_t sums = sp.splits > 1 ? (size_t)(tm * tn) * sp.splits * L::BM * L::BN * sizeof(int) : 0;
+    const size_t bytes = sums + (pack_a ? (size_t)p.m * k16 : 0) + (pack_w ? (size_t)p.n * k16 : 0);
+    if (bytes > 0) {
+        char* ws = (char*)workspace(bytes);
+        sp.counters = sums ? tile_counters((size_t)(tm * tn)) : nullptr;
+        if (!ws || (sums && !sp.counters)) return fail(NNC_HIP_ENOMEM, name, "no workspace for %zu bytes", bytes);
+        sp.sums = (int*)ws;
+        ws += sums;
+        if (pack_a || pack_w) {
+            Pack8Args q{{p.a, p.w}, {(int8_t*)ws, (int8_t*)ws + (pack_a ? p.m * k16 : 0)}, {pack_a ? p.m : 0, pack_w ? p.n : 0}, p.k, k16};
+            launch("nnc_hip_matmul_i8_pack", pack8_k, dim3(grid_for((q.rows[0] + q.rows[1]) * (k16 / 16), 1)), dim3(256), 0, q);
+            if (pack_a) p.a = q.to[0];
+            if (pack_w) p.w = q.to[1];
+            p.k = k16;
+        }
+    }
+    launch(name, kernel, dim3((unsigned)(tm * tn * sp.splits)), dim3(L::THREADS), L::LDS, p, sp);
 }
 
 // ---------------------------------------------------------------------------
@@ -233,7 +341,7 @@ __global__ void __launch_bounds__(64 * NW) gemm8_rows_k(Gemm8Args p) {
     const int8_t* w = p.w + min(n0 + i, p.n - 1) * p.k;
     const int8_t* a[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) a[t] = p.a + min(m0 + 16 * t + i, p.m - 1) * p.k;
+    for (int t = 0; t < MT; ++t) a[t] = m0 + 16 * t + i < p.m ? p.a + (m0 + 16 * t + i) * p.k : nullptr;  // no row: no loads
     ix4 acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = ix4{0, 0, 0, 0};
@@ -250,7 +358,7 @@ __global__ void __launch_bounds__(64 * NW) gemm8_rows_k(Gemm8Args p) {
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[t][j] = chunk(a[t], k0 + 16 * j);
+            for (int j = 0; j < 4; ++j) x[t][j] = a[t] ? chunk(a[t], k0 + 16 * j) : ix4{0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -284,19 +392,67 @@ static void launch_rows8(const char* name, const Gemm8Args& p, bool aligned) {
         launch(name, gemm8_rows_k<MT, NW, T, false>, grid, dim3(64 * NW), 0, p);
 }
 
+// Which kernel: the one whose time, in us past the launch, is least by what was
+// measured (256 CUs, K 1024 to 14336, M 1 to 8192, N 1001 to 4096). A row
+// kernel reads (16 + rows) K bytes per workgroup, all together at 9.8 TB/s and
+// one workgroup at 40 GB/s. A tile kernel takes so long for each slice and
+// round of workgroups; joining splits costs 1.5 us and 16 ns for every partial
+// tile written and read back; laying operands out for the tiles costs a launch
+// and their bytes. Against the neighbours, us: [64,4096]x[4096,4096] rows
+// 13.0, 64 x 64 tiles 10.7, in two splits 9.8; [64,14336]x[4096,14336] rows
+// 34.5, tiles 27.7, in four splits 14.5; [1024,4096]x[4096,4096] tiles of 64
+// 34.7, 128 24.8, 256 x 128 33.3, 256 48; with 8192 rows 225, 190, 158 and 133
+// (2.06 POPS; the stages' LDS conflicts gone that is 59% of the MFMA's cycles,
+// the rest waits for the next slice: one workgroup per CU, two stages).
+struct Plan8 {
+    int kernel = 0, splits = 1;
+    double us = 1e30;
+    void offer(int k, int s, double t) {
+        if (t < us) kernel = k, splits = s, us = t;
+    }
+};
+
+static Plan8 plan_gemm8(int64_t m, int64_t n, int64_t k, bool aligned) {
+    Plan8 best;
+    const double cus = cu_count(), slices = (double)ceil_div(k, 128);
+    // laying the operands out for the tile kernels: a launch, and their bytes
+    const double pack = aligned ? 0.0 : 2.5 + (double)(m + n) * k / 2e6;
+    for (int mt : {1, 2, 4}) {
+        if (m > 128) break;
+        const int64_t rows = m < 16 * mt ? m : 16 * mt;
+        const double each = (16.0 + rows) * k, all = each * ceil_div(n, 16) * ceil_div(m, 16 * mt);
+        best.offer(mt, 1, all / 9.8e6 > each / 40e3 ? all / 9.8e6 : each / 40e3);
+    }
+    const int64_t tiles64 = ceil_div(m, 64) * ceil_div(n, 64);
+    for (int s : {1, 2, 3, 4}) {
+        const double wgs = (double)tiles64 * s;
+        if (s > 1 && (wgs > cus || slices < 4 * s)) break;
+        best.offer(64, s, pack + ceil(slices / s) * (wgs <= cus ? 0.22 : 0.45 * ceil(wgs / (2 * cus))) + (s > 1 ? 1.5 + 0.016 * wgs : 0.0));
+    }
+    // a slice's time in one round of few tiles, of a tile for every CU, and in more
+    auto tile = [&](int kernel, int bm, int bn, double few, double full) {
+        const double wgs = (double)(ceil_div(m, bm) * ceil_div(n, bn)) / cus;
+        best.offer(kernel, 1, pack + slices * (wgs <= 1.0 ? few + (full - few) * wgs : full * ceil(wgs)));
+    };
+    tile(128, 128, 128, 0.47, 0.72);
+    tile(192, 256, 128, 0.80, 1.20);
+    tile(256, 256, 256, 1.25, 2.00);
+    return best;
+}
+
 template <typename T>
 static void launch_gemm8(const char* name, const Gemm8Args& p) {
-    const bool chunks = p.k % 16 == 0 && aligned16(p.a) && aligned16(p.w);
-    if (p.m <= 16) return launch_rows8<1, 16, T>(name, p, chunks);
-    if (p.m <= 32) return launch_rows8<2, 16, T>(name, p, chunks);
-    if (p.m <= 64) return launch_rows8<4, 8, T>(name, p, chunks);
-    if (!chunks) {
-        if (ceil_div(p.m, 128) * ceil_div(p.n, 128) >= cu_count()) return launch_tile8<Tile8<128, 128, 2, 2>, T, false>(name, p);
-        return launch_tile8<Tile8<64, 64, 2, 2>, T, false>(name, p);
+    const bool aligned = p.k % 16 == 0 && aligned16(p.a) && aligned16(p.w);
+    const Plan8 plan = plan_gemm8(p.m, p.n, p.k, aligned);
+    switch (plan.kernel) {
+        case 1: return launch_rows8<1, 8, T>(name, p, aligned);
+        case 2: return launch_rows8<2, 8, T>(name, p, aligned);
+        case 4: return launch_rows8<4, 8, T>(name, p, aligned);
+        case 64: return launch_tile8<Tile8<64, 64, 2, 2, 4, 4>, T>(name, p, plan.splits);
+        case 128: return launch_tile8<Tile8<128, 128, 2, 4, 4, 4>, T>(name, p, 1);
+        case 192: return launch_tile8<Tile8<256, 128, 4, 2, 3, 2>, T>(name, p, 1);
+        default: return launch_tile8<Tile8<256, 256, 2, 4, 2, 1>, T>(name, p, 1);
     }
-    if (ceil_div(p.m, 256) * ceil_div(p.n, 256) >= cu_count()) return launch_tile8<Tile8<256, 256, 2, 4>, T, true>(name, p);
-    if (ceil_div(p.m, 128) * ceil_div(p.n, 128) >= cu_count()) return launch_tile8<Tile8<128, 128, 2, 2>, T, true>(name, p);
-    return launch_tile8<Tile8<64, 64, 2, 2>, T, true>(name, p);
 }
 
 }  // namespace nnc
