@@ -81,6 +81,12 @@ struct PageShare {
     }
 };
 
+// The table slot of a group of 16 positions: t16 / page16, page16 = page / 16
+// from 1 to 16, by one multiplication: slot_magic(page16) * page16 is less than
+// 16 over 2^32, so the quotient is exact for t16 below 2^28. 0 stands for 2^32.
+RAGGED_HD uint32_t slot_magic(int page16) { return page16 == 1 ? 0u : (uint32_t)((0xffffffffu / (uint32_t)page16) + 1u); }
+RAGGED_HD uint32_t slot_of(uint32_t t16, uint32_t magic) { return magic ? (uint32_t)((uint64_t)t16 * magic >> 32) : t16; }
+
 // Attention: the rows of one cached head's `group` query heads, tokens
 // outermost, in tiles of `tile` rows.
 RAGGED_HD int query_tiles(const Span& s, int group, int tile) {

@@ -55,7 +55,7 @@ int main() {
                 if (hit[t] != (mine ? 1 : 0)) no("positions covered", trial);
             }
             for (int group : {1, 3, 16, 40})
-                for (int tile : {16, 64}) {
+                for (int tile : {16, 128}) {
                     const int tiles = query_tiles(s, group, tile);
                     if ((int64_t)tiles * tile < (int64_t)s.rows * group || (tiles && (int64_t)(tiles - 1) * tile >= (int64_t)s.rows * group))
                         no("tiles", trial);
@@ -64,7 +64,7 @@ int main() {
         if (sound) {
             if (touched > touched_bound(rows, batch, page)) no("bound of touched pages", trial);
             for (int group : {1, 3, 16, 40})
-                for (int tile : {16, 64}) {
+                for (int tile : {16, 128}) {
                     int64_t tiles = 0;
                     for (int b = 0; b < batch; ++b) tiles += query_tiles(span_of(g, b), group, tile);
                     if (tiles > query_tiles_bound(rows, batch, group, tile)) no("bound of tiles", trial);
@@ -80,6 +80,13 @@ int main() {
         if (window && k.lo > (first - window + 1 > 0 ? first - window + 1 : 0)) no("window", trial);
         if ((int64_t)k.lo + (int64_t)shares * k.chunk < k.hi) no("keys left over", trial);
         if (shares > 1 && (int64_t)k.lo + (int64_t)(shares - 1) * k.chunk >= k.hi) no("empty share", trial);
+    }
+    for (int page16 = 1; page16 <= 16; ++page16) {
+        const uint32_t magic = slot_magic(page16);
+        for (uint32_t t = 0; t < 1u << 20; ++t)
+            if (slot_of(t, magic) != t / page16) no("slot", (int)t);
+        for (uint32_t t = (1u << 28) - 100000; t < 1u << 28; ++t)
+            if (slot_of(t, magic) != t / page16) no("slot", (int)t);
     }
     printf("ok\n");
     return 0;
