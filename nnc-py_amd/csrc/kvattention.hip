@@ -25,8 +25,8 @@
 // bits), and so is p then (f16 outputs: p rounded to f16 once, 2^-12 of it).
 //
 // A workgroup takes 16 query rows - heads of one cached head, then tokens -
-// and a share of the keys, its four waves 64 keys each in turn; the waves'
-// sums are joined through LDS, the shares' through the workspace.
+// and a share of the keys, its waves 64 keys each in turn; the waves' sums are
+// joined through LDS, the shares' through the workspace.
 #include <limits.h>
 
 #include "mfma_tile.h"
@@ -40,10 +40,12 @@ struct KvAttnArgs {
     const float *k_scale, *v_scale;
     const void* q;
     void* out;
-    float* part;  // [row][head][split][dim + 2]: sums, maximum, divisor
+    float* part;    // [tile][cached head][split][row of the tile][dim + 4]: sums, maximum, divisor
+    int* counters;  // [tile][cached head], zero
     int64_t ld;
-    int q_col, heads, kv_heads, group, window, splits, chunk, tile;  // tile: query rows of a workgroup
+    int q_col, heads, kv_heads, group, window, splits, chunk, tiles;
     uint32_t slot_magic;
+    bool q_vec;  // query rows start on 16 bytes
     float scale;  // with log2(e)
 };
 
@@ -63,17 +65,101 @@ __device__ __forceinline__ f16x8 widen8(uint32_t lo, uint32_t hi) {
     return x.v + f16x8{c, c, c, c, c, c, c, c};
 }
 
-// p is scaled by this before it is rounded to f16: its smallest steps are
-// then 2^-36 of the row's largest
-static constexpr float kPLog = 12.f, kPScale = 4096.f;
+// The scale that a page's values are taken to have: a page of zeros (scale 0)
+// gets one that is small beside any page with values, whose p would otherwise
+// be small beside its own and lose bits as f16, and large enough for its
+// weights in the divisor to stay above 2^-126.
+__device__ __forceinline__ float value_unit(float scale) { return scale == 0.f ? 0x1p-64f : scale; }
+
+// p is scaled by 2^12 before it is rounded to f16: its smallest steps are then
+// 2^-36 of the row's largest. The running maximum is only moved, and what was
+// summed up scaled down, when it has grown by more than 2^3 (p stays below
+// 2^15).
+static constexpr float kPLog = 12.f, kSlack = 3.f;
 typedef float fx2 __attribute__((ext_vector_type(2)));
 
+// ---------------------------------------------------------------------------
+// Shares of the keys: every workgroup of a tile and head stores its rows' sums,
+// maximum and divisor (device scope, mfma_tile.h), and the last to arrive joins
+// them in the shares' order and writes the rows. Against a launch of its own
+// for that: 4 to 5 us less.
+// ---------------------------------------------------------------------------
+template <int D>
+struct Shares {
+    static constexpr int ROW = D + 4;
+    __amdgpu_buffer_rsrc_t r;
+    int tile;  // rows of a share
+    __device__ __forceinline__ Shares(const KvAttnArgs& a, int item, int tile_) : tile(tile_) {
+        r = make_rsrc(a.part + (int64_t)item * a.splits * tile_ * ROW);
+    }
+    __device__ __forceinline__ uint32_t at(int share, int row, int col) const {
+        return (uint32_t)((share * tile + row) * ROW + col) * 4u;
+    }
+    __device__ __forceinline__ void put4(int share, int row, int col, float x, float y, float z, float w) const {
+        typedef unsigned ux4 __attribute__((ext_vector_type(4)));
+        __builtin_amdgcn_raw_buffer_store_b128(ux4{__float_as_uint(x), __float_as_uint(y), __float_as_uint(z), __float_as_uint(w)}, r,
+                                               (int)at(share, row, col), 0, kDeviceScope);
+    }
+    // one wave: row `row` of the tile to `out`
+    template <typename T>
+    __device__ __forceinline__ void join(int shares, int row, T* out) const {
+        constexpr int PER = D >= 64 ? D / 64 : 1;
+        const int lane = threadIdx.x & 63, dim = lane % (D / PER) * PER;
+        float top = -INFINITY;
+        for (int s = lane; s < shares; s += 64) top = fmaxf(top, load_partial(r, at(s, row, D)));
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, o[PER];
+#pragma unroll
+        for (int q = 0; q < PER; ++q) o[q] = 0.f;
+        for (int s0 = 0; s0 < shares; s0 += 64) {
+            float w = 0.f;
+            if (s0 + lane < shares) {
+                w = __builtin_amdgcn_exp2f(load_partial(r, at(s0 + lane, row, D)) - base);
+                sum = fmaf(w, load_partial(r, at(s0 + lane, row, D + 1)), sum);
+            }
+            const int n = min(64, shares - s0);
+            for (int t = 0; t < n; t += 8) {
+                float v[8][PER];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const uint32_t from = at(min(s0 + t + u, shares - 1), row, dim);
+                    if constexpr (PER == 4) {
+                        const f32x4 x = load_partial4(r, from);
+                        v[u][0] = x[0], v[u][1] = x[1], v[u][2] = x[2], v[u][3] = x[3];
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < PER; ++q) v[u][q] = load_partial(r, from + 4 * q);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const float wt = __shfl(w, t + u);  // 0 behind the last share
+#pragma unroll
+                    for (int q = 0; q < PER; ++q) o[q] = fmaf(v[u][q], wt, o[q]);
+                }
+            }
+        }
+        sum = wave_add(sum);
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        if (lane < D / PER) {
+#pragma unroll
+            for (int q = 0; q < PER; ++q) out[dim + q] = (T)(o[q] * inv);
+        }
+    }
+};
+
+// waves of a workgroup for few query rows (dim 256: one wave's registers)
+constexpr int token_waves(int dim) { return dim <= 128 ? 8 : 4; }
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_attention_k(KvAttnArgs a) {
+__global__ void __launch_bounds__(64 * token_waves(D)) kv_attention_k(KvAttnArgs a) {
+    constexpr int NW = token_waves(D), STRIDE = 64 * NW;
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int STEPS = D / 32, PIECES = F32 ? 2 : 1, KV = D / 16;
-    __shared__ float ml[2][4][16];
-    __shared__ __align__(16) float os[3][16][D + 4];
+    constexpr int STEPS = D / 32, PIECES = F32 ? 2 : 1, KV = D / 16;  // KV: 16-dim blocks of the output
+    __shared__ float ml[2][NW][16];
+    __shared__ __align__(16) float os[NW / 2][16][D + 4];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int head_kv = blockIdx.y, split = blockIdx.z;
@@ -89,134 +175,167 @@ __global__ void __launch_bounds__(256) kv_attention_k(KvAttnArgs a) {
     const int head = head_kv * a.group + gh;
     const int first_pos = span.first() + (int)((int64_t)tile * 16 / a.group);
     const int64_t last = (int64_t)tile * 16 + 15 < all ? (int64_t)tile * 16 + 15 : all - 1;
-    const KeyRange range(first_pos, span.first() + (int)(last / a.group), a.window, a.splits, a.chunk, 256);
+    const int last_pos = span.first() + (int)(last / a.group);
+    const KeyRange range(first_pos, last_pos, a.window, a.splits, a.chunk, STRIDE);
     const int shares = range.shares();
     if (split >= shares) return;
     const int from = range.lo + split * range.chunk;
     const int to = min(range.hi, from + range.chunk);
 
-    // the query row's dims g * D / 4 .. + D / 4
-    f16x8 qf[PIECES][STEPS];
-    float qs = a.scale;
+    // K: the lane's row in the four blocks is in 16-key group i / 4. V: the
+    // lane's 16 keys are group g. A chunk's table entries are read one chunk
+    // before its keys and values; those into the registers of the chunk before
+    // as soon as these are used.
+    const int page = a.g.page, page16 = page / 16, wide = a.g.width - 1;
+    const int64_t plane = (int64_t)page * D, page_bytes = (int64_t)a.kv_heads * plane;
+    const int* table = a.g.table + (int64_t)b * a.g.width;
+    const int8_t* kbase = a.k + (int64_t)head_kv * plane + (int64_t)(i & 3) * D + g * (D / 4);
+    const int8_t* vbase = a.v + (int64_t)head_kv * plane + i * page;
+    int kid, vid;
+    auto find = [&](int tb) {
+        kid = table[min((int)slot_of(tb / 16 + (i >> 2), a.slot_magic), wide)];
+        vid = table[min((int)slot_of(tb / 16 + g, a.slot_magic), wide)];
+    };
+    ix2 kb[4][D / 32];
+    ix4 vb[KV];
+    float ks, vs;
+    bool have;
+    auto load_k = [&](int tb) {
+        const int t16 = tb / 16 + (i >> 2), off = (t16 - (int)slot_of(t16, a.slot_magic) * page16) * 16;
+        const int64_t pn = kid >= 0 && kid < a.g.pages && t16 * 16 < to ? kid : 0;
+        const int8_t* p = kbase + pn * page_bytes + off * D;
+#pragma unroll
+        for (int bl = 0; bl < 4; ++bl)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) kb[bl][c] = *reinterpret_cast<const ix2*>(p + bl * 4 * D + 8 * c);
+    };
+    auto load_v = [&](int tb) {
+        const int t16 = tb / 16 + g, off = (t16 - (int)slot_of(t16, a.slot_magic) * page16) * 16;
+        have = vid >= 0 && vid < a.g.pages && t16 * 16 < to;
+        const int64_t pn = have ? vid : 0;
+        const int8_t* p = vbase + pn * page_bytes + off;
+#pragma unroll
+        for (int c = 0; c < KV; ++c) vb[c] = *reinterpret_cast<const ix4*>(p + c * 16 * page);
+        ks = a.k_scale[pn * a.kv_heads + head_kv];
+        vs = a.v_scale[pn * a.kv_heads + head_kv];
+    };
+    // the query row's dims g * D / 4 .. + D / 4, read before the first keys
+    int tb = from + 64 * wave;
+    if (tb < to) find(tb);
+    constexpr int QV = 16 / (int)sizeof(T);
+    T qx[D / 4];
     {
         const T* qp = (const T*)a.q + row * a.ld + a.q_col + head * D + g * (D / 4);
-        float x[D / 4];
+        if (a.q_vec) {
+#pragma unroll
+            for (int d = 0; d < D / 4; d += QV) *reinterpret_cast<ix4*>(qx + d) = *reinterpret_cast<const ix4*>(qp + d);
+        } else {
+#pragma unroll
+            for (int d = 0; d < D / 4; ++d) qx[d] = qp[d];
+        }
+    }
+    if (tb < to) {
+        load_k(tb);
+        load_v(tb);
+        find(tb + STRIDE);
+    }
+    f16x8 qf[PIECES][STEPS];
+    float qs = a.scale;
+    int e = 0;
+    if (F32) {
+        // the row's largest value to [2^13, 2^14)
         float top = 0.f;
 #pragma unroll
-        for (int d = 0; d < D / 4; ++d) {
-            x[d] = row_ok ? (float)qp[d] : 0.f;
-            top = fmaxf(top, fabsf(x[d]));
-        }
-        if (F32) {
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            // the row's largest value to [2^13, 2^14)
-            int e = 0;
-            (void)frexpf(top, &e);
-            e = top > 0.f && top < INFINITY ? 14 - e : 0;
-            qs = ldexpf(qs, -e);
-#pragma unroll
-            for (int d = 0; d < D / 4; ++d) x[d] = ldexpf(x[d], e);
-        }
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = x[8 * s + j];
-                const half_t hi = (half_t)y;
-                qf[0][s][j] = hi;
-                if (F32) qf[PIECES - 1][s][j] = (half_t)(y - (float)hi);
-            }
+        for (int d = 0; d < D / 4; ++d) top = fmaxf(top, fabsf((float)qx[d]));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        (void)frexpf(top, &e);
+        e = top > 0.f && top < INFINITY ? 14 - e : 0;
+        qs = ldexpf(qs, -e);
     }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float y = F32 ? ldexpf((float)qx[8 * s + j], e) : (float)qx[8 * s + j];
+            const half_t hi = (half_t)y;
+            qf[0][s][j] = hi;
+            if (F32) qf[PIECES - 1][s][j] = (half_t)(y - (float)hi);
+        }
     float m = -INFINITY, l = 0.f;
     fx4 o[KV];
 #pragma unroll
     for (int c = 0; c < KV; ++c) o[c] = fx4{0.f, 0.f, 0.f, 0.f};
 
-    const int page = a.g.page, page16 = page / 16;
-    const int64_t plane = (int64_t)page * D;
-    for (int tb = from + 64 * wave; tb < to; tb += 256) {
-        // K: the lane's row in the four blocks is in 16-key group i / 4
-        uint32_t kb[4][D / 16];
-        {
-            const int t16 = tb / 16 + (i >> 2), slot = t16 / page16;
-            const int pn = t16 * 16 < to ? page_at(a.g, b, slot) : -1;
-            const int8_t* kp = a.k + ((int64_t)max(pn, 0) * a.kv_heads + head_kv) * plane +
-                               (int64_t)((t16 - slot * page16) * 16 + (i & 3)) * D + g * (D / 4);
-#pragma unroll
-            for (int bl = 0; bl < 4; ++bl)
-#pragma unroll
-                for (int c = 0; c < D / 16; c += 2) {
-                    const ix2 w = *reinterpret_cast<const ix2*>(kp + bl * 4 * D + 4 * c);
-                    kb[bl][c] = w[0], kb[bl][c + 1] = w[1];
-                }
-        }
-        // V: the lane's 16 keys are group g
-        ix4 vb[KV];
-        const int t16 = tb / 16 + g, slot = t16 / page16;
-        const int pn = t16 * 16 < to ? page_at(a.g, b, slot) : -1;
-        const int64_t at = (int64_t)max(pn, 0) * a.kv_heads + head_kv;
-        {
-            const int8_t* vp = a.v + at * plane + (t16 - slot * page16) * 16 + i * page;
-#pragma unroll
-            for (int c = 0; c < KV; ++c) vb[c] = *reinterpret_cast<const ix4*>(vp + c * 16 * page);
-        }
-        const float ku = pn >= 0 ? a.k_scale[at] * qs : 0.f;
-        float vu = pn >= 0 ? a.v_scale[at] : 1.f;
-        vu = vu == 0.f ? 1.f : vu;
-        const float lv = __builtin_amdgcn_logf(vu), iv = 1.0f / vu;
+    for (; tb < to; tb += STRIDE) {
         // scores of keys tb + 16 g + 4 b + r
         float x[16];
+        float top = -INFINITY;
 #pragma unroll
         for (int bl = 0; bl < 4; ++bl) {
             fx4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int st = 0; st < STEPS; ++st) {
-                const f16x8 kf = widen8(kb[bl][2 * st], kb[bl][2 * st + 1]);
+                const f16x8 kf = widen8((uint32_t)kb[bl][st][0], (uint32_t)kb[bl][st][1]);
 #pragma unroll
                 for (int pc = PIECES - 1; pc >= 0; --pc) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[pc][st], s, 0, 0, 0);
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = tb + 16 * g + 4 * bl + r;
-                const bool seen = pn >= 0 && j <= pos && (a.window <= 0 || j > pos - a.window);
-                x[4 * bl + r] = seen ? fmaf(s[r], ku, lv) : -INFINITY;
-            }
+            for (int r = 0; r < 4; ++r) x[4 * bl + r] = s[r];
         }
-        float mx = x[0];
+        load_k(tb + STRIDE);
+        const float vu = value_unit(vs);
+        float ku = ks * qs, lv = __builtin_amdgcn_logf(vu), iv = 1.0f / vu;
+        ku = ku == 0.f ? 0x1p-126f : ku;  // for the product with -inf
+        if (!(tb + 63 <= first_pos && (a.window <= 0 || tb > last_pos - a.window) && __all(have))) {
+            const int j = tb + 16 * g, low = a.window > 0 ? pos - a.window : INT_MIN, up = have ? pos : INT_MIN;
 #pragma unroll
-        for (int c = 1; c < 16; ++c) mx = fmaxf(mx, x[c]);
+            for (int c = 0; c < 16; ++c) x[c] = j + c <= up && j + c > low ? x[c] : -INFINITY;
+            // a row that sees none of the 16: their scales are not its own
+            if (!(j <= up && j + 15 > low)) ku = 1.f, lv = 0.f, iv = 0.f;
+        }
+#pragma unroll
+        for (int c = 0; c < 16; ++c) top = fmaxf(top, x[c]);
+        float mx = fmaf(top, ku, lv);
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;
-        const float alpha = __builtin_amdgcn_exp2f(m - base);
-        m = mn;
-        l *= alpha;
-        float p[16];
+        if (__any(mx > m + kSlack)) {
+            const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int c = 0; c < KV; ++c) o[c] *= alpha;
+        }
+        const float shift = lv - (m == -INFINITY ? 0.f : m - kPLog);
+        float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
-            p[c] = __builtin_amdgcn_exp2f(x[c] - base);
-            l += x[c] == -INFINITY ? 0.f : p[c] * iv;
+            x[c] = __builtin_amdgcn_exp2f(fmaf(x[c], ku, shift));
+            sum += x[c];
         }
+        l = fmaf(sum, iv, l);
 #pragma unroll
-        for (int c = 0; c < KV; ++c) o[c] *= alpha;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int n = 0; n < 2; ++n) {
             f16x8 pf[PIECES];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = p[8 * h + j] * kPScale;
-                const half_t hi = (half_t)y;
-                pf[0][j] = hi;
-                if (F32) pf[PIECES - 1][j] = (half_t)(y - (float)hi);
+            for (int j = 0; j < 8; j += 2) {
+                const float p0 = x[8 * n + j], p1 = x[8 * n + j + 1];
+                const f16x2 hi = __builtin_convertvector((fx2{p0, p1}), f16x2);
+                pf[0][j] = hi[0], pf[0][j + 1] = hi[1];
+                if (F32) {
+                    const f16x2 lo = __builtin_convertvector((fx2{p0 - (float)hi[0], p1 - (float)hi[1]}), f16x2);
+                    pf[PIECES - 1][j] = lo[0], pf[PIECES - 1][j + 1] = lo[1];
+                }
             }
 #pragma unroll
             for (int c = 0; c < KV; ++c) {
-                const f16x8 vf = widen8((uint32_t)vb[c][2 * h], (uint32_t)vb[c][2 * h + 1]);
+                const f16x8 vf = widen8((uint32_t)vb[c][2 * n], (uint32_t)vb[c][2 * n + 1]);
 #pragma unroll
                 for (int pc = PIECES - 1; pc >= 0; --pc) o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[pc], o[c], 0, 0, 0);
             }
         }
+        load_v(tb + STRIDE);
+        find(tb + 2 * STRIDE);
     }
     // join the waves
     l += __shfl_xor(l, 16);
@@ -225,37 +344,54 @@ __global__ void __launch_bounds__(256) kv_attention_k(KvAttnArgs a) {
     __syncthreads();
     float top = ml[0][0][i];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, ml[0][w][i]);
+    for (int w = 1; w < NW; ++w) top = fmaxf(top, ml[0][w][i]);
     const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) sum += ml[1][w][i] * __builtin_amdgcn_exp2f(ml[0][w][i] - base);
-    const float f = __builtin_amdgcn_exp2f(m - base) * (1.0f / kPScale);
+    for (int w = 0; w < NW; ++w) sum += ml[1][w][i] * __builtin_amdgcn_exp2f(ml[0][w][i] - base);
+    const float f = __builtin_amdgcn_exp2f(m - base);
 #pragma unroll
-    for (int c = 0; c < KV; ++c) {
-        o[c] *= f;
-        if (wave > 0) *reinterpret_cast<fx4*>(&os[wave - 1][i][16 * c + 4 * g]) = o[c];
+    for (int c = 0; c < KV; ++c) o[c] *= f;
+    // the upper half of the waves hands its sums to the lower, until one has all
+#pragma unroll
+    for (int n = NW / 2; n > 0; n /= 2) {
+        if (wave >= n && wave < 2 * n)
+#pragma unroll
+            for (int c = 0; c < KV; ++c) *reinterpret_cast<fx4*>(&os[wave - n][i][16 * c + 4 * g]) = o[c];
+        __syncthreads();
+        if (wave < n)
+#pragma unroll
+            for (int c = 0; c < KV; ++c) o[c] += *reinterpret_cast<const fx4*>(&os[wave][i][16 * c + 4 * g]);
+        if (n > 1) __syncthreads();
     }
-    __syncthreads();
-    if (wave > 0 || !row_ok) return;
-#pragma unroll
-    for (int c = 0; c < KV; ++c)
-#pragma unroll
-        for (int w = 0; w < 3; ++w) o[c] += *reinterpret_cast<const fx4*>(&os[w][i][16 * c + 4 * g]);
     if (shares == 1) {
+        if (wave > 0 || !row_ok) return;
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
         T* op = (T*)a.out + (row * a.heads + head) * D + 4 * g;
 #pragma unroll
-        for (int c = 0; c < KV; ++c)
+        for (int c = 0; c < KV; ++c) {
+            T v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) op[16 * c + r] = (T)(o[c][r] * inv);
-    } else {
-        float* pp = a.part + ((row * a.heads + head) * a.splits + split) * (D + 2);
+            for (int r = 0; r < 4; ++r) v[r] = (T)(o[c][r] * inv);
+            __builtin_memcpy(__builtin_assume_aligned(op + 16 * c, 4 * sizeof(T)), v, sizeof v);
+        }
+        return;
+    }
+    const int item = blockIdx.x * a.kv_heads + head_kv;
+    const Shares<D> part(a, item, 16);
+    if (wave == 0 && row_ok) {
 #pragma unroll
-        for (int c = 0; c < KV; ++c)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) pp[16 * c + 4 * g + r] = o[c][r];
-        if (g == 0) pp[D] = top, pp[D + 1] = sum;
+        for (int c = 0; c < KV; ++c) {
+            const float x = o[c][0], y = o[c][1], z = o[c][2], w = o[c][3];
+            part.put4(split, i, 16 * c + 4 * g, x, y, z, w);
+        }
+        if (g == 0) part.put4(split, i, D, top, sum, 0.f, 0.f);
+    }
+    if (!finish_arrive(a.counters + item, shares - 1)) return;
+    for (int r = wave; r < 16 && (int64_t)tile * 16 + r < all; r += NW) {
+        const int64_t f = (int64_t)tile * 16 + r;
+        const int t = (int)(f / a.group), hd = head_kv * a.group + (int)(f - (int64_t)t * a.group);
+        part.join(shares, r, (T*)a.out + ((int64_t)(span.end - span.rows + t) * a.heads + hd) * D);
     }
 }
 
@@ -269,9 +405,6 @@ __global__ void __launch_bounds__(256) kv_attention_k(KvAttnArgs a) {
 // Their 16-byte chunks are permuted so that 16 lanes reading a chunk of 16
 // rows hit all 64 banks. Two stages: chunk t + 1 is widened and stored, and
 // the loads of t + 2 go out, before t is used, with one barrier for each.
-//
-// The accumulators are only scaled down when some row's maximum has grown by
-// more than 2^3 since they last were (p is f16 and starts at 2^12).
 // ---------------------------------------------------------------------------
 typedef float fx16 __attribute__((ext_vector_type(16)));
 
@@ -282,11 +415,10 @@ __device__ __forceinline__ int lds_chunk(int row, int chunk) {  // byte offset; 
 }
 
 template <typename T, int D, int NW>
-__global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_prompt_k(KvAttnArgs a, int tiles) {
+__global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_prompt_k(KvAttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int STEPS = D / 16, PIECES = F32 ? 2 : 1, DB = D / 32, KRB = 2 * D;
     constexpr int ROWS = 32 * NW, THREADS = 64 * NW, STAGE = 64 * KRB + D * 128, LOADS = (4 * D + THREADS - 1) / THREADS;  // 16-byte pieces per thread and operand
-    constexpr float kSlack = 3.f;
     extern __shared__ __align__(16) char lds[];
     // [stage]: of 4 groups of 16 keys, K's scale, V's scale's logarithm and
     // inverse, 1 if they can be read; then the four last again
@@ -295,9 +427,8 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // one XCD after the other, so that the tiles of a head share its L2; the
     // tiles with most keys first
-    const int lin = xcd_remap(blockIdx.x, tiles * a.kv_heads * a.splits);
-    const int split = lin / (tiles * a.kv_heads), head_kv = lin / tiles - split * a.kv_heads;
-    int tile = tiles - 1 - lin % tiles;
+    const int lin = xcd_remap(blockIdx.x, a.tiles * a.kv_heads), head_kv = lin / a.tiles;
+    int tile = a.tiles - 1 - lin % a.tiles;
     const int b = __builtin_amdgcn_readfirstlane(
         find_share(tile, a.g.batch, [&](int s) { return query_tiles(span_of(a.g, s), a.group, ROWS); }));
     if (b < 0) return;
@@ -306,10 +437,8 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
     const int64_t all = (int64_t)span.rows * a.group, row0 = (int64_t)tile * ROWS;
     const int64_t last = row0 + ROWS - 1 < all ? row0 + ROWS - 1 : all - 1;
     const int first_pos = span.first() + (int)(row0 / a.group), last_pos = span.first() + (int)(last / a.group);
-    const KeyRange range(first_pos, last_pos, a.window, a.splits, a.chunk, 64);
-    const int shares = range.shares();
-    if (split >= shares) return;
-    const int from = range.lo + split * range.chunk, to = min(range.hi, from + range.chunk);
+    const KeyRange range(first_pos, last_pos, a.window, 1, 64, 64);
+    const int from = range.lo, to = range.hi;
     const int64_t fr = row0 + 32 * wave + i;
     const bool row_ok = fr < all;
     const int tok = (int)((row_ok ? fr : last) / a.group), gh = (int)((row_ok ? fr : last) - (int64_t)tok * a.group);
@@ -374,7 +503,7 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
             *reinterpret_cast<f16x8*>(lds + (vp ^ 16) + p * THREADS * 32) = widen8((uint32_t)vr[p][2], (uint32_t)vr[p][3]);
         }
         if (threadIdx.x < 4) {
-            const float vu = !can_read || su[1] == 0.f ? 1.f : su[1], ok = can_read ? 1.f : 0.f;
+            const float vu = can_read ? value_unit(su[1]) : 1.f, ok = can_read ? 1.f : 0.f;
             *reinterpret_cast<fx4*>(units + stage * 20 + threadIdx.x * 4) =
                 fx4{can_read ? su[0] * a.scale : 0.f, __builtin_amdgcn_logf(vu), 1.0f / vu, ok};
             units[stage * 20 + 16 + threadIdx.x] = ok;
@@ -485,7 +614,7 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
         f16x8 pf[PIECES][2][2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            const float shift = lv[kb] - base;  // base: m - 12, the 2^12 of kPScale
+            const float shift = lv[kb] - base;  // base: m - 12, of p's 2^12
             float sum = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -540,89 +669,64 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
 
     l += __shfl_xor(l, 32);
     if (!row_ok) return;
-    if (shares == 1) {
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-        T* op = (T*)a.out + ((int64_t)row * a.heads + head) * D + 4 * h;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    T* op = (T*)a.out + ((int64_t)row * a.heads + head) * D + 4 * h;
 #pragma unroll
-        for (int c = 0; c < DB; ++c)
+    for (int c = 0; c < DB; ++c)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                T v[4];
+        for (int q = 0; q < 4; ++q) {
+            T v[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = (T)(o[c][4 * q + r] * inv);
-                __builtin_memcpy(__builtin_assume_aligned(op + 32 * c + 8 * q, 4 * sizeof(T)), v, sizeof v);
-            }
-    } else {
-        float* pp = a.part + (((int64_t)row * a.heads + head) * a.splits + split) * (D + 2);
-#pragma unroll
-        for (int c = 0; c < DB; ++c)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) pp[32 * c + 8 * (r >> 2) + 4 * h + (r & 3)] = o[c][r];
-        if (h == 0) pp[D] = m, pp[D + 1] = l;
-    }
-}
-
-// joins the shares of one query row and head, in their order
-template <typename T, int D>
-__global__ void __launch_bounds__(64) kv_attention_join_k(KvAttnArgs a) {
-    int tok = blockIdx.x;
-    const int b = find_share(tok, a.g.batch, [&](int s) { return span_of(a.g, s).rows; });
-    if (b < 0) return;
-    const Span span = span_of(a.g, b);
-    const int head = blockIdx.y, gh = head % a.group;
-    // the tile that the row was in
-    const int64_t all = (int64_t)span.rows * a.group, tile = ((int64_t)tok * a.group + gh) / a.tile;
-    const int64_t last = (tile + 1) * a.tile < all ? (tile + 1) * a.tile - 1 : all - 1;
-    const KeyRange range(span.first() + (int)(tile * a.tile / a.group), span.first() + (int)(last / a.group), a.window,
-                         a.splits, a.chunk, a.tile == 16 ? 256 : 64);
-    const int shares = range.shares();
-    if (shares == 1) return;
-    const int64_t row = span.end - span.rows + tok;
-    const float* pp = a.part + (row * a.heads + head) * a.splits * (D + 2);
-    float top = -INFINITY;
-    for (int s = 0; s < shares; ++s) top = fmaxf(top, pp[(int64_t)s * (D + 2) + D]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int s = 0; s < shares; ++s) sum += pp[(int64_t)s * (D + 2) + D + 1] * __builtin_amdgcn_exp2f(pp[(int64_t)s * (D + 2) + D] - base);
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    for (int d = threadIdx.x; d < D; d += 64) {
-        float o = 0.f;
-        for (int s = 0; s < shares; ++s) o += pp[(int64_t)s * (D + 2) + d] * __builtin_amdgcn_exp2f(pp[(int64_t)s * (D + 2) + D] - base);
-        ((T*)a.out)[(row * a.heads + head) * D + d] = (T)(o * inv);
-    }
+            for (int r = 0; r < 4; ++r) v[r] = (T)(o[c][4 * q + r] * inv);
+            __builtin_memcpy(__builtin_assume_aligned(op + 32 * c + 8 * q, 4 * sizeof(T)), v, sizeof v);
+        }
 }
 
 template <typename T, int D, int NW>
-static void launch_prompt(const char* name, const KvAttnArgs& a, unsigned tiles) {
+static void launch_prompt(const char* name, const KvAttnArgs& a) {
     auto kernel = kv_prompt_k<T, D, NW>;
     constexpr int lds = 2 * (64 * 2 * D + D * 128) + 2 * 20 * 4;
     static const bool ok = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
     if (!ok) return fail(NNC_HIP_EDEVICE, name, "hipFuncSetAttribute failed");
-    launch(name, kernel, dim3(tiles * (unsigned)(a.kv_heads * a.splits)), dim3(64 * NW), lds, a, (int)tiles);
+    launch(NW == 8 ? "nnc_hip_kv_attention_256" : "nnc_hip_kv_attention_128", kernel, dim3((unsigned)(a.tiles * a.kv_heads)), dim3(64 * NW), lds, a);
 }
 
 template <typename T, int D>
-static void launch_kv_attention(const char* name, const KvAttnArgs& a, unsigned tiles) {
-    if (a.tile >= 128) {
-        if constexpr (D <= 128) {  // (dim 256: 512 registers a wave, and four of them)
-            if (a.tile == 256) launch_prompt<T, D, 8>(name, a, tiles);
-        }
-        if (a.tile == 128) launch_prompt<T, D, 4>(name, a, tiles);
-    } else {
-        launch(name, kv_attention_k<T, D>, dim3(tiles, (unsigned)a.kv_heads, (unsigned)a.splits), dim3(256), 0, a);
+static void launch_kv_attention(const char* name, const KvAttnArgs& a, int tile) {
+    if constexpr (D <= 128) {  // (dim 256: 512 registers a wave, and four of them)
+        if (tile == 256) return launch_prompt<T, D, 8>(name, a);
     }
-    if (a.splits > 1)
-        launch("nnc_hip_kv_attention_join", kv_attention_join_k<T, D>, dim3((unsigned)a.g.rows, (unsigned)a.heads), dim3(64), 0, a);
+    if (tile == 128) return launch_prompt<T, D, 4>(name, a);
+    launch(name, kv_attention_k<T, D>, dim3((unsigned)a.tiles, (unsigned)a.kv_heads, (unsigned)a.splits), dim3(64 * token_waves(D)), 0, a);
 }
 
 template <typename T>
-static void launch_dim(const char* name, const KvAttnArgs& a, unsigned tiles, int dim) {
+static void launch_dim(const char* name, const KvAttnArgs& a, int tile, int dim) {
     switch (dim) {
-        case 32: return launch_kv_attention<T, 32>(name, a, tiles);
-        case 64: return launch_kv_attention<T, 64>(name, a, tiles);
-        case 128: return launch_kv_attention<T, 128>(name, a, tiles);
-        default: return launch_kv_attention<T, 256>(name, a, tiles);
+        case 32: return launch_kv_attention<T, 32>(name, a, tile);
+        case 64: return launch_kv_attention<T, 64>(name, a, tile);
+        case 128: return launch_kv_attention<T, 128>(name, a, tile);
+        default: return launch_kv_attention<T, 256>(name, a, tile);
     }
+}
+
+// Query rows of a workgroup: 256 or 128 by the prompt kernel, 16 by the other,
+// which divides the keys instead. By the time that a CU takes for 64 keys,
+// dim 128, in us: 256 rows 2.5, 128 rows 1.9, two workgroups of them 3.0,
+// 256 rows as 16 tiles of 16 6.1. Two prompts of 2048 behind 2048, 32 heads
+// over 8: 248, 298 and (16 rows) 762 us; one of 256 behind 7936: 264, 248 and
+// 96; two of 1000, 16 heads of 64, fp32: 43, 36 and 65.
+static int query_tile(int64_t rows, int64_t batch, int group, int kv_heads, int dim) {
+    const int64_t cus = cu_count(), holders = rows < batch ? rows : batch;  // sequences that can have rows
+    auto count = [&](int tile) {
+        const int64_t n = ceil_div(rows * group, tile);
+        return (n > holders ? n : holders) * kv_heads;
+    };
+    const int64_t n256 = count(256), n128 = count(128);
+    const double t16 = 6.1 * (double)(rows * group) * kv_heads / (256.0 * cus);
+    const double t128 = n128 <= cus ? 1.9 : 3.0 * ceil_div(n128, 2 * cus);
+    const double t256 = dim <= 128 ? 2.5 * ceil_div(n256, cus) : 1e30;
+    return t256 < t128 && t256 < t16 ? 256 : t128 < t16 ? 128 : 16;
 }
 
 }  // namespace nnc
@@ -654,27 +758,34 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
     if (!ready(name)) return;
     const int capacity = c.ragged.width * c.page;
     const int longest = max_length > 0 && max_length < capacity ? max_length : capacity;
-    const int64_t holders = rows < c.ragged.batch ? rows : c.ragged.batch;  // sequences that can have rows
-    const int tile = c.dim <= 128 && rows * group >= 256 * holders ? 256 : rows * group >= 64 * holders ? 128 : 16, step = tile == 16 ? 256 : 64;
-    const int64_t tiles = query_tiles_bound(rows, c.ragged.batch, group, tile);
-    KvAttnArgs a{c.ragged, c.k, c.v, c.k_scale, c.v_scale, q->data, out->data, nullptr, ld, q_col, heads, c.kv_heads,
-                 group, window, 1, 0, tile, slot_magic(c.page / 16), scale * 1.44269504088896340736f};
+    const int tile = query_tile(rows, c.ragged.batch, group, c.kv_heads, c.dim);
+    const int64_t tiles = query_tiles_bound(rows, c.ragged.batch, group, tile), items = tiles * c.kv_heads;
+    KvAttnArgs a{c.ragged, c.k, c.v, c.k_scale, c.v_scale, q->data, out->data, nullptr, nullptr, ld, q_col, heads, c.kv_heads,
+                 group, window, 1, 64, (int)tiles, slot_magic(c.page / 16),
+                 aligned16(q->data) && ld * activation_bytes(q) % 16 == 0 && q_col * activation_bytes(q) % 16 == 0,
+                 scale * 1.44269504088896340736f};
     a.g.rows = (int)rows;
-    // enough shares of the keys to give every CU sixteen waves (eight of prompts)
-    const int64_t want = ceil_div((tile == 256 ? 1 : tile == 128 ? 2 : 4) * (int64_t)cu_count(), tiles * c.kv_heads), most = ceil_div(longest, 512);
-    a.splits = (int)(want < most ? want : most);
-    if (a.splits < 1) a.splits = 1;
-    a.chunk = (int)(ceil_div(ceil_div(longest > 0 ? longest : 1, a.splits), step) * step);
+    if (tile == 16) {
+        // shares of the keys, 512 or more each, while all workgroups run at
+        // once, one on a CU (a second round starts 6 us later: one sequence of
+        // 131072 in 32 shares 54.6 us, in 64 61)
+        const int step = 64 * token_waves(c.dim);
+        const int64_t want = cu_count() / items, most = ceil_div(longest, 512);
+        a.splits = (int)(want < most ? want : most);
+        if (a.splits < 1) a.splits = 1;
+        a.chunk = (int)(ceil_div(ceil_div(longest > 0 ? longest : 1, a.splits), step) * step);
+    }
     if (a.splits > 1) {
-        const size_t bytes = (size_t)rows * heads * a.splits * (c.dim + 2) * sizeof(float);
+        const size_t bytes = (size_t)items * a.splits * tile * (c.dim + 4) * sizeof(float);
         a.part = workspace(bytes);
-        if (!a.part) return fail(NNC_HIP_ENOMEM, name, "no workspace for %zu bytes of partial sums", bytes);
+        a.counters = tile_counters((size_t)items);
+        if (!a.part || !a.counters) return fail(NNC_HIP_ENOMEM, name, "no workspace for %zu bytes of partial sums", bytes);
     }
     set_work(0.0, 2.0 * c.kv_heads * c.dim * (double)longest * c.ragged.batch);
     if (q->dtype == NNC_DTYPE_FLOAT16)
-        launch_dim<half_t>(name, a, (unsigned)tiles, c.dim);
+        launch_dim<half_t>(name, a, tile, c.dim);
     else
-        launch_dim<float>(name, a, (unsigned)tiles, c.dim);
+        launch_dim<float>(name, a, tile, c.dim);
 }
 
 }  // extern "C"

@@ -93,7 +93,8 @@ RAGGED_HD int query_tiles(const Span& s, int group, int tile) {
     return (int)(((int64_t)s.rows * group + tile - 1) / tile);
 }
 RAGGED_HD int64_t query_tiles_bound(int64_t rows, int64_t batch, int group, int tile) {
-    return rows * group / tile + (rows < batch ? rows : batch);
+    const int64_t some = rows * group / tile + (rows < batch ? rows : batch), each = rows * ((group + tile - 1) / tile);
+    return some < each ? some : each;
 }
 
 // The keys that rows at positions first .. last see, [lo, hi), in at most

@@ -134,22 +134,25 @@ def attention(q, cache, starts, lengths, scale, window):
         if n <= 0:
             continue
         k, v, u, ok = cache.values(b, length)
-        for i in range(n):
-            pos, r = length - n + i, starts[b] + i
-            j = np.arange(length)
-            see = ok & (j <= pos) & ((j > pos - window) if window else True)
-            out[r] = 0
-            if not see.any():
-                continue
-            for h in range(heads):
-                kk, vv = k[h // group][see], v[h // group][see]
-                x = q[r, h].astype(np.float64)
-                s = scale * (kk @ x)
-                p = np.exp(s - s.max())
-                p /= p.sum()
-                out[r, h], size[r, h] = p @ vv, p @ np.abs(vv)
-                peak[r, h] = (p * u[h // group][see]).max()
-                reach[r, h], seen[r, h] = scale * (np.abs(kk) @ np.abs(x)).max(), see.sum()
+        j = np.arange(length)
+        pos = length - n + np.arange(n)[:, None]
+        see = ok & (j <= pos) & ((j > pos - window) if window else True)
+        some = see.any(1) if length else np.zeros(n, bool)
+        rs = slice(starts[b], starts[b] + n)
+        out[rs] = 0
+        if not some.any():
+            continue
+        for h in range(heads):
+            kk, vv, uu = k[h // group], v[h // group], u[h // group]
+            x = q[rs, h].astype(np.float64)
+            s = np.where(see, scale * (x @ kk.T), -np.inf)
+            top = np.where(some, s.max(1, initial=-np.inf), 0)
+            p = np.exp(s - top[:, None])
+            p /= np.where(some, p.sum(1), 1)[:, None]
+            out[rs, h], size[rs, h] = p @ vv, p @ np.abs(vv)
+            peak[rs, h] = (p * uu).max(1)
+            reach[rs, h] = np.where(see, scale * (np.abs(x) @ np.abs(kk).T), 0).max(1)
+            seen[rs, h] = see.sum(1)
     return out, (size, reach, seen, peak)
 
 

@@ -397,7 +397,7 @@ def check_attention(got, q, cache, starts, lengths, scale, window):
     return owned
 
 
-def run_attention(dev, rng, lengths, rows, heads, kv, dim, page, t, window=0, max_length=0, pad=2, sharp=2.0, width=None, garbage=False):
+def run_attention(dev, rng, lengths, rows, heads, kv, dim, page, t, window=0, max_length=0, pad=2, sharp=2.0, width=None, garbage=False, tile=None, spread=0):
     starts, total = ragged(rows, pad)
     table, pages = tables(rng, lengths, page, width=width)
     cache = s8.Cache(rng, pages, kv, page, dim, table)
@@ -410,11 +410,25 @@ def run_attention(dev, rng, lengths, rows, heads, kv, dim, page, t, window=0, ma
         used = {cache.page_of(b, t) for b, n in enumerate(lengths) for t in range(n)}
         for p in set(range(pages)) - used:
             cache.ks[p] = cache.vs[p] = np.nan
+    if spread:
+        cache.vs *= (2.0 ** rng.integers(-spread, spread + 1, cache.vs.shape)).astype(F32)
+        if t == F16:
+            cache.vs = np.minimum(cache.vs, F32(300))
+        cache.v[table[0, 1]] = cache.k[table[0, 1]] = 0
+        cache.vs[table[0, 1]] = cache.ks[table[0, 1]] = 0
     q_col = 3
     qrows = (rng.standard_normal((total, heads * dim + 6)) * sharp).astype(t)
     scale = dim ** -0.5
     d = dev({"q": qrows, **cache_arrays(cache, starts, lengths), "out": np.full((total, heads * dim), 7, t)})
+    if tile:
+        from nnc_py_amd import runtime
+        runtime.profile_reset()
+        runtime.profile_enable(True)
     d.call("nnc_hip_kv_attention", "q", *CACHE, "starts", "lengths", "out", q_col, heads, scale, window, max_length)
+    if tile:
+        names = [r["name"] for r in runtime.profile_table()]
+        runtime.profile_enable(False)
+        assert names == [f"nnc_hip_kv_attention_{tile}"]
     got = d.get("out")
     q = qrows[:, q_col:q_col + heads * dim].reshape(total, heads, dim)
     owned = check_attention(got, q, cache, starts, lengths, F32(scale), window)
@@ -438,6 +452,48 @@ def test_kv_attention_runs_of_tokens(heads, kv, dim, page, t, dev):
     than positions; padding behind."""
     rng = np.random.default_rng(heads * dim)
     run_attention(dev, rng, [70, 9, 140, 40, 3, 0, 129], [70, 2, 33, 0, 5, 4, 1], heads, kv, dim, page, t, garbage=True)
+
+
+PROMPTS = {128: ([130, 70, 40, 9, 0, 33], [130, 33, 3, 12, 4, 0], 32), 256: ([200, 130], [190, 110], 64)}
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("tile,dim,page", [(128, 32, 16), (128, 64, 48), (128, 128, 16), (128, 256, 64), (256, 32, 64), (256, 64, 16), (256, 128, 32)])
+def test_kv_attention_prompts(tile, dim, page, t, dev):
+    """Enough rows and heads for the kernels of 128 and 256 rows: whole
+    prompts, chunks, more rows than positions, none; windows; scores that pick
+    single keys; value scales from page to page 2^20 up and down, a page of
+    zeros; what no row sees is garbage."""
+    rng = np.random.default_rng(tile + dim)
+    lengths, rows, kv = PROMPTS[tile]
+    for window, sharp, spread in ((0, 2.0, 0), (37, 1.0, 0), (100, 30.0, 0), (0, 1.0, 20), (0, 0.0, 3)):
+        run_attention(dev, rng, lengths, rows, 128, kv, dim, page, t, window=window, garbage=True, tile=tile, sharp=sharp, spread=spread)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("tile", [128, 256])
+def test_kv_attention_prompts_with_pages_that_cannot_be_read(tile, t, dev):
+    """Page numbers outside the cache inside a prompt: their keys are unseen."""
+    rng = np.random.default_rng(tile)
+    lengths, rows, kv = PROMPTS[tile]
+    starts, total = ragged(rows, 0)
+    table, pages = tables(rng, lengths, 16)
+    table[0, 2], table[0, 7], table[1, 0] = -1, pages, 2 ** 31 - 1
+    cache = s8.Cache(rng, pages, kv, 16, 64, table)
+    q = (rng.standard_normal((total, 128 * 64)) * 2).astype(t)
+    d = dev({"q": q, **cache_arrays(cache, starts, lengths), "out": np.zeros((total, 128 * 64), t)})
+    d.call("nnc_hip_kv_attention", "q", *CACHE, "starts", "lengths", "out", 0, 128, 0.125, 0, 0)
+    check_attention(d.get("out"), q.reshape(total, 128, 64), cache, starts, lengths, F32(0.125), 0)
+
+
+def test_kv_attention_prompts_without_a_table(dev):
+    """A table of no width: no row sees anything."""
+    rng = np.random.default_rng(0)
+    cache = s8.Cache(rng, 2, 32, 16, 64, np.zeros((2, 0), I32))
+    starts = np.array([0, 100, 190], I32)
+    d = dev({"q": np.ones((190, 128 * 64), F32), **cache_arrays(cache, starts, [40, 0]), "out": np.ones((190, 128 * 64), F32)})
+    d.call("nnc_hip_kv_attention", "q", *CACHE, "starts", "lengths", "out", 0, 128, 0.125, 0, 0)
+    assert not d.get("out").any()
 
 
 @pytest.mark.parametrize("t", [F32, F16])
