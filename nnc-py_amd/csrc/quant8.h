@@ -37,18 +37,36 @@ __device__ __forceinline__ float max_nan(float a, float b) { return a > b || a !
 // number 0)
 __device__ __forceinline__ float inverse8(float unit) { return unit > 0.f ? 1.0f / unit : 0.f; }
 
-// The whole number nearest to x / unit, ties to even, as if the quotient were
-// exact: x * inverse is off by a few of its last bits, so the rounded
-// product can be the neighbour; the remainder x - q * unit, exact in one fused
-// operation, says so. |x| <= 127 units.
+// The whole numbers nearest to x / unit, ties to even, as if the quotient were
+// exact: x * inverse is off by a few of its last bits, so the rounded product
+// can be the neighbour; the remainder x - q * unit, exact in one fused
+// operation, says so, and only then (one value in 2^16) is there more to do.
+// |x| <= 127 units.
+template <int N>
+__device__ __forceinline__ void whole8_run(const float (&x)[N], float unit, float inverse, int8_t (&out)[N]) {
+    float q[N];
+    const float half = 0.5f * unit;
+    bool near = false;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        q[e] = rintf(x[e] * inverse);
+        near |= fabsf(fmaf(-q[e], unit, x[e])) >= half;
+    }
+    if (near) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float rest = fmaf(-q[e], unit, x[e]);
+            if (fabsf(rest) > half || (fabsf(rest) == half && ((int)q[e] & 1))) q[e] += copysignf(1.0f, rest);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) out[e] = inverse == 0.f ? (int8_t)0 : (int8_t)(int)q[e];
+}
 __device__ __forceinline__ int whole8(float x, float unit, float inverse) {
-    float q = rintf(x * inverse);
-    if (inverse == 0.f) return 0;
-    const float rest = fmaf(-q, unit, x), half = 0.5f * unit;
-    const bool odd = (int)q & 1;
-    if (rest > half || (rest == half && odd)) q += 1.0f;
-    if (rest < -half || (rest == -half && odd)) q -= 1.0f;
-    return (int)q;
+    const float v[1] = {x};
+    int8_t q[1];
+    whole8_run<1>(v, unit, inverse, q);
+    return q[0];
 }
 
 // Maximum (NaN if any is) and sum over a wave's 64 lanes, in every lane.

@@ -26,10 +26,159 @@ struct RowArgs {
     int64_t rows;
     int width;
     float eps;
+    bool nt;  // outputs of kNtStoreBytes or more
 };
 
-// One workgroup per row, the row read from memory (its later reads come from
-// the caches) for the squares, the largest value and the output.
+// A store of up to 16 bytes, non-temporal or not.
+template <typename P>
+__device__ __forceinline__ void store_pack(bool nt, P* to, const P& v) {
+    if constexpr (sizeof(P) == 16) {
+        const nt_u32x4 u = __builtin_bit_cast(nt_u32x4, v);
+        nt ? __builtin_nontemporal_store(u, (nt_u32x4*)to) : (void)(*(nt_u32x4*)to = u);
+    } else if constexpr (sizeof(P) == 8) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        nt ? __builtin_nontemporal_store(u, (uint64_t*)to) : (void)(*(uint64_t*)to = u);
+    } else if constexpr (sizeof(P) == 4) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v);
+        nt ? __builtin_nontemporal_store(u, (uint32_t*)to) : (void)(*(uint32_t*)to = u);
+    } else {
+        *to = v;
+    }
+}
+
+// N elements of a row, loaded and stored as one.
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Pack {
+    T v[N];
+};
+
+template <size_t BYTES>
+struct HeldAs;
+template <>
+struct HeldAs<16> {
+    typedef nt_u32x4 type;
+};
+template <>
+struct HeldAs<4> {
+    typedef uint32_t type;
+};
+template <>
+struct HeldAs<2> {
+    typedef uint16_t type;
+};
+
+// |x|'s bits: ordered like the values, NaN above infinity
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// Rows that fit the registers of TPR threads (64: a wave, 256: a workgroup),
+// PER packs of N elements each: one read, one write. The next row's loads go
+// out before the row is worked on, and the weights stay in registers over
+// all rows of a wave. Bound by HBM: about 22 vector operations per element are
+// 38 us for [16384, 4096], its bytes 103.
+template <typename T, int N, int TPR, int PER, int OUT, bool NORM>
+__global__ void __launch_bounds__(256) row_norm_reg_k(RowArgs a) {
+    typedef Pack<T, N> P;
+    typedef typename HeldAs<sizeof(P)>::type Held;  // (as an array of halves it takes twice the registers)
+    constexpr int ROWS = 256 / TPR;
+    __shared__ float part[2][4];
+    const int lane = threadIdx.x % TPR, packs = a.width / N;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+    if (TPR == 64 && row >= a.rows) return;
+    auto load = [&](Held (&v)[PER], const void* base, int64_t r) {
+        const P* p = (const P*)((const T*)base + r * a.width);
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int i = lane + TPR * q;
+            v[q] = i < packs ? __builtin_bit_cast(Held, p[i]) : Held{};
+        }
+    };
+    Held w[NORM ? PER : 1], x[PER], res[NORM ? PER : 1];
+    if constexpr (NORM) load(w, a.w, 0);
+    load(x, a.in, row);
+    if constexpr (NORM)
+        if (a.res) load(res, a.res, row);
+    for (; row < a.rows; row += step) {
+        // (not converted to 32 bits once for all rows: twice the registers)
+        if constexpr (NORM && N > 1)
+#pragma unroll
+            for (int q = 0; q < PER; ++q) asm volatile("" : "+v"(w[q]));
+        Held s[PER];
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            s[q] = x[q];
+            if constexpr (NORM) {
+                if (a.res) {
+                    P v = __builtin_bit_cast(P, x[q]), u = __builtin_bit_cast(P, res[q]);
+#pragma unroll
+                    for (int e = 0; e < N; ++e) v.v[e] = (T)((float)v.v[e] + (float)u.v[e]);
+                    s[q] = __builtin_bit_cast(Held, v);
+                }
+            }
+        }
+        if (TPR == 64 && row + step < a.rows) {
+            load(x, a.in, row + step);
+            if constexpr (NORM)
+                if (a.res) load(res, a.res, row + step);
+        }
+        float sq = 0.f;
+        uint32_t big = 0;
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const P v = __builtin_bit_cast(P, s[q]), u = __builtin_bit_cast(P, w[NORM ? q : 0]);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float y = (float)v.v[e];
+                if (NORM) sq = fmaf(y, y, sq);
+                if (OUT == kRowsInt8) big = max(big, abs_bits(NORM ? y * (float)u.v[e] : y));
+            }
+        }
+        float top = __uint_as_float(big);
+        if (NORM) sq = wave_add(sq);
+        if (OUT == kRowsInt8) {
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(__shfl_xor(top, o))));
+        }
+        if constexpr (TPR == 256) {
+            if ((threadIdx.x & 63) == 0) part[0][threadIdx.x >> 6] = sq, part[1][threadIdx.x >> 6] = top;
+            __syncthreads();
+            sq = (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]);
+            top = max_nan(max_nan(part[1][0], part[1][1]), max_nan(part[1][2], part[1][3]));
+            __syncthreads();
+        }
+        const float r = NORM ? 1.0f / sqrtf(sq / (float)a.width + a.eps) : 1.0f;
+        const float unit = unit8(top), inverse = inverse8(unit);
+        if (OUT == kRowsInt8 && lane == 0) a.scale[row] = r * unit;
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int i = lane + TPR * q;
+            if (i >= packs) continue;
+            const P v = __builtin_bit_cast(P, s[q]), u = __builtin_bit_cast(P, w[NORM ? q : 0]);
+            if (NORM && a.sum) store_pack(a.nt, (P*)((T*)a.sum + row * a.width) + i, v);
+            if constexpr (OUT == kRowsInt8) {
+                float t[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) t[e] = NORM ? (float)v.v[e] * (float)u.v[e] : (float)v.v[e];
+                Pack<int8_t, N> out;
+                whole8_run<N>(t, unit, inverse, out.v);
+                store_pack(a.nt, (Pack<int8_t, N>*)((int8_t*)a.out + row * a.width) + i, out);
+            } else if constexpr (NORM) {
+                P out;
+#pragma unroll
+                for (int e = 0; e < N; ++e) out.v[e] = (T)((float)v.v[e] * r * (float)u.v[e]);
+                store_pack(a.nt, (P*)((T*)a.out + row * a.width) + i, out);
+            }
+        }
+        if (TPR == 256 && row + step < a.rows) {
+            load(x, a.in, row + step);
+            if constexpr (NORM)
+                if (a.res) load(res, a.res, row + step);
+        }
+    }
+}
+
+// Longer rows: one workgroup per row, the row read from memory (its later reads
+// come from the caches) for the squares, the largest value and the output.
 template <typename T, int OUT, bool NORM>
 __global__ void __launch_bounds__(256) row_norm_k(RowArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -69,20 +218,70 @@ __global__ void __launch_bounds__(256) row_norm_k(RowArgs a) {
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) row_float_k(const int8_t* in, const float* scale, T* out, int64_t rows, int width) {
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+// N elements a thread.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) row_float_k(const int8_t* in, const float* scale, T* out, int64_t packs, uint32_t per_row, bool nt) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < packs; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = packs >> 32 ? i / per_row : (uint32_t)i / per_row;
         const float u = scale[row];
-        for (int i = threadIdx.x; i < width; i += 256) out[row * width + i] = (T)((float)in[row * width + i] * u);
+        const Pack<int8_t, N> q = ((const Pack<int8_t, N>*)in)[i];
+        Pack<T, N> v;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v.v[e] = (T)((float)q.v[e] * u);
+        store_pack(nt, (Pack<T, N>*)out + i, v);
     }
 }
 
+template <typename T>
+static void launch_float(const char* name, const int8_t* in, const float* scale, T* out, int64_t rows, int width) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const bool nt = rows * width * (int64_t)sizeof(T) >= kNtStoreBytes;
+    if (width % N == 0 && aligned16(out) && ((uintptr_t)in & (N - 1)) == 0) {
+        const int64_t packs = rows * (width / N);
+        launch(name, row_float_k<T, N>, dim3(grid_for(packs, 2)), dim3(256), 0, in, scale, out, packs, (uint32_t)(width / N), nt);
+    } else {
+        launch(name, row_float_k<T, 1>, dim3(grid_for(rows * width, 4)), dim3(256), 0, in, scale, out, rows * width, (uint32_t)width, false);
+    }
+}
+
+template <typename T, int N, int TPR, int PER, bool NORM>
+static void launch_rows_reg(const char* name, const RowArgs& a, bool int8) {
+    // every CU its fill of waves; each then walks its rows
+    const int64_t groups = ceil_div(a.rows, 256 / TPR), most = (int64_t)cu_count() * (TPR == 64 ? 8 : 16);
+    const dim3 grid((unsigned)(groups < most ? groups : most));
+    if (int8)
+        launch(name, row_norm_reg_k<T, N, TPR, PER, kRowsInt8, NORM>, grid, dim3(256), 0, a);
+    else if constexpr (NORM)
+        launch(name, row_norm_reg_k<T, N, TPR, PER, kRowsFloat, true>, grid, dim3(256), 0, a);
+}
+
+// A wave to a row while there are rows for every SIMD to have several, else a
+// workgroup, which has a row's elements sooner: [8, 4096] W256 us against W64.
 template <typename T, bool NORM>
-static void launch_rows(const char* name, const RowArgs& a, bool int8) {
+static void launch_rows(const char* name, RowArgs a, bool int8) {
+    constexpr int N = 16 / (int)sizeof(T);
+    a.nt = a.rows * a.width * (int64_t)(int8 ? 1 : sizeof(T)) >= kNtStoreBytes;
+    bool packed = a.width % N == 0 && ((uintptr_t)a.out & (int8 ? N - 1 : 15)) == 0;
+    for (const void* p : {a.in, a.res, a.w, (const void*)a.sum}) packed &= aligned16(p);
+    const int packs = a.width / N;
+    if (packed) {
+        if (a.rows >= 4 * cu_count()) {
+            if (packs <= 64) return launch_rows_reg<T, N, 64, 1, NORM>(name, a, int8);
+            if (packs <= 128) return launch_rows_reg<T, N, 64, 2, NORM>(name, a, int8);
+            if (packs <= 256) return launch_rows_reg<T, N, 64, 4, NORM>(name, a, int8);
+            if (packs <= 512) return launch_rows_reg<T, N, 64, 8, NORM>(name, a, int8);
+        }
+        if (packs <= 256) return launch_rows_reg<T, N, 256, 1, NORM>(name, a, int8);
+        if (packs <= 512) return launch_rows_reg<T, N, 256, 2, NORM>(name, a, int8);
+        if (packs <= 1024) return launch_rows_reg<T, N, 256, 4, NORM>(name, a, int8);
+        if (packs <= 2048) return launch_rows_reg<T, N, 256, 8, NORM>(name, a, int8);
+    } else if (a.width <= 256 * 8) {
+        return launch_rows_reg<T, 1, 256, 8, NORM>(name, a, int8);
+    }
     const unsigned grid = (unsigned)(a.rows < 65536 ? a.rows : 65536);
     if (int8)
         launch(name, row_norm_k<T, kRowsInt8, NORM>, dim3(grid), dim3(256), 0, a);
-    else if (NORM)
+    else if constexpr (NORM)
         launch(name, row_norm_k<T, kRowsFloat, true>, dim3(grid), dim3(256), 0, a);
 }
 
@@ -120,7 +319,7 @@ void nnc_hip_rms_norm(Tensor* in, Tensor* res, Tensor* weight, Tensor* sum, Tens
         return fail(NNC_HIP_EINVAL, name, "scale must be float32, one for each row");
     if (!ready(name)) return;
     RowArgs a{in->data, res ? res->data : nullptr, weight->data, sum ? sum->data : nullptr, out->data,
-              scale ? (float*)scale->data : nullptr, rows, (int)width, eps};
+              scale ? (float*)scale->data : nullptr, rows, (int)width, eps, false};
     const double e = activation_bytes(in);
     set_work(8.0 * rows * width, (double)rows * width * (e * (1 + !!res + !!sum) + (int8 ? 1.0 : e)));
     if (in->dtype == NNC_DTYPE_FLOAT16)
@@ -140,7 +339,7 @@ void nnc_hip_quantize_rows(Tensor* in, Tensor* out, Tensor* scale) {
     if (width > (1 << 30)) return fail(NNC_HIP_EUNSUPP, name, "rows of %lld elements", (long long)width);
     if (numel(scale) != rows) return fail(NNC_HIP_EINVAL, name, "scale must be one for each row");
     if (!ready(name)) return;
-    RowArgs a{in->data, nullptr, nullptr, nullptr, out->data, (float*)scale->data, rows, (int)width, 0.f};
+    RowArgs a{in->data, nullptr, nullptr, nullptr, out->data, (float*)scale->data, rows, (int)width, 0.f, false};
     set_work(4.0 * rows * width, (double)rows * width * (activation_bytes(in) + 1.0));
     if (in->dtype == NNC_DTYPE_FLOAT16)
         launch_rows<half_t, false>(name, a, true);
@@ -158,15 +357,12 @@ void nnc_hip_dequantize_rows(Tensor* in, Tensor* scale, Tensor* out) {
     const int64_t width = in->shape[in->ndim - 1], rows = numel(in) / width;
     if (width > (1 << 30)) return fail(NNC_HIP_EUNSUPP, name, "rows of %lld elements", (long long)width);
     if (numel(scale) != rows) return fail(NNC_HIP_EINVAL, name, "scale must be one for each row");
-    const unsigned grid = (unsigned)(rows < 65536 ? rows : 65536);
     if (!ready(name)) return;
     set_work(1.0 * rows * width, (double)rows * width * (activation_bytes(out) + 1.0));
     if (out->dtype == NNC_DTYPE_FLOAT16)
-        launch(name, row_float_k<half_t>, dim3(grid), dim3(256), 0, (const int8_t*)in->data, (const float*)scale->data,
-               (half_t*)out->data, rows, (int)width);
+        launch_float(name, (const int8_t*)in->data, (const float*)scale->data, (half_t*)out->data, rows, (int)width);
     else
-        launch(name, row_float_k<float>, dim3(grid), dim3(256), 0, (const int8_t*)in->data, (const float*)scale->data,
-               (float*)out->data, rows, (int)width);
+        launch_float(name, (const int8_t*)in->data, (const float*)scale->data, (float*)out->data, rows, (int)width);
 }
 
 }  // extern "C"
