@@ -69,6 +69,15 @@ __device__ __forceinline__ int whole8(float x, float unit, float inverse) {
     return q[0];
 }
 
+// N elements of a row, loaded and stored as one.
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Pack {
+    T v[N];
+};
+
+// |x|'s bits: ordered like the values, NaN above infinity
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
 // Maximum (NaN if any is) and sum over a wave's 64 lanes, in every lane.
 __device__ __forceinline__ float wave_max_nan(float v) {
 #pragma unroll
