@@ -14,8 +14,10 @@
 // q u_old / u; that is at most half a step more each time it does. Positions
 // behind the sequence's length are left as they were.
 //
-// One workgroup per touched page and head does all of this, so nothing is
-// shared between workgroups and no atomics are needed.
+// One wave or workgroup per touched page and head does all of this, so nothing
+// is shared between workgroups and no atomics are needed.
+#include <tuple>
+
 #include "quant8.h"
 
 namespace nnc {
@@ -86,6 +88,185 @@ struct KvArgs {
     int k_col, v_col, kv_heads, dim;
 };
 
+// ---------------------------------------------------------------------------
+// A group of TPG threads (a wave, or a workgroup) takes a page's K or V of one
+// head in quads: four consecutive positions by V dims, V of the rows' type in
+// 16 bytes. A quad is four 16-byte accesses of the rows; of K four runs of V
+// bytes, of V (one row of `page` bytes per dim) V words of four positions,
+// which go through LDS to whole 16-byte accesses of the cache.
+// ---------------------------------------------------------------------------
+template <typename T, int TPG>
+struct Quads {
+    static constexpr int V = 16 / (int)sizeof(T);
+    typedef Pack<T, V> Row;
+    typedef Pack<int8_t, V> Held;
+    int page, dim, chunks, count, thread;  // chunks: of V dims
+    __device__ __forceinline__ Quads(const KvArgs& a) : page(a.g.page), dim(a.dim), chunks(a.dim / V), count(a.g.page / 4 * chunks), thread(threadIdx.x % TPG) {}
+    // LDS bytes between two dims: a word past a multiple of 16, off the banks
+    __device__ __forceinline__ int stride() const { return page + 4; }
+    __device__ __forceinline__ static void sync() {
+        if (TPG == 64) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        } else {
+            __syncthreads();
+        }
+    }
+};
+
+template <typename T, int TPG, int QPER>
+__global__ void __launch_bounds__(256) kv_write_quads_k(KvArgs a) {
+    typedef Quads<T, TPG> Q;
+    extern __shared__ __align__(16) char lds[];
+    __shared__ float part[4];
+    const Q z(a);
+    const int pair = blockIdx.y * (256 / TPG) + threadIdx.x / TPG, which = pair & 1, head = pair >> 1;
+    int share = blockIdx.x;
+    const int b = find_share(share, a.g.batch, [&](int i) { return touched_pages(a.g, i); });
+    if (b < 0 || head >= a.kv_heads) return;  // (a workgroup of one group has one head)
+    const PageShare p(a.g, b, share);
+    if (p.page_no < 0) return;
+    const int64_t at = (int64_t)p.page_no * a.kv_heads + head, ld = which ? a.v_ld : a.k_ld;
+    const T* rows = (const T*)(which ? a.v_rows : a.k_rows) + (which ? a.v_col : a.k_col) + head * z.dim;
+    int8_t* held = (which ? a.v : a.k) + at * z.page * z.dim;
+    float* scale = (which ? a.v_scale : a.k_scale) + at;
+    const float before = *scale;
+    const int lo = p.fresh - p.begin, hi = p.stop - p.begin;
+    nt_u32x4 x[QPER][4];
+    uint32_t big = 0;
+#pragma unroll
+    for (int q = 0; q < QPER; ++q) {
+        const int e = z.thread + TPG * q, t4 = e / z.chunks * 4, d = e % z.chunks * Q::V;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const bool in = e < z.count && t4 + u >= lo && t4 + u < hi;
+            x[q][u] = in ? *(const nt_u32x4*)(rows + (int64_t)p.span.row(p.begin + t4 + u) * ld + d) : nt_u32x4{0, 0, 0, 0};
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < QPER; ++q)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const typename Q::Row v = __builtin_bit_cast(typename Q::Row, x[q][u]);
+#pragma unroll
+            for (int i = 0; i < Q::V; ++i) big = max(big, abs_bits((float)v.v[i]));
+        }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) big = max(big, (uint32_t)__shfl_xor((int)big, o));
+    float top = __uint_as_float(big);
+    if constexpr (TPG == 256) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+        __syncthreads();  // everybody has read the scale, too
+        top = max_nan(max_nan(part[0], part[1]), max_nan(part[2], part[3]));
+    }
+    float unit = unit8(top);
+    if (lo > 0) unit = max_nan(before, unit);
+    if (z.thread == 0) *scale = unit;
+    if (lo > 0 && !(unit == before)) {
+        for (int i = z.thread; i < lo * z.dim; i += TPG) {
+            int8_t* w = held + (which ? i % z.dim * z.page + i / z.dim : i);
+            *w = unit > 0.f ? (int8_t)rint((double)*w * (double)before / (double)unit) : 0;
+        }
+    }
+    const float inverse = inverse8(unit);
+    char* mine = lds + threadIdx.x / TPG * z.dim * z.stride();
+#pragma unroll
+    for (int q = 0; q < QPER; ++q) {
+        const int e = z.thread + TPG * q, t4 = e / z.chunks * 4, d = e % z.chunks * Q::V;
+        if (e >= z.count) continue;
+        typename Q::Held w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const typename Q::Row v = __builtin_bit_cast(typename Q::Row, x[q][u]);
+            float f[Q::V];
+#pragma unroll
+            for (int i = 0; i < Q::V; ++i) f[i] = (float)v.v[i];
+            whole8_run<Q::V>(f, unit, inverse, w[u].v);
+            if (!which && t4 + u >= lo && t4 + u < hi) *(typename Q::Held*)(held + (t4 + u) * z.dim + d) = w[u];
+        }
+        if (which) {
+#pragma unroll
+            for (int i = 0; i < Q::V; ++i) {
+                const uint32_t word = (uint8_t)w[0].v[i] | (uint32_t)(uint8_t)w[1].v[i] << 8 | (uint32_t)(uint8_t)w[2].v[i] << 16 | (uint32_t)(uint8_t)w[3].v[i] << 24;
+                *(uint32_t*)(mine + (d + i) * z.stride() + t4) = word;
+            }
+        }
+    }
+    Q::sync();
+    if (!which) return;
+    if (lo == 0 && hi == z.page) {
+        for (int o = z.thread * 16; o < z.dim * z.page; o += TPG * 16) {
+            const uint32_t* w = (const uint32_t*)(mine + o / z.page * z.stride() + o % z.page);
+            *(nt_u32x4*)(held + o) = nt_u32x4{w[0], w[1], w[2], w[3]};
+        }
+    } else {
+        // part of a page: the positions of the call and no others
+        const int from = lo & ~3, words = (hi - from + 3) / 4;
+        for (int i = z.thread; i < words * z.dim; i += TPG) {
+            const int d = i / words, t = from + i % words * 4;
+            const char* w = mine + d * z.stride() + t;
+            if (t >= lo && t + 4 <= hi) {
+                *(uint32_t*)(held + d * z.page + t) = *(const uint32_t*)w;
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (t + u >= lo && t + u < hi) held[d * z.page + t + u] = (int8_t)w[u];
+            }
+        }
+    }
+}
+
+template <typename T, int TPG>
+__global__ void __launch_bounds__(256) kv_read_quads_k(KvArgs a) {
+    typedef Quads<T, TPG> Q;
+    extern __shared__ __align__(16) char lds[];
+    const Q z(a);
+    const int pair = blockIdx.y * (256 / TPG) + threadIdx.x / TPG, which = pair & 1, head = pair >> 1;
+    int share = blockIdx.x;
+    const int b = find_share(share, a.g.batch, [&](int i) { return touched_pages(a.g, i); });
+    if (b < 0 || head >= a.kv_heads) return;
+    const PageShare p(a.g, b, share);
+    if (p.page_no < 0) return;
+    const int64_t at = (int64_t)p.page_no * a.kv_heads + head, ld = which ? a.v_ld : a.k_ld;
+    T* rows = (T*)(which ? a.v_rows : a.k_rows) + (which ? a.v_col : a.k_col) + head * z.dim;
+    const int8_t* held = (which ? a.v : a.k) + at * z.page * z.dim;
+    const float unit = (which ? a.v_scale : a.k_scale)[at];
+    const int lo = p.fresh - p.begin, hi = p.stop - p.begin;
+    char* mine = lds + threadIdx.x / TPG * z.dim * z.stride();
+    if (which)
+        for (int o = z.thread * 16; o < z.dim * z.page; o += TPG * 16) {
+            const nt_u32x4 v = *(const nt_u32x4*)(held + o);
+            uint32_t* w = (uint32_t*)(mine + o / z.page * z.stride() + o % z.page);
+            w[0] = v[0], w[1] = v[1], w[2] = v[2], w[3] = v[3];
+        }
+    Q::sync();
+    for (int e = z.thread; e < z.count; e += TPG) {
+        const int t4 = e / z.chunks * 4, d = e % z.chunks * Q::V;
+        if (t4 + 3 < lo || t4 >= hi) continue;
+        uint32_t word[Q::V];
+        if (which)
+#pragma unroll
+            for (int i = 0; i < Q::V; ++i) word[i] = *(const uint32_t*)(mine + (d + i) * z.stride() + t4);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (t4 + u < lo || t4 + u >= hi) continue;
+            typename Q::Held w;
+            if (which) {
+#pragma unroll
+                for (int i = 0; i < Q::V; ++i) w.v[i] = (int8_t)(word[i] >> 8 * u);
+            } else {
+                w = *(const typename Q::Held*)(held + (t4 + u) * z.dim + d);
+            }
+            typename Q::Row v;
+#pragma unroll
+            for (int i = 0; i < Q::V; ++i) v.v[i] = (T)((float)w.v[i] * unit);
+            *(typename Q::Row*)(rows + (int64_t)p.span.row(p.begin + t4 + u) * ld + d) = v;
+        }
+    }
+}
+
+// Rows that start on no 16 bytes, and pages of more than 1024 quads: one
+// workgroup per page and head, element by element.
 template <typename T>
 __global__ void __launch_bounds__(256) kv_write_k(KvArgs a) {
     const int head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -155,6 +336,56 @@ __global__ void __launch_bounds__(256) kv_read_k(KvArgs a) {
     }
 }
 
+template <typename T>
+static bool quads(const KvArgs& a, int* count) {
+    *count = a.g.page * a.dim / (4 * (16 / (int)sizeof(T)));
+    for (auto [p, col, ld] : {std::tuple(a.k_rows, a.k_col, a.k_ld), std::tuple(a.v_rows, a.v_col, a.v_ld)})
+        if (!aligned16(p) || col * sizeof(T) % 16 != 0 || ld * (int64_t)sizeof(T) % 16 != 0) return false;
+    return true;
+}
+
+// grid of the quads kernels and their LDS
+template <int TPG>
+static dim3 quads_grid(const KvArgs& a, size_t* lds) {
+    *lds = (size_t)(256 / TPG) * a.dim * (a.g.page + 4);
+    return dim3((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)ceil_div(2 * a.kv_heads, 256 / TPG));
+}
+
+// A wave to a page's K or V of a head while that is one quad a lane (16
+// positions by 128 in f16), else a workgroup: 8 prompts of 1024 in fp32, 16
+// heads of 64 in pages of 64, 15.5 us with a wave and four quads a lane, 11.7
+// with a workgroup and one (read 12.2 and 10.6). The bytes alone are 7.2 us each
+// way at a copy's rate, the rest is the chain of lengths, table, scale and rows
+// that each page waits for, about 5 us, as for one new token in each of 32
+// sequences (5.5 us). Bytes one by one took 32 us each.
+template <typename T>
+static void launch_write(const char* name, const KvArgs& a) {
+    int n;
+    size_t lds;
+    if (!quads<T>(a, &n) || n > 1024)
+        return launch(name, kv_write_k<T>, dim3((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)a.kv_heads), dim3(256), 0, a);
+    const dim3 one = quads_grid<64>(a, &lds);
+    if (n <= 64) return launch(name, kv_write_quads_k<T, 64, 1>, one, dim3(256), lds, a);
+    const dim3 all = quads_grid<256>(a, &lds);
+    if (n <= 256) return launch(name, kv_write_quads_k<T, 256, 1>, all, dim3(256), lds, a);
+    if (n <= 512) return launch(name, kv_write_quads_k<T, 256, 2>, all, dim3(256), lds, a);
+    return launch(name, kv_write_quads_k<T, 256, 4>, all, dim3(256), lds, a);
+}
+
+template <typename T>
+static void launch_read(const char* name, const KvArgs& a) {
+    int n;
+    size_t lds;
+    if (!quads<T>(a, &n) || a.dim * (a.g.page + 4) > 65536)
+        return launch(name, kv_read_k<T>, dim3((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)a.kv_heads), dim3(256), 0, a);
+    if (n <= 64) {
+        const dim3 one = quads_grid<64>(a, &lds);
+        return launch(name, kv_read_quads_k<T, 64>, one, dim3(256), lds, a);
+    }
+    const dim3 all = quads_grid<256>(a, &lds);
+    launch(name, kv_read_quads_k<T, 256>, all, dim3(256), lds, a);
+}
+
 static bool kv_args(const char* name, Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale,
                     Tensor* v_scale, Tensor* table, Tensor* starts, Tensor* lengths, int k_col, int v_col, KvArgs* a) {
     CacheArgs c;
@@ -185,13 +416,12 @@ void nnc_hip_kv_write(Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Te
     if (!kv_args(name, k, v, k_cache, v_cache, k_scale, v_scale, table, starts, lengths, k_col, v_col, &a)) return;
     if (a.g.rows == 0 || a.g.batch == 0 || a.g.width == 0) return;
     if (!ready(name)) return;
-    const dim3 grid((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)a.kv_heads);
     const double n = 2.0 * a.g.rows * a.kv_heads * a.dim;
     set_work(6.0 * n, n * (activation_bytes(k) + 1));
     if (k->dtype == NNC_DTYPE_FLOAT16)
-        launch(name, kv_write_k<half_t>, grid, dim3(256), 0, a);
+        launch_write<half_t>(name, a);
     else
-        launch(name, kv_write_k<float>, grid, dim3(256), 0, a);
+        launch_write<float>(name, a);
 }
 
 void nnc_hip_kv_read(Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table, Tensor* starts,
@@ -201,13 +431,12 @@ void nnc_hip_kv_read(Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* 
     if (!kv_args(name, k, v, k_cache, v_cache, k_scale, v_scale, table, starts, lengths, k_col, v_col, &a)) return;
     if (a.g.rows == 0 || a.g.batch == 0 || a.g.width == 0) return;
     if (!ready(name)) return;
-    const dim3 grid((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)a.kv_heads);
     const double n = 2.0 * a.g.rows * a.kv_heads * a.dim;
     set_work(n, n * (activation_bytes(k) + 1));
     if (k->dtype == NNC_DTYPE_FLOAT16)
-        launch(name, kv_read_k<half_t>, grid, dim3(256), 0, a);
+        launch_read<half_t>(name, a);
     else
-        launch(name, kv_read_k<float>, grid, dim3(256), 0, a);
+        launch_read<float>(name, a);
 }
 
 }  // extern "C"

@@ -273,10 +273,22 @@ def check_cache(d, cache):
         np.testing.assert_array_equal(d.get(name), want, err_msg=name)
 
 
+KV_SIZES = [(1, 16, 32), (2, 16, 128), (3, 48, 64), (2, 64, 64), (1, 128, 128), (2, 256, 256), (5, 32, 64), (1, 240, 32)]
+
+
 @pytest.mark.parametrize("t", [F32, F16])
-@pytest.mark.parametrize("kv,page,dim", [(1, 16, 32), (2, 16, 128), (3, 48, 64), (2, 64, 64), (1, 128, 128), (2, 256, 256),
-                                         (5, 32, 64), (1, 240, 32)])
+@pytest.mark.parametrize("kv,page,dim", KV_SIZES)
 def test_kv_write_and_read(kv, page, dim, t, dev):
+    write_and_read(kv, page, dim, t, dev, 1, 3, 4, 7)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("kv,page,dim", KV_SIZES + [(3, 16, 64), (1, 112, 64), (2, 128, 256), (1, 64, 128)])
+def test_kv_write_and_read_aligned(kv, page, dim, t, dev):
+    write_and_read(kv, page, dim, t, dev, 0, 8, 8, 8)
+
+
+def write_and_read(kv, page, dim, t, dev, k_shift, v_shift, back_col, back_pad):
     """Ragged rows: new sequences, rows that begin inside a page, at its first
     and last position, none, a sequence of one position; rows of a fused
     projection; padding behind the last."""
@@ -287,13 +299,13 @@ def test_kv_write_and_read(kv, page, dim, t, dev):
     table, pages = tables(rng, lengths, page)
     cache = s8.Cache(rng, pages, kv, page, dim, table)
     heads = 2
-    x = rng.standard_normal((total, (heads + 2 * kv) * dim + 5)).astype(t)
+    x = rng.standard_normal((total, (heads + 2 * kv) * dim + (5 if k_shift else 8))).astype(t)
     x[2] *= 20  # scales that grow
-    k_col, v_col = heads * dim + 1, (heads + kv) * dim + 3
+    k_col, v_col = heads * dim + k_shift, (heads + kv) * dim + v_shift
     back_rows = [min(n, r + page - 1) for n, r in zip(lengths, rows)]
     back, back_total = ragged(back_rows, pad=2)
     d = dev({"x": x, **cache_arrays(cache, starts, lengths), "back": back,
-             "kr": np.full((back_total, kv * dim), 9, t), "vr": np.full((back_total, kv * dim + 7), 9, t)})
+             "kr": np.full((back_total, kv * dim), 9, t), "vr": np.full((back_total, kv * dim + back_pad), 9, t)})
     d.call("nnc_hip_kv_write", "x", "x", *CACHE, "starts", "lengths", k_col, v_col)
     want = cache.copy()
     want.write(x[:, k_col:k_col + kv * dim].reshape(total, kv, dim), x[:, v_col:v_col + kv * dim].reshape(total, kv, dim), starts, lengths)
@@ -301,14 +313,14 @@ def test_kv_write_and_read(kv, page, dim, t, dev):
     # once more: nothing changes
     d.call("nnc_hip_kv_write", "x", "x", *CACHE, "starts", "lengths", k_col, v_col)
     check_cache(d, want)
-    d.call("nnc_hip_kv_read", *CACHE, "back", "lengths", "kr", "vr", 0, 4)
-    kr, vr = np.full((back_total, kv * dim), 9, t), np.full((back_total, kv * dim + 7), 9, t)
+    d.call("nnc_hip_kv_read", *CACHE, "back", "lengths", "kr", "vr", 0, back_col)
+    kr, vr = np.full((back_total, kv * dim), 9, t), np.full((back_total, kv * dim + back_pad), 9, t)
     for b, n in enumerate(lengths):
         for i in range(back_rows[b]):
             pos = n - back_rows[b] + i
             p = want.page_of(b, pos)
             kr[back[b] + i] = (want.k[p, :, pos % page].astype(F32) * want.ks[p][:, None]).reshape(-1).astype(t)
-            vr[back[b] + i, 4:4 + kv * dim] = (want.v[p, :, :, pos % page].astype(F32) * want.vs[p][:, None]).reshape(-1).astype(t)
+            vr[back[b] + i, back_col:back_col + kv * dim] = (want.v[p, :, :, pos % page].astype(F32) * want.vs[p][:, None]).reshape(-1).astype(t)
     np.testing.assert_array_equal(d.get("kr"), kr)
     np.testing.assert_array_equal(d.get("vr"), vr)
 
