@@ -171,6 +171,58 @@ class GraphBuilder:
         self._node("LayerNormalization", ins, [y], name, axis=int(axis), epsilon=float(epsilon))
         return y
 
+    # -- 8-bit serving operators (include/nnc_hip.h) --------------------------------
+    def _rows8(self, x, name, out, scale=None):
+        s = self.shape(x)
+        return [self._out(name, s, "int8", name=out), self._out(f"{name}_scale", s[:-1], name=scale)]
+
+    def rms_norm(self, x, weight, residual=None, epsilon=1e-6, int8=False, name=None, out=None):
+        """Output, its row scales if `int8`, and the sum if there is a
+        `residual`: one name, or a tuple in that order."""
+        nm = name or "rms_norm"
+        ys = self._rows8(x, nm, out) if int8 else [self._out(nm, self.shape(x), self.g.tensors[x].dtype, name=out)]
+        if residual is not None:
+            ys.append(self._out(f"{nm}_sum", self.shape(x), self.g.tensors[x].dtype))
+        self._node("RmsNormalization", [x, weight] + ([residual] if residual is not None else []), ys, name,
+                   epsilon=float(epsilon), int8=bool(int8))
+        return ys[0] if len(ys) == 1 else tuple(ys)
+
+    def quantize_rows(self, x, name=None, out=None):
+        """Whole numbers and row scales."""
+        ys = self._rows8(x, name or "quantize_rows", out)
+        self._node("QuantizeRows", [x], ys, name)
+        return tuple(ys)
+
+    def dequantize_rows(self, x, scale, name=None, out=None):
+        y = self._out(name or "dequantize_rows", self.shape(x), name=out)
+        self._node("DequantizeRows", [x, scale], [y], name)
+        return y
+
+    def matmul_i8(self, a, a_scale, w, w_scale, bias=None, name=None, out=None):
+        y = self._out(name or "matmul_i8", tuple(self.shape(a)[:-1]) + (self.shape(w)[0],), name=out)
+        self._node("MatMulRows8", [a, a_scale, w, w_scale] + ([bias] if bias is not None else []), [y], name)
+        return y
+
+    def kv_cache(self, name, pages, kv_heads, page, dim):
+        """An empty paged cache: tensors that stay from run to run, for
+        kv_write and kv_attention (k_cache, v_cache, k_scale, v_scale)."""
+        return (self.const(f"{name}_k", np.zeros((pages, kv_heads, page, dim), np.int8)),
+                self.const(f"{name}_v", np.zeros((pages, kv_heads, dim, page), np.int8)),
+                self.const(f"{name}_k_scale", np.zeros((pages, kv_heads), np.float32)),
+                self.const(f"{name}_v_scale", np.zeros((pages, kv_heads), np.float32)))
+
+    def kv_write(self, k, v, cache, table, starts, lengths, k_col=0, v_col=0, name=None):
+        """Changes `cache`; nodes added after it see the new rows."""
+        self._node("KvWrite", [k, v, *cache, table, starts, lengths], list(cache), name, k_col=int(k_col), v_col=int(v_col))
+
+    def kv_attention(self, q, cache, table, starts, lengths, heads, q_col=0, scale=None, window=0, max_length=0, name=None,
+                     out=None):
+        dim = self.shape(cache[0])[3]
+        y = self._out(name or "kv_attention", tuple(self.shape(q)[:-1]) + (heads * dim,), name=out)
+        self._node("KvAttention", [q, *cache, table, starts, lengths], [y], name, q_col=int(q_col), heads=int(heads),
+                   scale=float(dim ** -0.5 if scale is None else scale), window=int(window), max_length=int(max_length))
+        return y
+
     def _reduce(self, op, x, axes, keepdims, name, out):
         s = list(self.shape(x))
         nd = len(s)

@@ -132,6 +132,7 @@ _GENERIC = {
     "Equal": "nnc_equal", "And": "nnc_and", "Greater": "nnc_greater", "Or": "nnc_or",
     "Not": "nnc_not", "Identity": "nnc_identity", "MatMul": "nnc_matmul",
     "FusedAddRelu": "nnc_add_relu", "FusedAddSigmoid": "nnc_add_sigmoid",
+    "QuantizeRows": "nnc_hip_quantize_rows", "DequantizeRows": "nnc_hip_dequantize_rows",
 }
 
 _CAST = {"float32": 0, "float16": 1, "int32": 2, "int8": 3, "uint8": 4, "bool": 5, "int64": 6}
@@ -199,6 +200,22 @@ def lower_node(g: Graph, node: Node) -> Call:
     if op == "ScaledSoftmax":  # Div by one element + softmax in one pass (include/nnc_hip.h)
         return Call("nnc_hip_scaled_softmax", [_t(ins[0]), _t(ins[1]), _t(outs[0]),
                                                ("i", int(node.attrs.get("axis", -1)))], node.name)
+    if op == "RmsNormalization":  # the 8-bit serving operators (include/nnc_hip.h)
+        int8 = bool(node.attrs.get("int8"))
+        res = len(ins) > 2 and bool(ins[2])
+        return Call("nnc_hip_rms_norm", [_t(ins[0]), _opt(node, 2), _t(ins[1]), _t(outs[-1]) if res else ("null",),
+                                         _t(outs[0]), _t(outs[1]) if int8 else ("null",),
+                                         ("f", float(node.attrs.get("epsilon", 1e-6)))], node.name)
+    if op == "MatMulRows8":
+        return Call("nnc_hip_matmul_i8", [_t(i) for i in ins[:4]] + [_opt(node, 4), _t(outs[0])], node.name)
+    if op == "KvWrite":  # its outputs are the cache tensors among its inputs
+        return Call("nnc_hip_kv_write", [_t(i) for i in ins] + [("i", int(node.attrs[k])) for k in ("k_col", "v_col")],
+                    node.name)
+    if op == "KvAttention":
+        a = node.attrs
+        return Call("nnc_hip_kv_attention", [_t(i) for i in ins] + [_t(outs[0]), ("i", int(a["q_col"])), ("i", int(a["heads"])),
+                                                                    ("f", float(a["scale"])), ("i", int(a["window"])),
+                                                                    ("i", int(a["max_length"]))], node.name)
     if op == "FusedEltwise":  # an element-wise chain in one pass (include/nnc_hip.h)
         steps = node.attrs["steps"]
         prog = [v for st in steps for v in (st[0], st[1], st[2])]

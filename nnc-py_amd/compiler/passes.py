@@ -58,13 +58,18 @@ def eliminate_identity(g: Graph) -> int:
     return removed
 
 
+# ops that change tensors which stay from run to run
+LASTING_OPS = {"KvWrite"}
+
+
 def eliminate_dead_code(g: Graph) -> int:
     """Drop nodes none of whose outputs reach a graph output
-    (passes/dead_code_elimination.py:13), then unreferenced tensors."""
+    (passes/dead_code_elimination.py:13) or stay from run to run, then
+    unreferenced tensors."""
     live = set(g.outputs)
     keep = []
     for node in reversed(g.topological_sort()):
-        if any(o in live for o in node.outputs):
+        if node.op_type in LASTING_OPS or any(o in live for o in node.outputs):
             keep.append(node)
             live.update(i for i in node.inputs if i)
     removed = len(g.nodes) - len(keep)

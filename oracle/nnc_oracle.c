@@ -1256,3 +1256,217 @@ void nnc_hip_attention(Tensor* qkv, Tensor* div, Tensor* out, int batch, int seq
         }
     free(q), free(kt), free(v), free(s), free(s2), free(p), free(c);
 }
+
+/* ------------------------------------------------------------------------
+ * The 8-bit serving operators (include/nnc_hip.h): target-only, no reference
+ * counterpart. Their definitions on float32 activations, sums in double. The
+ * whole numbers and steps are those of the target exactly; sums differ by
+ * its float32 roundings. Pinned against float64 numpy by
+ * tests/test_serving8_graph.py.
+ * ---------------------------------------------------------------------- */
+static float largest_of(const float* x, int64_t n, int64_t step) {
+    float top = 0.f;
+    for (int64_t i = 0; i < n; ++i) {
+        const float v = fabsf(x[i * step]);
+        if (isnan(v) || v > top) top = v;
+        if (isnan(v)) break;
+    }
+    return top;
+}
+
+static float unit8(float top) {
+    if (!isfinite(top)) return NAN;
+    return top < 0x1p-100f ? 0.f : (float)((double)top / 127);
+}
+
+static int8_t whole8(double x, float unit) { return unit > 0.f ? (int8_t)rint(x / (double)unit) : 0; }
+
+static int is_float32(const char* name, const Tensor* t) {
+    if (t->dtype == NNC_DTYPE_FLOAT32) return 1;
+    fprintf(stderr, "%s: float32 activations only\n", name);
+    return 0;
+}
+
+void nnc_hip_rms_norm(Tensor* in, Tensor* res, Tensor* weight, Tensor* sum, Tensor* out, Tensor* scale, float eps) {
+    if (!is_float32("nnc_hip_rms_norm", in)) return;
+    const int64_t width = in->shape[in->ndim - 1], rows = width > 0 ? numel(in) / width : 0;
+    const float* w = (const float*)weight->data;
+    float* s = (float*)malloc((size_t)(width > 0 ? width : 1) * sizeof(float));
+    for (int64_t row = 0; row < rows; ++row) {
+        const int64_t at = row * width;
+        double squares = 0;
+        for (int64_t i = 0; i < width; ++i) {
+            s[i] = ((const float*)in->data)[at + i];
+            if (res) s[i] += ((const float*)res->data)[at + i];
+            squares += (double)s[i] * s[i];
+        }
+        const double r = 1 / sqrt(squares / (double)width + (double)eps);
+        if (sum) memcpy((float*)sum->data + at, s, (size_t)width * sizeof(float));
+        if (out->dtype != NNC_DTYPE_INT8) {
+            for (int64_t i = 0; i < width; ++i) ((float*)out->data)[at + i] = (float)(s[i] * r * w[i]);
+            continue;
+        }
+        for (int64_t i = 0; i < width; ++i) s[i] *= w[i];
+        const float unit = unit8(largest_of(s, width, 1));
+        for (int64_t i = 0; i < width; ++i) ((int8_t*)out->data)[at + i] = whole8(s[i], unit);
+        ((float*)scale->data)[row] = (float)(r * unit);
+    }
+    free(s);
+}
+
+void nnc_hip_quantize_rows(Tensor* in, Tensor* out, Tensor* scale) {
+    if (!is_float32("nnc_hip_quantize_rows", in)) return;
+    const int64_t width = in->shape[in->ndim - 1], rows = width > 0 ? numel(in) / width : 0;
+    for (int64_t row = 0; row < rows; ++row) {
+        const float* x = (const float*)in->data + row * width;
+        const float unit = unit8(largest_of(x, width, 1));
+        for (int64_t i = 0; i < width; ++i) ((int8_t*)out->data)[row * width + i] = whole8(x[i], unit);
+        ((float*)scale->data)[row] = unit;
+    }
+}
+
+void nnc_hip_dequantize_rows(Tensor* in, Tensor* scale, Tensor* out) {
+    if (!is_float32("nnc_hip_dequantize_rows", out)) return;
+    const int64_t width = in->shape[in->ndim - 1], n = numel(in);
+    for (int64_t i = 0; i < n; ++i) ((float*)out->data)[i] = ((const int8_t*)in->data)[i] * ((const float*)scale->data)[i / width];
+}
+
+void nnc_hip_matmul_i8(Tensor* a, Tensor* a_scale, Tensor* w, Tensor* w_scale, Tensor* bias, Tensor* out) {
+    if (!is_float32("nnc_hip_matmul_i8", out)) return;
+    const int64_t k = a->shape[a->ndim - 1], m = k > 0 ? numel(a) / k : 0, n = w->shape[0];
+    for (int64_t i = 0; i < m; ++i)
+        for (int64_t j = 0; j < n; ++j) {
+            const int8_t *x = (const int8_t*)a->data + i * k, *y = (const int8_t*)w->data + j * k;
+            int32_t sum = 0;
+            for (int64_t l = 0; l < k; ++l) sum += x[l] * y[l];
+            const double v = (double)sum * ((const float*)a_scale->data)[i] * ((const float*)w_scale->data)[j];
+            ((float*)out->data)[i * n + j] = (float)(v + (bias ? ((const float*)bias->data)[j] : 0.f));
+        }
+}
+
+/* The positions of sequence b that its rows are: [first, stop), position t in
+ * row `shift` + t. Extents are taken as they are (the target clamps them). */
+typedef struct {
+    int64_t first, stop, shift;
+} Rows8;
+
+static Rows8 rows_of(const Tensor* starts, const Tensor* lengths, int b) {
+    const int32_t *s = (const int32_t*)starts->data, length = ((const int32_t*)lengths->data)[b];
+    const int64_t n = s[b + 1] - s[b];
+    Rows8 r = {length > n ? length - n : 0, n > 0 ? length : 0, (int64_t)s[b + 1] - length};
+    return r;
+}
+
+static int64_t page_at(const Tensor* table, const Tensor* cache, int b, int64_t slot) {
+    const int32_t p = ((const int32_t*)table->data)[b * table->shape[1] + slot];
+    return p >= 0 && p < cache->shape[0] ? p : -1;
+}
+
+/* One page and head: `rows` new rows of dim values (ld apart) from position lo
+ * on; position t, dim d at held[t * step_t + d * step_d]. */
+static void write_page(const float* x, int64_t ld, int64_t rows, int64_t dim, int64_t lo, int8_t* held, int64_t step_t,
+                       int64_t step_d, float* scale) {
+    float top = 0.f;
+    for (int64_t r = 0; r < rows; ++r) {
+        const float v = largest_of(x + r * ld, dim, 1);
+        if (isnan(v) || v > top) top = v;
+        if (isnan(v)) break;
+    }
+    const float before = *scale;
+    float unit = unit8(top);
+    if (lo > 0 && (isnan(before) || before > unit)) unit = before;
+    for (int64_t t = 0; lo > 0 && t < lo && !(unit == before); ++t)
+        for (int64_t d = 0; d < dim; ++d) {
+            int8_t* q = held + t * step_t + d * step_d;
+            *q = unit > 0.f ? (int8_t)rint((double)*q * (double)before / (double)unit) : 0;
+        }
+    for (int64_t r = 0; r < rows; ++r)
+        for (int64_t d = 0; d < dim; ++d) held[(lo + r) * step_t + d * step_d] = whole8(x[r * ld + d], unit);
+    *scale = unit;
+}
+
+void nnc_hip_kv_write(Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale,
+                      Tensor* table, Tensor* starts, Tensor* lengths, int k_col, int v_col) {
+    if (!is_float32("nnc_hip_kv_write", k)) return;
+    const int64_t heads = k_cache->shape[1], page = k_cache->shape[2], dim = k_cache->shape[3];
+    const int64_t k_ld = k->shape[k->ndim - 1], v_ld = v->shape[v->ndim - 1];
+    for (int b = 0; b < table->shape[0]; ++b) {
+        const Rows8 r = rows_of(starts, lengths, b);
+        for (int64_t t = r.first; t < r.stop;) {
+            const int64_t slot = t / page, lo = t % page, stop = (slot + 1) * page < r.stop ? (slot + 1) * page : r.stop;
+            const int64_t p = page_at(table, k_cache, b, slot);
+            for (int64_t h = 0; p >= 0 && h < heads; ++h) {
+                const int64_t at = p * heads + h, row = r.shift + t;
+                write_page((const float*)k->data + row * k_ld + k_col + h * dim, k_ld, stop - t, dim, lo,
+                           (int8_t*)k_cache->data + at * page * dim, dim, 1, (float*)k_scale->data + at);
+                write_page((const float*)v->data + row * v_ld + v_col + h * dim, v_ld, stop - t, dim, lo,
+                           (int8_t*)v_cache->data + at * page * dim, 1, page, (float*)v_scale->data + at);
+            }
+            t = stop;
+        }
+    }
+}
+
+void nnc_hip_kv_read(Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table, Tensor* starts,
+                     Tensor* lengths, Tensor* k, Tensor* v, int k_col, int v_col) {
+    if (!is_float32("nnc_hip_kv_read", k)) return;
+    const int64_t heads = k_cache->shape[1], page = k_cache->shape[2], dim = k_cache->shape[3];
+    const int64_t k_ld = k->shape[k->ndim - 1], v_ld = v->shape[v->ndim - 1];
+    for (int b = 0; b < table->shape[0]; ++b) {
+        const Rows8 r = rows_of(starts, lengths, b);
+        for (int64_t t = r.first; t < r.stop; ++t) {
+            const int64_t p = page_at(table, k_cache, b, t / page), row = r.shift + t;
+            for (int64_t h = 0; p >= 0 && h < heads; ++h)
+                for (int64_t d = 0; d < dim; ++d) {
+                    const int64_t at = p * heads + h;
+                    ((float*)k->data)[row * k_ld + k_col + h * dim + d] =
+                        ((const int8_t*)k_cache->data)[(at * page + t % page) * dim + d] * ((const float*)k_scale->data)[at];
+                    ((float*)v->data)[row * v_ld + v_col + h * dim + d] =
+                        ((const int8_t*)v_cache->data)[(at * dim + d) * page + t % page] * ((const float*)v_scale->data)[at];
+                }
+        }
+    }
+}
+
+void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table,
+                          Tensor* starts, Tensor* lengths, Tensor* out, int q_col, int heads, float scale, int window,
+                          int max_length) {
+    (void)max_length;
+    if (!is_float32("nnc_hip_kv_attention", q)) return;
+    const int64_t kv = k_cache->shape[1], page = k_cache->shape[2], dim = k_cache->shape[3], group = heads / kv;
+    const int64_t ld = q->shape[q->ndim - 1], most = table->shape[1] * page;
+    double* p = (double*)malloc((size_t)(most > 0 ? most : 1) * sizeof(double));
+    double* y = (double*)malloc((size_t)(dim > 0 ? dim : 1) * sizeof(double));
+    const int32_t* s = (const int32_t*)starts->data;
+    for (int b = 0; b < table->shape[0]; ++b) {
+        const int64_t length = ((const int32_t*)lengths->data)[b];
+        for (int64_t row = s[b]; row < s[b + 1]; ++row)
+            for (int64_t h = 0; h < heads; ++h) {
+                const int64_t pos = length - s[b + 1] + row, from = window > 0 && pos >= window ? pos - window + 1 : 0;
+                const float* x = (const float*)q->data + row * ld + q_col + h * dim;
+                double top = -INFINITY, sum = 0;
+                for (int64_t j = from; j <= pos; ++j) {
+                    const int64_t slot = page_at(table, k_cache, b, j / page), at = slot * kv + h / group;
+                    p[j] = -INFINITY;
+                    if (slot < 0) continue;
+                    const int8_t* key = (const int8_t*)k_cache->data + (at * page + j % page) * dim;
+                    double dot = 0;
+                    for (int64_t d = 0; d < dim; ++d) dot += (double)x[d] * key[d];
+                    p[j] = dot * scale * ((const float*)k_scale->data)[at];
+                    if (isnan(p[j]) || p[j] > top) top = p[j];
+                }
+                for (int64_t d = 0; d < dim; ++d) y[d] = 0;
+                for (int64_t j = from; j <= pos; ++j) {
+                    const int64_t slot = page_at(table, k_cache, b, j / page), at = slot * kv + h / group;
+                    if (slot < 0) continue;
+                    const double e = exp(p[j] - top);
+                    const double u = e * ((const float*)v_scale->data)[at];
+                    sum += e;
+                    for (int64_t d = 0; d < dim; ++d) y[d] += u * ((const int8_t*)v_cache->data)[(at * dim + d) * page + j % page];
+                }
+                for (int64_t d = 0; d < dim; ++d)
+                    ((float*)out->data)[(row * heads + h) * dim + d] = sum == 0 ? 0.f : (float)(y[d] / sum);
+            }
+    }
+    free(p), free(y);
+}
