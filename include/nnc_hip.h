@@ -346,7 +346,8 @@ void nnc_hip_conv_packed_noalloc(Tensor* in, Tensor* w, Tensor* b, Tensor* res, 
  * `in`, and `out` the same as `in`). weight: one row. out of in's type: y, scale NULL. out int8:
  * the product s * w, rounded to float32, is quantised row by row and `scale`
  * (one for each row) is its step u times 1 / sqrt(...), so the whole numbers
- * do not depend on the order of the sum of squares.
+ * do not depend on the order of the sum of squares, which is float32's:
+ * values up to 2^60 for rows of any length.
  *
  * nnc_hip_quantize_rows / nnc_hip_dequantize_rows: rows (of the last extent)
  * to 8 bits with a scale each, and back: activations between an attention or
@@ -378,8 +379,10 @@ void nnc_hip_matmul_i8(Tensor* a, Tensor* a_scale, Tensor* w, Tensor* w_scale, T
  * the larger of its old scale and the new rows'; if that is larger than the
  * old one, the kept whole numbers become the nearest to their value under it.
  * A page that the new rows begin in gets theirs. Positions behind the length
- * stay as they were. No page may belong to two sequences that write to it in
- * one call; pages of a common prefix that no row touches may be shared.
+ * stay as they were. Scales are 0, 2^-107 or more (values of 2^-100), or NaN;
+ * attention takes any up to 2^102. No page may belong to two sequences that write to it in
+ * one call, nor be in its table twice; pages of a common prefix that no row
+ * touches may be shared.
  *
  * nnc_hip_kv_read: the opposite: rows starts[b] .. starts[b + 1] of k and v
  * receive sequence b's last positions.

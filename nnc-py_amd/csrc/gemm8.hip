@@ -482,7 +482,7 @@ void nnc_hip_matmul_i8(Tensor* a, Tensor* a_scale, Tensor* w, Tensor* w_scale, T
         return fail(NNC_HIP_EINVAL, name, "a_scale and out need %lld rows, w_scale and bias %lld", (long long)m, (long long)n);
     if (m == 0 || n == 0) return;
     if (k < 1 || k > 131071) return fail(NNC_HIP_EUNSUPP, name, "K = %lld (1 to 131071)", (long long)k);
-    if (m > (int64_t)65535 * 64 || n > (int64_t)1 << 30) return fail(NNC_HIP_EUNSUPP, name, "too many rows");
+    if (m > (int64_t)65535 * 64 || n > (int64_t)1 << 26) return fail(NNC_HIP_EUNSUPP, name, "too many rows");
     if (!ready(name)) return;
     Gemm8Args p{(const int8_t*)a->data, (const int8_t*)w->data, (const float*)a_scale->data, (const float*)w_scale->data,
                 bias ? (const float*)bias->data : nullptr, out->data, m, n, (int)k,

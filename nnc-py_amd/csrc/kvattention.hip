@@ -22,7 +22,8 @@
 // consecutive keys 16g .. 16g + 15: one scale each, and 16 consecutive bytes
 // of V. Whole numbers of 8 bits are exact in f16. Query rows are f16 as they
 // are; fp32 ones are scaled by a power of two and cut into two f16 pieces (22
-// bits), and so is p then (f16 outputs: p rounded to f16 once, 2^-12 of it).
+// bits), and so is p then (f16 outputs: p rounded to f16 once, 2^-11 of it at most, as their own
+// rounding is).
 //
 // A workgroup takes 16 query rows - heads of one cached head, then tokens -
 // and a share of the keys, its waves 64 keys each in turn; the waves' sums are
@@ -70,6 +71,12 @@ __device__ __forceinline__ f16x8 widen8(uint32_t lo, uint32_t hi) {
 // be small beside its own and lose bits as f16, and large enough for its
 // weights in the divisor to stay above 2^-126.
 __device__ __forceinline__ float value_unit(float scale) { return scale == 0.f ? 0x1p-64f : scale; }
+
+// The divisor sum_j p_j / u_j is kept 2^24 smaller, and the sums of values are
+// made so before they are divided: p up to 2^15 over the smallest scale that
+// is not 0, 2^-107, stays finite then for as many keys as there can be, and
+// 1 / u a normal number for scales up to 2^102.
+static constexpr float kWeight = 0x1p-24f;
 
 // p is scaled by 2^12 before it is rounded to f16: its smallest steps are then
 // 2^-36 of the row's largest. The running maximum is only moved, and what was
@@ -145,7 +152,7 @@ struct Shares {
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
         if (lane < D / PER) {
 #pragma unroll
-            for (int q = 0; q < PER; ++q) out[dim + q] = (T)(o[q] * inv);
+            for (int q = 0; q < PER; ++q) out[dim + q] = (T)(o[q] * kWeight * inv);
         }
     }
 };
@@ -285,7 +292,7 @@ __global__ void __launch_bounds__(64 * token_waves(D)) kv_attention_k(KvAttnArgs
         }
         load_k(tb + STRIDE);
         const float vu = value_unit(vs);
-        float ku = ks * qs, lv = __builtin_amdgcn_logf(vu), iv = 1.0f / vu;
+        float ku = ks * qs, lv = __builtin_amdgcn_logf(vu), iv = kWeight / vu;
         ku = ku == 0.f ? 0x1p-126f : ku;  // for the product with -inf
         if (!(tb + 63 <= first_pos && (a.window <= 0 || tb > last_pos - a.window) && __all(have))) {
             const int j = tb + 16 * g, low = a.window > 0 ? pos - a.window : INT_MIN, up = have ? pos : INT_MIN;
@@ -372,7 +379,7 @@ __global__ void __launch_bounds__(64 * token_waves(D)) kv_attention_k(KvAttnArgs
         for (int c = 0; c < KV; ++c) {
             T v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (T)(o[c][r] * inv);
+            for (int r = 0; r < 4; ++r) v[r] = (T)(o[c][r] * kWeight * inv);
             __builtin_memcpy(__builtin_assume_aligned(op + 16 * c, 4 * sizeof(T)), v, sizeof v);
         }
         return;
@@ -505,7 +512,7 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
         if (threadIdx.x < 4) {
             const float vu = can_read ? value_unit(su[1]) : 1.f, ok = can_read ? 1.f : 0.f;
             *reinterpret_cast<fx4*>(units + stage * 20 + threadIdx.x * 4) =
-                fx4{can_read ? su[0] * a.scale : 0.f, __builtin_amdgcn_logf(vu), 1.0f / vu, ok};
+                fx4{can_read ? su[0] * a.scale : 0.f, __builtin_amdgcn_logf(vu), kWeight / vu, ok};
             units[stage * 20 + 16 + threadIdx.x] = ok;
         }
     };
@@ -677,7 +684,7 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
         for (int q = 0; q < 4; ++q) {
             T v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (T)(o[c][4 * q + r] * inv);
+            for (int r = 0; r < 4; ++r) v[r] = (T)(o[c][4 * q + r] * kWeight * inv);
             __builtin_memcpy(__builtin_assume_aligned(op + 32 * c + 8 * q, 4 * sizeof(T)), v, sizeof v);
         }
 }
@@ -760,6 +767,7 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
     const int longest = max_length > 0 && max_length < capacity ? max_length : capacity;
     const int tile = query_tile(rows, c.ragged.batch, group, c.kv_heads, c.dim);
     const int64_t tiles = query_tiles_bound(rows, c.ragged.batch, group, tile), items = tiles * c.kv_heads;
+    if (items * 64 * 8 > UINT32_MAX) return fail(NNC_HIP_EUNSUPP, name, "%lld rows of %d heads", (long long)rows, heads);
     KvAttnArgs a{c.ragged, c.k, c.v, c.k_scale, c.v_scale, q->data, out->data, nullptr, nullptr, ld, q_col, heads, c.kv_heads,
                  group, window, 1, 64, (int)tiles, slot_magic(c.page / 16),
                  aligned16(q->data) && ld * activation_bytes(q) % 16 == 0 && q_col * activation_bytes(q) % 16 == 0,

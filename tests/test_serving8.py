@@ -562,6 +562,22 @@ def test_kv_attention_pages_of_different_size(rows, t, dev):
     check_attention(d.get("out"), q.reshape(rows, heads, dim), cache, starts, [length], F32(0.125), 0)
 
 
+@pytest.mark.parametrize("rows,heads,length", [(1, 4, 9000), (600, 64, 700)])
+@pytest.mark.parametrize("power", [-100, 90])
+def test_kv_attention_values_very_small_and_large(power, rows, heads, length, dev):
+    """Values from the smallest that the cache holds to far beyond a product's:
+    neither the sums nor the divisor overflow or vanish."""
+    rng = np.random.default_rng(abs(power) + rows)
+    table, pages = tables(rng, [length], 64)
+    cache = s8.Cache(rng, pages, 1, 64, 32, table)
+    cache.vs = (rng.uniform(1, 4, cache.vs.shape) * 2.0 ** power).astype(F32)
+    starts = np.array([0, rows], I32)
+    q = rng.standard_normal((rows, heads * 32)).astype(F32)
+    d = dev({"q": q, **cache_arrays(cache, starts, [length]), "out": np.zeros((rows, heads * 32), F32)})
+    d.call("nnc_hip_kv_attention", "q", *CACHE, "starts", "lengths", "out", 0, heads, 0.1, 0, 0)
+    check_attention(d.get("out"), q.reshape(rows, heads, 32), cache, starts, [length], F32(0.1), 0)
+
+
 def test_kv_attention_query_sizes(dev):
     """fp32 queries from very small to very large: the pieces hold 22 bits of
     each row at any size; a row that is not finite stays by itself."""
