@@ -5,9 +5,13 @@
 // The sum is exact (32-bit integers: K up to 131071); the scales, the bias
 // and the output's rounding follow in 32 bits. No reference counterpart.
 //
-// v_mfma_i32_16x16x64_i8: lane (i = lane % 16, g = lane / 16) holds 16 k of
-// row i of either operand; the k order is the same in both, so it does not
-// matter which 16 of the 64 a lane group has. Result register r is row
+// [8192,4096]x[4096,4096] to f16 130 us, 2.11 POPS (a library's product of the
+// same operands to 32-bit integers 133 us); 8 rows 6.0 us, of which the
+// weights' 16.8 MB are 3.2 at a copy's rate.
+//
+// v_mfma_i32_16x16x64_i8 (few rows): lane (i = lane % 16, g = lane / 16) holds
+// 16 k of row i of either operand; the k order is the same in both, so it does
+// not matter which 16 of the 64 a lane group has. Result register r is row
 // 4g + r, column i.
 #include "mfma_tile.h"
 #include "quant8.h"
