@@ -97,6 +97,7 @@ struct KvArgs {
 // ---------------------------------------------------------------------------
 template <typename T, int TPG>
 struct Quads {
+    static constexpr int THREADS = TPG < 256 ? 256 : TPG, GROUPS = THREADS / TPG;  // of a workgroup
     static constexpr int V = 16 / (int)sizeof(T);
     typedef Pack<T, V> Row;
     typedef Pack<int8_t, V> Held;
@@ -115,12 +116,12 @@ struct Quads {
 };
 
 template <typename T, int TPG, int QPER>
-__global__ void __launch_bounds__(256) kv_write_quads_k(KvArgs a) {
+__global__ void __launch_bounds__((Quads<T, TPG>::THREADS)) kv_write_quads_k(KvArgs a) {
     typedef Quads<T, TPG> Q;
     extern __shared__ __align__(16) char lds[];
-    __shared__ float part[4];
+    __shared__ float part[Q::THREADS / 64];
     const Q z(a);
-    const int pair = blockIdx.y * (256 / TPG) + threadIdx.x / TPG, which = pair & 1, head = pair >> 1;
+    const int pair = blockIdx.y * Q::GROUPS + threadIdx.x / TPG, which = pair & 1, head = pair >> 1;
     int share = blockIdx.x;
     const int b = find_share(share, a.g.batch, [&](int i) { return touched_pages(a.g, i); });
     if (b < 0 || head >= a.kv_heads) return;  // (a workgroup of one group has one head)
@@ -154,10 +155,12 @@ __global__ void __launch_bounds__(256) kv_write_quads_k(KvArgs a) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) big = max(big, (uint32_t)__shfl_xor((int)big, o));
     float top = __uint_as_float(big);
-    if constexpr (TPG == 256) {
+    if constexpr (TPG > 64) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
         __syncthreads();  // everybody has read the scale, too
-        top = max_nan(max_nan(part[0], part[1]), max_nan(part[2], part[3]));
+        top = part[0];
+#pragma unroll
+        for (int i = 1; i < TPG / 64; ++i) top = max_nan(top, part[i]);
     }
     float unit = unit8(top);
     if (lo > 0) unit = max_nan(before, unit);
@@ -217,11 +220,11 @@ __global__ void __launch_bounds__(256) kv_write_quads_k(KvArgs a) {
 }
 
 template <typename T, int TPG>
-__global__ void __launch_bounds__(256) kv_read_quads_k(KvArgs a) {
+__global__ void __launch_bounds__((Quads<T, TPG>::THREADS)) kv_read_quads_k(KvArgs a) {
     typedef Quads<T, TPG> Q;
     extern __shared__ __align__(16) char lds[];
     const Q z(a);
-    const int pair = blockIdx.y * (256 / TPG) + threadIdx.x / TPG, which = pair & 1, head = pair >> 1;
+    const int pair = blockIdx.y * Q::GROUPS + threadIdx.x / TPG, which = pair & 1, head = pair >> 1;
     int share = blockIdx.x;
     const int b = find_share(share, a.g.batch, [&](int i) { return touched_pages(a.g, i); });
     if (b < 0 || head >= a.kv_heads) return;
@@ -265,8 +268,8 @@ __global__ void __launch_bounds__(256) kv_read_quads_k(KvArgs a) {
     }
 }
 
-// Rows that start on no 16 bytes, and pages of more than 1024 quads: one
-// workgroup per page and head, element by element.
+// Rows that start on no 16 bytes: one workgroup per page and head, element by
+// element.
 template <typename T>
 __global__ void __launch_bounds__(256) kv_write_k(KvArgs a) {
     const int head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -337,18 +340,22 @@ __global__ void __launch_bounds__(256) kv_read_k(KvArgs a) {
 }
 
 template <typename T>
-static bool quads(const KvArgs& a, int* count) {
-    *count = a.g.page * a.dim / (4 * (16 / (int)sizeof(T)));
+static bool quads(const KvArgs& a) {
     for (auto [p, col, ld] : {std::tuple(a.k_rows, a.k_col, a.k_ld), std::tuple(a.v_rows, a.v_col, a.v_ld)})
         if (!aligned16(p) || col * sizeof(T) % 16 != 0 || ld * (int64_t)sizeof(T) % 16 != 0) return false;
     return true;
 }
 
-// grid of the quads kernels and their LDS
-template <int TPG>
-static dim3 quads_grid(const KvArgs& a, size_t* lds) {
-    *lds = (size_t)(256 / TPG) * a.dim * (a.g.page + 4);
-    return dim3((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)ceil_div(2 * a.kv_heads, 256 / TPG));
+template <typename T, int TPG, typename Kernel>
+static void launch_quads(const char* name, Kernel kernel, const KvArgs& a) {
+    typedef Quads<T, TPG> Q;
+    const size_t lds = (size_t)Q::GROUPS * a.dim * (a.g.page + 4);
+    if (TPG == 1024) {  // the largest pages: 66560 bytes
+        static const bool ok = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 256 * 260) == hipSuccess;
+        if (!ok) return fail(NNC_HIP_EDEVICE, name, "hipFuncSetAttribute failed");
+    }
+    launch(name, kernel, dim3((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)ceil_div(2 * a.kv_heads, Q::GROUPS)),
+           dim3(Q::THREADS), lds, a);
 }
 
 // A wave to a page's K or V of a head while that is one quad a lane (16
@@ -357,33 +364,32 @@ static dim3 quads_grid(const KvArgs& a, size_t* lds) {
 // with a workgroup and one (read 12.2 and 10.6). The bytes alone are 7.2 us each
 // way at a copy's rate, the rest is the chain of lengths, table, scale and rows
 // that each page waits for, about 5 us, as for one new token in each of 32
-// sequences (5.5 us). Bytes one by one took 32 us each.
+// sequences (5.5 us). Bytes one by one took 32 us each. Pages of more than 1024
+// quads (256 positions by 128 in fp32) get workgroups of 1024, whose lanes hold
+// no more than others'.
 template <typename T>
 static void launch_write(const char* name, const KvArgs& a) {
-    int n;
-    size_t lds;
-    if (!quads<T>(a, &n) || n > 1024)
+    const int n = a.g.page * a.dim * (int)sizeof(T) / 64;
+    if (!quads<T>(a))
         return launch(name, kv_write_k<T>, dim3((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)a.kv_heads), dim3(256), 0, a);
-    const dim3 one = quads_grid<64>(a, &lds);
-    if (n <= 64) return launch(name, kv_write_quads_k<T, 64, 1>, one, dim3(256), lds, a);
-    const dim3 all = quads_grid<256>(a, &lds);
-    if (n <= 256) return launch(name, kv_write_quads_k<T, 256, 1>, all, dim3(256), lds, a);
-    if (n <= 512) return launch(name, kv_write_quads_k<T, 256, 2>, all, dim3(256), lds, a);
-    return launch(name, kv_write_quads_k<T, 256, 4>, all, dim3(256), lds, a);
+    if (n <= 64) return launch_quads<T, 64>(name, kv_write_quads_k<T, 64, 1>, a);
+    if (n <= 256) return launch_quads<T, 256>(name, kv_write_quads_k<T, 256, 1>, a);
+    if (n <= 512) return launch_quads<T, 256>(name, kv_write_quads_k<T, 256, 2>, a);
+    if (n <= 1024) return launch_quads<T, 256>(name, kv_write_quads_k<T, 256, 4>, a);
+    if constexpr (sizeof(T) == 4) {
+        if (n > 2048) return launch_quads<T, 1024>(name, kv_write_quads_k<T, 1024, 4>, a);
+    }
+    launch_quads<T, 1024>(name, kv_write_quads_k<T, 1024, 2>, a);
 }
 
 template <typename T>
 static void launch_read(const char* name, const KvArgs& a) {
-    int n;
-    size_t lds;
-    if (!quads<T>(a, &n) || a.dim * (a.g.page + 4) > 65536)
+    const int n = a.g.page * a.dim * (int)sizeof(T) / 64;
+    if (!quads<T>(a))
         return launch(name, kv_read_k<T>, dim3((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)a.kv_heads), dim3(256), 0, a);
-    if (n <= 64) {
-        const dim3 one = quads_grid<64>(a, &lds);
-        return launch(name, kv_read_quads_k<T, 64>, one, dim3(256), lds, a);
-    }
-    const dim3 all = quads_grid<256>(a, &lds);
-    launch(name, kv_read_quads_k<T, 256>, all, dim3(256), lds, a);
+    if (n <= 64) return launch_quads<T, 64>(name, kv_read_quads_k<T, 64>, a);
+    if (n <= 1024) return launch_quads<T, 256>(name, kv_read_quads_k<T, 256>, a);
+    launch_quads<T, 1024>(name, kv_read_quads_k<T, 1024>, a);
 }
 
 static bool kv_args(const char* name, Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale,

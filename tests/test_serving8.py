@@ -283,7 +283,8 @@ def test_kv_write_and_read(kv, page, dim, t, dev):
 
 
 @pytest.mark.parametrize("t", [F32, F16])
-@pytest.mark.parametrize("kv,page,dim", KV_SIZES + [(3, 16, 64), (1, 112, 64), (2, 128, 256), (1, 64, 128)])
+@pytest.mark.parametrize("kv,page,dim", KV_SIZES + [(3, 16, 64), (1, 112, 64), (2, 128, 256), (1, 64, 128),
+                                                     (1, 256, 128), (1, 176, 256)])
 def test_kv_write_and_read_aligned(kv, page, dim, t, dev):
     write_and_read(kv, page, dim, t, dev, 0, 8, 8, 8)
 
