@@ -51,6 +51,7 @@ struct KvAttnArgs {
     int q_col, heads, kv_heads, group, window, splits, chunk, tiles;
     uint32_t slot_magic;
     bool q_vec;  // query rows start on 16 bytes
+    bool by_length;  // long sequences' workgroups first
     float scale;  // with log2(e)
 };
 
@@ -161,6 +162,41 @@ struct Shares {
     }
 };
 
+// Where workgroups come in several rounds, those of long sequences go first, in
+// eighths of the longest: the `tile`-th sequence in that order, -1 behind the
+// last, -2 if a sequence has more than one tile.
+static constexpr int kOrdered = 256;  // sequences
+__device__ __forceinline__ int longest_first(const Ragged& g, int group, int tile) {
+    const int lane = threadIdx.x & 63, passes = (g.batch + 63) / 64;
+    float length[kOrdered / 64], most = 0.f;
+    bool one = true;
+#pragma unroll
+    for (int u = 0; u < kOrdered / 64; ++u) {
+        length[u] = -1.f;
+        if (u < passes && 64 * u + lane < g.batch) {
+            const Span span = span_of(g, 64 * u + lane);
+            const int tiles = query_tiles(span, group, 16);
+            if (tiles > 0) length[u] = (float)span.length;
+            one &= tiles <= 1;
+            most = fmaxf(most, length[u]);
+        }
+    }
+    if (!__all(one)) return -2;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+    const float eighths = 8.f / (most + 1.f);
+    for (int c = 7; c >= 0; --c)
+#pragma unroll
+        for (int u = 0; u < kOrdered / 64; ++u) {
+            if (u >= passes) continue;
+            const uint64_t in = __ballot(length[u] >= 0.f && min((int)(length[u] * eighths), 7) == c);
+            const int n = __popcll(in);
+            if (tile < n) return 64 * u + __ffsll(__ballot((in >> lane & 1) && __popcll(in & ((1ull << lane) - 1)) == tile)) - 1;
+            tile -= n;
+        }
+    return -1;
+}
+
 // waves of a workgroup for few query rows (dim 256: one wave's registers)
 constexpr int token_waves(int dim) { return dim <= 128 ? 8 : 4; }
 
@@ -173,9 +209,15 @@ __global__ void __launch_bounds__(64 * token_waves(D)) kv_attention_k(KvAttnArgs
     __shared__ __align__(16) float os[NW / 2][16][D + 4];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int head_kv = blockIdx.y, split = blockIdx.z;
-    int tile = blockIdx.x;
-    const int b = find_share(tile, a.g.batch, [&](int s) { return query_tiles(span_of(a.g, s), a.group, 16); });
+    const int split = blockIdx.z;
+    int head_kv = blockIdx.y, tile = blockIdx.x, b = -2;
+    if (a.by_length) {  // all heads of a sequence, then the next one's
+        const int lin = blockIdx.y * a.tiles + blockIdx.x;
+        tile = lin / a.kv_heads, head_kv = lin - tile * a.kv_heads;
+        b = longest_first(a.g, a.group, tile);
+        if (b >= 0) tile = 0;
+    }
+    if (b == -2) b = find_share(tile, a.g.batch, [&](int s) { return query_tiles(span_of(a.g, s), a.group, 16); });
     if (b < 0) return;
     const Span span = span_of(a.g, b);
     const int64_t all = (int64_t)span.rows * a.group, fr = (int64_t)tile * 16 + i;
@@ -778,9 +820,10 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
     if (items * 64 * 8 > UINT32_MAX) return fail(NNC_HIP_EUNSUPP, name, "%lld rows of %d heads", (long long)rows, heads);
     KvAttnArgs a{c.ragged, c.k, c.v, c.k_scale, c.v_scale, q->data, out->data, nullptr, nullptr, ld, q_col, heads, c.kv_heads,
                  group, window, 1, 64, (int)tiles, slot_magic(c.page / 16),
-                 aligned16(q->data) && ld * activation_bytes(q) % 16 == 0 && q_col * activation_bytes(q) % 16 == 0,
+                 aligned16(q->data) && ld * activation_bytes(q) % 16 == 0 && q_col * activation_bytes(q) % 16 == 0, false,
                  scale * 1.44269504088896340736f};
     a.g.rows = (int)rows;
+    a.by_length = tile == 16 && items > cu_count() && c.ragged.batch <= kOrdered && rows <= kOrdered;
     if (tile == 16) {
         // shares of the keys, 512 or more each, while all workgroups run at
         // once, one on a CU (a second round starts 6 us later: one sequence of

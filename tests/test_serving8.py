@@ -563,6 +563,23 @@ def test_kv_attention_pages_of_different_size(rows, t, dev):
     check_attention(d.get("out"), q.reshape(rows, heads, dim), cache, starts, [length], F32(0.125), 0)
 
 
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("batch,kv,several", [(40, 8, False), (70, 4, False), (256, 2, False), (300, 1, False), (90, 4, True)])
+def test_kv_attention_many_sequences(batch, kv, several, t, dev):
+    """More workgroups than fit at once: every sequence answered once, in
+    whatever order, those without rows or positions among them; with one
+    sequence of several tiles too."""
+    rng = np.random.default_rng(batch)
+    lengths = rng.integers(0, 150, batch)
+    lengths[:3] = [700, 0, 1]
+    rows = rng.integers(0, 5, batch) > 0
+    rows = [int(r) for r in rows]
+    rows[0] = 1
+    if several:
+        rows[5] = 20
+    run_attention(dev, rng, [int(n) for n in lengths], rows, 2 * kv, kv, 32, 16, t, garbage=True)
+
+
 @pytest.mark.parametrize("rows,heads,length", [(1, 4, 9000), (600, 64, 700)])
 @pytest.mark.parametrize("power", [-100, 90])
 def test_kv_attention_values_very_small_and_large(power, rows, heads, length, dev):
