@@ -28,9 +28,9 @@
 // A workgroup takes 16 query rows - heads of one cached head, then tokens -
 // and a share of the keys, its waves 64 keys each in turn; the waves' sums are
 // joined through LDS, the shares' through the workspace. The cache's bytes
-// bound it: 64 sequences of up to 8192 positions (32 heads over 8 of 128) 130 us,
-// 552 MB at 4.25 TB/s, its longest ones ending last; one of 131072 54.2 us,
-// 4.95 TB/s, where a large copy reaches 5.2. A short call is a chain of dependent
+// bound it: 64 sequences of up to 8192 positions (32 heads over 8 of 128) 105 us,
+// 552 MB at 5.2 TB/s, as a large copy (in the batch's own order, whose longest
+// ended last, 130); one of 131072 54.2 us, 4.95 TB/s. A short call is a chain of dependent
 // loads (lengths, table, page) and joins, 7.2 us for four of 333.
 #include <limits.h>
 
@@ -197,12 +197,12 @@ __device__ __forceinline__ int longest_first(const Ragged& g, int group, int til
     return -1;
 }
 
-// waves of a workgroup for few query rows (dim 256: one wave's registers)
+// most waves of a workgroup for few query rows (dim 256: one wave's registers)
 constexpr int token_waves(int dim) { return dim <= 128 ? 8 : 4; }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(64 * token_waves(D)) kv_attention_k(KvAttnArgs a) {
-    constexpr int NW = token_waves(D), STRIDE = 64 * NW;
+template <typename T, int D, int NW>
+__global__ void __launch_bounds__(64 * NW) kv_attention_k(KvAttnArgs a) {
+    constexpr int STRIDE = 64 * NW;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int STEPS = D / 32, PIECES = F32 ? 2 : 1, KV = D / 16;  // KV: 16-dim blocks of the output
     __shared__ float ml[2][NW][16];
@@ -749,21 +749,26 @@ static void launch_prompt(const char* name, const KvAttnArgs& a) {
 }
 
 template <typename T, int D>
-static void launch_kv_attention(const char* name, const KvAttnArgs& a, int tile) {
+static void launch_kv_attention(const char* name, const KvAttnArgs& a, int tile, int waves) {
     if constexpr (D <= 128) {  // (dim 256: 512 registers a wave, and four of them)
         if (tile == 256) return launch_prompt<T, D, 8>(name, a);
     }
     if (tile == 128) return launch_prompt<T, D, 4>(name, a);
-    launch(name, kv_attention_k<T, D>, dim3((unsigned)a.tiles, (unsigned)a.kv_heads, (unsigned)a.splits), dim3(64 * token_waves(D)), 0, a);
+    const dim3 grid((unsigned)a.tiles, (unsigned)a.kv_heads, (unsigned)a.splits);
+    if constexpr (D <= 128) {
+        if (waves == 4) return launch(name, kv_attention_k<T, D, 4>, grid, dim3(256), 0, a);
+        if (waves == 2) return launch(name, kv_attention_k<T, D, 2>, grid, dim3(128), 0, a);
+    }
+    launch(name, kv_attention_k<T, D, token_waves(D)>, grid, dim3(64 * token_waves(D)), 0, a);
 }
 
 template <typename T>
-static void launch_dim(const char* name, const KvAttnArgs& a, int tile, int dim) {
+static void launch_dim(const char* name, const KvAttnArgs& a, int tile, int waves, int dim) {
     switch (dim) {
-        case 32: return launch_kv_attention<T, 32>(name, a, tile);
-        case 64: return launch_kv_attention<T, 64>(name, a, tile);
-        case 128: return launch_kv_attention<T, 128>(name, a, tile);
-        default: return launch_kv_attention<T, 256>(name, a, tile);
+        case 32: return launch_kv_attention<T, 32>(name, a, tile, waves);
+        case 64: return launch_kv_attention<T, 64>(name, a, tile, waves);
+        case 128: return launch_kv_attention<T, 128>(name, a, tile, waves);
+        default: return launch_kv_attention<T, 256>(name, a, tile, waves);
     }
 }
 
@@ -784,6 +789,20 @@ static int query_tile(int64_t rows, int64_t batch, int group, int kv_heads, int 
     const double t128 = n128 <= cus ? 1.9 : 3.0 * ceil_div(n128, 2 * cus);
     const double t256 = dim <= 128 ? 2.5 * ceil_div(n256, cus) : 1e30;
     return t256 < t128 && t256 < t16 ? 256 : t128 < t16 ? 128 : 16;
+}
+
+// Waves of a workgroup of 16 query rows. All workgroups at once: as many as
+// there can be. In several rounds, fewer waves leave room for other
+// workgroups on the CU, whose keys arrive while one starts or joins; more
+// have a long sequence done sooner. 8, 4 and 2 waves, us, 32 heads over 8 of
+// 128, f16: 64 sequences of up to 8192 107, 113, 128; 64 of 4096 99, 96, 101;
+// 64 of up to 1024 25, 21, 22; 128 of up to 4096 110, 100, 114; 128 of up to 512
+// 37, 25, 20; 256 of up to 1024 97, 66, 54; 512 of up to 4096 425, 381, 400; 512
+// of up to 300, 8 heads of 64, fp32 117, 51, 35.
+static int query_waves(int64_t items, int longest) {
+    const double rounds = (double)items / cu_count();
+    if (rounds <= 1.0 || longest > 2048 * rounds) return 8;
+    return rounds >= 4.0 && longest <= 128 * rounds ? 2 : 4;
 }
 
 }  // namespace nnc
@@ -823,6 +842,7 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
                  aligned16(q->data) && ld * activation_bytes(q) % 16 == 0 && q_col * activation_bytes(q) % 16 == 0, false,
                  scale * 1.44269504088896340736f};
     a.g.rows = (int)rows;
+    const int waves = query_waves(items, longest);
     a.by_length = tile == 16 && items > cu_count() && c.ragged.batch <= kOrdered && rows <= kOrdered;
     if (tile == 16) {
         // shares of the keys, 512 or more each, while all workgroups run at
@@ -842,9 +862,9 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
     }
     set_work(0.0, 2.0 * c.kv_heads * c.dim * (double)longest * c.ragged.batch);
     if (q->dtype == NNC_DTYPE_FLOAT16)
-        launch_dim<half_t>(name, a, tile, c.dim);
+        launch_dim<half_t>(name, a, tile, waves, c.dim);
     else
-        launch_dim<float>(name, a, tile, c.dim);
+        launch_dim<float>(name, a, tile, waves, c.dim);
 }
 
 }  // extern "C"

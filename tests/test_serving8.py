@@ -564,9 +564,11 @@ def test_kv_attention_pages_of_different_size(rows, t, dev):
 
 
 @pytest.mark.parametrize("t", [F32, F16])
-@pytest.mark.parametrize("batch,kv,several", [(40, 8, False), (70, 4, False), (256, 2, False), (300, 1, False), (90, 4, True)])
-def test_kv_attention_many_sequences(batch, kv, several, t, dev):
-    """More workgroups than fit at once: every sequence answered once, in
+@pytest.mark.parametrize("batch,kv,several", [(40, 8, False), (70, 4, False), (256, 2, False), (256, 8, False), (300, 1, False),
+                                              (600, 4, False), (90, 4, True)])
+@pytest.mark.parametrize("dim", [32, 128])
+def test_kv_attention_many_sequences(dim, batch, kv, several, t, dev):
+    """More workgroups than fit at once, of different sizes: every sequence answered once, in
     whatever order, those without rows or positions among them; with one
     sequence of several tiles too."""
     rng = np.random.default_rng(batch)
@@ -577,7 +579,7 @@ def test_kv_attention_many_sequences(batch, kv, several, t, dev):
     rows[0] = 1
     if several:
         rows[5] = 20
-    run_attention(dev, rng, [int(n) for n in lengths], rows, 2 * kv, kv, 32, 16, t, garbage=True)
+    run_attention(dev, rng, [int(n) for n in lengths], rows, 2 * kv, kv, dim, 16, t, garbage=True)
 
 
 @pytest.mark.parametrize("rows,heads,length", [(1, 4, 9000), (600, 64, 700)])
