@@ -396,7 +396,8 @@ void nnc_hip_matmul_i8(Tensor* a, Tensor* a_scale, Tensor* w, Tensor* w_scale, T
  * positions, only pages that cannot be read) gets zeros; what is in the cache
  * at positions that a row does not see does not reach its result. max_length:
  * the longest sequence if the caller knows it, 0 otherwise (then the
- * table's width); it decides how the work is divided, not the result. */
+ * table's width); like the batch it decides how the work is divided, and so the
+ * order of the sums, but not which positions are seen. */
 void nnc_hip_kv_write(Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale,
                       Tensor* table, Tensor* starts, Tensor* lengths, int k_col, int v_col);
 void nnc_hip_kv_read(Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table, Tensor* starts,
