@@ -775,9 +775,11 @@ static void launch_dim(const char* name, const KvAttnArgs& a, int tile, int wave
 // Query rows of a workgroup: 256 or 128 by the prompt kernel, 16 by the other,
 // which divides the keys instead. By the time that a CU takes for 64 keys,
 // dim 128, in us: 256 rows 2.5, 128 rows 1.9, two workgroups of them 3.0,
-// 256 rows as 16 tiles of 16 6.1. Two prompts of 2048 behind 2048, 32 heads
-// over 8: 248, 298 and (16 rows) 762 us; one of 256 behind 7936: 264, 248 and
-// 96; two of 1000, 16 heads of 64, fp32: 43, 36 and 65.
+// 256 rows as 16 tiles of 16 6.1. With 256, 128 and 16 rows, us, 32 heads over 8
+// of 128, f16: two prompts of 2048 behind 2048 243, 292, 595; 16 of 1024 248, 256,
+// 554; four of 256 behind 1792 74, 71, 115; one of 256 behind 7936 261, 243, 101;
+// one of 256 18, 16, 11; 64 of 16 behind 1008 83, 55, 85, of 4 behind 4092 307,
+// 201, 99.
 static int query_tile(int64_t rows, int64_t batch, int group, int kv_heads, int dim) {
     const int64_t cus = cu_count(), holders = rows < batch ? rows : batch;  // sequences that can have rows
     auto count = [&](int tile) {
