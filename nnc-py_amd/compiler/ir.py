@@ -99,19 +99,55 @@ class Graph:
                 return n
         return None
 
+    def updated(self) -> set[str]:
+        """Tensors that a node changes in place: among its inputs and its
+        outputs (a cache that rows are written to)."""
+        return {t for n in self.nodes for t in n.outputs if t and t in n.inputs}
+
+    def fixed(self) -> set[str]:
+        """Tensors that no pass may take away: the graph's outputs, and what
+        nodes read or make that read or write an updated tensor. Such a node
+        stays the node it was, at its place among the others of that tensor:
+        fused with an earlier or a later one it would see another state."""
+        fixed, updated = set(self.outputs), self.updated()
+        for n in self.nodes if updated else ():
+            if any(t in updated for t in n.inputs + n.outputs):
+                fixed.update(t for t in n.inputs + n.outputs if t)
+        return fixed
+
+    def _state_order(self) -> dict[int, list[Node]]:
+        """Nodes that have to run before a node (by id), for the tensors that
+        nodes change in place: a writer after every reader and writer inserted
+        before it, a reader after the writer before it."""
+        before: dict[int, list[Node]] = {}
+        for t in self.updated():
+            writer, readers = None, []
+            for n in self.nodes:
+                if t in n.outputs:
+                    before.setdefault(id(n), []).extend(readers + ([writer] if writer else []))
+                    writer, readers = n, []
+                elif t in n.inputs:
+                    before.setdefault(id(n), []).extend([writer] if writer else [])
+                    readers.append(n)
+        return before
+
     def topological_sort(self) -> list[Node]:
         """Nodes ordered so every input is produced before use; stable with
         respect to insertion order (the reference sorts with networkx,
         graph.py:55-60; insertion order is already topological here unless a
-        pass appended nodes out of order)."""
+        pass appended nodes out of order). Nodes that read or write a tensor
+        which one of them changes in place keep their order of insertion: the
+        tensor's name does not tell its states apart."""
         ready = set(self.inputs) | set(self.constants)
+        before, done = self._state_order(), set()
         order, pending = [], list(self.nodes)
         while pending:
             progressed = False
             rest = []
             for n in pending:
-                if all(i in ready or i == "" for i in n.inputs):
+                if all(i in ready or i == "" for i in n.inputs) and all(id(b) in done for b in before.get(id(n), ())):
                     order.append(n)
+                    done.add(id(n))
                     ready.update(n.outputs)
                     progressed = True
                 else:

@@ -44,10 +44,14 @@ INPLACE_INPUTS = {"FusedConvAddRelu": (3,)}
 # ---------------------------------------------------------------------------
 def eliminate_identity(g: Graph) -> int:
     """Bypass Identity nodes (passes/identity_elimination.py:13): consumers read
-    the Identity's input. An Identity producing a graph output is kept."""
+    the Identity's input. An Identity producing a graph output is kept, and one
+    from or to a tensor that a node changes in place: the two differ then."""
     removed = 0
+    updated = g.updated()
     for node in list(g.nodes):
         if node.op_type != "Identity" or node.outputs[0] in g.outputs:
+            continue
+        if node.inputs[0] in updated or node.outputs[0] in updated:
             continue
         src, dst = node.inputs[0], node.outputs[0]
         for c in g.nodes:
@@ -100,10 +104,10 @@ _PATTERNS = [  # (producer, consumer, fused op), in priority order
 def fuse_patterns(g: Graph) -> int:
     """producer().only_used_by(consumer()) -> one fused node carrying the
     producer's inputs/attrs and the consumer's output."""
-    fused = 0
+    fused, fixed = 0, g.fixed()
     for prod_op, cons_op, fused_op in _PATTERNS:
         for node in list(g.nodes):
-            if node.op_type != prod_op or node.outputs[0] in g.outputs:
+            if node.op_type != prod_op or node.outputs[0] in fixed:
                 continue
             users = g.consumers(node.outputs[0])
             if len(users) != 1 or users[0].op_type != cons_op:
@@ -127,14 +131,14 @@ def fuse_residual(g: Graph) -> int:
     is added in the conv epilogue instead of a separate pass over both
     tensors. The Add's first operand is preferred (the block's main-path
     conv in ResNet; the shortcut conv stays a plain conv)."""
-    fused = 0
+    fused, fixed = 0, g.fixed()
     for add in list(g.nodes):
         if add.op_type != "FusedAddRelu" or len(add.inputs) != 2 or add.inputs[0] == add.inputs[1]:
             continue
         for k in (0, 1):
             mid, res = add.inputs[k], add.inputs[1 - k]
             prod = g.producer(mid)
-            if prod is None or prod.op_type != "Conv" or mid in g.outputs:
+            if prod is None or prod.op_type != "Conv" or mid in fixed:
                 continue
             if len(g.consumers(mid)) != 1:
                 continue
@@ -206,7 +210,7 @@ def fuse_projection(g: Graph) -> int:
     ([Co][9*Ci + Cx]), the two biases summed, and P's input read by F's
     contraction, so the projection needs no launch and no tensor. Inputs:
     x, w, bias or "", projection input; attrs: F's, plus proj_strides."""
-    fused = 0
+    fused, fixed = 0, g.fixed()
     for f in list(g.nodes):
         if f.op_type != "FusedConvAddRelu" or len(f.inputs) != 4:
             continue
@@ -217,7 +221,7 @@ def fuse_projection(g: Graph) -> int:
         if wf.data is None or wf.data.ndim != 4 or wf.data.shape[1:3] != (3, 3):
             continue
         p = g.producer(res)
-        if p is None or p.op_type != "Conv" or res in g.outputs or len(g.consumers(res)) != 1:
+        if p is None or p.op_type != "Conv" or res in fixed or len(g.consumers(res)) != 1:
             continue
         if len(p.inputs) < 2 or not g.tensors[p.inputs[1]].is_constant or len(g.consumers(p.inputs[1])) != 1:
             continue
@@ -265,9 +269,9 @@ def fuse_matmul_bias(g: Graph) -> int:
     views, W packed to [N, K] at compile time) or, when the Add was fused
     with a Relu, FusedMatMulBiasRelu (lowered to nnc_matmul_relu with the
     bias). The sum is the same fp32 add of the bias to the product."""
-    fused = 0
+    fused, fixed = 0, g.fixed()
     for mm in list(g.nodes):
-        if mm.op_type != "MatMul" or len(mm.inputs) != 2 or mm.outputs[0] in g.outputs:
+        if mm.op_type != "MatMul" or len(mm.inputs) != 2 or mm.outputs[0] in fixed:
             continue
         a, w = mm.inputs
         wt = g.tensors[w]
@@ -399,14 +403,14 @@ def _stream_conv_pool(g: Graph, lds_budget: int) -> int:
     kernel's shapes, 224x224 or 64x64 input)."""
     if CONV_POOL_MIN_ROWS is None:
         return 0
-    fused = 0
+    fused, fixed = 0, g.fixed()
     for conv in list(g.nodes):
         if conv.op_type != "FusedConvRelu" or len(conv.inputs) < 2:
             continue
         w = g.tensors[conv.inputs[1]]
         x = g.tensors[conv.inputs[0]]
         mid = conv.outputs[0]
-        if len(w.shape) != 2 or len(x.shape) != 4 or x.shape[1] != 3 or mid in g.outputs:
+        if len(w.shape) != 2 or len(x.shape) != 4 or x.shape[1] != 3 or mid in fixed:
             continue
         if list(conv.attrs.get("kernel_shape", [])) != [7, 7] or w.shape[0] > 64:
             continue
@@ -447,13 +451,13 @@ def stream_tiles(g: Graph, lds_budget: int = LDS_BUDGET) -> int:
     intermediate (an image's C means, its w blocks and partial sums) fits
     `lds_budget`, at batches up to GAP_GEMM_MAX_BATCH. The decision and its
     footprint are recorded in the node's metadata["tile_stream"]."""
-    fused = _stream_conv_pool(g, lds_budget)
+    fused, fixed = _stream_conv_pool(g, lds_budget), g.fixed()
     for gap in list(g.nodes):
         if gap.op_type != "GlobalAveragePool" or len(gap.inputs) != 1:
             continue
         x, pooled = gap.inputs[0], gap.outputs[0]
         xs = g.tensors[x].shape
-        if len(xs) != 4 or pooled in g.outputs or g.tensors[x].dtype != "float32" or xs[0] > GAP_GEMM_MAX_BATCH:
+        if len(xs) != 4 or pooled in fixed or g.tensors[x].dtype != "float32" or xs[0] > GAP_GEMM_MAX_BATCH:
             continue
         if xs[1] % 4 or xs[1] > 1024:
             continue
@@ -463,7 +467,7 @@ def stream_tiles(g: Graph, lds_budget: int = LDS_BUDGET) -> int:
         flat = users[0]
         flat_out = flat.outputs[0]
         gemms = g.consumers(flat_out)
-        if flat_out in g.outputs or len(gemms) != 1 or gemms[0].op_type != "Gemm":
+        if flat_out in fixed or len(gemms) != 1 or gemms[0].op_type != "Gemm":
             continue
         gm = gemms[0]
         if gm.inputs[0] != flat_out or int(gm.attrs.get("transA", 0)) != 0 or int(gm.attrs.get("transB", 0)) != 1:
@@ -526,7 +530,7 @@ def fuse_eltwise_chains(g: Graph) -> int:
     so the values are those of the op-by-op calls."""
     from .lower import clip_bounds
     from ..abi import EW_OPS
-    fused = 0
+    fused, fixed = 0, g.fixed()
     done: set[str] = set()
     for head in g.topological_sort():
         if head.name in done or not _ew_node_ok(g, head):
@@ -547,7 +551,7 @@ def fuse_eltwise_chains(g: Graph) -> int:
             chain.append(node)
             prev = node.outputs[0]
             users = g.consumers(prev)
-            if prev in g.outputs or len(users) != 1 or not _ew_node_ok(g, users[0]):
+            if prev in fixed or len(users) != 1 or not _ew_node_ok(g, users[0]):
                 break
             nxt = users[0]
             if nxt.name in done or prev not in nxt.inputs[:EW_STEPS[nxt.op_type][1]]:
@@ -580,9 +584,9 @@ def fuse_add_layernorm(g: Graph) -> int:
     FusedAddLayerNorm node (inputs: a, b, scale, bias; the LayerNorm's
     attrs), lowered to nnc_hip_add_layernorm: the sum stays in registers.
     The same bits as the Add and the LayerNorm run one after the other."""
-    fused = 0
+    fused, fixed = 0, g.fixed()
     for add in list(g.nodes):
-        if add.op_type != "Add" or len(add.inputs) != 2 or add.outputs[0] in g.outputs:
+        if add.op_type != "Add" or len(add.inputs) != 2 or add.outputs[0] in fixed:
             continue
         s = add.outputs[0]
         t = g.tensors[s]
@@ -610,9 +614,9 @@ def fuse_scaled_softmax(g: Graph) -> int:
     nnc_hip_scaled_softmax: attention's score scaling applied as the rows
     are loaded. The same bits as the Div and the Softmax one after the
     other."""
-    fused = 0
+    fused, fixed = 0, g.fixed()
     for div in list(g.nodes):
-        if div.op_type != "Div" or len(div.inputs) != 2 or div.outputs[0] in g.outputs:
+        if div.op_type != "Div" or len(div.inputs) != 2 or div.outputs[0] in fixed:
             continue
         q = div.outputs[0]
         x, d = (g.tensors[i] for i in div.inputs)
@@ -640,7 +644,7 @@ def fuse_split_transposes(g: Graph) -> int:
     Transpose becomes a SliceTranspose of the unsplit tensor (attrs perm,
     col0, width), lowered to nnc_hip_transpose_slice. A copy of the same
     elements: the bits of the Split, the Reshape and the Transpose."""
-    fused = 0
+    fused, fixed = 0, g.fixed()
     for split in list(g.nodes):
         if split.op_type != "Split" or not split.inputs or not split.outputs:
             continue
@@ -651,11 +655,11 @@ def fuse_split_transposes(g: Graph) -> int:
         chains = []
         for piece in split.outputs:
             users = g.consumers(piece)
-            if piece in g.outputs or len(users) != 1 or users[0].op_type != "Reshape" or users[0].inputs[0] != piece:
+            if piece in fixed or len(users) != 1 or users[0].op_type != "Reshape" or users[0].inputs[0] != piece:
                 break
             rs = users[0]
             tr = g.consumers(rs.outputs[0])
-            if rs.outputs[0] in g.outputs or len(tr) != 1 or tr[0].op_type != "Transpose" or tr[0].inputs[0] != rs.outputs[0]:
+            if rs.outputs[0] in fixed or len(tr) != 1 or tr[0].op_type != "Transpose" or tr[0].inputs[0] != rs.outputs[0]:
                 break
             chains.append((piece, rs, tr[0]))
         if len(chains) != len(split.outputs):
@@ -676,7 +680,7 @@ def fuse_split_transposes(g: Graph) -> int:
             for t in rs.outputs + [piece]:
                 g.tensors.pop(t, None)
             for c in rs.inputs[1:]:
-                if c in g.tensors and not g.consumers(c) and c not in g.outputs:
+                if c in g.tensors and not g.consumers(c) and c not in fixed:
                     g.tensors.pop(c, None)
         g.nodes.remove(split)
         fused += 1
@@ -690,7 +694,7 @@ ATTENTION_MAX_SEQ = 128
 def _only_reader(g: Graph, tensor: str, op_type: str, index: int | None = 0):
     """The one node reading `tensor` (no graph output), if it is an
     `op_type` reading it at input `index` (any input if None)."""
-    if tensor in g.outputs:
+    if tensor in g.fixed():
         return None
     users = g.consumers(tensor)
     if len(users) != 1 or users[0].op_type != op_type:
@@ -778,12 +782,12 @@ def compose_transposes(g: Graph) -> int:
     else (and no graph output) becomes one Transpose of the first's input
     with the composed permutation: out.shape[i] = x.shape[p1[p2[i]]], the
     same element moves, one copy instead of two."""
-    merged = 0
+    merged, fixed = 0, g.fixed()
     for t2 in list(g.nodes):
         if t2.op_type != "Transpose" or not t2.inputs:
             continue
         t1 = g.producer(t2.inputs[0])
-        if t1 is None or t1.op_type != "Transpose" or t1.outputs[0] in g.outputs:
+        if t1 is None or t1.op_type != "Transpose" or t1.outputs[0] in fixed:
             continue
         if len(g.consumers(t1.outputs[0])) != 1:
             continue
@@ -807,14 +811,14 @@ def eliminate_concat_split(g: Graph) -> int:
     pieces (the Concat's output read by nothing else, neither result a graph
     output) hands the Concat's inputs straight to the Split's readers: both
     copies disappear and every value is unchanged."""
-    removed = 0
+    removed, fixed = 0, g.fixed()
     for split in list(g.nodes):
         if split.op_type != "Split" or not split.inputs:
             continue
         cat = g.producer(split.inputs[0])
-        if cat is None or cat.op_type != "Concat" or cat.outputs[0] in g.outputs:
+        if cat is None or cat.op_type != "Concat" or cat.outputs[0] in fixed:
             continue
-        if len(g.consumers(cat.outputs[0])) != 1 or any(o in g.outputs for o in split.outputs):
+        if len(g.consumers(cat.outputs[0])) != 1 or any(o in fixed for o in split.outputs):
             continue
         nd = len(g.tensors[cat.outputs[0]].shape)
         ax_c, ax_s = int(cat.attrs.get("axis", 0)) % nd, int(split.attrs.get("axis", 0)) % nd
@@ -1180,6 +1184,7 @@ def find_branches(g: Graph, order: list[Node], max_flops: float) -> list[Branch]
         for t in n.inputs:
             consumers.setdefault(t, []).append(n)
     taken: set[str] = set()
+    fixed = g.fixed()
     out: list[Branch] = []
     for d in order:
         if d.op_type not in CONV_OPS or d.name in taken:
@@ -1189,7 +1194,7 @@ def find_branches(g: Graph, order: list[Node], max_flops: float) -> list[Branch]
             continue
         others = [c for c in consumers.get(acts[0], []) if c.name != d.name]
         readers = consumers.get(d.outputs[0], [])
-        if len(others) != 1 or len(readers) != 1 or d.outputs[0] in g.outputs:
+        if len(others) != 1 or len(readers) != 1 or d.outputs[0] in fixed:
             continue
         a, j = others[0], readers[0]
         lo, hi = min(pos[a.name], pos[d.name]), pos[j.name]
