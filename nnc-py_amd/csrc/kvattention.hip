@@ -840,7 +840,7 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
     const int64_t tiles = query_tiles_bound(rows, c.ragged.batch, group, tile), items = tiles * c.kv_heads;
     if (items * 64 * 8 > UINT32_MAX) return fail(NNC_HIP_EUNSUPP, name, "%lld rows of %d heads", (long long)rows, heads);
     KvAttnArgs a{c.ragged, c.k, c.v, c.k_scale, c.v_scale, q->data, out->data, nullptr, nullptr, ld, q_col, heads, c.kv_heads,
-                 group, window, 1, 64, (int)tiles, slot_magic(c.page / 16),
+                 group, window_of(window, capacity), 1, 64, (int)tiles, slot_magic(c.page / 16),
                  aligned16(q->data) && ld * activation_bytes(q) % 16 == 0 && q_col * activation_bytes(q) % 16 == 0, false,
                  scale * 1.44269504088896340736f};
     a.g.rows = (int)rows;

@@ -97,6 +97,10 @@ RAGGED_HD int64_t query_tiles_bound(int64_t rows, int64_t batch, int group, int 
     return some < each ? some : each;
 }
 
+// The window that is compared: none (0) if it is as long as a sequence can be,
+// so that positions less it stay far from the smallest number.
+RAGGED_HD int window_of(int window, int capacity) { return window < capacity ? window : 0; }
+
 // The keys that rows at positions first .. last see, [lo, hi), in at most
 // `splits` shares of at least `least` keys (a multiple of `step`): share s has
 // [lo + s * chunk, ...).
@@ -104,7 +108,7 @@ struct KeyRange {
     int lo, hi, chunk;
     RAGGED_HD KeyRange(int first, int last, int window, int splits, int least, int step) {
         hi = imax(last + 1, 0);
-        lo = window > 0 ? imax(first - window + 1, 0) & ~63 : 0;
+        lo = window > 0 && first >= window ? (first - window + 1) & ~63 : 0;
         const int each = (imax(hi - lo, 0) + splits - 1) / splits;
         chunk = imax(least, (each + step - 1) / step * step);
     }
