@@ -379,10 +379,9 @@ void nnc_hip_matmul_i8(Tensor* a, Tensor* a_scale, Tensor* w, Tensor* w_scale, T
  * the larger of its old scale and the new rows'; if that is larger than the
  * old one, the kept whole numbers become the nearest to their value under it.
  * A page that the new rows begin in gets theirs. Positions behind the length
- * stay as they were. Scales are 0, 2^-107 or more (values of 2^-100), or NaN;
- * attention takes any up to 2^102. No page may belong to two sequences that write to it in
- * one call, nor be in its table twice; pages of a common prefix that no row
- * touches may be shared.
+ * stay as they were. Scales are 0, 2^-107 or more (values of 2^-100), or NaN.
+ * No page may belong to two sequences that write to it in one call, nor be in
+ * its table twice; pages of a common prefix that no row touches may be shared.
  *
  * nnc_hip_kv_read: the opposite: rows starts[b] .. starts[b + 1] of k and v
  * receive sequence b's last positions.
@@ -394,10 +393,12 @@ void nnc_hip_matmul_i8(Tensor* a, Tensor* a_scale, Tensor* w, Tensor* w_scale, T
  * head h reading cached head h / (heads / kv_heads). out [rows][heads * dim],
  * 16-byte aligned. A row that sees nothing (no length, more rows than
  * positions, only pages that cannot be read) gets zeros; what is in the cache
- * at positions that a row does not see does not reach its result. max_length:
- * the longest sequence if the caller knows it, 0 otherwise (then the
- * table's width); like the batch it decides how the work is divided, and so the
- * order of the sums, but not which positions are seen. */
+ * at positions that a row does not see does not reach its result. The pages'
+ * scales may be any that kv_write makes, in any mix: a key has its weight in
+ * the divisor whatever the size of its page's values. max_length: the longest
+ * sequence if the caller knows it, 0 otherwise (then the table's width); like
+ * the batch it decides how the work is divided, and so the order of the sums,
+ * but not which positions are seen. */
 void nnc_hip_kv_write(Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale,
                       Tensor* table, Tensor* starts, Tensor* lengths, int k_col, int v_col);
 void nnc_hip_kv_read(Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table, Tensor* starts,

@@ -5,13 +5,16 @@
 //   j <= pos_i, j > pos_i - window;  k_j = K_j u_k(page), v_j = V_j u_v(page)
 //
 // with K, V whole numbers and one scale for each page and head. One pass over
-// the keys: in units of powers of two, x_j = scale log2(e) u_k (q . K_j) +
-// log2(u_v), running maximum m of x, p_j = 2^(x_j - m); then
+// the keys: in units of powers of two, s_j = scale log2(e) u_k (q . K_j) and
+// x_j = s_j + log2(u_v); m a running maximum of x, p_j = 2^(x_j - m); then
 //
-//   out = (sum_j p_j V_j) / (sum_j p_j / u_v(j))
+//   out = 2^e (sum_j p_j V_j) / l,   l = sum_j 2^(s_j - m + e) = sum_j p_j 2^e / u_v
 //
 // so that the pages' value scales cost nothing in the second product, and p
-// has the size of what it contributes.
+// has the size of what it contributes. e is a whole number that keeps l near 1:
+// m - e is about the largest s. The factor 2^e / u_v of a page serves as long as
+// p did not lose what l needs: where it is over 2^60 (a page of values far below
+// another's, or of zeros) l takes its own exponentials.
 //
 // v_mfma_f32_16x16x32_f16, keys as the first operand's rows and query rows as
 // the second's columns (S^T = K Q^T, then O^T = V^T P^T): lane (i = lane % 16,
@@ -22,8 +25,8 @@
 // consecutive keys 16g .. 16g + 15: one scale each, and 16 consecutive bytes
 // of V. Whole numbers of 8 bits are exact in f16. Query rows are f16 as they
 // are; fp32 ones are scaled by a power of two and cut into two f16 pieces (22
-// bits), and so is p then (f16 outputs: p rounded to f16 once, 2^-11 of it at most, as their own
-// rounding is).
+// bits), and so is p then. For f16 outputs p is rounded to f16 once, which moves a
+// weight by 2^-11 of it at most, as the output's own rounding moves the result.
 //
 // A workgroup takes 16 query rows - heads of one cached head, then tokens -
 // and a share of the keys, its waves 64 keys each in turn; the waves' sums are
@@ -45,7 +48,7 @@ struct KvAttnArgs {
     const float *k_scale, *v_scale;
     const void* q;
     void* out;
-    float* part;    // [tile][cached head][split][row of the tile][dim + 4]: sums, maximum, divisor
+    float* part;    // [tile][cached head][split][row of the tile][dim + 4]: sums, m, l, e
     int* counters;  // [tile][cached head], zero
     int64_t ld;
     int q_col, heads, kv_heads, group, window, splits, chunk, tiles;
@@ -71,24 +74,39 @@ __device__ __forceinline__ f16x8 widen8(uint32_t lo, uint32_t hi) {
     return x.v + f16x8{c, c, c, c, c, c, c, c};
 }
 
-// The scale that a page's values are taken to have: a page of zeros (scale 0)
-// gets one that is small beside any page with values, whose p would otherwise
-// be small beside its own and lose bits as f16, and large enough for its
-// weights in the divisor to stay above 2^-126.
-__device__ __forceinline__ float value_unit(float scale) { return scale == 0.f ? 0x1p-64f : scale; }
-
-// The divisor sum_j p_j / u_j is kept 2^24 smaller, and the sums of values are
-// made so before they are divided: p up to 2^15 over the smallest scale that
-// is not 0, 2^-107, stays finite then for as many keys as there can be, and
-// 1 / u a normal number for scales up to 2^102.
-static constexpr float kWeight = 0x1p-24f;
-
 // p is scaled by 2^12 before it is rounded to f16: its smallest steps are then
 // 2^-36 of the row's largest. The running maximum is only moved, and what was
 // summed up scaled down, when it has grown by more than 2^3 (p stays below
-// 2^15).
-static constexpr float kPLog = 12.f, kSlack = 3.f;
+// 2^15). It is the largest x itself, so that the p of a key that outweighs the
+// others is 2^12, exact in f16: the next power of two in its place makes f16
+// results of 64 sequences of up to 8192 worse by a third (2.9e-4 for 2.2e-4).
+static constexpr float kSlack = 3.f;
+static constexpr float kPLog = 12.f;
+// A page's factor is used up to here. A p that l needs (2^-41: 2^17 such keys
+// change its last bit) is 2^-101 then, still a normal number; and as e, each
+// lane's own, is chosen where m is moved or the factor is larger only, a term of
+// l is up to 2^75, of which 2^28 leave it finite.
+static constexpr float kMostFactor = 0x1p60f;
+// m before anything was seen: x is above, and 2^(kNone - x) is 0
+static constexpr float kNone = -3.402823466e38f;
+// a page of zeros has the logarithm of a scale so small that none of its p
+// shows beside a page of values, and no factor
+static constexpr float kZeros = -200.f;
 typedef float fx2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float scale_log(float scale) {
+    const float log = __builtin_amdgcn_logf(scale);
+    return log < kZeros ? kZeros : log;  // (NaN stays)
+}
+// The s against which l is taken (2^12 of p go with e), and e for the largest s.
+__device__ __forceinline__ float reference(float m, float e) { return m - (e + kPLog); }
+__device__ __forceinline__ float exponent(float m, float largest) { return floorf(__builtin_amdgcn_fmed3f(m - largest, -400.f, 400.f)) - kPLog; }
+// What l becomes when m and e do: times o's factor and a power of two. (In one
+// exponential where either may not be a normal number: the sum is rounded, by
+// less than a weight's last bit.)
+__device__ __forceinline__ float rescale(float m, float e, float to_m, float to_e) { return __builtin_amdgcn_exp2f((m - to_m) + (to_e - e)); }
+// nothing seen: no lane's own s is below this reference
+static constexpr float kUnseen = 400.f - kPLog;
 
 // ---------------------------------------------------------------------------
 // Shares of the keys: every workgroup of a tile and head stores its rows' sums,
@@ -117,19 +135,24 @@ struct Shares {
     __device__ __forceinline__ void join(int shares, int row, T* out) const {
         constexpr int PER = D >= 64 ? D / 64 : 1;
         const int lane = threadIdx.x & 63, dim = lane % (D / PER) * PER;
-        float top = -INFINITY;
-        for (int s = lane; s < shares; s += 64) top = fmaxf(top, load_partial(r, at(s, row, D)));
+        float top = kNone, far = kNone;
+        for (int s = lane; s < shares; s += 64) {
+            const float m = load_partial(r, at(s, row, D));
+            top = fmaxf(top, m);
+            far = fmaxf(far, reference(m, load_partial(r, at(s, row, D + 2))));
+        }
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-        const float base = top == -INFINITY ? 0.f : top;
+        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o)), far = fmaxf(far, __shfl_xor(far, o));
+        const float e = exponent(top, far);
         float sum = 0.f, o[PER];
 #pragma unroll
         for (int q = 0; q < PER; ++q) o[q] = 0.f;
         for (int s0 = 0; s0 < shares; s0 += 64) {
             float w = 0.f;
             if (s0 + lane < shares) {
-                w = __builtin_amdgcn_exp2f(load_partial(r, at(s0 + lane, row, D)) - base);
-                sum = fmaf(w, load_partial(r, at(s0 + lane, row, D + 1)), sum);
+                const float m = load_partial(r, at(s0 + lane, row, D));
+                w = __builtin_amdgcn_exp2f(m - top);
+                sum = fmaf(rescale(m, load_partial(r, at(s0 + lane, row, D + 2)), top, e), load_partial(r, at(s0 + lane, row, D + 1)), sum);
             }
             const int n = min(64, shares - s0);
             for (int t = 0; t < n; t += 8) {
@@ -157,7 +180,7 @@ struct Shares {
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
         if (lane < D / PER) {
 #pragma unroll
-            for (int q = 0; q < PER; ++q) out[dim + q] = (T)(o[q] * kWeight * inv);
+            for (int q = 0; q < PER; ++q) out[dim + q] = (T)ldexpf(o[q] * inv, (int)e);
         }
     }
 };
@@ -200,12 +223,14 @@ __device__ __forceinline__ int longest_first(const Ragged& g, int group, int til
 // most waves of a workgroup for few query rows (dim 256: one wave's registers)
 constexpr int token_waves(int dim) { return dim <= 128 ? 8 : 4; }
 
+// (dim 32: four waves a SIMD; three, where the compiler takes a few registers
+// more, are 29 us and not 25 for 512 sequences of up to 300, 8 heads, fp32)
 template <typename T, int D, int NW>
-__global__ void __launch_bounds__(64 * NW) kv_attention_k(KvAttnArgs a) {
+__global__ void __launch_bounds__(64 * NW, D == 32 ? 4 : 1) kv_attention_k(KvAttnArgs a) {
     constexpr int STRIDE = 64 * NW;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int STEPS = D / 32, PIECES = F32 ? 2 : 1, KV = D / 16;  // KV: 16-dim blocks of the output
-    __shared__ float ml[2][NW][16];
+    __shared__ float ml[3][NW][16];
     __shared__ __align__(16) float os[NW / 2][16][D + 4];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -315,7 +340,8 @@ __global__ void __launch_bounds__(64 * NW) kv_attention_k(KvAttnArgs a) {
             qf[0][s][j] = hi;
             if (F32) qf[PIECES - 1][s][j] = (half_t)(y - (float)hi);
         }
-    float m = -INFINITY, l = 0.f;
+    float m = kNone, l = 0.f;  // m the row's, l the lane's
+    float ex = kUnseen;
     fx4 o[KV];
 #pragma unroll
     for (int c = 0; c < KV; ++c) o[c] = fx4{0.f, 0.f, 0.f, 0.f};
@@ -337,8 +363,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attention_k(KvAttnArgs a) {
             for (int r = 0; r < 4; ++r) x[4 * bl + r] = s[r];
         }
         load_k(tb + STRIDE);
-        const float vu = value_unit(vs);
-        float ku = ks * qs, lv = __builtin_amdgcn_logf(vu), iv = kWeight / vu;
+        float ku = ks * qs, lv = scale_log(vs), iv = 1.0f / vs;
         ku = ku == 0.f ? 0x1p-126f : ku;  // for the product with -inf
         if (!(tb + 63 <= first_pos && (a.window <= 0 || tb > last_pos - a.window) && __all(have))) {
             const int j = tb + 16 * g, low = a.window > 0 ? pos - a.window : INT_MIN, up = have ? pos : INT_MIN;
@@ -352,21 +377,29 @@ __global__ void __launch_bounds__(64 * NW) kv_attention_k(KvAttnArgs a) {
         float mx = fmaf(top, ku, lv);
         mx = fmaxf(mx, __shfl_xor(mx, 16));
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        if (__any(mx > m + kSlack)) {
-            const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= alpha;
+        float factor = ldexpf(iv, (int)ex), sum = 0.f;
+        if (__any(mx > m + kSlack || factor > kMostFactor)) {
+            const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - mn);
+            const float en = exponent(mn, fmaxf(reference(m, ex), top * ku));
+            l *= rescale(m, ex, mn, en);
+            m = mn, ex = en;
 #pragma unroll
             for (int c = 0; c < KV; ++c) o[c] *= alpha;
+            factor = ldexpf(iv, (int)ex);
+            if (__any(factor > kMostFactor)) {
+                const float base = reference(m, ex);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) l += __builtin_amdgcn_exp2f(fmaf(x[c], ku, -base));
+                factor = 0.f;
+            }
         }
-        const float shift = lv - (m == -INFINITY ? 0.f : m - kPLog);
-        float sum = 0.f;
+        const float shift = lv - (m - kPLog);
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
             x[c] = __builtin_amdgcn_exp2f(fmaf(x[c], ku, shift));
             sum += x[c];
         }
-        l = fmaf(sum, iv, l);
+        l = fmaf(sum, factor, l);
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             f16x8 pf[PIECES];
@@ -391,18 +424,19 @@ __global__ void __launch_bounds__(64 * NW) kv_attention_k(KvAttnArgs a) {
         find(tb + 2 * STRIDE);
     }
     // join the waves
+    const float er = fminf(fminf(ex, __shfl_xor(ex, 16)), fminf(__shfl_xor(ex, 32), __shfl_xor(ex, 48)));
+    l = ldexpf(l, (int)(er - ex));
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (g == 0) ml[0][wave][i] = m, ml[1][wave][i] = l;
+    if (g == 0) ml[0][wave][i] = m, ml[1][wave][i] = l, ml[2][wave][i] = er;
     __syncthreads();
-    float top = ml[0][0][i];
+    float top = kNone, far = kNone, sum = 0.f;
 #pragma unroll
-    for (int w = 1; w < NW; ++w) top = fmaxf(top, ml[0][w][i]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[0][w][i]), far = fmaxf(far, reference(ml[0][w][i], ml[2][w][i]));
+    ex = exponent(top, far);
 #pragma unroll
-    for (int w = 0; w < NW; ++w) sum += ml[1][w][i] * __builtin_amdgcn_exp2f(ml[0][w][i] - base);
-    const float f = __builtin_amdgcn_exp2f(m - base);
+    for (int w = 0; w < NW; ++w) sum += ml[1][w][i] * rescale(ml[0][w][i], ml[2][w][i], top, ex);
+    const float f = __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
     for (int c = 0; c < KV; ++c) o[c] *= f;
     // the upper half of the waves hands its sums to the lower, until one has all
@@ -425,7 +459,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attention_k(KvAttnArgs a) {
         for (int c = 0; c < KV; ++c) {
             T v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (T)(o[c][r] * kWeight * inv);
+            for (int r = 0; r < 4; ++r) v[r] = (T)ldexpf(o[c][r] * inv, (int)ex);
             __builtin_memcpy(__builtin_assume_aligned(op + 16 * c, 4 * sizeof(T)), v, sizeof v);
         }
         return;
@@ -438,7 +472,7 @@ __global__ void __launch_bounds__(64 * NW) kv_attention_k(KvAttnArgs a) {
             const float x = o[c][0], y = o[c][1], z = o[c][2], w = o[c][3];
             part.put4(split, i, 16 * c + 4 * g, x, y, z, w);
         }
-        if (g == 0) part.put4(split, i, D, top, sum, 0.f, 0.f);
+        if (g == 0) part.put4(split, i, D, top, sum, ex, 0.f);
     }
     if (!finish_arrive(a.counters + item, shares - 1)) return;
     for (int r = wave; r < 16 && (int64_t)tile * 16 + r < all; r += NW) {
@@ -560,9 +594,9 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
             *reinterpret_cast<f16x8*>(lds + (vp ^ 16) + p * THREADS * 32) = widen8((uint32_t)vr[p][2], (uint32_t)vr[p][3]);
         }
         if (threadIdx.x < 4) {
-            const float vu = can_read ? value_unit(su[1]) : 1.f, ok = can_read ? 1.f : 0.f;
+            const float vu = can_read ? su[1] : 1.f, ok = can_read ? 1.f : 0.f;
             *reinterpret_cast<fx4*>(units + stage * 20 + threadIdx.x * 4) =
-                fx4{can_read ? su[0] * a.scale : 0.f, __builtin_amdgcn_logf(vu), kWeight / vu, ok};
+                fx4{can_read ? su[0] * a.scale : 0.f, scale_log(vu), 1.0f / vu, ok};
             units[stage * 20 + 16 + threadIdx.x] = ok;
         }
     };
@@ -592,7 +626,8 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
                 if (F32) qf[PIECES - 1][s][j] = (half_t)(y - (float)hi);
             }
     }
-    float m = -INFINITY, l = 0.f;
+    float m = kNone, l = 0.f;  // m the row's, l the lane's
+    float ex = kUnseen;
     fx16 o[DB];
 #pragma unroll
     for (int c = 0; c < DB; ++c)
@@ -602,7 +637,7 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
     auto attend = [&](int tb, int stage, bool masked) {
         const int ka = kget + stage * STAGE, va = vget + stage * STAGE;
         fx16 x[2];
-        float ku[2], lv[2], iv[2], mx = -INFINITY;
+        float ku[2], lv[2], iv[2], top[2], mx = -INFINITY;
         // operands are read in groups, one group ahead of its MFMAs
         constexpr int GK = STEPS < 4 || D > 128 || (D == 128 && F32) ? 2 : 4, GV = GK, GROUPS = 2 * STEPS / GK;
         f16x8 kf[2][GK], vf[2][GV];
@@ -645,29 +680,44 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
             // key tb + 32 kb + 16 h + r is in x[kb][r]
             if (masked) {
                 const int j = tb + 32 * kb, low = a.window > 0 ? posh - a.window : INT_MIN;
-                const int top = un[3] != 0.f ? posh : INT_MIN;
+                const int up = un[3] != 0.f ? posh : INT_MIN;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const float y = x[kb][r];
-                    x[kb][r] = j + r <= top && j + r > low ? y : -INFINITY;
+                    x[kb][r] = j + r <= up && j + r > low ? y : -INFINITY;
                 }
                 // a row that sees none of the 16: their scales are not its own
-                if (!(j <= top && j + 15 > low)) ku[kb] = 1.f, lv[kb] = 0.f, iv[kb] = 0.f;
+                if (!(j <= up && j + 15 > low)) ku[kb] = 1.f, lv[kb] = 0.f, iv[kb] = 0.f;
             }
-            float top = -INFINITY;
+            top[kb] = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, x[kb][r]);
-            mx = fmaxf(mx, fmaf(top, ku[kb], lv[kb]));
+            for (int r = 0; r < 16; ++r) top[kb] = fmaxf(top[kb], x[kb][r]);
+            mx = fmaxf(mx, fmaf(top[kb], ku[kb], lv[kb]));
         }
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        if (__any(mx > m + kSlack)) {
-            const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= alpha;
+        float factor[2] = {ldexpf(iv[0], (int)ex), ldexpf(iv[1], (int)ex)};
+        if (__any(mx > m + kSlack || fmaxf(factor[0], factor[1]) > kMostFactor)) {
+            const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - mn);
+            const float en = exponent(mn, fmaxf(reference(m, ex), fmaxf(top[0] * ku[0], top[1] * ku[1])));
+            l *= rescale(m, ex, mn, en);
+            m = mn, ex = en;
 #pragma unroll
             for (int c = 0; c < DB; ++c) o[c] *= alpha;
+            factor[0] = ldexpf(iv[0], (int)ex), factor[1] = ldexpf(iv[1], (int)ex);
+            if (__any(fmaxf(factor[0], factor[1]) > kMostFactor)) {
+                const float base = reference(m, ex);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float s = x[kb][r];
+                        l += __builtin_amdgcn_exp2f(fmaf(s, ku[kb], -base));
+                    }
+                    factor[kb] = 0.f;
+                }
+            }
         }
-        const float base = m == -INFINITY ? 0.f : m - kPLog;
+        const float base = m - kPLog;
         f16x8 pf[PIECES][2][2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
@@ -689,7 +739,7 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
                     pf[PIECES - 1][kb][r / 8][r % 8] = lo[0], pf[PIECES - 1][kb][r / 8][r % 8 + 1] = lo[1];
                 }
             }
-            l = fmaf(sum, iv[kb], l);
+            l = fmaf(sum, factor[kb], l);
         }
 #pragma unroll
         for (int n = 0; n < DB * 4 / GV; ++n) {
@@ -724,6 +774,8 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
         attend(tb, stage, !whole || !__all(ok[0] * ok[1] * ok[2] * ok[3] != 0.f));
     }
 
+    const float er = fminf(ex, __shfl_xor(ex, 32));
+    l = ldexpf(l, (int)(er - ex));
     l += __shfl_xor(l, 32);
     if (!row_ok) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -734,7 +786,7 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
         for (int q = 0; q < 4; ++q) {
             T v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (T)(o[c][4 * q + r] * kWeight * inv);
+            for (int r = 0; r < 4; ++r) v[r] = (T)ldexpf(o[c][4 * q + r] * inv, (int)er);
             __builtin_memcpy(__builtin_assume_aligned(op + 32 * c + 8 * q, 4 * sizeof(T)), v, sizeof v);
         }
 }

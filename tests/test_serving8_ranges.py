@@ -39,3 +39,100 @@ def test_windows_of_any_size_with_rows_without_a_position(heads, kv, rows, windo
     good as none."""
     rng = np.random.default_rng(heads)
     run_attention(dev, rng, [5, 2, 40], rows, heads, kv, 64, 16, t, window=window, garbage=True, tile=128 if heads == 128 else None)
+
+
+# ---------------------------------------------------------------------------
+# value scales
+# ---------------------------------------------------------------------------
+
+# name: scales (powers of two) of a sequence's pages in turn, None a page of zeros
+SCALES = {
+    "zeros among 2^90": [90, None],
+    "zeros among 2^114": [114, None, None, 113],
+    "zeros among 2^-100": [-100, None],
+    "zeros among the smallest": [-107, None, -106],
+    "zeros and both ends": [100, None, -107, 0],
+    "zeros alone": [None],
+    "zeros first": [None, None, None, None, None, -3],
+    "the smallest first": [-107, -107, -107, -107, -107, 110],
+    "the largest first": [110, -107, -107, -107, -107, -107],
+    "a step up each page": list(range(-100, 110, 15)),
+    "a step down each page": list(range(110, -100, -15)),
+    "far apart in turn": [-60, 60, -20, 100, -100],
+}
+
+
+# and such as float16 outputs can hold
+SCALES16 = {"zeros among 2^7": [7, None], "zeros first": [None, None, None, None, None, -3], "the smallest first": [-107] * 5 + [7],
+            "far apart in turn": [-60, 7, -20, -100], "zeros alone": [None]}
+
+
+def far_bound(out, dim, about, t):
+    """Scales far from 1: the logarithm of a scale under 2^128 is off by its
+    last bit (2^-17), its sum with the scores and the maximum by half of one
+    each; a weight by ln 2 times that, and the divisor's weights need not be off
+    alike. A row whose weight is all on a page of zeros may have a result below
+    float32's smallest step, 2^-149: it is rounded to a whole number of them."""
+    size = about[0]
+    return s8.attention_bound(t, dim, out, *about) + 2 * 0.6932 * 2.0 ** -16 * size + 2.0 ** -150
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sharp", [0.0, 0.3, 4.0, 60.0])
+@pytest.mark.parametrize("name,t", [(n, F32) for n in SCALES] + [(n, F16) for n in SCALES16])
+@pytest.mark.parametrize("rows,heads,kv,dim,length", [(1, 2, 1, 32, 9000), (1, 8, 2, 64, 700), (3, 4, 2, 256, 700), (700, 64, 1, 32, 700),
+                                                      (200, 128, 32, 64, 300)])
+def test_attention_over_pages_of_any_scale(rows, heads, kv, dim, length, name, t, sharp, dev):  # noqa: F811
+    """Pages whose value scales lie anywhere from 2^-107 up, with pages of
+    zeros among them: each key has its weight in the divisor however small its
+    page's values are beside another's. Flat scores, and such as pick a page."""
+    powers = (SCALES if t == F32 else SCALES16)[name]
+    rng = np.random.default_rng(rows + dim)
+    page = 16
+    table, pages = tables(rng, [length], page)
+    cache = s8.Cache(rng, pages, kv, page, dim, table)
+    for slot, p in enumerate(table[0]):
+        power = powers[slot % len(powers)]
+        if power is None:
+            cache.vs[p] = 0
+            if slot % 3:  # values are whole numbers times 0 either way
+                cache.v[p] = 0
+        else:
+            cache.vs[p] = (rng.uniform(1, 2, kv) * 2.0 ** power).astype(F32)
+    starts = np.array([0, rows], I32)
+    q = (rng.standard_normal((rows, heads * dim)) * sharp).astype(t)
+    scale = F32(dim ** -0.5)
+    d = dev({"q": q, **cache_arrays(cache, starts, [length]), "out": np.full((rows, heads * dim), 7, t)})
+    d.call("nnc_hip_kv_attention", "q", *CACHE, "starts", "lengths", "out", 0, heads, float(scale), 0, 0)
+    got = d.get("out").astype(np.float64)
+    some = slice(None) if rows < 50 else slice(0, heads, 9)  # every head's answer has the same code
+    shown = np.arange(rows) if rows < 50 else np.unique(np.linspace(0, rows - 1, 40).astype(int))
+    out, about = attention_of(q.reshape(rows, heads, dim), cache, length, scale, shown, some)
+    bound = far_bound(out, dim, about, t)
+    off = np.abs(got.reshape(rows, heads, dim)[shown][:, some] - out)
+    bad = ~(off <= bound)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4].tolist(), off[bad][:4], out[bad][:4])
+
+
+def attention_of(q, cache, length, scale, shown, some):
+    """serving8.attention for some rows and heads of one sequence whose rows
+    are all `length` positions' last: out and what its bound needs."""
+    rows, heads, dim = q.shape
+    group = heads // cache.kv
+    k, v, u, _ = cache.values(0, length)
+    pos = length - rows + shown
+    see = np.arange(length) <= pos[:, None]
+    hs = np.arange(heads)[some]
+    out, size = np.zeros((2, len(shown), len(hs), dim))
+    reach, seen, peak = np.zeros((3, len(shown), len(hs)))
+    for i, h in enumerate(hs):
+        kk, vv, uu = k[h // group], v[h // group], u[h // group]
+        x = q[shown, h].astype(np.float64)
+        s = np.where(see, float(scale) * (x @ kk.T), -np.inf)
+        p = np.exp(s - s.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        out[:, i], size[:, i] = p @ vv, p @ np.abs(vv)
+        peak[:, i] = (p * uu).max(1)
+        reach[:, i] = np.where(see, float(scale) * (np.abs(x) @ np.abs(kk).T), 0).max(1)
+        seen[:, i] = see.sum(1)
+    return out, (size, reach, seen, peak)
