@@ -343,11 +343,11 @@ void nnc_hip_conv_packed_noalloc(Tensor* in, Tensor* w, Tensor* b, Tensor* res, 
  * nnc_hip_rms_norm: s = in (+ res), rounded to the activations' type;
  * y = s * w / sqrt(mean(s^2) + eps) over the last extent. `res` may be NULL;
  * `sum`, if not NULL, receives s (it may be the same buffer as `res` or
- * `in`); `out` may be the same as `in` if `sum` is not. weight: one row. out of in's type: y, scale NULL. out int8:
- * the product s * w, rounded to float32, is quantised row by row and `scale`
- * (one for each row) is its step u times 1 / sqrt(...), so the whole numbers
- * do not depend on the order of the sum of squares, which is float32's:
- * values up to 2^60 for rows of any length.
+ * `in`); `out` may be the same as `in` if `sum` is not. weight: one row. out of
+ * in's type: y, scale NULL. out int8: the product s * w, rounded to float32, is
+ * quantised row by row and `scale` (one for each row) is its step u times
+ * 1 / sqrt(...), so the whole numbers do not depend on the order of the sum of
+ * squares. That is float32's; values may be of any finite size.
  *
  * nnc_hip_quantize_rows / nnc_hip_dequantize_rows: rows (of the last extent)
  * to 8 bits with a scale each, and back: activations between an attention or

@@ -9,7 +9,9 @@
 //   whole number, scale = r * u                            (8-bit output)
 //
 // r cancels out of y / scale, so q does not depend on it: the whole numbers
-// are exactly defined whatever order the squares are summed in.
+// are exactly defined whatever order the squares are summed in. Where the sum of
+// squares passes the largest number (values over 2^49 at least), it is taken
+// once more of values 2^80 smaller, a sum under 2^126 for rows of 2^30.
 #include "quant8.h"
 
 namespace nnc {
@@ -28,6 +30,16 @@ struct RowArgs {
     float eps;
     bool nt;  // outputs of kNtStoreBytes or more
 };
+
+static constexpr float kSmaller = 0x1p-80f;
+
+// r, from the sum of squares of values 2^80 smaller if SMALLER
+template <bool SMALLER>
+__device__ __forceinline__ float inverse_root(float squares, int width, float eps) {
+    if (SMALLER) return kSmaller / sqrtf(squares / (float)width + eps * kSmaller * kSmaller);
+    return 1.0f / sqrtf(squares / (float)width + eps);
+}
+__device__ __forceinline__ bool too_large(float squares, int width, float eps) { return !(squares / (float)width + eps < INFINITY); }
 
 // A store of up to 16 bytes, non-temporal or not.
 template <typename P>
@@ -137,7 +149,27 @@ __global__ void __launch_bounds__(256) row_norm_reg_k(RowArgs a) {
             top = max_nan(max_nan(part[1][0], part[1][1]), max_nan(part[1][2], part[1][3]));
             __syncthreads();
         }
-        const float r = NORM ? 1.0f / sqrtf(sq / (float)a.width + a.eps) : 1.0f;
+        float r = NORM ? inverse_root<false>(sq, a.width, a.eps) : 1.0f;
+        if (NORM && too_large(sq, a.width, a.eps)) {
+            sq = 0.f;
+#pragma unroll
+            for (int q = 0; q < PER; ++q) {
+                const P v = __builtin_bit_cast(P, s[q]);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const float y = (float)v.v[e] * kSmaller;
+                    sq = fmaf(y, y, sq);
+                }
+            }
+            sq = wave_add(sq);
+            if constexpr (TPR == 256) {
+                if ((threadIdx.x & 63) == 0) part[0][threadIdx.x >> 6] = sq;
+                __syncthreads();
+                sq = (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]);
+                __syncthreads();
+            }
+            r = inverse_root<true>(sq, a.width, a.eps);
+        }
         const float unit = unit8(top), inverse = inverse8(unit);
         if (OUT == kRowsInt8 && lane == 0) a.scale[row] = r * unit;
 #pragma unroll
@@ -193,7 +225,22 @@ __global__ void __launch_bounds__(256) row_norm_k(RowArgs a) {
         sq = (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]);
         top = max_nan(max_nan(part[1][0], part[1][1]), max_nan(part[1][2], part[1][3]));
         __syncthreads();
-        const float r = NORM ? 1.0f / sqrtf(sq / (float)a.width + a.eps) : 1.0f;
+        float r = NORM ? inverse_root<false>(sq, a.width, a.eps) : 1.0f;
+        if (NORM && too_large(sq, a.width, a.eps)) {
+            sq = 0.f;
+            for (int i = threadIdx.x; i < a.width; i += 256) {
+                float s = (float)in[i];
+                if (res) s = (float)(T)(s + (float)res[i]);
+                s *= kSmaller;
+                sq = fmaf(s, s, sq);
+            }
+            sq = wave_add(sq);
+            if (lane == 0) part[0][wave] = sq;
+            __syncthreads();
+            sq = (part[0][0] + part[0][1]) + (part[0][2] + part[0][3]);
+            __syncthreads();
+            r = inverse_root<true>(sq, a.width, a.eps);
+        }
         const float unit = unit8(top), inverse = inverse8(unit);
         if (OUT == kRowsInt8 && threadIdx.x == 0) a.scale[row] = r * unit;
         for (int i = threadIdx.x; i < a.width; i += 256) {

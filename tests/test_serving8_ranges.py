@@ -10,8 +10,8 @@ import numpy as np
 import pytest
 
 import serving8 as s8
-from serving8 import F16, F32, I8, I32
-from test_serving8 import CACHE, cache_arrays, check_attention, dev, ragged, run_attention, tables  # noqa: F401 (dev: fixture)
+from serving8 import F16, F32, I32
+from test_serving8 import CACHE, cache_arrays, check_norm, dev, run_attention, tables  # noqa: F401 (dev: fixture)
 
 ROOT = Path(__file__).resolve().parent.parent
 
@@ -136,3 +136,46 @@ def attention_of(q, cache, length, scale, shown, some):
         reach[:, i] = np.where(see, float(scale) * (np.abs(x) @ np.abs(kk).T), 0).max(1)
         seen[:, i] = see.sum(1)
     return out, (size, reach, seen, peak)
+
+
+# ---------------------------------------------------------------------------
+# norms of large values
+# ---------------------------------------------------------------------------
+
+def large_rows(rng, rows, width, power):
+    """Rows around 2^power (one of ordinary size, one of zeros but for one
+    element), below the largest number with a residual of a quarter."""
+    x = rng.uniform(-1, 1, (rows, width)) * 2.0 ** power
+    res = rng.uniform(-0.25, 0.25, (rows, width)) * 2.0 ** power
+    if rows > 2:
+        x[1], res[1] = x[1] * 2.0 ** -power, res[1] * 2.0 ** -power
+        x[2], res[2] = 0, 0
+        x[2, width // 2] = 2.0 ** power
+    return x.astype(F32), res.astype(F32), rng.uniform(0.1, 0.5, width).astype(F32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [55, 60, 64, 90, 126, 127])
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("rows,width", [(1, 1), (3, 256), (5, 4096), (4, 1345), (3, 8192), (3, 8200), (2, 40000), (4100, 64),
+                                        (4100, 500), (4097, 1000)])
+def test_rms_norm_of_large_values(rows, width, int8, power, dev):  # noqa: F811
+    """Squares that pass the largest float32 number: the root is finite and
+    every output has its value, in the kernel of each width and row count."""
+    rng = np.random.default_rng(rows + width + power)
+    x, res, w = large_rows(rng, rows, width, power)
+    check_norm(dev, x, None, w, int8)
+    check_norm(dev, x, res, w, int8, alias=rows > 4000)
+    if rows < 10:
+        check_norm(dev, x, res, w, int8, shift={"x": 4})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eps", [3e38, 1e30, 1e-30, 1e-38])
+def test_rms_norm_of_any_epsilon(eps, dev):  # noqa: F811
+    rng = np.random.default_rng(1)
+    eps = float(F32(eps))
+    for power in (-40, 0, 62, 127):
+        x, res, w = large_rows(rng, 4, 700, power)
+        for int8 in (False, True):
+            check_norm(dev, x, res, w, int8, eps=eps)
