@@ -346,11 +346,11 @@ static bool quads(const KvArgs& a) {
     return true;
 }
 
-template <typename T, int TPG, typename Kernel>
-static void launch_quads(const char* name, Kernel kernel, const KvArgs& a) {
+template <typename T, int TPG, void (*kernel)(KvArgs)>
+static void launch_quads(const char* name, const KvArgs& a) {
     typedef Quads<T, TPG> Q;
     const size_t lds = (size_t)Q::GROUPS * a.dim * (a.g.page + 4);
-    if (TPG == 1024) {  // the largest pages: 66560 bytes
+    if constexpr (TPG == 1024) {  // the largest pages: 66560 bytes, allowed once for each kernel
         static const bool ok = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 256 * 260) == hipSuccess;
         if (!ok) return fail(NNC_HIP_EDEVICE, name, "hipFuncSetAttribute failed");
     }
@@ -372,14 +372,14 @@ static void launch_write(const char* name, const KvArgs& a) {
     const int n = a.g.page * a.dim * (int)sizeof(T) / 64;
     if (!quads<T>(a))
         return launch(name, kv_write_k<T>, dim3((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)a.kv_heads), dim3(256), 0, a);
-    if (n <= 64) return launch_quads<T, 64>(name, kv_write_quads_k<T, 64, 1>, a);
-    if (n <= 256) return launch_quads<T, 256>(name, kv_write_quads_k<T, 256, 1>, a);
-    if (n <= 512) return launch_quads<T, 256>(name, kv_write_quads_k<T, 256, 2>, a);
-    if (n <= 1024) return launch_quads<T, 256>(name, kv_write_quads_k<T, 256, 4>, a);
+    if (n <= 64) return launch_quads<T, 64, kv_write_quads_k<T, 64, 1>>(name, a);
+    if (n <= 256) return launch_quads<T, 256, kv_write_quads_k<T, 256, 1>>(name, a);
+    if (n <= 512) return launch_quads<T, 256, kv_write_quads_k<T, 256, 2>>(name, a);
+    if (n <= 1024) return launch_quads<T, 256, kv_write_quads_k<T, 256, 4>>(name, a);
     if constexpr (sizeof(T) == 4) {
-        if (n > 2048) return launch_quads<T, 1024>(name, kv_write_quads_k<T, 1024, 4>, a);
+        if (n > 2048) return launch_quads<T, 1024, kv_write_quads_k<T, 1024, 4>>(name, a);
     }
-    launch_quads<T, 1024>(name, kv_write_quads_k<T, 1024, 2>, a);
+    launch_quads<T, 1024, kv_write_quads_k<T, 1024, 2>>(name, a);
 }
 
 template <typename T>
@@ -387,9 +387,9 @@ static void launch_read(const char* name, const KvArgs& a) {
     const int n = a.g.page * a.dim * (int)sizeof(T) / 64;
     if (!quads<T>(a))
         return launch(name, kv_read_k<T>, dim3((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)a.kv_heads), dim3(256), 0, a);
-    if (n <= 64) return launch_quads<T, 64>(name, kv_read_quads_k<T, 64>, a);
-    if (n <= 1024) return launch_quads<T, 256>(name, kv_read_quads_k<T, 256>, a);
-    launch_quads<T, 1024>(name, kv_read_quads_k<T, 1024>, a);
+    if (n <= 64) return launch_quads<T, 64, kv_read_quads_k<T, 64>>(name, a);
+    if (n <= 1024) return launch_quads<T, 256, kv_read_quads_k<T, 256>>(name, a);
+    launch_quads<T, 1024, kv_read_quads_k<T, 1024>>(name, a);
 }
 
 static bool kv_args(const char* name, Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale,

@@ -4,6 +4,7 @@ index arithmetic of ragged batches with any numbers in the device arrays."""
 from __future__ import annotations
 
 import ctypes
+import re
 import subprocess
 from pathlib import Path
 
@@ -153,3 +154,16 @@ def test_kv_attention_refusals(lib):
         ("output rows", {"out": t(F32, 8, 256)}, EINVAL), ("output shape", {"out": t(F32, 7 * 256)}, EINVAL), ("window", {"window": -1}, EINVAL),
         ("max_length", {"max_length": -1}, EINVAL), ("scale", {"scale": 0.0}, EINVAL), ("scale", {"scale": float("inf")}, EINVAL),
         ("scale", {"scale": float("nan")}, EINVAL), ("unaligned", {"out": t(F32, 7, 256, data=4100)}, EUNSUPP)])
+
+
+def test_every_kernel_with_large_lds_raises_its_own_limit(pkg):
+    """The limit of dynamic LDS belongs to a kernel: each one that is launched
+    with more than 64 KB (pages of 256 positions by 256) has a flag of its own
+    for having raised it."""
+    from nnc_py_amd import runtime
+    names = subprocess.run(["nm", str(runtime.LIB_PATH)], check=True, capture_output=True, text=True).stdout.split()
+    kernels = {n.removeprefix("_ZN3nnc") for n in names if re.fullmatch(r"_ZN3nnc\d+kv_\w+_quads_k\w+Li1024E\w+", n)}
+    assert len(kernels) == 5
+    flags = [n for n in names if n.startswith("_ZGV") and "launch_quads" in n]
+    for k in kernels:
+        assert any(k in f for f in flags), k
