@@ -299,6 +299,12 @@ __global__ void __launch_bounds__(256) pack8_k(Pack8Args p) {
     }
 }
 
+// The operation's work, for the launch that does it (an operand laid out again
+// first is a launch of its own, with its bytes).
+static void set_product_work(const Gemm8Args& p, size_t out_bytes) {
+    set_work(2.0 * p.m * p.n * p.k, (double)p.m * p.k + (double)p.n * p.k + (double)p.m * p.n * out_bytes);
+}
+
 template <class L, typename T>
 static void launch_tile8(const char* name, Gemm8Args p, int splits) {
     auto kernel = gemm8_tile_k<L, T>;
@@ -320,12 +326,14 @@ static void launch_tile8(const char* name, Gemm8Args p, int splits) {
         ws += sums;
         if (pack_a || pack_w) {
             Pack8Args q{{p.a, p.w}, {(int8_t*)ws, (int8_t*)ws + (pack_a ? p.m * k16 : 0)}, {pack_a ? p.m : 0, pack_w ? p.n : 0}, p.k, k16};
+            set_work(0.0, (double)(q.rows[0] + q.rows[1]) * (p.k + k16));
             launch("nnc_hip_matmul_i8_pack", pack8_k, dim3(grid_for((q.rows[0] + q.rows[1]) * (k16 / 16), 1)), dim3(256), 0, q);
             if (pack_a) p.a = q.to[0];
             if (pack_w) p.w = q.to[1];
-            p.k = k16;
         }
     }
+    set_product_work(p, sizeof(T));
+    if (pack_a || pack_w) p.k = k16;
     launch(name, kernel, dim3((unsigned)(tm * tn * sp.splits)), dim3(L::THREADS), L::LDS, p, sp);
 }
 
@@ -390,6 +398,7 @@ __global__ void __launch_bounds__(64 * NW) gemm8_rows_k(Gemm8Args p) {
 template <int MT, int NW, typename T>
 static void launch_rows8(const char* name, const Gemm8Args& p, bool aligned) {
     const dim3 grid((unsigned)ceil_div(p.n, 16), (unsigned)ceil_div(p.m, 16 * MT));
+    set_product_work(p, sizeof(T));
     if (aligned)
         launch(name, gemm8_rows_k<MT, NW, T, true>, grid, dim3(64 * NW), 0, p);
     else
@@ -445,17 +454,19 @@ static Plan8 plan_gemm8(int64_t m, int64_t n, int64_t k, bool aligned) {
 }
 
 template <typename T>
-static void launch_gemm8(const char* name, const Gemm8Args& p) {
+static void launch_gemm8(const Gemm8Args& p) {
     const bool aligned = p.k % 16 == 0 && aligned16(p.a) && aligned16(p.w);
     const Plan8 plan = plan_gemm8(p.m, p.n, p.k, aligned);
     switch (plan.kernel) {
-        case 1: return launch_rows8<1, 8, T>(name, p, aligned);
-        case 2: return launch_rows8<2, 8, T>(name, p, aligned);
-        case 4: return launch_rows8<4, 8, T>(name, p, aligned);
-        case 64: return launch_tile8<Tile8<64, 64, 2, 2, 4, 4>, T>(name, p, plan.splits);
-        case 128: return launch_tile8<Tile8<128, 128, 2, 4, 4, 4>, T>(name, p, 1);
-        case 192: return launch_tile8<Tile8<256, 128, 4, 2, 3, 2>, T>(name, p, 1);
-        default: return launch_tile8<Tile8<256, 256, 2, 4, 2, 1>, T>(name, p, 1);
+        case 1: return launch_rows8<1, 8, T>("nnc_hip_matmul_i8_rows16", p, aligned);
+        case 2: return launch_rows8<2, 8, T>("nnc_hip_matmul_i8_rows32", p, aligned);
+        case 4: return launch_rows8<4, 8, T>("nnc_hip_matmul_i8_rows64", p, aligned);
+        case 64:
+            return launch_tile8<Tile8<64, 64, 2, 2, 4, 4>, T>(plan.splits > 1 ? "nnc_hip_matmul_i8_64x64_split" : "nnc_hip_matmul_i8_64x64", p,
+                                                              plan.splits);
+        case 128: return launch_tile8<Tile8<128, 128, 2, 4, 4, 4>, T>("nnc_hip_matmul_i8_128x128", p, 1);
+        case 192: return launch_tile8<Tile8<256, 128, 4, 2, 3, 2>, T>("nnc_hip_matmul_i8_256x128", p, 1);
+        default: return launch_tile8<Tile8<256, 256, 2, 4, 2, 1>, T>("nnc_hip_matmul_i8_256x256", p, 1);
     }
 }
 
@@ -491,11 +502,10 @@ void nnc_hip_matmul_i8(Tensor* a, Tensor* a_scale, Tensor* w, Tensor* w_scale, T
     Gemm8Args p{(const int8_t*)a->data, (const int8_t*)w->data, (const float*)a_scale->data, (const float*)w_scale->data,
                 bias ? (const float*)bias->data : nullptr, out->data, m, n, (int)k,
                 aligned16(out->data) && n * activation_bytes(out) % 16 == 0};
-    set_work(2.0 * m * n * k, (double)m * k + (double)n * k + (double)m * n * activation_bytes(out));
     if (out->dtype == NNC_DTYPE_FLOAT16)
-        launch_gemm8<half_t>(name, p);
+        launch_gemm8<half_t>(p);
     else
-        launch_gemm8<float>(name, p);
+        launch_gemm8<float>(p);
 }
 
 }  // extern "C"
