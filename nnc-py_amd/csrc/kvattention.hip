@@ -914,7 +914,9 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
         a.counters = tile_counters((size_t)items);
         if (!a.part || !a.counters) return fail(NNC_HIP_ENOMEM, name, "no workspace for %zu bytes of partial sums", bytes);
     }
-    set_work(0.0, 2.0 * c.kv_heads * c.dim * (double)longest * c.ragged.batch);
+    // every sequence taken as the longest; of it, what its rows' windows reach
+    const int64_t reach = a.window > 0 ? (int64_t)a.window - 1 + ceil_div(rows, c.ragged.batch) : longest;
+    set_work(0.0, 2.0 * c.kv_heads * c.dim * (double)(reach < longest ? reach : longest) * c.ragged.batch);
     if (q->dtype == NNC_DTYPE_FLOAT16)
         launch_dim<half_t>(name, a, tile, waves, c.dim);
     else

@@ -10,7 +10,7 @@ import pytest
 
 import serving8 as s8
 from serving8 import F16, F32, I8
-from test_serving8 import check_norm, check_product, dev, norm_inputs  # noqa: F401 (dev: fixture)
+from test_serving8 import check_norm, check_product, dev, norm_inputs, run_attention  # noqa: F401 (dev: fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -90,6 +90,14 @@ def test_matmul_i8_work_in_the_timing_table(size, dev):  # noqa: F811
     assert (pack is not None) == (k % 16 != 0)
     if pack:
         assert pack["flops"] == 0 and pack["bytes"] == (m + n) * (k + -(-k // 16) * 16)
+
+
+@pytest.mark.parametrize("window,rows,reach", [(0, 1, 4000), (1, 1, 1), (700, 1, 700), (700, 5, 704), (3999, 5, 4000), (2 ** 31 - 1, 1, 4000)])
+def test_kv_attention_work_in_the_timing_table(window, rows, reach, dev):  # noqa: F811
+    """The cache's bytes once: as far as the longest sequence or its window reaches."""
+    rng = np.random.default_rng(2)
+    table = ran(lambda: run_attention(dev, rng, [4000, 4000], [rows, rows], 4, 2, 64, 16, F16, window=window, max_length=4000, pad=0))
+    assert [r["bytes"] for r in table.values()] == [2.0 * 2 * 64 * reach * 2]
 
 
 # rows for every wave of the GPU and short ones (a wave a row: one, two and four
