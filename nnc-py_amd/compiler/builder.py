@@ -218,7 +218,7 @@ class GraphBuilder:
     def kv_attention(self, q, cache, table, starts, lengths, heads, q_col=0, scale=None, window=0, max_length=0, name=None,
                      out=None):
         dim = self.shape(cache[0])[3]
-        y = self._out(name or "kv_attention", tuple(self.shape(q)[:-1]) + (heads * dim,), name=out)
+        y = self._out(name or "kv_attention", tuple(self.shape(q)[:-1]) + (heads * dim,), self.g.tensors[q].dtype, name=out)
         self._node("KvAttention", [q, *cache, table, starts, lengths], [y], name, q_col=int(q_col), heads=int(heads),
                    scale=float(dim ** -0.5 if scale is None else scale), window=int(window), max_length=int(max_length))
         return y

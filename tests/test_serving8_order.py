@@ -217,3 +217,47 @@ def test_fusion_beside_a_cache_goes_on(pkg):
     b.output(b.sigmoid(b.add(m.attend(q), x)))
     calls = [c.op for c in build_program(b.build(), 3).calls]
     assert calls == ["nnc_add_relu", "nnc_hip_kv_write", "nnc_hip_kv_attention", "nnc_add_sigmoid"]
+
+
+def half_graph(pkg):
+    """Rows of a fused projection in float16: written, attended, normed."""
+    from nnc_py_amd.compiler.builder import GraphBuilder
+    b = GraphBuilder("half")
+    qkv = b.input("qkv", (ROWS, 3 * WIDTH), "float16")
+    cache = b.kv_cache("cache", PAGES, KV, PAGE, DIM)
+    place = [b.input("table", (1, 2), "int32"), b.input("starts", (2,), "int32"), b.input("lengths", (1,), "int32")]
+    b.kv_write(qkv, qkv, cache, *place, k_col=WIDTH, v_col=2 * WIDTH)
+    a = b.output(b.kv_attention(qkv, cache, *place, heads=KV))
+    b.output(b.rms_norm(a, b.const("w", np.ones(WIDTH, np.float16))))
+    return b.build()
+
+
+def test_attention_answers_in_the_queries_type(pkg):
+    g = half_graph(pkg)
+    assert [g.tensors[o].dtype for o in g.outputs] == ["float16", "float16"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("level", [0, 3])
+def test_a_half_precision_graph_on_the_device(level, hip, pkg):
+    import serving8 as s8
+    from nnc_py_amd import runtime
+    from nnc_py_amd.compiler.executor import Executor, build_program
+    runtime.clear_error()
+    ex = Executor(build_program(half_graph(pkg), level), True, hip)
+    rng = np.random.default_rng(3)
+    table, starts = np.array([[2, 0]], I32), np.array([0, ROWS], I32)
+    cache = s8.Cache(rng, PAGES, KV, PAGE, DIM, table, filled=False)
+    for n in range(1, 20):  # (the first call's row before the sequence has no position)
+        qkv = rng.standard_normal((ROWS, 3 * WIDTH)).astype(np.float16)
+        for name, a in (("qkv", qkv), ("table", table), ("starts", starts), ("lengths", np.array([n], I32))):
+            ex.set_input(name, a)
+        ex.run()
+        q, k, v = qkv.reshape(ROWS, 3, KV, DIM).transpose(1, 0, 2, 3)
+        cache.write(k, v, starts, [n])
+        out, about = s8.attention(q, cache, starts, [n], F32(DIM ** -0.5), 0)
+        a, y = (ex.get(o) for o in ex.prog.graph.outputs)
+        assert (np.abs(a.reshape(out.shape).astype(np.float64) - out) <= s8.attention_bound(np.float16, DIM, out, *about)).all()
+        want = s8.rms_norm(a, None, np.ones(WIDTH, np.float16), 1e-6)[3]
+        assert (np.abs(y.astype(np.float64) - want) <= s8.U16 * 1.01 * np.abs(want) + s8.SUB16).all()
+    assert runtime.last_error()[0] == 0
