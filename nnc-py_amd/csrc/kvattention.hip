@@ -318,7 +318,6 @@ __global__ void __launch_bounds__(64 * NW, D == 32 ? 4 : 1) kv_attention_k(KvAtt
         find(tb + STRIDE);
     }
     f16x8 qf[PIECES][STEPS];
-    float qs = a.scale;
     int e = 0;
     if (F32) {
         // the row's largest value to [2^13, 2^14)
@@ -329,7 +328,6 @@ __global__ void __launch_bounds__(64 * NW, D == 32 ? 4 : 1) kv_attention_k(KvAtt
         top = fmaxf(top, __shfl_xor(top, 32));
         (void)frexpf(top, &e);
         e = top > 0.f && top < INFINITY ? 14 - e : 0;
-        qs = ldexpf(qs, -e);
     }
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
@@ -363,7 +361,7 @@ __global__ void __launch_bounds__(64 * NW, D == 32 ? 4 : 1) kv_attention_k(KvAtt
             for (int r = 0; r < 4; ++r) x[4 * bl + r] = s[r];
         }
         load_k(tb + STRIDE);
-        float ku = ks * qs, lv = scale_log(vs), iv = 1.0f / vs;
+        float ku = F32 ? ldexpf(ks * a.scale, -e) : ks * a.scale, lv = scale_log(vs), iv = 1.0f / vs;
         ku = ku == 0.f ? 0x1p-126f : ku;  // for the product with -inf
         if (!(tb + 63 <= first_pos && (a.window <= 0 || tb > last_pos - a.window) && __all(have))) {
             const int j = tb + 16 * g, low = a.window > 0 ? pos - a.window : INT_MIN, up = have ? pos : INT_MIN;
@@ -603,10 +601,9 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
 
     // the query row
     f16x8 qf[PIECES][STEPS];
-    float qscale = 1.f;
+    int e = 0;
     {
         const T* qp = (const T*)a.q + (int64_t)row * a.ld + a.q_col + head * D + 8 * h;
-        int e = 0;
         if (F32) {
             float top = 0.f;
             for (int s = 0; s < STEPS; ++s)
@@ -614,7 +611,6 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
             top = fmaxf(top, __shfl_xor(top, 32));
             (void)frexpf(top, &e);
             e = top > 0.f && top < INFINITY ? 14 - e : 0;
-            qscale = ldexpf(1.f, -e);
         }
 #pragma unroll
         for (int s = 0; s < STEPS; ++s)
@@ -675,7 +671,7 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
                     }
             }
             const fx4 un = *reinterpret_cast<const fx4*>(units + stage * 20 + (2 * kb + h) * 4);
-            ku[kb] = un[0] * qscale, lv[kb] = un[1], iv[kb] = un[2];
+            ku[kb] = F32 ? ldexpf(un[0], -e) : un[0], lv[kb] = un[1], iv[kb] = un[2];
             ku[kb] = ku[kb] == 0.f ? 0x1p-126f : ku[kb];  // for the product with -inf
             // key tb + 32 kb + 16 h + r is in x[kb][r]
             if (masked) {

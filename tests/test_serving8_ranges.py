@@ -179,3 +179,29 @@ def test_rms_norm_of_any_epsilon(eps, dev):  # noqa: F811
         x, res, w = large_rows(rng, 4, 700, power)
         for int8 in (False, True):
             check_norm(dev, x, res, w, int8, eps=eps)
+
+
+# ---------------------------------------------------------------------------
+# query sizes
+# ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_power,k_power", [(-125, 126), (-120, 124), (-100, 97), (60, -60), (104, -105), (101, -104)])
+@pytest.mark.parametrize("rows,heads,kv", [(1, 4, 2), (200, 128, 32)])
+def test_queries_and_key_scales_far_from_one(rows, heads, kv, q_power, k_power, dev):  # noqa: F811
+    """Scores of ordinary size from queries and keys that are not."""
+    rng = np.random.default_rng(rows)
+    page, dim, length = 16, 64, 300
+    table, pages = tables(rng, [length], page)
+    cache = s8.Cache(rng, pages, kv, page, dim, table)
+    cache.ks = (rng.uniform(0.004, 0.02, cache.ks.shape) * 2.0 ** k_power).astype(F32)
+    starts = np.array([0, rows], I32)
+    q = (rng.standard_normal((rows, heads * dim)) * 2.0 ** q_power).astype(F32)
+    scale = F32(0.125)
+    d = dev({"q": q, **cache_arrays(cache, starts, [length]), "out": np.zeros((rows, heads * dim), F32)})
+    d.call("nnc_hip_kv_attention", "q", *CACHE, "starts", "lengths", "out", 0, heads, float(scale), 0, 0)
+    some = slice(None) if rows == 1 else slice(0, heads, 9)
+    shown = np.unique(np.linspace(0, rows - 1, 20).astype(int))
+    out, about = attention_of(q.reshape(rows, heads, dim), cache, length, scale, shown, some)
+    off = np.abs(d.get("out").reshape(rows, heads, dim)[shown][:, some].astype(np.float64) - out)
+    assert (off <= s8.attention_bound(F32, dim, out, *about)).all(), off.max()
