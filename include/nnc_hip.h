@@ -332,8 +332,11 @@ void nnc_hip_conv_packed_noalloc(Tensor* in, Tensor* w, Tensor* b, Tensor* res, 
  * counterpart in the reference ABI. Activations are float32 or float16, all
  * tensors of a call that hold activations of one type; 8-bit values are int8
  * whole numbers -127 .. 127 with float32 scales, value = whole number * scale.
- * Sums, statistics and scales are float32 or wider. Rows, heads, dims and
- * batches are any size (0: nothing happens) where no limit is named.
+ * Sums, statistics and scales are float32 or wider; attention's weights are
+ * rounded before they meet the values, to float16 for float16 outputs and to 22
+ * bits for float32 ones, whose queries have 22 bits of the row's largest.
+ * Rows, heads, dims and batches are any size (0: nothing happens) where no
+ * limit is named.
  *
  * To 8 bits: u = the largest absolute value / 127, rounded once; each whole
  * number is the nearest to x / u, ties to even. Largest value below 2^-100:
@@ -343,11 +346,12 @@ void nnc_hip_conv_packed_noalloc(Tensor* in, Tensor* w, Tensor* b, Tensor* res, 
  * nnc_hip_rms_norm: s = in (+ res), rounded to the activations' type;
  * y = s * w / sqrt(mean(s^2) + eps) over the last extent. `res` may be NULL;
  * `sum`, if not NULL, receives s (it may be the same buffer as `res` or
- * `in`); `out` may be the same as `in` if `sum` is not. weight: one row. out of
- * in's type: y, scale NULL. out int8: the product s * w, rounded to float32, is
- * quantised row by row and `scale` (one for each row) is its step u times
- * 1 / sqrt(...), so the whole numbers do not depend on the order of the sum of
- * squares. That is float32's; values may be of any finite size.
+ * `in`); `out` of in's type may be the same as `in` if `sum` is not. weight:
+ * one row. out of in's type: y, scale NULL. out int8: the product s * w,
+ * rounded to float32, is quantised row by row and `scale` (one for each row) is
+ * its step u times 1 / sqrt(...), so the whole numbers do not depend on the
+ * order of the sum of squares. That is float32's; values may be of any finite
+ * size.
  *
  * nnc_hip_quantize_rows / nnc_hip_dequantize_rows: rows (of the last extent)
  * to 8 bits with a scale each, and back: activations between an attention or
@@ -363,9 +367,9 @@ void nnc_hip_matmul_i8(Tensor* a, Tensor* a_scale, Tensor* w, Tensor* w_scale, T
 
 /* A paged cache: k_cache int8 [pages][kv_heads][page][dim], v_cache int8
  * [pages][kv_heads][dim][page], k_scale and v_scale float32 [pages][kv_heads];
- * page a multiple of 16 up to 256, dim 32, 64, 128 or 256, 16-byte aligned.
- * table int32 [batch][width]: position t of sequence b is in page
- * table[b][t / page]. starts int32 [batch + 1], lengths int32 [batch]:
+ * page a multiple of 16 up to 256, dim 32, 64, 128 or 256, kv_heads up to
+ * 32767, 16-byte aligned. table int32 [batch][width]: position t of sequence b
+ * is in page table[b][t / page]. starts int32 [batch + 1], lengths int32 [batch]:
  * sequence b's rows of the activations are starts[b] .. starts[b + 1] (never
  * decreasing), and they are its last positions, lengths[b] being its length
  * with them. table, starts and lengths are device memory, read when the call

@@ -51,7 +51,8 @@ bool cache_args(const char* name, Tensor* k_cache, Tensor* v_cache, Tensor* k_sc
     const int64_t page = ks[2], dim = ks[3];
     if (vs[0] != ks[0] || vs[1] != ks[1] || vs[2] != dim || vs[3] != page)
         return fail(NNC_HIP_EINVAL, name, "K must be [pages][heads][page][dim] and V [pages][heads][dim][page]"), false;
-    if (ks[0] < 1 || ks[1] < 1 || ks[0] > INT32_MAX || ks[1] > 65535)
+    // (a page's K and V of a head are rows of a grid of at most 65535)
+    if (ks[0] < 1 || ks[1] < 1 || ks[0] > INT32_MAX || ks[1] > 32767)
         return fail(NNC_HIP_EINVAL, name, "bad page or head count"), false;
     if (page < 16 || page > 256 || page % 16 != 0)
         return fail(NNC_HIP_EUNSUPP, name, "pages of %lld positions (a multiple of 16 up to 256)", (long long)page), false;

@@ -156,6 +156,18 @@ def test_kv_attention_refusals(lib):
         ("scale", {"scale": float("nan")}, EINVAL), ("unaligned", {"out": t(F32, 7, 256, data=4100)}, EUNSUPP)])
 
 
+def test_as_many_cached_heads_as_a_grid_has_rows_for(lib):
+    """K and V of a page and head are rows of a grid: 32767 heads at most."""
+    t = lib.t
+    for heads, code in ((32767, ESTATE), (32768, EINVAL)):
+        args = {**cache(lib, k_cache=t(I8, 1, heads, 256, 256), v_cache=t(I8, 1, heads, 256, 256), k_scale=t(F32, 1, heads),
+                        v_scale=t(F32, 1, heads))}
+        x = t(F16, 7, heads * 256)
+        assert lib.code("nnc_hip_kv_write", x, x, *args.values(), 0, 0) == code
+        assert lib.code("nnc_hip_kv_read", *args.values(), x, x, 0, 0) == code
+        assert lib.code("nnc_hip_kv_attention", x, *args.values(), x, 0, heads, 1.0, 0, 0) == code
+
+
 def test_every_kernel_with_large_lds_raises_its_own_limit(pkg):
     """The limit of dynamic LDS belongs to a kernel: each one that is launched
     with more than 64 KB (pages of 256 positions by 256) has a flag of its own
