@@ -129,3 +129,41 @@ def test_quantize_and_dequantize_kernels(rows, width, t, dev):  # noqa: F811
     np.testing.assert_array_equal(d.get("q"), q)
     d.call("nnc_hip_dequantize_rows", "q", "s", "y")
     np.testing.assert_array_equal(d.get("y"), (q.astype(F32) * unit[:, None]).astype(t))
+
+
+def test_captured_products_replayed(dev, hip):  # noqa: F811
+    """A norm to 8 bits and products that lay operands out, split k and take the
+    largest tiles, captured together (they share the workspace) and replayed
+    with other inputs, eager calls in between: the same bits as eager."""
+    from nnc_py_amd import runtime
+    rng = np.random.default_rng(5)
+    jobs = []
+    for m, n, k in ((200, 64, 2064), (300, 400, 513), (2048, 4096, 144), (4, 512, 256)):
+        w = rng.integers(-127, 128, (n, k)).astype(I8)
+        d = dev({"x": rng.standard_normal((m, k)).astype(F16), "one": np.ones(k, F16), "a": np.zeros((m, k), I8), "sa": np.zeros(m, F32),
+                 "w": w, "sw": rng.uniform(0.01, 0.02, n).astype(F32), "b": rng.standard_normal(n).astype(F32), "out": np.zeros((m, n), F16)})
+        jobs.append((d, (m, k)))
+
+    def calls(d):
+        hip.nnc_hip_rms_norm(d.t("x"), None, d.t("one"), None, d.t("a"), d.t("sa"), 1e-6)
+        hip.nnc_hip_matmul_i8(d.t("a"), d.t("sa"), d.t("w"), d.t("sw"), d.t("b"), d.t("out"))
+    for d, _ in jobs:  # the workspace has its size before the capture
+        calls(d)
+    runtime.sync()
+    runtime.check(hip.nnc_hip_graph_begin(), "begin")
+    for d, _ in jobs:
+        calls(d)
+    runtime.check(hip.nnc_hip_graph_end(), "end")
+    for i in range(5):
+        for d, shape in jobs:
+            d.set("x", (rng.standard_normal(shape) * (i + 1)).astype(F16))
+        runtime.check(hip.nnc_hip_graph_launch(), "launch")
+        runtime.sync()
+        got = [d.get("out") for d, _ in jobs]
+        for (d, _), replayed in zip(jobs, got):
+            assert replayed.any()
+            calls(d)
+            runtime.sync()
+            np.testing.assert_array_equal(d.get("out"), replayed)
+    assert runtime.last_error()[0] == 0
+    hip.nnc_hip_graph_destroy()

@@ -11,7 +11,7 @@ import pytest
 
 import serving8 as s8
 from serving8 import F16, F32, I32
-from test_serving8 import CACHE, cache_arrays, check_norm, dev, run_attention, tables  # noqa: F401 (dev: fixture)
+from test_serving8 import CACHE, cache_arrays, check_attention, check_norm, dev, run_attention, tables  # noqa: F401 (dev: fixture)
 
 ROOT = Path(__file__).resolve().parent.parent
 
@@ -205,3 +205,64 @@ def test_queries_and_key_scales_far_from_one(rows, heads, kv, q_power, k_power, 
     out, about = attention_of(q.reshape(rows, heads, dim), cache, length, scale, shown, some)
     off = np.abs(d.get("out").reshape(rows, heads, dim)[shown][:, some].astype(np.float64) - out)
     assert (off <= s8.attention_bound(F32, dim, out, *about)).all(), off.max()
+
+
+# ---------------------------------------------------------------------------
+# caches of more than 4 GiB
+# ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("lengths,rows,heads", [([40, 17, 33], [40, 1, 2], 16), ([300, 250], [250, 250], 64)])
+def test_pages_behind_four_gib(lengths, rows, heads, t, hip, abi):
+    """Pages at the far end of a cache: written, read back and attended to, by
+    both attention kernels, as by a small cache that holds them alone."""
+    from nnc_py_amd import runtime
+    runtime.clear_error()
+    kv, page, dim, pages = 8, 16, 128, 280000
+    assert pages * kv * page * dim > 2 ** 32
+    rng = np.random.default_rng(len(lengths))
+    table, used = tables(rng, lengths, page, extra=0)
+    small = s8.Cache(rng, used, kv, page, dim, table, filled=False)
+    far = np.concatenate([np.arange(pages - used + 1, pages), [0]]).astype(I32)  # the small cache's page -> the large one's
+    far_table = np.where(table < used, far[np.minimum(table, used - 1)], table).astype(I32)
+    starts = np.concatenate([[0], np.cumsum(rows)]).astype(I32)
+    total = int(starts[-1])
+    x = rng.standard_normal((total, (heads + 2 * kv) * dim)).astype(t)
+    d = s8.Dev(hip, abi, runtime, {"x": x, "table": far_table, "starts": starts, "lengths": np.array(lengths, I32),
+                                   "k_scale": np.zeros((pages, kv), F32), "v_scale": np.zeros((pages, kv), F32),
+                                   "kr": np.zeros((total, kv * dim), t), "vr": np.zeros((total, kv * dim), t),
+                                   "out": np.zeros((total, heads * dim), t)})
+    big = [runtime.DeviceBuffer.empty((pages, kv, *s), np.int8) for s in ((page, dim), (dim, page))]
+    try:
+        for name, b in zip(("k_cache", "v_cache"), big):
+            d.desc[name], shape = b.tensor()
+            d.kept.append(shape)
+        before = [n - min(n, r) for n, r in zip(lengths, rows)]
+        if any(before):  # the positions before the rows
+            b_starts = np.concatenate([[0], np.cumsum(before)]).astype(I32)
+            y = rng.standard_normal((int(b_starts[-1]), 2 * kv * dim)).astype(t)
+            e = s8.Dev(hip, abi, runtime, {"x": y, "starts": b_starts, "lengths": np.array(before, I32)})
+            args = [d.t(n) for n in CACHE]
+            hip.nnc_hip_kv_write(e.t("x"), e.t("x"), *args, e.t("starts"), e.t("lengths"), 0, kv * dim)
+            runtime.sync()
+            small.write(y[:, :kv * dim].reshape(-1, kv, dim), y[:, kv * dim:].reshape(-1, kv, dim), b_starts, before)
+            e.free()
+        k_col, v_col = heads * dim, (heads + kv) * dim
+        d.call("nnc_hip_kv_write", "x", "x", *CACHE, "starts", "lengths", k_col, v_col)
+        parts = x.reshape(total, heads + 2 * kv, dim)
+        small.write(parts[:, heads:heads + kv], parts[:, heads + kv:], starts, lengths)
+        d.call("nnc_hip_kv_read", *CACHE, "starts", "lengths", "kr", "vr", 0, 0)
+        kr, vr = (d.get(n).reshape(total, kv, dim) for n in ("kr", "vr"))
+        for b, n in enumerate(lengths):
+            for i in range(max(0, rows[b] - n), rows[b]):
+                pos = n - rows[b] + i
+                p = small.page_of(b, pos)
+                np.testing.assert_array_equal(kr[starts[b] + i], (small.k[p, :, pos % page].astype(F32) * small.ks[p][:, None]).astype(t))
+                np.testing.assert_array_equal(vr[starts[b] + i], (small.v[p, :, :, pos % page].astype(F32) * small.vs[p][:, None]).astype(t))
+        d.call("nnc_hip_kv_attention", "x", *CACHE, "starts", "lengths", "out", 0, heads, float(F32(dim ** -0.5)), 0, 0)
+        check_attention(d.get("out"), parts[:, :heads], small, starts, lengths, F32(dim ** -0.5), 0)
+    finally:
+        d.free()
+        for b in big:
+            b.free()
