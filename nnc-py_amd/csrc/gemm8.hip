@@ -5,9 +5,10 @@
 // The sum is exact (32-bit integers: K up to 131071); the scales, the bias
 // and the output's rounding follow in 32 bits. No reference counterpart.
 //
-// [8192,4096]x[4096,4096] to f16 130 us, 2.11 POPS (a library's product of the
-// same operands to 32-bit integers 133 us); 8 rows 6.0 us, of which the
-// weights' 16.8 MB are 3.2 at a copy's rate.
+// [8192,4096]x[4096,4096] to f16 130 to 135 us from card to card, 2.04 to 2.11
+// POPS (a library's product of the same operands to 32-bit integers 133 us on
+// one of them); 8 rows 6.0 us, of which the weights' 16.8 MB are 3.2 at a
+// copy's rate.
 //
 // v_mfma_i32_16x16x64_i8 (few rows): lane (i = lane % 16, g = lane / 16) holds
 // 16 k of row i of either operand; the k order is the same in both, so it does
@@ -56,7 +57,7 @@ __device__ __forceinline__ ix4 row_chunk(const int8_t* row, int k, int K) {
 // gets an offset past the buffer (zeros). Other operands are laid out so
 // first (pack8_k): chunks through registers instead took 107 us for
 // [2048,4001]x[4096,4001], 96 with 128 x 128 tiles, unaligned loads being
-// split up; with the layout 59.
+// split up; with the layout 54.
 //
 // An LDS row is 128 k of one row of a or w, its 16-byte chunk c at position
 // c ^ (row / 2 % 8): LDS has 64 banks, and 16 lanes reading a chunk of 16 rows
@@ -412,11 +413,12 @@ static void launch_rows8(const char* name, const Gemm8Args& p, bool aligned) {
 // round of workgroups; joining splits costs 1.5 us and 16 ns for every partial
 // tile written and read back; laying operands out for the tiles costs a launch
 // and their bytes. Against the neighbours, us: [64,4096]x[4096,4096] rows
-// 13.0, 64 x 64 tiles 10.7, in two splits 9.8; [64,14336]x[4096,14336] rows
-// 34.5, tiles 27.7, in four splits 14.5; [1024,4096]x[4096,4096] tiles of 64
-// 34.7, 128 24.8, 256 x 128 33.3, 256 48; with 8192 rows 225, 190, 158 and 133
-// (2.06 POPS; the stages' LDS conflicts gone that is 59% of the MFMA's cycles,
-// the rest waits for the next slice: one workgroup per CU, two stages).
+// 12.2, 64 x 64 tiles 10.6, in two splits 9.6; [64,14336]x[4096,14336] rows
+// 34.4, tiles 27.9, in four splits 14.7; [512,4096]x[4096,4096] tiles of 64 16.2
+// (14.4 by the rule), 128 19.1; [1024,4096]x[4096,4096] tiles of 64 31.9, 128 24.3, 256 x 128 30.1,
+// 256 47.9; with 8192 rows 227, 179, 154 and 130 (the matrix units busy 61% of
+// the cycles, the rest waits for the next slice: one workgroup per CU, two
+// stages).
 struct Plan8 {
     int kernel = 0, splits = 1;
     double us = 1e30;

@@ -33,8 +33,8 @@
 // joined through LDS, the shares' through the workspace. The cache's bytes
 // bound it: 64 sequences of up to 8192 positions (32 heads over 8 of 128) 105 us,
 // 552 MB at 5.2 TB/s, as a large copy (in the batch's own order, whose longest
-// ended last, 130); one of 131072 54.2 us, 4.95 TB/s. A short call is a chain of dependent
-// loads (lengths, table, page) and joins, 7.2 us for four of 333.
+// ended last, 130); one of 131072 54.6 us, 4.9 TB/s. A short call is a chain of
+// dependent loads (lengths, table, page) and joins, 7.4 us for four of 333.
 #include <limits.h>
 
 #include "mfma_tile.h"
@@ -483,10 +483,10 @@ __global__ void __launch_bounds__(64 * NW, D == 32 ? 4 : 1) kv_attention_k(KvAtt
 // ---------------------------------------------------------------------------
 // Many query rows (prompts): 32 rows per wave, 4 or 8 waves, the keys 64 at a
 // time through LDS, where they are kept as f16: widened once for all waves.
-// Two prompts of 2048 rows behind 2048 positions, 32 heads over 8 of 128: 236
-// us, 873 TFLOP/s of the 1334 that a large f16 product reaches. The matrix units
+// Two prompts of 2048 rows behind 2048 positions, 32 heads over 8 of 128: 240
+// us, 860 TFLOP/s of the 1334 that a large f16 product reaches. The matrix units
 // are busy for 40% of the cycles and the vector units, with masks, exponentials
-// and conversions, for 58%; the two overlap only in part.
+// and conversions, for 59%; the two overlap only in part.
 // v_mfma_f32_32x32x16_f16 as above; query row i = lane % 32, lane half h. Row 8q + 4h + u of a block of 32 keys is key 16h + 4q + u: lane half h
 // has the scores of 16 consecutive keys, which one page's scales serve.
 //
@@ -824,10 +824,11 @@ static void launch_dim(const char* name, const KvAttnArgs& a, int tile, int wave
 // which divides the keys instead. By the time that a CU takes for 64 keys,
 // dim 128, in us: 256 rows 2.5, 128 rows 1.9, two workgroups of them 3.0,
 // 256 rows as 16 tiles of 16 6.1. With 256, 128 and 16 rows, us, 32 heads over 8
-// of 128, f16: two prompts of 2048 behind 2048 243, 292, 595; 16 of 1024 248, 256,
-// 554; four of 256 behind 1792 74, 71, 115; one of 256 behind 7936 261, 243, 101;
-// one of 256 18, 16, 11; 64 of 16 behind 1008 83, 55, 85, of 4 behind 4092 307,
-// 201, 99.
+// of 128, f16: two prompts of 2048 behind 2048 241, 285, 592; 16 of 1024 256, 253,
+// 523; four of 256 behind 1792 76, 68, 101; one of 256 behind 7936 264, 242, 92;
+// one of 256 17, 15, 10; 64 of 16 behind 1008 79, 52, 85, of 4 behind 4092 298,
+// 192, 99. fp32: two of 2048 375, 426, 643; 16 of 1024 374, 373, 630; four of 256
+// 107, 89, 120; one of 256 behind 7936 372, 311, 106.
 static int query_tile(int64_t rows, int64_t batch, int group, int kv_heads, int dim) {
     const int64_t cus = cu_count(), holders = rows < batch ? rows : batch;  // sequences that can have rows
     auto count = [&](int tile) {
@@ -845,10 +846,10 @@ static int query_tile(int64_t rows, int64_t batch, int group, int kv_heads, int 
 // there can be. In several rounds, fewer waves leave room for other
 // workgroups on the CU, whose keys arrive while one starts or joins; more
 // have a long sequence done sooner. 8, 4 and 2 waves, us, 32 heads over 8 of
-// 128, f16: 64 sequences of up to 8192 107, 113, 128; 64 of 4096 99, 96, 101;
-// 64 of up to 1024 25, 21, 22; 128 of up to 4096 110, 100, 114; 128 of up to 512
-// 37, 25, 20; 256 of up to 1024 97, 66, 54; 512 of up to 4096 425, 381, 400; 512
-// of up to 300, 8 heads of 64, fp32 117, 51, 35.
+// 128, f16: 64 sequences of up to 8192 106, 112, 127; 64 of 4096 100, 97, 101;
+// 64 of up to 1024 25, 20, 22; 128 of up to 4096 114, 102, 117; 128 of up to 512
+// 38, 25, 20; 256 of up to 1024 99, 66, 53; 512 of up to 4096 448, 403, 423; 512
+// of up to 300, 8 heads of 64, fp32 121, 50, 34.
 static int query_waves(int64_t items, int longest) {
     const double rounds = (double)items / cu_count();
     if (rounds <= 1.0 || longest > 2048 * rounds) return 8;
@@ -897,7 +898,9 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
     if (tile == 16) {
         // shares of the keys, 512 or more each, while all workgroups run at
         // once, one on a CU (a second round starts 6 us later: one sequence of
-        // 131072 in 32 shares 54.6 us, in 64 61)
+        // 131072 in 32 shares 48.2 us, in 64 54.9, call after call on one cache).
+        // By the longest sequence: a window leaves most shares empty, and one
+        // token behind 131072 takes 31 us under a window of 8192
         const int step = 64 * token_waves(c.dim);
         const int64_t want = cu_count() / items, most = ceil_div(longest, 512);
         a.splits = (int)(want < most ? want : most);
