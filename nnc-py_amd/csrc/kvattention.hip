@@ -83,9 +83,9 @@ __device__ __forceinline__ f16x8 widen8(uint32_t lo, uint32_t hi) {
 static constexpr float kSlack = 3.f;
 static constexpr float kPLog = 12.f;
 // A page's factor is used up to here. A p that l needs (2^-41: 2^17 such keys
-// change its last bit) is 2^-101 then, still a normal number; and as e, each
-// lane's own, is chosen where m is moved or the factor is larger only, a term of
-// l is up to 2^75, of which 2^28 leave it finite.
+// change its last bit) is 2^-101 then, still a normal number; and as e is chosen
+// where m is moved or the factor is larger only, a term of l is up to 2^75, of
+// which 2^28 leave it finite.
 static constexpr float kMostFactor = 0x1p60f;
 // m before anything was seen: x is above, and 2^(kNone - x) is 0
 static constexpr float kNone = -3.402823466e38f;
@@ -105,7 +105,7 @@ __device__ __forceinline__ float exponent(float m, float largest) { return floor
 // exponential where either may not be a normal number: the sum is rounded, by
 // less than a weight's last bit.)
 __device__ __forceinline__ float rescale(float m, float e, float to_m, float to_e) { return __builtin_amdgcn_exp2f((m - to_m) + (to_e - e)); }
-// nothing seen: no lane's own s is below this reference
+// e before anything was seen
 static constexpr float kUnseen = 400.f - kPLog;
 
 // ---------------------------------------------------------------------------
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(64 * NW, D == 32 ? 4 : 1) kv_attention_k(KvAtt
             qf[0][s][j] = hi;
             if (F32) qf[PIECES - 1][s][j] = (half_t)(y - (float)hi);
         }
-    float m = kNone, l = 0.f;  // m the row's, l the lane's
+    float m = kNone, l = 0.f;  // m and ex the row's, l the lane's
     float ex = kUnseen;
     fx4 o[KV];
 #pragma unroll
@@ -378,7 +378,10 @@ __global__ void __launch_bounds__(64 * NW, D == 32 ? 4 : 1) kv_attention_k(KvAtt
         float factor = ldexpf(iv, (int)ex), sum = 0.f;
         if (__any(mx > m + kSlack || factor > kMostFactor)) {
             const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - mn);
-            const float en = exponent(mn, fmaxf(reference(m, ex), top * ku));
+            float far = fmaxf(reference(m, ex), top * ku);
+            far = fmaxf(far, __shfl_xor(far, 16));
+            far = fmaxf(far, __shfl_xor(far, 32));
+            const float en = exponent(mn, far);
             l *= rescale(m, ex, mn, en);
             m = mn, ex = en;
 #pragma unroll
@@ -422,11 +425,9 @@ __global__ void __launch_bounds__(64 * NW, D == 32 ? 4 : 1) kv_attention_k(KvAtt
         find(tb + 2 * STRIDE);
     }
     // join the waves
-    const float er = fminf(fminf(ex, __shfl_xor(ex, 16)), fminf(__shfl_xor(ex, 32), __shfl_xor(ex, 48)));
-    l = ldexpf(l, (int)(er - ex));
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    if (g == 0) ml[0][wave][i] = m, ml[1][wave][i] = l, ml[2][wave][i] = er;
+    if (g == 0) ml[0][wave][i] = m, ml[1][wave][i] = l, ml[2][wave][i] = ex;
     __syncthreads();
     float top = kNone, far = kNone, sum = 0.f;
 #pragma unroll
@@ -622,7 +623,7 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
                 if (F32) qf[PIECES - 1][s][j] = (half_t)(y - (float)hi);
             }
     }
-    float m = kNone, l = 0.f;  // m the row's, l the lane's
+    float m = kNone, l = 0.f;  // m and ex the row's, l the lane's
     float ex = kUnseen;
     fx16 o[DB];
 #pragma unroll
@@ -694,7 +695,9 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
         float factor[2] = {ldexpf(iv[0], (int)ex), ldexpf(iv[1], (int)ex)};
         if (__any(mx > m + kSlack || fmaxf(factor[0], factor[1]) > kMostFactor)) {
             const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - mn);
-            const float en = exponent(mn, fmaxf(reference(m, ex), fmaxf(top[0] * ku[0], top[1] * ku[1])));
+            float far = fmaxf(reference(m, ex), fmaxf(top[0] * ku[0], top[1] * ku[1]));
+            far = fmaxf(far, __shfl_xor(far, 32));
+            const float en = exponent(mn, far);
             l *= rescale(m, ex, mn, en);
             m = mn, ex = en;
 #pragma unroll
@@ -770,8 +773,6 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
         attend(tb, stage, !whole || !__all(ok[0] * ok[1] * ok[2] * ok[3] != 0.f));
     }
 
-    const float er = fminf(ex, __shfl_xor(ex, 32));
-    l = ldexpf(l, (int)(er - ex));
     l += __shfl_xor(l, 32);
     if (!row_ok) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -782,7 +783,7 @@ __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_promp
         for (int q = 0; q < 4; ++q) {
             T v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (T)ldexpf(o[c][4 * q + r] * inv, (int)er);
+            for (int r = 0; r < 4; ++r) v[r] = (T)ldexpf(o[c][4 * q + r] * inv, (int)ex);
             __builtin_memcpy(__builtin_assume_aligned(op + 32 * c + 8 * q, 4 * sizeof(T)), v, sizeof v);
         }
 }
