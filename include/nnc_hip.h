@@ -411,6 +411,67 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
                           Tensor* starts, Tensor* lengths, Tensor* out, int q_col, int heads, float scale, int window,
                           int max_length);
 
+/* ---- positions, drafted tokens, answers -------------------------------------
+ * The rest of a decoder's serving path, float32 or float16 activations as
+ * above. No counterpart in the reference ABI.
+ *
+ * nnc_hip_rope: norms of query and key heads and their rotation by position, in
+ * one pass. in [rows][ld], its columns from col being `heads` heads of `dim`
+ * values; out likewise from out_col, of in's type: the same columns of the
+ * same buffer, or columns that do not overlap in's (NNC_HIP_EINVAL). For each
+ * head y = x * w / sqrt(mean(x^2) + eps) over its dim values if `weight` (in's
+ * type, [dim] or [heads][dim]) is not NULL, else y = x. Then, if `angles` is
+ * not NULL, its first rot dims are rotated: angles float32 [places][rot] holds
+ * rot / 2 cosines and then as many sines for each place, rot even, 2 to dim;
+ * positions int32 [rows] names each row's place (device memory, clamped to
+ * those that there are). Pair i is dims i and i + rot / 2, or 2 i and 2 i + 1
+ * if `interleaved`: (y_a, y_b) becomes (y_a cos - y_b sin, y_b cos + y_a sin).
+ * Computed in float64, rounded to float32 and then to in's type. Queries and
+ * keys that lie side by side are one call: heads = both, weight a row each.
+ *
+ * nnc_hip_rope_kv_write: nnc_hip_rope of a call's queries and keys, the keys
+ * and the values going into the paged cache as by nnc_hip_kv_write; the
+ * results are those of the three calls, bit for bit. q's columns from q_col:
+ * heads * dim, to q_out ([rows][heads * dim]), or in place if that is NULL; no
+ * queries if q is NULL. q, k and v may be one tensor, but rotated queries must
+ * not lie over keys or values (NNC_HIP_EINVAL). q_weight [dim] or
+ * [heads][dim], k_weight [dim] or [kv_heads][dim], either may be NULL. angles
+ * as above, NULL: none; positions NULL: each row's place is its position in
+ * its sequence (drafts that share one have to name it). Rows of no sequence
+ * are neither read nor written. May use the stream's scratch.
+ *
+ * nnc_hip_kv_tree_attention: nnc_hip_kv_attention for drafted tokens: the
+ * sequence's rows do not see each other in order but by masks. tree int32
+ * [rows][words] (device memory): row i sees row m of its sequence if bit m %
+ * 32 of word m / 32 of its mask is set (itself by its own bit; rows that the
+ * words do not reach are not seen). Every row sees the positions before the
+ * sequence's first row; with window > 0 those of them that are later than p -
+ * window, p = the first row's position + the row's set bits - 1, which is its
+ * position if its mask names the drafts that lead to it and itself. Drafts that
+ * a mask names are seen whatever the window. Everything else as for
+ * nnc_hip_kv_attention.
+ *
+ * nnc_hip_token_logprobs: of rows of logits [rows][vocab], p = softmax(scale *
+ * logits): logprob float32 [rows] = log p[tokens[row]] (tokens int32 [rows]);
+ * entropy float32 [rows] = -sum p log p; top_index int32 and top_logprob
+ * float32 [rows][n]: the n likeliest tokens (n from 1 to 64), the earlier of
+ * equal ones first, and their log p. Any of the three may be NULL (tokens with
+ * logprob). Logits of -infinity have probability 0; a row whose largest is not
+ * finite (a NaN or +infinity in it, or nothing but -infinity) has NaN for
+ * results and -1 for tokens. A token outside [0, vocab): NaN. Where there are
+ * fewer than n tokens: -1, -infinity. Sums are float64. */
+void nnc_hip_rope(Tensor* in, Tensor* weight, Tensor* angles, Tensor* positions, Tensor* out, int col, int out_col,
+                  int heads, int dim, int interleaved, float eps);
+void nnc_hip_rope_kv_write(Tensor* q, Tensor* k, Tensor* v, Tensor* q_weight, Tensor* k_weight, Tensor* angles,
+                           Tensor* positions, Tensor* q_out, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale,
+                           Tensor* v_scale, Tensor* table, Tensor* starts, Tensor* lengths, int q_col, int heads,
+                           int k_col, int v_col, int interleaved, float eps);
+void nnc_hip_kv_tree_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale,
+                               Tensor* table, Tensor* starts, Tensor* lengths, Tensor* tree, Tensor* out, int q_col,
+                               int heads, float scale, int window, int max_length);
+void nnc_hip_token_logprobs(Tensor* logits, Tensor* tokens, Tensor* logprob, Tensor* entropy, Tensor* top_index,
+                            Tensor* top_logprob, float scale);
+
 #ifdef __cplusplus
 }
 #endif

@@ -137,6 +137,10 @@ TARGET_SIGNATURES = {
     "nnc_hip_kv_write": [TP] * 9 + [c_int, c_int],
     "nnc_hip_kv_read": [TP] * 9 + [c_int, c_int],
     "nnc_hip_kv_attention": [TP] * 9 + [c_int, c_int, c_float, c_int, c_int],
+    "nnc_hip_rope": [TP] * 5 + [c_int] * 5 + [c_float],
+    "nnc_hip_rope_kv_write": [TP] * 15 + [c_int] * 5 + [c_float],
+    "nnc_hip_kv_tree_attention": [TP] * 10 + [c_int, c_int, c_float, c_int, c_int],
+    "nnc_hip_token_logprobs": [TP] * 6 + [c_float],
 }
 
 # nnc_hip_fused_eltwise's op codes (include/nnc_hip.h NNC_EW_*)

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import numpy as np
 
+from ..rotary import angles
 from .ir import Graph, Node, TensorInfo
 
 
@@ -222,6 +223,45 @@ class GraphBuilder:
         self._node("KvAttention", [q, *cache, table, starts, lengths], [y], name, q_col=int(q_col), heads=int(heads),
                    scale=float(dim ** -0.5 if scale is None else scale), window=int(window), max_length=int(max_length))
         return y
+
+    def rope_angles(self, name, positions, rot, base=10000.0, **scaling):
+        """A table of angles as a constant (rotary.angles)."""
+        return self.const(name, angles(positions, rot, base, **scaling))
+
+    def rope(self, x, heads, dim, angles=None, positions=None, weight=None, col=0, interleaved=False, epsilon=1e-6, name=None,
+             out=None):
+        y = self._out(name or "rope", tuple(self.shape(x)[:-1]) + (heads * dim,), self.g.tensors[x].dtype, name=out)
+        self._node("Rope", [x, weight or "", angles or "", positions or ""], [y], name, col=int(col), heads=int(heads), dim=int(dim),
+                   interleaved=int(interleaved), epsilon=float(epsilon))
+        return y
+
+    def rope_kv_write(self, q, k, v, cache, table, starts, lengths, heads, angles=None, positions=None, q_weight=None, k_weight=None,
+                      q_col=0, k_col=0, v_col=0, interleaved=False, epsilon=1e-6, name=None, out=None):
+        """The rotated queries. Changes `cache`; nodes added after it see the new rows."""
+        dim = self.shape(cache[0])[3]
+        y = self._out(name or "rope_kv_write", tuple(self.shape(q)[:-1]) + (heads * dim,), self.g.tensors[q].dtype, name=out)
+        self._node("RopeKvWrite", [q, k, v, q_weight or "", k_weight or "", angles or "", positions or "", *cache, table, starts, lengths],
+                   [y, *cache], name, q_col=int(q_col), heads=int(heads), k_col=int(k_col), v_col=int(v_col),
+                   interleaved=int(interleaved), epsilon=float(epsilon))
+        return y
+
+    def kv_tree_attention(self, q, cache, table, starts, lengths, tree, heads, q_col=0, scale=None, window=0, max_length=0, name=None,
+                          out=None):
+        dim = self.shape(cache[0])[3]
+        y = self._out(name or "kv_tree_attention", tuple(self.shape(q)[:-1]) + (heads * dim,), self.g.tensors[q].dtype, name=out)
+        self._node("KvTreeAttention", [q, *cache, table, starts, lengths, tree], [y], name, q_col=int(q_col), heads=int(heads),
+                   scale=float(dim ** -0.5 if scale is None else scale), window=int(window), max_length=int(max_length))
+        return y
+
+    def token_logprobs(self, logits, tokens, top=0, scale=1.0, name=None):
+        """Log probabilities and entropies; with `top`, tokens and their log
+        probabilities besides."""
+        nm, s = name or "token_logprobs", tuple(self.shape(logits)[:-1])
+        ys = [self._out(nm, s), self._out(f"{nm}_entropy", s)]
+        if top:
+            ys += [self._out(f"{nm}_index", s + (top,), "int32"), self._out(f"{nm}_top", s + (top,))]
+        self._node("TokenLogprobs", [logits, tokens], ys, name, scale=float(scale))
+        return tuple(ys)
 
     def _reduce(self, op, x, axes, keepdims, name, out):
         s = list(self.shape(x))

@@ -216,6 +216,23 @@ def lower_node(g: Graph, node: Node) -> Call:
         return Call("nnc_hip_kv_attention", [_t(i) for i in ins] + [_t(outs[0]), ("i", int(a["q_col"])), ("i", int(a["heads"])),
                                                                     ("f", float(a["scale"])), ("i", int(a["window"])),
                                                                     ("i", int(a["max_length"]))], node.name)
+    if op == "Rope":
+        a = node.attrs
+        return Call("nnc_hip_rope", [_t(ins[0])] + [_opt(node, i) for i in (1, 2, 3)] + [_t(outs[0]), ("i", int(a["col"])), ("i", 0)]
+                    + [("i", int(a[k])) for k in ("heads", "dim", "interleaved")] + [("f", float(a["epsilon"]))], node.name)
+    if op == "RopeKvWrite":  # its outputs are the rotated queries and the cache tensors among its inputs
+        a = node.attrs
+        return Call("nnc_hip_rope_kv_write", [_t(i) for i in ins[:3]] + [_opt(node, i) for i in (3, 4, 5, 6)] + [_t(outs[0])]
+                    + [_t(i) for i in ins[7:]] + [("i", int(a[k])) for k in ("q_col", "heads", "k_col", "v_col", "interleaved")]
+                    + [("f", float(a["epsilon"]))], node.name)
+    if op == "KvTreeAttention":
+        a = node.attrs
+        return Call("nnc_hip_kv_tree_attention", [_t(i) for i in ins] + [_t(outs[0]), ("i", int(a["q_col"])), ("i", int(a["heads"])),
+                                                                         ("f", float(a["scale"])), ("i", int(a["window"])),
+                                                                         ("i", int(a["max_length"]))], node.name)
+    if op == "TokenLogprobs":
+        return Call("nnc_hip_token_logprobs", [_t(i) for i in ins] + [_t(o) for o in outs] + [("null",)] * (4 - len(outs))
+                    + [("f", float(node.attrs["scale"]))], node.name)
     if op == "FusedEltwise":  # an element-wise chain in one pass (include/nnc_hip.h)
         steps = node.attrs["steps"]
         prog = [v for st in steps for v in (st[0], st[1], st[2])]

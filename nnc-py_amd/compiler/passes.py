@@ -63,7 +63,7 @@ def eliminate_identity(g: Graph) -> int:
 
 
 # ops that change tensors which stay from run to run
-LASTING_OPS = {"KvWrite"}
+LASTING_OPS = {"KvWrite", "RopeKvWrite"}
 
 
 def eliminate_dead_code(g: Graph) -> int:

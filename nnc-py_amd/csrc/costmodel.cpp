@@ -816,6 +816,43 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* kc, Tensor* vc, Tensor* ks, Tensor*
     record("nnc_hip_kv_attention", "nnc_hip_kv_attention",
            kLaunchUs + fmax(flops / (kMfmaI8 / 4), bytes / (kHbm * kStreamEff)) * 1e6, flops, bytes);
 }
+// positions, drafted tokens and answers: their bytes once
+static double used_bytes(Tensor* t, int64_t width) {  // of a matrix of which `width` columns are used
+    const int64_t ld = t && t->shape && t->ndim > 0 ? t->shape[t->ndim - 1] : 0;
+    return ld > 0 ? (double)nbytes(t) * (double)width / (double)ld : 0.0;
+}
+void nnc_hip_rope(Tensor* in, Tensor* weight, Tensor* angles, Tensor* positions, Tensor* out, int col, int out_col, int heads,
+                  int dim, int interleaved, float eps) {
+    (void)weight, (void)angles, (void)positions, (void)col, (void)out_col, (void)interleaved, (void)eps;
+    if (in && out && numel(in) > 0) stream_kernel("nnc_hip_rope", "nnc_hip_rope", 2.0 * used_bytes(in, (int64_t)heads * dim));
+}
+void nnc_hip_rope_kv_write(Tensor* q, Tensor* k, Tensor* v, Tensor* q_weight, Tensor* k_weight, Tensor* angles, Tensor* positions,
+                           Tensor* q_out, Tensor* kc, Tensor* vc, Tensor* ks, Tensor* vs, Tensor* table, Tensor* starts,
+                           Tensor* lengths, int q_col, int heads, int k_col, int v_col, int interleaved, float eps) {
+    (void)q_weight, (void)k_weight, (void)angles, (void)positions, (void)q_out, (void)vc, (void)ks, (void)vs, (void)table;
+    (void)starts, (void)lengths, (void)q_col, (void)k_col, (void)v_col, (void)interleaved, (void)eps;
+    if (!k || !v || !kc || !kc->shape || kc->ndim != 4 || numel(k) <= 0) return;
+    const int64_t dim = kc->shape[3], row = kc->shape[1] * dim;
+    stream_kernel("nnc_hip_rope_kv_write", "nnc_hip_rope_kv_write",
+                  (q ? 2.0 * used_bytes(q, heads * dim) : 0.0) + 1.25 * (used_bytes(k, row) + used_bytes(v, row)));
+}
+void nnc_hip_kv_tree_attention(Tensor* q, Tensor* kc, Tensor* vc, Tensor* ks, Tensor* vs, Tensor* table, Tensor* starts,
+                               Tensor* lengths, Tensor* tree, Tensor* out, int q_col, int heads, float scale, int window,
+                               int max_length) {
+    (void)vc, (void)ks, (void)vs, (void)starts, (void)lengths, (void)tree, (void)q_col, (void)heads, (void)scale, (void)window;
+    if (!q || !kc || !table || !out || !kc->shape || !table->shape || kc->ndim != 4 || table->ndim != 2) return;
+    const double length = max_length > 0 ? max_length : (double)table->shape[1] * (double)kc->shape[2];
+    const double bytes = 2.0 * (double)table->shape[0] * length * (double)(kc->shape[1] * kc->shape[3]) + 2.0 * nbytes(out);
+    const double flops = 4.0 * (double)numel(out) * length;
+    record("nnc_hip_kv_tree_attention", "nnc_hip_kv_tree_attention",
+           kLaunchUs + fmax(flops / (kMfmaI8 / 4), bytes / (kHbm * kStreamEff)) * 1e6, flops, bytes);
+}
+void nnc_hip_token_logprobs(Tensor* logits, Tensor* tokens, Tensor* logprob, Tensor* entropy, Tensor* top_index,
+                            Tensor* top_logprob, float scale) {
+    (void)tokens, (void)logprob, (void)entropy, (void)scale;
+    if (logits && numel(logits) > 0)
+        stream_kernel("nnc_hip_token_logprobs", "nnc_hip_token_logprobs", nbytes(logits) + nbytes(top_index) + nbytes(top_logprob));
+}
 // eltwise.hip nnc_hip_fused_eltwise: one streaming pass, each input read and
 // the output written once
 void nnc_hip_fused_eltwise(Tensor** ins, int n_in, const int* prog, int n_steps, const float* consts, Tensor* out) {

@@ -18,7 +18,7 @@
 // is shared between workgroups and no atomics are needed.
 #include <tuple>
 
-#include "quant8.h"
+#include "kvcache.h"
 
 namespace nnc {
 
@@ -79,15 +79,6 @@ bool cache_args(const char* name, Tensor* k_cache, Tensor* v_cache, Tensor* k_sc
                          (int)width, (int)rows, (int)page, ks[0]};
     return true;
 }
-
-struct KvArgs {
-    Ragged g;
-    int8_t *k, *v;
-    float *k_scale, *v_scale;
-    void *k_rows, *v_rows;
-    int64_t k_ld, v_ld;
-    int k_col, v_col, kv_heads, dim;
-};
 
 // ---------------------------------------------------------------------------
 // A group of TPG threads (a wave, or a workgroup) takes a page's K or V of one
@@ -369,7 +360,7 @@ static void launch_quads(const char* name, const KvArgs& a) {
 // quads (256 positions by 128 in fp32) get workgroups of 1024, whose lanes hold
 // no more than others'.
 template <typename T>
-static void launch_write(const char* name, const KvArgs& a) {
+static void launch_write_rows(const char* name, const KvArgs& a) {
     const int n = a.g.page * a.dim * (int)sizeof(T) / 64;
     if (!quads<T>(a))
         return launch(name, kv_write_k<T>, dim3((unsigned)touched_bound(a.g.rows, a.g.batch, a.g.page), (unsigned)a.kv_heads), dim3(256), 0, a);
@@ -383,6 +374,13 @@ static void launch_write(const char* name, const KvArgs& a) {
     launch_quads<T, 1024, kv_write_quads_k<T, 1024, 2>>(name, a);
 }
 
+void launch_write(const char* name, bool f16, const KvArgs& a) {
+    if (f16)
+        launch_write_rows<half_t>(name, a);
+    else
+        launch_write_rows<float>(name, a);
+}
+
 template <typename T>
 static void launch_read(const char* name, const KvArgs& a) {
     const int n = a.g.page * a.dim * (int)sizeof(T) / 64;
@@ -393,8 +391,8 @@ static void launch_read(const char* name, const KvArgs& a) {
     launch_quads<T, 1024, kv_read_quads_k<T, 1024>>(name, a);
 }
 
-static bool kv_args(const char* name, Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale,
-                    Tensor* v_scale, Tensor* table, Tensor* starts, Tensor* lengths, int k_col, int v_col, KvArgs* a) {
+bool kv_args(const char* name, Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale,
+             Tensor* v_scale, Tensor* table, Tensor* starts, Tensor* lengths, int k_col, int v_col, KvArgs* a) {
     CacheArgs c;
     int64_t rows = 0, v_rows = 0;
     if (!cache_args(name, k_cache, v_cache, k_scale, v_scale, table, starts, lengths, 0, &c)) return false;
@@ -425,10 +423,7 @@ void nnc_hip_kv_write(Tensor* k, Tensor* v, Tensor* k_cache, Tensor* v_cache, Te
     if (!ready(name)) return;
     const double n = 2.0 * a.g.rows * a.kv_heads * a.dim;
     set_work(6.0 * n, n * (activation_bytes(k) + 1));
-    if (k->dtype == NNC_DTYPE_FLOAT16)
-        launch_write<half_t>(name, a);
-    else
-        launch_write<float>(name, a);
+    launch_write(name, k->dtype == NNC_DTYPE_FLOAT16, a);
 }
 
 void nnc_hip_kv_read(Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table, Tensor* starts,

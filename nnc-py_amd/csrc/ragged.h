@@ -97,6 +97,42 @@ RAGGED_HD int64_t query_tiles_bound(int64_t rows, int64_t batch, int group, int 
     return some < each ? some : each;
 }
 
+// Drafted rows see each other by a mask of `words` words a row: bit m % 32 of
+// word m / 32 is set if the row sees row m of its sequence. Which of the 16
+// positions from `at` on a row sees, position at + c in bit c: all before
+// `first`, the drafts' first position, the mask's own from there to `length`.
+RAGGED_HD uint32_t tree_word(const int* mask, int words, int64_t w) { return w >= 0 && w < words ? (uint32_t)mask[w] : 0u; }
+RAGGED_HD uint32_t tree_bits(const int* mask, int words, int first, int length, int at) {
+    const int64_t d = (int64_t)at - first;
+    uint32_t bits;
+    if (d <= -16) {
+        bits = 0xffffu;
+    } else if (d < 0) {
+        bits = ((1u << -d) - 1u) | tree_word(mask, words, 0) << -d;
+    } else {
+        const uint32_t s = (uint32_t)(d & 31);
+        bits = tree_word(mask, words, d >> 5) >> s;
+        if (s > 16) bits |= tree_word(mask, words, (d >> 5) + 1) << (32 - s);
+    }
+    const int64_t left = (int64_t)length - at;
+    return left >= 16 ? bits & 0xffffu : left > 0 ? bits & ((1u << left) - 1u) : 0u;
+}
+// How many of the sequence's `rows` rows a row sees: with the context they are
+// its position, a draft being the last of those that lead to it.
+RAGGED_HD int tree_depth(const int* mask, int words, int rows) {
+    int n = 0;
+    for (int w = 0; w < words && 32 * (int64_t)w < rows; ++w) {
+        uint32_t x = (uint32_t)mask[w];
+        if (rows - 32 * w < 32) x &= (1u << (rows - 32 * w)) - 1u;
+#ifdef __HIP_DEVICE_COMPILE__
+        n += __popc(x);
+#else
+        n += __builtin_popcount(x);
+#endif
+    }
+    return n;
+}
+
 // The window that is compared: none (0) if it is as long as a sequence can be,
 // so that positions less it stay far from the smallest number.
 RAGGED_HD int window_of(int window, int capacity) { return window < capacity ? window : 0; }

@@ -1,0 +1,264 @@
+// Rotary positions: norms of query and key heads and their rotation by position
+// (nnc_hip_rope), and the same on the way into the paged 8-bit cache
+// (nnc_hip_rope_kv_write). No reference counterpart.
+//
+//   y = x w / sqrt(mean(x^2) + eps)           over a head's dim values, if there are weights
+//   (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)   for the rot / 2 pairs of its first rot dims
+//
+// with the pair's cosine c and sine s from the row of the angle table that the
+// position names. All of it in float64 and rounded to float32 and the
+// activations' type at the end: keys are then cut to whole numbers, and a
+// result that depended on the order of a sum would be another whole number now
+// and then. A float64 operation takes no longer than a float32 one here.
+#include "kvcache.h"
+
+namespace nnc {
+
+struct RopeArgs {
+    const void* in;
+    void* out;
+    const void* weight;   // [dim], or [heads][dim]; null: no norm
+    const float* angles;  // [places][rot]; null: no rotation
+    const int* positions;  // [rows]; null: places in the sequences of g
+    Ragged g;             // batch 0: every row is taken
+    int64_t in_ld, out_ld;
+    int64_t rows, places;
+    int col, out_col, heads, dim, rot;
+    bool interleaved, weight_each;
+    double eps;
+};
+
+// The sequence that a row belongs to, -1 if it is none's: the first whose rows
+// end behind it. All lanes of a wave ask for the same row; 64 sequences are
+// compared at a time. What starts holds only decides which of 0 .. batch - 1.
+__device__ __forceinline__ int owner_of(const Ragged& g, int row) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = g.batch;  // the answer is one of lo .. hi
+    while (lo < hi) {
+        const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+        const uint64_t past = __ballot(at < hi && g.starts[min(at, g.batch - 1) + 1] > row);
+        const int probes = (hi - lo + step - 1) / step;
+        const int f = past ? __ffsll((unsigned long long)past) - 1 : probes;
+        if (f < probes) hi = lo + f * step;
+        if (f > 0) lo += (f - 1) * step + 1;
+    }
+    if (lo >= g.batch) return -1;
+    const Span s = span_of(g, lo);
+    return row >= s.end - s.rows && row < s.end ? lo : -1;
+}
+
+// The row of the angle table for a row of the activations; -1 if the row is to
+// be left alone.
+__device__ __forceinline__ int64_t rope_place(const RopeArgs& a, int64_t row) {
+    int64_t at = 0;
+    if (a.g.batch > 0) {
+        const int b = owner_of(a.g, (int)row);
+        if (b < 0) return -1;
+        const Span s = span_of(a.g, b);
+        at = row - s.end + s.length;
+    }
+    if (a.positions) at = a.positions[row];
+    return at < 0 ? 0 : at < a.places ? at : a.places - 1;
+}
+
+// To float32, then to the activations' type. (The compiler would make one
+// conversion of the two, which takes twenty operations for float16.)
+template <typename T>
+__device__ __forceinline__ T rounded(double y) {
+    float f = (float)y;
+    asm("" : "+v"(f));
+    return (T)f;
+}
+
+__device__ __forceinline__ double wave_add(double v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Any sizes: a wave to a head of a row, a pair or an unpaired dim a lane.
+template <typename T>
+__global__ void __launch_bounds__(256) rope_k(RopeArgs a) {
+    const int lane = threadIdx.x & 63, half = a.rot / 2;
+    const int64_t items = a.rows * a.heads, step = (int64_t)gridDim.x * 4;
+    for (int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); item < items; item += step) {
+        const int64_t row = item / a.heads;
+        const int head = (int)(item - row * a.heads);
+        const int64_t place = rope_place(a, row);
+        if (place < 0) continue;
+        const T* x = (const T*)a.in + row * a.in_ld + a.col + (int64_t)head * a.dim;
+        T* y = (T*)a.out + row * a.out_ld + a.out_col + (int64_t)head * a.dim;
+        const T* w = (const T*)a.weight + (a.weight_each ? (int64_t)head * a.dim : 0);
+        double r = 1.0;
+        if (a.weight) {
+            double sum = 0.0;
+            for (int d = lane; d < a.dim; d += 64) sum += (double)(float)x[d] * (double)(float)x[d];
+            r = 1.0 / sqrt(wave_add(sum) / a.dim + a.eps);
+        }
+        auto normed = [&](int d) { return a.weight ? (double)(float)x[d] * r * (double)(float)w[d] : (double)(float)x[d]; };
+        for (int u = lane; u < a.dim - half; u += 64) {
+            if (u >= half) {
+                y[u + half] = rounded<T>(normed(u + half));
+                continue;
+            }
+            const int one = a.interleaved ? 2 * u : u, other = a.interleaved ? 2 * u + 1 : u + half;
+            const double c = a.angles[place * a.rot + u], s = a.angles[place * a.rot + half + u];
+            const double p = normed(one), q = normed(other);
+            y[one] = rounded<T>(p * c - q * s);
+            y[other] = rounded<T>(q * c + p * s);
+        }
+    }
+}
+
+static void launch_rope(const char* name, bool f16, const RopeArgs& a) {
+    const int64_t blocks = ceil_div(a.rows * a.heads, 4), most = (int64_t)cu_count() * 32;
+    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    if (f16)
+        launch(name, rope_k<half_t>, grid, dim3(256), 0, a);
+    else
+        launch(name, rope_k<float>, grid, dim3(256), 0, a);
+}
+
+// ---------------------------------------------------------------------------
+// arguments
+// ---------------------------------------------------------------------------
+
+// Columns of a matrix as memory: rows of `width` bytes, ld bytes apart.
+struct Columns {
+    uintptr_t at;
+    int64_t rows, ld, width;
+};
+static Columns columns(const Tensor* t, int64_t rows, int64_t ld, int64_t col, int64_t width) {
+    const int64_t e = activation_bytes(t);
+    return Columns{(uintptr_t)t->data + (uintptr_t)(col * e), rows, ld * e, width * e};
+}
+// Whether two may have a byte in common.
+static bool share_bytes(const Columns& a, const Columns& b) {
+    if (a.rows < 1 || b.rows < 1) return false;
+    if (a.at + (uintptr_t)((a.rows - 1) * a.ld + a.width) <= b.at || b.at + (uintptr_t)((b.rows - 1) * b.ld + b.width) <= a.at) return false;
+    if (a.ld != b.ld) return true;
+    int64_t d = ((int64_t)b.at - (int64_t)a.at) % a.ld;
+    if (d < 0) d += a.ld;
+    return d < a.width || d + b.width > a.ld;
+}
+
+static bool rope_weight(const char* name, const char* what, const Tensor* in, Tensor* weight, int heads, int dim, float eps, RopeArgs* a) {
+    a->weight = nullptr, a->weight_each = false, a->eps = eps;
+    if (!weight) return true;
+    if (!has_data(weight) || !good_shape(weight)) return fail(NNC_HIP_EINVAL, name, "%s: NULL data or bad shape", what), false;
+    if (weight->dtype != in->dtype) return fail(NNC_HIP_EUNSUPP, name, "%s: of another type than the rows", what), false;
+    const int64_t n = numel(weight);
+    if (n != dim && n != (int64_t)heads * dim) return fail(NNC_HIP_EINVAL, name, "%s must be [dim] or [heads][dim]", what), false;
+    if (!(eps >= 0.f) || !(eps < INFINITY)) return fail(NNC_HIP_EINVAL, name, "eps must not be negative"), false;
+    a->weight = weight->data, a->weight_each = n != dim;
+    return true;
+}
+
+static bool rope_angles(const char* name, Tensor* angles, Tensor* positions, int64_t rows, int dim, bool needs_positions, RopeArgs* a) {
+    a->angles = nullptr, a->positions = nullptr, a->places = 1, a->rot = 0;
+    if (!angles) {
+        if (positions) return fail(NNC_HIP_EINVAL, name, "positions without angles"), false;
+        return true;
+    }
+    if (!has_data(angles) || !good_shape(angles) || angles->ndim != 2 || angles->shape[0] < 1)
+        return fail(NNC_HIP_EINVAL, name, "angles must be [positions][rot]"), false;
+    if (angles->dtype != NNC_DTYPE_FLOAT32) return fail(NNC_HIP_EUNSUPP, name, "float32 angles only"), false;
+    const int64_t rot = angles->shape[1];
+    if (rot < 2 || rot % 2 != 0 || rot > dim) return fail(NNC_HIP_EINVAL, name, "%lld of %d dims turned", (long long)rot, dim), false;
+    if (angles->shape[0] > INT32_MAX) return fail(NNC_HIP_EUNSUPP, name, "too many angles"), false;
+    if (!positions && needs_positions) return fail(NNC_HIP_EINVAL, name, "angles without positions"), false;
+    if (positions) {
+        if (!has_data(positions) || !good_shape(positions) || numel(positions) != rows)
+            return fail(NNC_HIP_EINVAL, name, "positions must be one for each row"), false;
+        if (positions->dtype != NNC_DTYPE_INT32) return fail(NNC_HIP_EUNSUPP, name, "int32 positions only"), false;
+        a->positions = (const int*)positions->data;
+    }
+    a->angles = (const float*)angles->data, a->places = angles->shape[0], a->rot = (int)rot;
+    return true;
+}
+
+// Where the rotated rows go: out's columns, apart from the rows' own or the same.
+static bool rope_out(const char* name, const Tensor* in, Tensor* out, int col, int out_col, int64_t width, int64_t rows, int64_t ld, RopeArgs* a) {
+    int64_t out_rows = 0, out_ld = 0;
+    if (!rows_arg(name, "out", out, out_col, width, &out_rows, &out_ld)) return false;
+    if (out->dtype != in->dtype || out_rows != rows) return fail(NNC_HIP_EINVAL, name, "out differs from the input in rows or type"), false;
+    const Columns from = columns(in, rows, ld, col, width), to = columns(out, rows, out_ld, out_col, width);
+    if (!(from.at == to.at && from.ld == to.ld) && share_bytes(from, to))
+        return fail(NNC_HIP_EINVAL, name, "out overlaps the input without being the same columns"), false;
+    a->out = out->data, a->out_ld = out_ld, a->out_col = out_col;
+    return true;
+}
+
+}  // namespace nnc
+
+using namespace nnc;
+
+extern "C" {
+
+void nnc_hip_rope(Tensor* in, Tensor* weight, Tensor* angles, Tensor* positions, Tensor* out, int col, int out_col, int heads,
+                  int dim, int interleaved, float eps) {
+    const char* name = "nnc_hip_rope";
+    RopeArgs a{};
+    if (heads < 1 || dim < 1 || heads > 65535 || dim > 65536) return fail(NNC_HIP_EINVAL, name, "%d heads of %d", heads, dim);
+    const int64_t width = (int64_t)heads * dim;
+    if (!rows_arg(name, "in", in, col, width, &a.rows, &a.in_ld)) return;
+    if (!rope_weight(name, "weight", in, weight, heads, dim, eps, &a) || !rope_angles(name, angles, positions, a.rows, dim, true, &a) ||
+        !rope_out(name, in, out, col, out_col, width, a.rows, a.in_ld, &a))
+        return;
+    a.in = in->data, a.col = col, a.heads = heads, a.dim = dim, a.interleaved = interleaved != 0;
+    if (a.rows == 0) return;
+    if (!ready(name)) return;
+    const double n = (double)a.rows * (double)width;
+    set_work(8.0 * n, 2.0 * n * activation_bytes(in) + 4.0 * (double)a.rows * a.rot);
+    launch_rope(name, in->dtype == NNC_DTYPE_FLOAT16, a);
+}
+
+void nnc_hip_rope_kv_write(Tensor* q, Tensor* k, Tensor* v, Tensor* q_weight, Tensor* k_weight, Tensor* angles, Tensor* positions,
+                           Tensor* q_out, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table,
+                           Tensor* starts, Tensor* lengths, int q_col, int heads, int k_col, int v_col, int interleaved, float eps) {
+    const char* name = "nnc_hip_rope_kv_write";
+    KvArgs w;
+    if (!kv_args(name, k, v, k_cache, v_cache, k_scale, v_scale, table, starts, lengths, k_col, v_col, &w)) return;
+    const int64_t rows = w.g.rows, kv_width = (int64_t)w.kv_heads * w.dim;
+    RopeArgs ka{}, qa{};
+    if (!rope_weight(name, "k_weight", k, k_weight, w.kv_heads, w.dim, eps, &ka) || !rope_angles(name, angles, positions, rows, w.dim, false, &ka)) return;
+    ka.in = k->data, ka.in_ld = w.k_ld, ka.col = k_col, ka.heads = w.kv_heads;
+    ka.rows = rows, ka.dim = w.dim, ka.interleaved = interleaved != 0, ka.g = w.g;
+    if (q) {
+        qa = ka;
+        if (heads < 1 || heads > 65535) return fail(NNC_HIP_EINVAL, name, "%d heads", heads);
+        const int64_t width = (int64_t)heads * w.dim;
+        int64_t q_rows = 0;
+        if (!rows_arg(name, "q", q, q_col, width, &q_rows, &qa.in_ld)) return;
+        if (q_rows != rows || q->dtype != k->dtype) return fail(NNC_HIP_EINVAL, name, "q and k differ in rows or type");
+        if (!rope_weight(name, "q_weight", q, q_weight, heads, w.dim, eps, &qa)) return;
+        qa.in = q->data, qa.col = q_col, qa.heads = heads;
+        Tensor* out = q_out ? q_out : q;
+        if (!rope_out(name, q, out, q_col, q_out ? 0 : q_col, width, rows, qa.in_ld, &qa)) return;
+        const Columns to = columns(out, rows, qa.out_ld, qa.out_col, width);
+        if (share_bytes(to, columns(k, rows, w.k_ld, k_col, kv_width)) || share_bytes(to, columns(v, rows, w.v_ld, v_col, kv_width)))
+            return fail(NNC_HIP_EINVAL, name, "the rotated queries would lie over keys or values");
+    } else if (q_weight || q_out) {
+        return fail(NNC_HIP_EINVAL, name, "q_weight or q_out without q");
+    }
+    if (rows == 0 || w.g.batch == 0 || w.g.width == 0) return;
+    if (!ready(name)) return;
+    const bool f16 = k->dtype == NNC_DTYPE_FLOAT16;
+    // the rotated keys pass through scratch
+    const size_t bytes = (size_t)rows * kv_width * activation_bytes(k);
+    ka.out = workspace(bytes);
+    if (!ka.out) return fail(NNC_HIP_ENOMEM, name, "no workspace for %zu bytes of rotated keys", bytes);
+    ka.out_ld = kv_width, ka.out_col = 0;
+    w.k_rows = ka.out, w.k_ld = kv_width, w.k_col = 0;
+    const double n = (double)rows * activation_bytes(k);
+    if (q) {
+        set_work(8.0 * rows * heads * w.dim, 2.0 * n * heads * w.dim);
+        launch_rope("nnc_hip_rope_kv_write_q", f16, qa);
+    }
+    set_work(8.0 * rows * kv_width, 2.0 * n * kv_width);
+    launch_rope("nnc_hip_rope_kv_write_k", f16, ka);
+    set_work(12.0 * rows * kv_width, 2.0 * (n + rows) * kv_width);
+    launch_write(name, f16, w);
+}
+
+}  // extern "C"

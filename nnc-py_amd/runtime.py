@@ -83,6 +83,10 @@ _HIP_SIGNATURES = {
     "nnc_hip_kv_write": (abi.TARGET_SIGNATURES["nnc_hip_kv_write"], None),
     "nnc_hip_kv_read": (abi.TARGET_SIGNATURES["nnc_hip_kv_read"], None),
     "nnc_hip_kv_attention": (abi.TARGET_SIGNATURES["nnc_hip_kv_attention"], None),
+    "nnc_hip_rope": (abi.TARGET_SIGNATURES["nnc_hip_rope"], None),
+    "nnc_hip_rope_kv_write": (abi.TARGET_SIGNATURES["nnc_hip_rope_kv_write"], None),
+    "nnc_hip_kv_tree_attention": (abi.TARGET_SIGNATURES["nnc_hip_kv_tree_attention"], None),
+    "nnc_hip_token_logprobs": (abi.TARGET_SIGNATURES["nnc_hip_token_logprobs"], None),
     "nnc_hip_ew_chain_specialized": ([ctypes.c_int, abi.I32P, ctypes.c_int], ctypes.c_int),
 }
 

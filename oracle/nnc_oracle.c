@@ -1470,3 +1470,157 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
     }
     free(p), free(y);
 }
+
+/* One head: norm and rotation of x[0 .. dim) to y, in double. */
+static void rope_head(const float* x, const float* w, const float* angles, int64_t dim, int64_t rot, int interleaved, double eps,
+                      double* t, float* y) {
+    double sum = 0;
+    for (int64_t d = 0; d < dim; ++d) sum += (double)x[d] * x[d];
+    const double r = 1 / sqrt(sum / (double)dim + eps);
+    for (int64_t d = 0; d < dim; ++d) t[d] = w ? x[d] * r * w[d] : x[d];
+    for (int64_t i = 0; i < rot / 2; ++i) {
+        const int64_t a = interleaved ? 2 * i : i, b = interleaved ? 2 * i + 1 : i + rot / 2;
+        const double c = angles[i], s = angles[rot / 2 + i], p = t[a], q = t[b];
+        t[a] = p * c - q * s, t[b] = q * c + p * s;
+    }
+    for (int64_t d = 0; d < dim; ++d) y[d] = (float)t[d];
+}
+
+/* All heads of a row; `place`: the row's row of angles before it is clamped. */
+static void rope_row(const float* x, const Tensor* weight, const Tensor* angles, int64_t place, int64_t heads, int64_t dim,
+                     int interleaved, float eps, float* y) {
+    const int64_t rot = angles ? angles->shape[1] : 0, last = angles ? angles->shape[0] - 1 : 0;
+    const float* turn = angles ? (const float*)angles->data + (place < 0 ? 0 : place > last ? last : place) * rot : NULL;
+    double* t = (double*)malloc((size_t)dim * sizeof(double));
+    for (int64_t h = 0; h < heads; ++h) {
+        const float* w = weight ? (const float*)weight->data + (numel(weight) == dim ? 0 : h * dim) : NULL;
+        rope_head(x + h * dim, w, turn, dim, rot, interleaved, eps, t, y + h * dim);
+    }
+    free(t);
+}
+
+void nnc_hip_rope(Tensor* in, Tensor* weight, Tensor* angles, Tensor* positions, Tensor* out, int col, int out_col, int heads,
+                  int dim, int interleaved, float eps) {
+    if (!is_float32("nnc_hip_rope", in)) return;
+    const int64_t ld = in->shape[in->ndim - 1], out_ld = out->shape[out->ndim - 1], rows = ld > 0 ? numel(in) / ld : 0;
+    for (int64_t r = 0; r < rows; ++r)
+        rope_row((const float*)in->data + r * ld + col, weight, angles, positions ? ((const int32_t*)positions->data)[r] : 0, heads, dim,
+                 interleaved, eps, (float*)out->data + r * out_ld + out_col);
+}
+
+void nnc_hip_rope_kv_write(Tensor* q, Tensor* k, Tensor* v, Tensor* q_weight, Tensor* k_weight, Tensor* angles, Tensor* positions,
+                           Tensor* q_out, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table,
+                           Tensor* starts, Tensor* lengths, int q_col, int heads, int k_col, int v_col, int interleaved, float eps) {
+    if (!is_float32("nnc_hip_rope_kv_write", k)) return;
+    const int64_t dim = k_cache->shape[3], kv = k_cache->shape[1];
+    const int64_t k_ld = k->shape[k->ndim - 1], rows = k_ld > 0 ? numel(k) / k_ld : 0;
+    float* turned = (float*)calloc((size_t)(rows * kv * dim + 1), sizeof(float));
+    const int32_t* s = (const int32_t*)starts->data;
+    for (int b = 0; b < table->shape[0]; ++b)
+        for (int64_t r = s[b]; r < s[b + 1]; ++r) {
+            int64_t place = ((const int32_t*)lengths->data)[b] - s[b + 1] + r;
+            if (positions) place = ((const int32_t*)positions->data)[r];
+            rope_row((const float*)k->data + r * k_ld + k_col, k_weight, angles, place, kv, dim, interleaved, eps, turned + r * kv * dim);
+            if (!q) continue;
+            Tensor* to = q_out ? q_out : q;
+            rope_row((const float*)q->data + r * q->shape[q->ndim - 1] + q_col, q_weight, angles, place, heads, dim, interleaved, eps,
+                     (float*)to->data + r * to->shape[to->ndim - 1] + (q_out ? 0 : q_col));
+        }
+    int64_t shape[2] = {rows, kv * dim};
+    Tensor t = {turned, NNC_DTYPE_FLOAT32, shape, 2, rows * kv * dim * 4};
+    nnc_hip_kv_write(&t, v, k_cache, v_cache, k_scale, v_scale, table, starts, lengths, 0, v_col);
+    free(turned);
+}
+
+void nnc_hip_kv_tree_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k_scale, Tensor* v_scale, Tensor* table,
+                               Tensor* starts, Tensor* lengths, Tensor* tree, Tensor* out, int q_col, int heads, float scale,
+                               int window, int max_length) {
+    (void)max_length;
+    if (!is_float32("nnc_hip_kv_tree_attention", q)) return;
+    const int64_t kv = k_cache->shape[1], page = k_cache->shape[2], dim = k_cache->shape[3], group = heads / kv;
+    const int64_t ld = q->shape[q->ndim - 1], most = table->shape[1] * page, words = tree->shape[1];
+    double* p = (double*)malloc((size_t)(most > 0 ? most : 1) * sizeof(double));
+    double* y = (double*)malloc((size_t)(dim > 0 ? dim : 1) * sizeof(double));
+    const int32_t* s = (const int32_t*)starts->data;
+    for (int b = 0; b < table->shape[0]; ++b) {
+        const int64_t length = ((const int32_t*)lengths->data)[b], n = s[b + 1] - s[b], first = length - n;
+        for (int64_t row = s[b]; row < s[b + 1]; ++row) {
+            const uint32_t* mask = (const uint32_t*)tree->data + row * words;
+            int64_t pos = first - 1;
+            for (int64_t m = 0; m < n && m < 32 * words; ++m) pos += mask[m / 32] >> m % 32 & 1;
+            for (int64_t h = 0; h < heads; ++h) {
+                const float* x = (const float*)q->data + row * ld + q_col + h * dim;
+                double top = -INFINITY, sum = 0;
+                for (int64_t j = 0; j < length; ++j) {
+                    const int64_t slot = page_at(table, k_cache, b, j / page), at = slot * kv + h / group, m = j - first;
+                    const int seen = m < 0 ? window <= 0 || j > pos - window : m < 32 * words && (mask[m / 32] >> m % 32 & 1);
+                    p[j] = -INFINITY;
+                    if (slot < 0 || !seen) continue;
+                    const int8_t* key = (const int8_t*)k_cache->data + (at * page + j % page) * dim;
+                    double dot = 0;
+                    for (int64_t d = 0; d < dim; ++d) dot += (double)x[d] * key[d];
+                    p[j] = dot * scale * ((const float*)k_scale->data)[at];
+                    if (isnan(p[j]) || p[j] > top) top = p[j];
+                }
+                for (int64_t d = 0; d < dim; ++d) y[d] = 0;
+                for (int64_t j = 0; j < length; ++j) {
+                    if (p[j] == -INFINITY) continue;
+                    const int64_t slot = page_at(table, k_cache, b, j / page), at = slot * kv + h / group;
+                    const double e = exp(p[j] - top), u = e * ((const float*)v_scale->data)[at];
+                    sum += e;
+                    for (int64_t d = 0; d < dim; ++d) y[d] += u * ((const int8_t*)v_cache->data)[(at * dim + d) * page + j % page];
+                }
+                for (int64_t d = 0; d < dim; ++d)
+                    ((float*)out->data)[(row * heads + h) * dim + d] = sum == 0 ? 0.f : (float)(y[d] / sum);
+            }
+        }
+    }
+    free(p), free(y);
+}
+
+void nnc_hip_token_logprobs(Tensor* logits, Tensor* tokens, Tensor* logprob, Tensor* entropy, Tensor* top_index, Tensor* top_logprob,
+                            float scale) {
+    if (!is_float32("nnc_hip_token_logprobs", logits)) return;
+    const int64_t vocab = logits->shape[logits->ndim - 1], rows = vocab > 0 ? numel(logits) / vocab : 0;
+    const int64_t n = top_index ? top_index->shape[top_index->ndim - 1] : 0;
+    for (int64_t r = 0; r < rows; ++r) {
+        const float* x = (const float*)logits->data + r * vocab;
+        float top = -INFINITY;
+        for (int64_t i = 0; i < vocab; ++i) {
+            if (isnan(x[i]) || x[i] > top) top = x[i];
+            if (isnan(x[i])) break;
+        }
+        double sum = 0, weighted = 0;
+        for (int64_t i = 0; i < vocab; ++i) {
+            const double d = (double)scale * ((double)x[i] - top), e = exp(d);
+            sum += e;
+            if (e > 0) weighted += d * e;
+        }
+        const int ok = isfinite(top);
+        const double log_sum = log(sum);
+        if (entropy) ((float*)entropy->data)[r] = ok ? (float)(log_sum - weighted / sum) : NAN;
+        if (logprob) {
+            const int32_t t = ((const int32_t*)tokens->data)[r];
+            ((float*)logprob->data)[r] = ok && t >= 0 && t < vocab ? (float)((double)scale * ((double)x[t] - top) - log_sum) : NAN;
+        }
+        int64_t last = -1;
+        for (int64_t a = 0; a < n; ++a) {
+            int64_t best = -1;
+            for (int64_t i = 0; ok && i < vocab; ++i) {
+                const int after = last < 0 || x[i] < x[last] || (x[i] == x[last] && i > last);
+                if (after && (best < 0 || x[i] > x[best])) best = i;
+            }
+            ((int32_t*)top_index->data)[r * n + a] = (int32_t)best;
+            ((float*)top_logprob->data)[r * n + a] =
+                best < 0 ? (ok ? -INFINITY : NAN) : (float)((double)scale * ((double)x[best] - top) - log_sum);
+            if (best < 0) {
+                for (++a; a < n; ++a) {
+                    ((int32_t*)top_index->data)[r * n + a] = -1;
+                    ((float*)top_logprob->data)[r * n + a] = ok ? -INFINITY : NAN;
+                }
+                break;
+            }
+            last = best;
+        }
+    }
+}
