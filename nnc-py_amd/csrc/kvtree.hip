@@ -5,10 +5,22 @@
 //   j < first, or j = first + m for the rows m that row i's mask names
 //
 // with first the position of the sequence's first new row: a tree of drafts,
-// whose branches do not see each other, behind a common context.
+// whose branches do not see each other, behind a common context. Scores, weights
+// and sums as in kvattention.hip, a lane having the scores of 16 consecutive
+// keys for a query row.
+//
+// Drafts are many rows for one cached head - tokens times the heads of a group -
+// but not enough to hide that the cache has to be read, and the keys are many.
+// So a wave takes up to 64 query rows (4 blocks of 16) with 64 keys at a time:
+// a key's whole numbers are made f16 once for all of them and stay in
+// registers, and waves need no barrier until their rows are joined. The keys of
+// all sequences and heads, in units of 64 for each wave, are one line that is cut
+// into as many runs as there are CUs, so that ragged lengths leave none idle:
+// what a run has of a sequence that others share is stored, and the last to
+// arrive joins the shares in their order.
 #include <limits.h>
 
-#include "quant8.h"
+#include "kvattn.h"
 
 namespace nnc {
 
@@ -19,97 +31,552 @@ struct TreeArgs {
     const int* tree;  // [rows][words]
     const void* q;
     void* out;
+    float* part;    // [run][2][row of the tile][dim + 4]: sums, m, l, e
+    int* counters;  // [cached head][tile], zero
     int64_t ld;
-    int q_col, heads, kv_heads, group, window, words;
+    int64_t tiles;  // for each cached head, at most
+    int q_col, heads, kv_heads, group, window, words, least;
+    uint32_t slot_magic;
+    bool q_vec;   // query rows start on 16 bytes
     float scale;  // with log2(e)
 };
 
-// A workgroup to a row and head, a wave to 64 keys at a time, a key a lane for
-// the scores and a dim a lane for the values. Float32 throughout.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_tree_k(TreeArgs a) {
-    constexpr int PER = D / 64 ? D / 64 : 1;
-    __shared__ float qs[D], ps[4][64], os[4][D], ml[2][4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int head = blockIdx.y, head_kv = head / a.group;
-    int at = blockIdx.x;
-    const int b = find_share(at, a.g.batch, [&](int s) { return span_of(a.g, s).rows; });
-    if (b < 0) return;
-    const Span span = span_of(a.g, b);
-    const int first = span.first();
-    const int64_t row = span.end - span.rows + at;
-    const int* mask = a.tree + row * a.words;
-    int low = INT_MIN;
-    if (a.window > 0) low = first + tree_depth(mask, a.words, span.rows) - 1 - a.window;
-    const T* qp = (const T*)a.q + row * a.ld + a.q_col + (int64_t)head * D;
-    for (int d = threadIdx.x; d < D; d += 256) qs[d] = (float)qp[d];
-    __syncthreads();
-    const int page = a.g.page;
-    float m = -INFINITY, l = 0.f, o[PER] = {};
-    for (int tb = 64 * wave; tb < span.length; tb += 256) {
-        const int j = tb + lane;
-        const uint32_t bits = tree_bits(mask, a.words, first, span.length, j & ~15);
-        const int pn = j < span.length ? page_at(a.g, b, j / page) : -1;
-        float s = -INFINITY, u = 0.f;
-        if (pn >= 0 && (bits >> (j & 15) & 1) && (j >= first || j > low)) {
-            const int64_t plane = (int64_t)pn * a.kv_heads + head_kv;
-            const int8_t* k = a.k + (plane * page + j % page) * D;
-            float dot = 0.f;
-            for (int d = 0; d < D; ++d) dot = fmaf(qs[d], (float)k[d], dot);
-            s = dot * (a.k_scale[plane] * a.scale);
-            u = a.v_scale[plane];
+// The keys that rows of a sequence see, [lo, hi), and the tiles and units that
+// they make for each cached head.
+struct TreeSpan {
+    Span span;
+    int lo, tiles, units;
+    __device__ __forceinline__ TreeSpan(const TreeArgs& a, int b, int tile, int stride) : span(span_of(a.g, b)) {
+        tiles = query_tiles(span, a.group, tile);
+        // a row's position is first - 1 at least
+        const int first = span.first();
+        lo = a.window > 0 && first > a.window ? (first - a.window) & ~63 : 0;
+        units = max(1, (span.length - lo + stride - 1) / stride);
+    }
+};
+
+// Unit u of one cached head's: the sequence, u's place in it, and the tiles
+// before; how many units there are if u is -1. Every wave for itself, 64 sequences at a time.
+struct TreePlace {
+    int b;
+    int64_t u;
+    int64_t tiles;
+};
+__device__ __forceinline__ TreePlace locate(const TreeArgs& a, int64_t u, int tile, int stride) {
+    const int lane = threadIdx.x & 63;
+    int64_t units = 0, tiles = 0;
+    for (int base = 0; base < a.g.batch; base += 64) {
+        int64_t mine = 0, units_each = 0;
+        int t = 0;
+        if (base + lane < a.g.batch) {
+            const TreeSpan s(a, base + lane, tile, stride);
+            units_each = s.units, t = s.tiles;
+            mine = t * units_each;
         }
-        float top = s;
+        // (starts that decrease would make more tiles than there are counters for)
+        int upto_t = t;
 #pragma unroll
-        for (int x = 1; x < 64; x <<= 1) top = max_nan(top, __shfl_xor(top, x));
-        const float mn = max_nan(m, top), base = mn == -INFINITY ? 0.f : mn;
-        const float alpha = exp2f(m - base), p = s == -INFINITY ? 0.f : exp2f(s - base);
-        l = l * alpha + wave_add(p);
-        m = mn;
-        ps[wave][lane] = p == 0.f ? 0.f : p * u;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        for (int o = 1; o < 64; o <<= 1) {
+            const int below = __shfl_up(upto_t, o);
+            if (lane >= o) upto_t += below;
+        }
+        const int before_t = upto_t - t;
+        const int64_t room = a.tiles - tiles - before_t;
+        if (room < t) t = room > 0 ? (int)room : 0, mine = t * units_each;
+        int64_t upto = mine;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int d = lane + 64 * i;
-            o[i] *= alpha;
-            if (d < D)
-                for (int c = 0; c < 64; c += 16) {
-                    const int pc = tb + c < span.length ? page_at(a.g, b, (tb + c) / page) : -1;
-                    if (pc < 0) continue;
-                    const int8_t* v = a.v + (((int64_t)pc * a.kv_heads + head_kv) * D + d) * page + (tb + c) % page;
-                    for (int e = 0; e < 16; ++e)
-                        if (ps[wave][c + e] != 0.f) o[i] = fmaf(ps[wave][c + e], (float)v[e], o[i]);
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t below = __shfl_up((long long)upto, o);
+            if (lane >= o) upto += below;
+        }
+        const int64_t all = __shfl((long long)upto, 63);
+        if (u >= 0 && u - units < all) {
+            const int at = __ffsll((unsigned long long)__ballot(upto > u - units)) - 1;
+            return TreePlace{base + at, u - units - __shfl((long long)(upto - mine), at), tiles + __shfl(before_t, at)};
+        }
+        units += all;
+        tiles += __shfl(upto_t, 63);
+        if (tiles >= a.tiles) break;
+    }
+    return TreePlace{-1, units, a.tiles};
+}
+
+// A run's share of an item: units [unit, unit + n) of a tile and cached head.
+struct TreeShare {
+    Span span;
+    int b, tile, head_kv, lo, unit, n;
+    bool whole;
+};
+
+template <int D, int R>
+struct TreePlaces {
+    static constexpr int ROW = D + 4;
+    __amdgpu_buffer_rsrc_t r;
+    __device__ __forceinline__ explicit TreePlaces(const TreeArgs& a) : r(make_rsrc(a.part)) {}
+    __device__ __forceinline__ uint32_t at(int place, int row, int col) const { return (uint32_t)((place * R + row) * ROW + col) * 4u; }
+    __device__ __forceinline__ void put4(int place, int row, int col, float x, float y, float z, float w) const {
+        typedef unsigned ux4 __attribute__((ext_vector_type(4)));
+        __builtin_amdgcn_raw_buffer_store_b128(ux4{__float_as_uint(x), __float_as_uint(y), __float_as_uint(z), __float_as_uint(w)}, r,
+                                               (int)at(place, row, col), 0, kDeviceScope);
+    }
+};
+
+// The shares of an item, joined by the workgroup that arrives last: kJoin of
+// them at a time, each row's maxima and divisors first, then 4 dims of a row a
+// thread. place(s) is where share s is; out(row) the row's output.
+static constexpr int kJoin = 32;
+template <typename T, int D, int R, int THREADS, class Place, class Out>
+__device__ __forceinline__ void join_shares(const TreePlaces<D, R>& from, int rows, int shares, Place place, Out out, float* lds) {
+    constexpr int QUADS = D / 4, PER = (R * QUADS + THREADS - 1) / THREADS, AHEAD = PER >= 8 ? 4 : 8;
+    static_assert(R <= THREADS && kJoin <= THREADS, "a thread each");
+    float (*ms)[R] = reinterpret_cast<float (*)[R]>(lds);             // [kJoin][R]
+    float (*ls)[R] = reinterpret_cast<float (*)[R]>(lds + kJoin * R), (*es)[R] = reinterpret_cast<float (*)[R]>(lds + 2 * kJoin * R);
+    float* scale = lds + 3 * kJoin * R;  // [R]
+    float* exps = scale + R;             // [R]
+    int* places = reinterpret_cast<int*>(exps + R);  // [kJoin]
+    const int tid = threadIdx.x;
+    auto row_of = [&](int q) { return min((tid + THREADS * q) / QUADS, R - 1); };
+    float top = kNone, e = kUnseen, sum = 0.f;  // of row tid
+    f32x4 o[PER];
+#pragma unroll
+    for (int q = 0; q < PER; ++q) o[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < shares; s0 += kJoin) {
+        const int n = min(kJoin, shares - s0);
+        __syncthreads();
+        if (tid < n) places[tid] = place(s0 + tid);
+        __syncthreads();
+        for (int k = tid; k < n * R; k += THREADS) {
+            const int sh = k / R, row = k % R;
+            const f32x4 x = load_partial4(from.r, from.at(places[sh], min(row, rows - 1), D));
+            ms[sh][row] = x[0], ls[sh][row] = x[1], es[sh][row] = x[2];
+        }
+        __syncthreads();
+        if (tid < R) {
+            float m = top, far = reference(top, e);
+            for (int sh = 0; sh < n; ++sh) m = fmaxf(m, ms[sh][tid]), far = fmaxf(far, reference(ms[sh][tid], es[sh][tid]));
+            const float en = exponent(m, far);
+            sum *= rescale(top, e, m, en);
+            for (int sh = 0; sh < n; ++sh) {
+                sum = fmaf(rescale(ms[sh][tid], es[sh][tid], m, en), ls[sh][tid], sum);
+                ms[sh][tid] = __builtin_amdgcn_exp2f(ms[sh][tid] - m);
+            }
+            scale[tid] = __builtin_amdgcn_exp2f(top - m);
+            top = m, e = en;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < PER; ++q) o[q] *= scale[row_of(q)];
+        for (int t = 0; t < n; t += AHEAD) {
+            f32x4 v[AHEAD][PER];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int q = 0; q < PER; ++q)
+                    v[u][q] = load_partial4(from.r, from.at(places[min(t + u, n - 1)], min(row_of(q), rows - 1), (tid + THREADS * q) % QUADS * 4));
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int q = 0; q < PER; ++q) {
+                    const float w = t + u < n ? ms[min(t + u, n - 1)][row_of(q)] : 0.f;
+                    o[q] += v[u][q] * w;
                 }
         }
-        __builtin_amdgcn_wave_barrier();
     }
-    if (lane == 0) ml[0][wave] = m, ml[1][wave] = l;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (lane + 64 * i < D) os[wave][lane + 64 * i] = o[i];
     __syncthreads();
-    float top = -INFINITY, sum = 0.f;
-    for (int w = 0; w < 4; ++w) top = max_nan(top, ml[0][w]);
-    const float base = top == -INFINITY ? 0.f : top;
-    for (int w = 0; w < 4; ++w) sum += ml[1][w] * exp2f(ml[0][w] - base);
-    T* out = (T*)a.out + (row * a.heads + head) * D;
-    for (int d = threadIdx.x; d < D; d += 256) {
-        float y = 0.f;
-        for (int w = 0; w < 4; ++w) y += os[w][d] * exp2f(ml[0][w] - base);
-        out[d] = (T)(sum == 0.f ? 0.f : y / sum);
+    if (tid < R) scale[tid] = sum == 0.f ? 0.f : 1.0f / sum, exps[tid] = e;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+        const int row = row_of(q), d = (tid + THREADS * q) % QUADS * 4;
+        if (row >= rows || tid + THREADS * q >= R * QUADS) continue;
+        T v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float y = o[q][r];
+            v[r] = (T)ldexpf(y * scale[row], (int)exps[row]);
+        }
+        __builtin_memcpy(__builtin_assume_aligned(out(row) + d, 4 * sizeof(T)), v, sizeof v);
     }
 }
 
-template <typename T>
-static void launch_tree(const char* name, const TreeArgs& a, int dim) {
-    const dim3 grid((unsigned)a.g.rows, (unsigned)a.heads);
-    switch (dim) {
-        case 32: return launch(name, kv_tree_k<T, 32>, grid, dim3(256), 0, a);
-        case 64: return launch(name, kv_tree_k<T, 64>, grid, dim3(256), 0, a);
-        case 128: return launch(name, kv_tree_k<T, 128>, grid, dim3(256), 0, a);
-        default: return launch(name, kv_tree_k<T, 256>, grid, dim3(256), 0, a);
+// NB blocks of 16 query rows of a tile of R against a share's keys: to the
+// output if the share is whole, else to its place.
+template <typename T, int D, int R, int NB, int NW>
+__device__ __forceinline__ void tree_share(const TreeArgs& a, const TreeShare& w, int place, float* lds) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int STRIDE = 64 * NW, STEPS = D / 32, PIECES = F32 ? 2 : 1, KV = D / 16;
+    f16x8* qs = reinterpret_cast<f16x8*>(lds);                    // [NB][STEPS][PIECES][lane]
+    int* rows = reinterpret_cast<int*>(lds + R * D / 2 * PIECES);  // [R]: row of the activations, -1: none
+    int* lows = rows + R;                                          // [R]: the last position that a window hides
+    int* ups = lows + R;                                           // [R]: the power of two that the row's pieces are scaled by
+    float* ml = reinterpret_cast<float*>(ups + R);                 // [3][NW][R]
+    float* os = ml + 3 * NW * R;                                   // [NW / 2][R][D + 4]
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Span& span = w.span;
+    const int first = span.first();
+    const int64_t all = (int64_t)span.rows * a.group;
+    const int to = min(span.length, w.lo + (w.unit + w.n) * STRIDE);
+
+    const int page = a.g.page, page16 = page / 16, wide = a.g.width - 1;
+    const int64_t plane = (int64_t)page * D, page_bytes = (int64_t)a.kv_heads * plane;
+    const int* table = a.g.table + (int64_t)w.b * a.g.width;
+    const int8_t* kbase = a.k + (int64_t)w.head_kv * plane + (int64_t)(i & 3) * D + g * (D / 4);
+    const int8_t* vbase = a.v + (int64_t)w.head_kv * plane + i * page;
+    int kid, vid;
+    auto find = [&](int tb) {
+        kid = table[min((int)slot_of(tb / 16 + (i >> 2), a.slot_magic), wide)];
+        vid = table[min((int)slot_of(tb / 16 + g, a.slot_magic), wide)];
+    };
+    ix2 kb[4][D / 32];
+    ix4 vb[KV];
+    float ks, vs;
+    bool have;
+    auto load_k = [&](int tb) {
+        const int t16 = tb / 16 + (i >> 2), off = (t16 - (int)slot_of(t16, a.slot_magic) * page16) * 16;
+        const int64_t pn = kid >= 0 && kid < a.g.pages && t16 * 16 < to ? kid : 0;
+        const int8_t* p = kbase + pn * page_bytes + off * D;
+#pragma unroll
+        for (int bl = 0; bl < 4; ++bl)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) kb[bl][c] = *reinterpret_cast<const ix2*>(p + bl * 4 * D + 8 * c);
+    };
+    auto load_v = [&](int tb) {
+        const int t16 = tb / 16 + g, off = (t16 - (int)slot_of(t16, a.slot_magic) * page16) * 16;
+        have = vid >= 0 && vid < a.g.pages && t16 * 16 < to;
+        const int64_t pn = have ? vid : 0;
+        const int8_t* p = vbase + pn * page_bytes + off;
+#pragma unroll
+        for (int c = 0; c < KV; ++c) vb[c] = *reinterpret_cast<const ix4*>(p + c * 16 * page);
+        ks = a.k_scale[pn * a.kv_heads + w.head_kv];
+        vs = a.v_scale[pn * a.kv_heads + w.head_kv];
+    };
+    int tb = w.lo + w.unit * STRIDE + 64 * wave;
+    if (tb < to) find(tb);
+
+    // the query rows' dims g * D / 4 .. + D / 4, by a wave for each block
+    constexpr int QV = 16 / (int)sizeof(T);
+    for (int rb = wave; rb < NB; rb += NW) {
+        const int64_t fr = (int64_t)w.tile * R + 16 * rb + i;
+        const bool ok = fr < all;
+        const int tok = (int)((ok ? fr : 0) / a.group), gh = (int)((ok ? fr : 0) - (int64_t)tok * a.group);
+        const int row = span.end - span.rows + tok;
+        T qx[D / 4];
+        const T* qp = (const T*)a.q + (int64_t)row * a.ld + a.q_col + (w.head_kv * a.group + gh) * D + g * (D / 4);
+        if (a.q_vec) {
+#pragma unroll
+            for (int d = 0; d < D / 4; d += QV) *reinterpret_cast<ix4*>(qx + d) = *reinterpret_cast<const ix4*>(qp + d);
+        } else {
+#pragma unroll
+            for (int d = 0; d < D / 4; ++d) qx[d] = qp[d];
+        }
+        int e = 0;
+        if (F32) {
+            // the row's largest value to [2^13, 2^14)
+            float top = 0.f;
+#pragma unroll
+            for (int d = 0; d < D / 4; ++d) top = fmaxf(top, fabsf((float)qx[d]));
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            (void)frexpf(top, &e);
+            e = top > 0.f && top < INFINITY ? 14 - e : 0;
+        }
+        if (g == 0) {
+            rows[16 * rb + i] = ok ? row : -1;
+            ups[16 * rb + i] = e;
+            lows[16 * rb + i] = a.window > 0 ? first + tree_depth(a.tree + (int64_t)row * a.words, a.words, span.rows) - 1 - a.window : INT_MIN;
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            f16x8 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = F32 ? ldexpf((float)qx[8 * s + j], e) : (float)qx[8 * s + j];
+                hi[j] = (half_t)y;
+                lo[j] = (half_t)(y - (float)hi[j]);
+            }
+            qs[((rb * STEPS + s) * PIECES) * 64 + lane] = hi;
+            if (F32) qs[((rb * STEPS + s) * PIECES + 1) * 64 + lane] = lo;
+        }
     }
+    if (tb < to) {
+        load_k(tb);
+        load_v(tb);
+        find(tb + STRIDE);
+    }
+    __syncthreads();
+    float m[NB], l[NB], ex[NB];  // m and ex the row's, l the lane's
+    fx4 o[NB][KV];
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) {
+        m[rb] = kNone, l[rb] = 0.f, ex[rb] = kUnseen;
+#pragma unroll
+        for (int c = 0; c < KV; ++c) o[rb][c] = fx4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    for (; tb < to; tb += STRIDE) {
+        // scores of keys tb + 16 g + 4 b + r
+        fx4 x[NB][4];
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            f16x8 qf[NB][PIECES];
+#pragma unroll
+            for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+                for (int pc = 0; pc < PIECES; ++pc) qf[rb][pc] = qs[((rb * STEPS + st) * PIECES + pc) * 64 + lane];
+#pragma unroll
+            for (int bl = 0; bl < 4; ++bl) {
+                const f16x8 kf = widen8((uint32_t)kb[bl][st][0], (uint32_t)kb[bl][st][1]);
+#pragma unroll
+                for (int pc = PIECES - 1; pc >= 0; --pc)
+#pragma unroll
+                    for (int rb = 0; rb < NB; ++rb)
+                        x[rb][bl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rb][pc], st == 0 && pc == PIECES - 1 ? fx4{} : x[rb][bl], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(tb + STRIDE);
+        __builtin_amdgcn_sched_barrier(0);
+        const float u = ks * a.scale, log_v = scale_log(vs), inv_v = 1.0f / vs;
+        const bool clear = tb + 64 <= first && a.window <= 0 && __all(have);
+        f16x8 pf[NB][PIECES][2];
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) {
+            float ku = F32 ? ldexpf(u, -ups[16 * rb + i]) : u, lv = log_v, iv = inv_v;
+            ku = ku == 0.f ? 0x1p-126f : ku;  // for the product with -inf
+            float y[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) y[c] = x[rb][c / 4][c % 4];
+            if (!clear) {
+                const int j = tb + 16 * g, row = rows[16 * rb + i];
+                uint32_t bits = have && row >= 0 ? tree_bits(a.tree + (int64_t)row * a.words, a.words, first, span.length, j) : 0u;
+                if (a.window > 0) {  // of the context, up to low
+                    const int n = min(min(lows[16 * rb + i] + 1, first) - j, 16);
+                    if (n > 0) bits &= 0xffffffffu << n;
+                }
+#pragma unroll
+                for (int c = 0; c < 16; ++c) y[c] = bits >> c & 1 ? y[c] : -INFINITY;
+                // a row that sees none of the 16: their scales are not its own
+                if (!bits) ku = 1.f, lv = 0.f, iv = 0.f;
+            }
+            float top = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) top = fmaxf(top, y[c]);
+            float mx = fmaf(top, ku, lv);
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            float factor = ldexpf(iv, (int)ex[rb]);
+            if (__any(mx > m[rb] + kSlack || factor > kMostFactor)) {
+                const float mn = fmaxf(m[rb], mx), alpha = __builtin_amdgcn_exp2f(m[rb] - mn);
+                float far = fmaxf(reference(m[rb], ex[rb]), top * ku);
+                far = fmaxf(far, __shfl_xor(far, 16));
+                far = fmaxf(far, __shfl_xor(far, 32));
+                const float en = exponent(mn, far);
+                l[rb] *= rescale(m[rb], ex[rb], mn, en);
+                m[rb] = mn, ex[rb] = en;
+#pragma unroll
+                for (int c = 0; c < KV; ++c) o[rb][c] *= alpha;
+                factor = ldexpf(iv, (int)ex[rb]);
+                if (__any(factor > kMostFactor)) {
+                    const float base = reference(m[rb], ex[rb]);
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) l[rb] += __builtin_amdgcn_exp2f(fmaf(y[c], ku, -base));
+                    factor = 0.f;
+                }
+            }
+            const float shift = lv - (m[rb] - kPLog);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+                y[c] = __builtin_amdgcn_exp2f(fmaf(y[c], ku, shift));
+                sum += y[c];
+            }
+            l[rb] = fmaf(sum, factor, l[rb]);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const float p0 = y[8 * n + j], p1 = y[8 * n + j + 1];
+                    const f16x2 hi = __builtin_convertvector((fx2{p0, p1}), f16x2);
+                    pf[rb][0][n][j] = hi[0], pf[rb][0][n][j + 1] = hi[1];
+                    if (F32) {
+                        const f16x2 lo = __builtin_convertvector((fx2{p0 - (float)hi[0], p1 - (float)hi[1]}), f16x2);
+                        pf[rb][PIECES - 1][n][j] = lo[0], pf[rb][PIECES - 1][n][j + 1] = lo[1];
+                    }
+                }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int c = 0; c < KV; ++c) {
+                const f16x8 vf = widen8((uint32_t)vb[c][2 * n], (uint32_t)vb[c][2 * n + 1]);
+#pragma unroll
+                for (int pc = PIECES - 1; pc >= 0; --pc)
+#pragma unroll
+                    for (int rb = 0; rb < NB; ++rb) o[rb][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rb][pc][n], o[rb][c], 0, 0, 0);
+            }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(tb + STRIDE);
+        find(tb + 2 * STRIDE);
+    }
+
+    // join the waves: each row's maximum, divisor and exponent, then the upper
+    // half of the waves hands its sums to the lower, until one has all
+    float inv[NB];
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) {
+        l[rb] += __shfl_xor(l[rb], 16);
+        l[rb] += __shfl_xor(l[rb], 32);
+        if (g == 0) {
+            float* mine = ml + wave * R + 16 * rb + i;
+            mine[0] = m[rb], mine[NW * R] = l[rb], mine[2 * NW * R] = ex[rb];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) {
+        const float* r = ml + 16 * rb + i;
+        float top = kNone, far = kNone, sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < NW; ++v) top = fmaxf(top, r[v * R]), far = fmaxf(far, reference(r[v * R], r[(2 * NW + v) * R]));
+        ex[rb] = exponent(top, far);
+#pragma unroll
+        for (int v = 0; v < NW; ++v) sum += r[(NW + v) * R] * rescale(r[v * R], r[(2 * NW + v) * R], top, ex[rb]);
+        const float f = __builtin_amdgcn_exp2f(m[rb] - top);
+#pragma unroll
+        for (int c = 0; c < KV; ++c) o[rb][c] *= f;
+        m[rb] = top, l[rb] = sum;
+        inv[rb] = sum == 0.f ? 0.f : 1.0f / sum;
+    }
+#pragma unroll
+    for (int n = NW / 2; n > 0; n /= 2) {
+        if (wave >= n && wave < 2 * n)
+#pragma unroll
+            for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+                for (int c = 0; c < KV; ++c) *reinterpret_cast<fx4*>(os + ((wave - n) * R + 16 * rb + i) * (D + 4) + 16 * c + 4 * g) = o[rb][c];
+        __syncthreads();
+        if (wave < n)
+#pragma unroll
+            for (int rb = 0; rb < NB; ++rb)
+#pragma unroll
+                for (int c = 0; c < KV; ++c) o[rb][c] += *reinterpret_cast<const fx4*>(os + (wave * R + 16 * rb + i) * (D + 4) + 16 * c + 4 * g);
+        __syncthreads();
+    }
+    if (wave > 0) return;
+    const TreePlaces<D, R> places(a);
+#pragma unroll
+    for (int rb = 0; rb < NB; ++rb) {
+        const int row = rows[16 * rb + i];
+        if (row < 0) continue;
+        if (w.whole) {
+            const int tok = row - (span.end - span.rows), gh = (int)((int64_t)w.tile * R + 16 * rb + i - (int64_t)tok * a.group);
+            T* op = (T*)a.out + ((int64_t)row * a.heads + w.head_kv * a.group + gh) * D + 4 * g;
+#pragma unroll
+            for (int c = 0; c < KV; ++c) {
+                T v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = (T)ldexpf(o[rb][c][r] * inv[rb], (int)ex[rb]);
+                __builtin_memcpy(__builtin_assume_aligned(op + 16 * c, 4 * sizeof(T)), v, sizeof v);
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < KV; ++c) {
+                const float p = o[rb][c][0], q = o[rb][c][1], r = o[rb][c][2], s = o[rb][c][3];
+                places.put4(place, 16 * rb + i, 16 * c + 4 * g, p, q, r, s);
+            }
+            if (g == 0) places.put4(place, 16 * rb + i, D, m[rb], l[rb], ex[rb], 0.f);
+        }
+    }
+}
+
+template <typename T, int D, int RB, int NW>
+__global__ void __launch_bounds__(64 * NW, NW / 4) kv_tree_k(TreeArgs a) {
+    constexpr int STRIDE = 64 * NW, R = 16 * RB;
+    extern __shared__ __align__(16) float tree_lds[];
+    const TreePlace sum = locate(a, -1, R, STRIDE);
+    const int64_t total = sum.u * a.kv_heads;
+    // runs of `least` units or more
+    const int64_t useful = (total + a.least - 1) / a.least;
+    const int runs = __builtin_amdgcn_readfirstlane((int)(useful < gridDim.x ? useful : gridDim.x));
+    if ((int)blockIdx.x >= runs) return;
+    const int run = xcd_remap(blockIdx.x, runs);
+    const int64_t end = run_begin(run + 1, total, runs);
+    for (int64_t at = run_begin(run, total, runs); at < end;) {
+        const int head_kv = (int)(at / sum.u);
+        const TreePlace p = locate(a, at - head_kv * sum.u, R, STRIDE);
+        const int b = __builtin_amdgcn_readfirstlane(p.b);
+        const TreeSpan s(a, b, R, STRIDE);
+        TreeShare w;
+        w.span = s.span, w.b = b, w.head_kv = __builtin_amdgcn_readfirstlane(head_kv), w.lo = s.lo;
+        w.tile = __builtin_amdgcn_readfirstlane((int)(p.u / s.units));
+        w.unit = __builtin_amdgcn_readfirstlane((int)(p.u - (int64_t)w.tile * s.units));
+        w.n = __builtin_amdgcn_readfirstlane((int)(end - at < s.units - w.unit ? end - at : s.units - w.unit));
+        w.whole = w.n == s.units;
+        const int64_t begin = at - w.unit;  // of the item
+        const int place = share_place(run, begin, total, runs);
+        const int64_t left = (int64_t)s.span.rows * a.group - (int64_t)w.tile * R;
+        const int blocks = left >= R ? RB : (int)((left + 15) / 16);
+        if (RB > 2 && blocks > 2)
+            tree_share<T, D, R, RB, NW>(a, w, place, tree_lds);
+        else if (RB > 1 && blocks > 1)
+            tree_share<T, D, R, 2, NW>(a, w, place, tree_lds);
+        else
+            tree_share<T, D, R, 1, NW>(a, w, place, tree_lds);
+        if (!w.whole) {
+            const int run0 = run_of(begin, total, runs), shares = run_of(begin + s.units - 1, total, runs) - run0 + 1;
+            if (finish_arrive(a.counters + (int64_t)head_kv * a.tiles + p.tiles + w.tile, shares - 1)) {
+                const TreePlaces<D, R> places(a);
+                join_shares<T, D, R, 64 * NW>(
+                    places, (int)min((int64_t)R, left), shares, [&](int sh) { return share_place(run0 + sh, begin, total, runs); },
+                    [&](int r) {
+                        const int64_t f = (int64_t)w.tile * R + r;
+                        const int t = (int)(f / a.group), head = w.head_kv * a.group + (int)(f - (int64_t)t * a.group);
+                        return (T*)a.out + ((int64_t)(s.span.end - s.span.rows + t) * a.heads + head) * D;
+                    },
+                    tree_lds);
+            }
+        }
+        at += w.n;
+        __syncthreads();  // the LDS is the next share's
+    }
+}
+
+template <typename T, int D, int RB, int NW>
+constexpr int tree_lds_bytes() {
+    constexpr int share = 4 * 16 * RB * (D / 2 * (sizeof(T) == 4 ? 2 : 1) + 3 + 3 * NW + NW / 2 * (D + 4)), join = 4 * (16 * RB * (3 * kJoin + 2) + kJoin);
+    return share > join ? share : join;
+}
+
+template <typename T, int D, int RB, int NW>
+static void launch_blocks(const char* name, TreeArgs& a, int64_t rows) {
+    auto kernel = kv_tree_k<T, D, RB, NW>;
+    constexpr int lds = tree_lds_bytes<T, D, RB, NW>();
+    static const bool ok = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
+    if (!ok) return fail(NNC_HIP_EDEVICE, name, "hipFuncSetAttribute failed");
+    const int runs = cu_count();
+    a.tiles = query_tiles_bound(rows, a.g.batch, a.group, 16 * RB);
+    const int64_t items = a.tiles * a.kv_heads;
+    const size_t bytes = (size_t)runs * 2 * 16 * RB * (D + 4) * sizeof(float);
+    if (items > INT32_MAX) return fail(NNC_HIP_EUNSUPP, name, "%lld rows of %d heads", (long long)rows, a.heads);
+    a.part = workspace(bytes);
+    a.counters = tile_counters((size_t)items);
+    if (!a.part || !a.counters) return fail(NNC_HIP_ENOMEM, name, "no workspace for %zu bytes of partial sums", bytes);
+    launch(name, kernel, dim3((unsigned)runs), dim3(64 * NW), lds, a);
+}
+
+// Blocks of 16 query rows of a tile
+template <typename T, int D>
+static void launch_tree(const char* name, TreeArgs& a, int64_t rows) {
+    const int64_t holders = rows < a.g.batch ? rows : a.g.batch, each = ceil_div(rows * a.group, holders);
+    constexpr int MOST = D <= 64 ? 4 : D == 128 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T) == 2 ? 2 : 1;
+    if constexpr (MOST >= 4) {
+        if (each > 32) return launch_blocks<T, D, 4, 4>(name, a, rows);
+    }
+    if constexpr (MOST >= 2) {
+        if (each > 16) return launch_blocks<T, D, 2, 4>(name, a, rows);
+    }
+    launch_blocks<T, D, 1, 4>(name, a, rows);
 }
 
 }  // namespace nnc
@@ -146,15 +613,20 @@ void nnc_hip_kv_tree_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tens
     if (!ready(name)) return;
     const int capacity = c.ragged.width * c.page;
     const int longest = max_length > 0 && max_length < capacity ? max_length : capacity;
-    TreeArgs a{c.ragged, c.k, c.v, c.k_scale, c.v_scale, (const int*)tree->data, q->data, out->data, ld, q_col, heads, c.kv_heads,
-               group, window_of(window, capacity), (int)tree->shape[1], scale * 1.44269504088896340736f};
+    TreeArgs a{c.ragged, c.k, c.v, c.k_scale, c.v_scale, (const int*)tree->data, q->data, out->data, nullptr, nullptr, ld, 0, q_col, heads,
+               c.kv_heads, group, window_of(window, capacity), (int)tree->shape[1], 2, slot_magic(c.page / 16),
+               aligned16(q->data) && ld * activation_bytes(q) % 16 == 0 && q_col * activation_bytes(q) % 16 == 0,
+               scale * 1.44269504088896340736f};
     a.g.rows = (int)rows;
     const int64_t reach = a.window > 0 ? (int64_t)a.window - 1 + ceil_div(rows, c.ragged.batch) : longest;
     set_work(0.0, 2.0 * c.kv_heads * c.dim * (double)(reach < longest ? reach : longest) * c.ragged.batch);
-    if (q->dtype == NNC_DTYPE_FLOAT16)
-        launch_tree<half_t>(name, a, c.dim);
-    else
-        launch_tree<float>(name, a, c.dim);
+    const bool f16 = q->dtype == NNC_DTYPE_FLOAT16;
+    switch (c.dim) {
+        case 32: return f16 ? launch_tree<half_t, 32>(name, a, rows) : launch_tree<float, 32>(name, a, rows);
+        case 64: return f16 ? launch_tree<half_t, 64>(name, a, rows) : launch_tree<float, 64>(name, a, rows);
+        case 128: return f16 ? launch_tree<half_t, 128>(name, a, rows) : launch_tree<float, 128>(name, a, rows);
+        default: return f16 ? launch_tree<half_t, 256>(name, a, rows) : launch_tree<float, 256>(name, a, rows);
+    }
 }
 
 }  // extern "C"

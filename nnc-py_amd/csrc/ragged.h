@@ -133,6 +133,17 @@ RAGGED_HD int tree_depth(const int* mask, int words, int rows) {
     return n;
 }
 
+// `total` units of work, one after the other, in `parts` runs of equal length:
+// run p has [run_begin(p), run_begin(p + 1)), and unit i is in run_of(i). An
+// item, a range of units, that several runs have a share of is put together
+// from a place for each: a run has two, as its first or a later range is such a
+// share; those between are whole items.
+RAGGED_HD int64_t run_begin(int64_t p, int64_t total, int parts) { return p * total / parts; }
+RAGGED_HD int run_of(int64_t i, int64_t total, int parts) { return (int)(((i + 1) * parts - 1) / total); }
+RAGGED_HD int share_place(int run, int64_t item_begin, int64_t total, int parts) {
+    return 2 * run + (item_begin > run_begin(run, total, parts) ? 1 : 0);
+}
+
 // The window that is compared: none (0) if it is as long as a sequence can be,
 // so that positions less it stay far from the smallest number.
 RAGGED_HD int window_of(int window, int capacity) { return window < capacity ? window : 0; }

@@ -34,5 +34,29 @@ int main() {
         for (int m = 0; m < rows; ++m) depth += bit(m);
         if (tree_depth(mask.data(), words, rows) != depth) return printf("depth in trial %d\n", trial), 1;
     }
+    // runs cover the units once, and the shares of an item have places of their own
+    for (int trial = 0; trial < 3000; ++trial) {
+        const int parts = rnd(1, 40), items = rnd(1, 30);
+        std::vector<int64_t> begin(1, 0);
+        for (int n = 0; n < items; ++n) begin.push_back(begin.back() + rnd(1, rnd(0, 1) ? 3 : 60));
+        const int64_t total = begin.back();
+        if (parts > total) continue;
+        std::vector<int> seen(total, 0), taken(2 * parts, 0);
+        for (int p = 0; p < parts; ++p)
+            for (int64_t i = run_begin(p, total, parts); i < run_begin(p + 1, total, parts); ++i) {
+                ++seen[i];
+                if (run_of(i, total, parts) != p) return printf("run of %lld in trial %d\n", (long long)i, trial), 1;
+            }
+        for (int n : seen)
+            if (n != 1) return printf("units in trial %d\n", trial), 1;
+        for (int n = 0; n < items; ++n) {
+            const int first = run_of(begin[n], total, parts), last = run_of(begin[n + 1] - 1, total, parts);
+            if (first == last) continue;  // whole
+            for (int p = first; p <= last; ++p) {
+                const int at = share_place(p, begin[n], total, parts);
+                if (at < 0 || at >= 2 * parts || taken[at]++) return printf("place in trial %d\n", trial), 1;
+            }
+        }
+    }
     puts("ok");
 }
