@@ -339,15 +339,15 @@ __device__ __forceinline__ void tree_share(const TreeArgs& a, const TreeShare& w
         __builtin_amdgcn_sched_barrier(0);
         const float u = ks * a.scale, log_v = scale_log(vs), inv_v = 1.0f / vs;
         const bool clear = tb + 64 <= first && a.window <= 0 && __all(have);
-        f16x8 pf[NB][PIECES][2];
+        float ku[NB], lv[NB], iv[NB], top[NB], mx[NB], factor[NB];
 #pragma unroll
         for (int rb = 0; rb < NB; ++rb) {
-            float ku = F32 ? ldexpf(u, -ups[16 * rb + i]) : u, lv = log_v, iv = inv_v;
-            ku = ku == 0.f ? 0x1p-126f : ku;  // for the product with -inf
-            float y[16];
+            ku[rb] = F32 ? ldexpf(u, -ups[16 * rb + i]) : u, lv[rb] = log_v, iv[rb] = inv_v;
+            ku[rb] = ku[rb] == 0.f ? 0x1p-126f : ku[rb];  // for the product with -inf
+        }
+        if (!clear) {
 #pragma unroll
-            for (int c = 0; c < 16; ++c) y[c] = x[rb][c / 4][c % 4];
-            if (!clear) {
+            for (int rb = 0; rb < NB; ++rb) {
                 const int j = tb + 16 * g, row = rows[16 * rb + i];
                 uint32_t bits = have && row >= 0 ? tree_bits(a.tree + (int64_t)row * a.words, a.words, first, span.length, j) : 0u;
                 if (a.window > 0) {  // of the context, up to low
@@ -355,20 +355,35 @@ __device__ __forceinline__ void tree_share(const TreeArgs& a, const TreeShare& w
                     if (n > 0) bits &= 0xffffffffu << n;
                 }
 #pragma unroll
-                for (int c = 0; c < 16; ++c) y[c] = bits >> c & 1 ? y[c] : -INFINITY;
+                for (int c = 0; c < 16; ++c) {
+                    const float y = x[rb][c / 4][c % 4];
+                    x[rb][c / 4][c % 4] = bits >> c & 1 ? y : -INFINITY;
+                }
                 // a row that sees none of the 16: their scales are not its own
-                if (!bits) ku = 1.f, lv = 0.f, iv = 0.f;
+                if (!bits) ku[rb] = 1.f, lv[rb] = 0.f, iv[rb] = 0.f;
             }
-            float top = -INFINITY, sum = 0.f;
+        }
+        bool move = false;
 #pragma unroll
-            for (int c = 0; c < 16; ++c) top = fmaxf(top, y[c]);
-            float mx = fmaf(top, ku, lv);
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            float factor = ldexpf(iv, (int)ex[rb]);
-            if (__any(mx > m[rb] + kSlack || factor > kMostFactor)) {
-                const float mn = fmaxf(m[rb], mx), alpha = __builtin_amdgcn_exp2f(m[rb] - mn);
-                float far = fmaxf(reference(m[rb], ex[rb]), top * ku);
+        for (int rb = 0; rb < NB; ++rb) {
+            top[rb] = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) top[rb] = fmaxf(top[rb], x[rb][c / 4][c % 4]);
+            mx[rb] = fmaf(top[rb], ku[rb], lv[rb]);
+        }
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) mx[rb] = fmaxf(mx[rb], __shfl_xor(mx[rb], 16));
+#pragma unroll
+        for (int rb = 0; rb < NB; ++rb) {
+            mx[rb] = fmaxf(mx[rb], __shfl_xor(mx[rb], 32));
+            factor[rb] = ldexpf(iv[rb], (int)ex[rb]);
+            move |= mx[rb] > m[rb] + kSlack || factor[rb] > kMostFactor;
+        }
+        if (__any(move)) {
+#pragma unroll
+            for (int rb = 0; rb < NB; ++rb) {
+                const float mn = fmaxf(m[rb], mx[rb]), alpha = __builtin_amdgcn_exp2f(m[rb] - mn);
+                float far = fmaxf(reference(m[rb], ex[rb]), top[rb] * ku[rb]);
                 far = fmaxf(far, __shfl_xor(far, 16));
                 far = fmaxf(far, __shfl_xor(far, 32));
                 const float en = exponent(mn, far);
@@ -376,26 +391,31 @@ __device__ __forceinline__ void tree_share(const TreeArgs& a, const TreeShare& w
                 m[rb] = mn, ex[rb] = en;
 #pragma unroll
                 for (int c = 0; c < KV; ++c) o[rb][c] *= alpha;
-                factor = ldexpf(iv, (int)ex[rb]);
-                if (__any(factor > kMostFactor)) {
-                    const float base = reference(m[rb], ex[rb]);
+                factor[rb] = ldexpf(iv[rb], (int)en);
+                if (__any(factor[rb] > kMostFactor)) {
+                    const float base = reference(m[rb], en);
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) l[rb] += __builtin_amdgcn_exp2f(fmaf(y[c], ku, -base));
-                    factor = 0.f;
+                    for (int c = 0; c < 16; ++c) {
+                        const float y = x[rb][c / 4][c % 4];
+                        l[rb] += __builtin_amdgcn_exp2f(fmaf(y, ku[rb], -base));
+                    }
+                    factor[rb] = 0.f;
                 }
             }
-            const float shift = lv - (m[rb] - kPLog);
+        }
+        f16x8 pf[NB][PIECES][2];
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-                y[c] = __builtin_amdgcn_exp2f(fmaf(y[c], ku, shift));
-                sum += y[c];
-            }
-            l[rb] = fmaf(sum, factor, l[rb]);
+        for (int rb = 0; rb < NB; ++rb) {
+            const float shift = lv[rb] - (m[rb] - kPLog);
+            float sum = 0.f;
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
-                    const float p0 = y[8 * n + j], p1 = y[8 * n + j + 1];
+                    const float s0 = x[rb][2 * n + j / 4][j % 4], s1 = x[rb][2 * n + j / 4][j % 4 + 1];
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s0, ku[rb], shift)), p1 = __builtin_amdgcn_exp2f(fmaf(s1, ku[rb], shift));
+                    sum += p0;
+                    sum += p1;
                     const f16x2 hi = __builtin_convertvector((fx2{p0, p1}), f16x2);
                     pf[rb][0][n][j] = hi[0], pf[rb][0][n][j + 1] = hi[1];
                     if (F32) {
@@ -403,7 +423,7 @@ __device__ __forceinline__ void tree_share(const TreeArgs& a, const TreeShare& w
                         pf[rb][PIECES - 1][n][j] = lo[0], pf[rb][PIECES - 1][n][j + 1] = lo[1];
                     }
                 }
-            __builtin_amdgcn_sched_barrier(0);
+            l[rb] = fmaf(sum, factor[rb], l[rb]);
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -490,8 +510,8 @@ __device__ __forceinline__ void tree_share(const TreeArgs& a, const TreeShare& w
     }
 }
 
-template <typename T, int D, int RB, int NW>
-__global__ void __launch_bounds__(64 * NW, NW / 4) kv_tree_k(TreeArgs a) {
+template <typename T, int D, int RB, int NW, int OCC>
+__global__ void __launch_bounds__(64 * NW, OCC) kv_tree_k(TreeArgs a) {
     constexpr int STRIDE = 64 * NW, R = 16 * RB;
     extern __shared__ __align__(16) float tree_lds[];
     const TreePlace sum = locate(a, -1, R, STRIDE);
@@ -548,13 +568,13 @@ constexpr int tree_lds_bytes() {
     return share > join ? share : join;
 }
 
-template <typename T, int D, int RB, int NW>
+template <typename T, int D, int RB, int NW, int OCC>
 static void launch_blocks(const char* name, TreeArgs& a, int64_t rows) {
-    auto kernel = kv_tree_k<T, D, RB, NW>;
+    auto kernel = kv_tree_k<T, D, RB, NW, OCC>;
     constexpr int lds = tree_lds_bytes<T, D, RB, NW>();
     static const bool ok = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
     if (!ok) return fail(NNC_HIP_EDEVICE, name, "hipFuncSetAttribute failed");
-    const int runs = cu_count();
+    const int runs = cu_count() * OCC;
     a.tiles = query_tiles_bound(rows, a.g.batch, a.group, 16 * RB);
     const int64_t items = a.tiles * a.kv_heads;
     const size_t bytes = (size_t)runs * 2 * 16 * RB * (D + 4) * sizeof(float);
@@ -569,14 +589,11 @@ static void launch_blocks(const char* name, TreeArgs& a, int64_t rows) {
 template <typename T, int D>
 static void launch_tree(const char* name, TreeArgs& a, int64_t rows) {
     const int64_t holders = rows < a.g.batch ? rows : a.g.batch, each = ceil_div(rows * a.group, holders);
-    constexpr int MOST = D <= 64 ? 4 : D == 128 ? (sizeof(T) == 2 ? 4 : 2) : sizeof(T) == 2 ? 2 : 1;
-    if constexpr (MOST >= 4) {
-        if (each > 32) return launch_blocks<T, D, 4, 4>(name, a, rows);
+    if (D <= 128 && each > 32) return launch_blocks<T, D, 2, 4, D <= 128 ? 2 : 1>(name, a, rows);
+    if (D <= 128 || sizeof(T) == 2) {
+        if (each > 16) return launch_blocks<T, D, 2, 4, 1>(name, a, rows);
     }
-    if constexpr (MOST >= 2) {
-        if (each > 16) return launch_blocks<T, D, 2, 4>(name, a, rows);
-    }
-    launch_blocks<T, D, 1, 4>(name, a, rows);
+    launch_blocks<T, D, 1, 4, 1>(name, a, rows);
 }
 
 }  // namespace nnc

@@ -110,9 +110,13 @@ def logprobs(x, scale):
     """log p in float64, entropies, and for each row how far its sum may be off,
     relative, and its entropy besides.
 
-    A term e^d is off by two units of float32's last place (2^-22 of it) and by
-    what rounding d, the difference and its product, does (2^-23 of |d|); the
-    largest, e^0, is exact."""
+    A term e^d is off by the exponential's last place (2^-23), by what rounding
+    the difference, log2 e times the scale, their product and log2 e itself does
+    to d (3.5 * 2^-24 of it) and by the float32 sum of the 32 values that a lane
+    takes at once, two by two (5 * 2^-24): together under 2^-21 + 2^-22 |d|. It is
+    scaled once for each time that a larger maximum turns up in its lane and
+    where lanes (6 steps), waves and segments are joined, each off by 2^-23: 20
+    times at most here. The largest, e^0, is counted."""
     x = x.astype(np.float64)
     with np.errstate(invalid="ignore", over="ignore"):
         top = x.max(1, keepdims=True)
@@ -123,9 +127,9 @@ def logprobs(x, scale):
         lp = np.where(ok[:, None], d - np.log(total)[:, None], np.nan)
         de = np.where(e > 0, np.abs(d) * e, 0)
         h = np.where(ok, np.log(total) + de.sum(1) / total, np.nan)
-        term = np.where(e > 0, (2.0 ** -22 + 2.0 ** -23 * np.where(e > 0, np.abs(d), 0)) * e, 0)
+        term = np.where(e > 0, (2.0 ** -21 + 20 * 2.0 ** -23 + 2.0 ** -22 * np.where(e > 0, np.abs(d), 0)) * e, 0)
         off = (np.where(d == 0, 0, term)).sum(1) / total + 2.0 ** -45
-        off_h = (np.where(e > 0, (np.abs(d) * term + 2.0 ** -23 * de), 0)).sum(1) / total + off * (1 + de.sum(1) / total)
+        off_h = (np.where(e > 0, (np.abs(d) * term + 2.0 ** -22 * de), 0)).sum(1) / total + off * (1 + de.sum(1) / total)
     return lp, h, off, off_h
 
 
