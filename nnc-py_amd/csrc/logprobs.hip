@@ -5,21 +5,19 @@
 //   m = max_i x_i,  S = sum_i e^(t (x_i - m));  log p_i = t (x_i - m) - log S
 //   entropy = log S - sum_i t (x_i - m) e^(t (x_i - m)) / S
 //
-// in one pass with a running maximum for each lane. A row's largest term is 1,
-// and where it leaves 2^-24 and less to all others, entropy and the largest
-// token's log probability are made of those: so terms of the lane's maximum are
-// counted, the others summed for themselves, 16 or 32 of them in float32 and
-// these sums in float64.
+// A workgroup has a segment of a row in registers, so it is read once: maximum,
+// then the sums against it, then the likeliest. A row's largest term is 1, and
+// where it leaves 2^-24 and less to all others, entropy and the largest token's
+// log probability are made of those: so terms that are 1 are counted, the others
+// summed for themselves, two packs of them in float32 and these sums in float64.
 //
-// The likeliest tokens: a wave keeps 64 of them in order, one a lane, as whole
-// numbers that compare as (value, earlier index) do. A batch of a few packs a
-// lane only looks for tokens if one is above the n-th that the wave has; they
-// gather in LDS, and 64 at a time are sorted and merged, which a row needs about
-// n log(vocab / n) / 64 times for each wave. The first bar is the n-th largest of
-// the lanes' maxima in the first batch.
-//
-// Rows are cut into segments while there are fewer than the GPU has room for;
-// the last to arrive joins them.
+// The likeliest tokens: n values at least reach the n-th largest of a wave's lane
+// maxima, and the least of the waves' (n / waves)-th largest; the highest of these
+// bars is what few more than n reach. Those gather in LDS, are sorted, 64 to a
+// wave, as whole numbers that compare as (value, earlier index) do, and merged.
+// If more than 256 reach it (equal values, rows of -infinity), each wave keeps a
+// list of its best 64, one a lane, and merges 64 at a time into it. The last
+// segment to arrive joins a row's segments.
 #include "mfma_tile.h"
 #include "quant8.h"
 
@@ -34,7 +32,8 @@ struct LogprobArgs {
     float* part;    // [row][segment][SLOT]: a segment's sums and tokens
     int* counters;  // [row], zero
     int64_t rows, vocab;
-    int top, segments;
+    int top, segments, each;  // packs of a segment
+    int64_t row0;   // of the launch
     float scale;
 };
 
@@ -57,30 +56,66 @@ __device__ __forceinline__ K larger(K a, K b) { return a > b ? a : b; }
 template <typename K>
 __device__ __forceinline__ K smaller(K a, K b) { return a > b ? b : a; }
 
+// The word of lane ^ J, without a way through LDS: by DPP within 16 lanes, beyond
+// by exchanging rows of 16 and halves of 32.
+template <int J>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
+    const int v = (int)x;
+    if constexpr (J == 1) return (uint32_t)__builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);  // quads 1 0 3 2
+    if constexpr (J == 2) return (uint32_t)__builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);  // quads 2 3 0 1
+    if constexpr (J == 4)  // 7 - i in eights, then 3 - i in quads
+        return (uint32_t)__builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true), 0x1b, 0xf, 0xf, true);
+    if constexpr (J == 8) return (uint32_t)__builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);  // turned by 8
+    if constexpr (J == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return threadIdx.x & 16 ? r[0] : r[1];
+    }
+    if constexpr (J == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return threadIdx.x & 32 ? r[0] : r[1];
+    }
+}
+template <int J>
+__device__ __forceinline__ float lane_xor(float x) { return __uint_as_float(lane_xor<J>(__float_as_uint(x))); }
+template <int J>
+__device__ __forceinline__ u64 lane_xor(u64 x) { return (u64)lane_xor<J>((uint32_t)(x >> 32)) << 32 | lane_xor<J>((uint32_t)x); }
+template <int J>
+__device__ __forceinline__ double lane_xor(double x) { return __longlong_as_double((long long)lane_xor<J>((u64)__double_as_longlong(x))); }
+
 // 64 keys, one a lane, in rising order
-template <typename K>
-__device__ __forceinline__ K sort_rising(K key) {
+template <int RUN, int J, typename K>
+__device__ __forceinline__ K sort_step(K key) {
     const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            const K other = __shfl_xor(key, j);
-            const bool up = (lane & k) == 0, low = (lane & j) == 0;
-            key = up == low ? smaller(key, other) : larger(key, other);
-        }
+    const K other = lane_xor<J>(key);
+    key = ((lane & RUN) == 0) == ((lane & J) == 0) ? smaller(key, other) : larger(key, other);
+    if constexpr (J > 1) return sort_step<RUN, J / 2>(key);
     return key;
 }
+template <typename K>
+__device__ __forceinline__ K sort_rising(K key) {
+    key = sort_step<2, 1>(key);
+    key = sort_step<4, 2>(key);
+    key = sort_step<8, 4>(key);
+    key = sort_step<16, 8>(key);
+    key = sort_step<32, 16>(key);
+    return sort_step<64, 32>(key);
+}
 // The 64 largest of a falling and a rising sequence, falling
-__device__ __forceinline__ u64 merge_falling(u64 falling, u64 rising) {
-    const int lane = threadIdx.x & 63;
-    u64 key = larger(falling, rising);
-#pragma unroll
-    for (int j = 32; j > 0; j >>= 1) {
-        const u64 other = __shfl_xor(key, j);
-        key = (lane & j) == 0 ? larger(key, other) : smaller(key, other);
-    }
+template <int J>
+__device__ __forceinline__ u64 merge_step(u64 key) {
+    const u64 other = lane_xor<J>(key);
+    key = (threadIdx.x & J) == 0 ? larger(key, other) : smaller(key, other);
+    if constexpr (J > 1) return merge_step<J / 2>(key);
     return key;
+}
+__device__ __forceinline__ u64 merge_falling(u64 falling, u64 rising) { return merge_step<32>(larger(falling, rising)); }
+
+// What `op` makes of all lanes' values
+template <int J = 32, typename K, class Op>
+__device__ __forceinline__ K over_lanes(K x, Op op) {
+    x = op(x, lane_xor<J>(x));
+    if constexpr (J > 1) return over_lanes<J / 2>(x, op);
+    return x;
 }
 
 // Sums of a part of a row: the terms e^(t (x - m)) that are less than 1, how
@@ -107,22 +142,95 @@ __device__ __forceinline__ void add_sums(RowSums& s, RowSums t, float c) {
     rebase(s, m, c), rebase(t, m, c);
     s.rest += t.rest, s.ones += t.ones, s.weighted += t.weighted;
 }
-__device__ __forceinline__ RowSums shuffled(const RowSums& s, int o) {
-    return RowSums{__shfl_xor(s.m, o), __shfl_xor(s.rest, o), __shfl_xor(s.ones, o), __shfl_xor(s.weighted, o)};
+
+// 16 bytes of a row, kept as words
+template <typename T>
+struct Words {
+    static constexpr int V = 16 / (int)sizeof(T);
+    static constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xfc00fc00u;  // -infinity
+    __device__ __forceinline__ static float at(nt_u32x4 w, int u) {
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t x = w[u];
+            return __uint_as_float(x);
+        } else {
+            const uint32_t x = w[u / 2];
+            return (float)__builtin_bit_cast(f16x2, x)[u % 2];
+        }
+    }
+    // the words with the next value first
+    __device__ __forceinline__ static nt_u32x4 next(nt_u32x4 w) {
+        if constexpr (sizeof(T) == 4) return nt_u32x4{w[1], w[2], w[3], w[0]};
+        return nt_u32x4{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16};
+    }
+    __device__ __forceinline__ static uint32_t max_of(uint32_t x, uint32_t y) {
+        if constexpr (sizeof(T) == 4)
+            return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+        else
+            return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(f16x2, x), __builtin_bit_cast(f16x2, y)));
+    }
+};
+
+// Takes the values that are the maximum out of a lane's packs; how many.
+template <typename T, int PACKS>
+__device__ __forceinline__ float take_out(nt_u32x4 (&raw)[PACKS], float m) {
+    float ones = 0.f;
+#pragma unroll
+    for (int p = 0; p < PACKS; ++p)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t w = raw[p][u];
+            if constexpr (sizeof(T) == 4) {
+                const bool one = __uint_as_float(w) == m;
+                raw[p][u] = one ? Words<T>::NONE : w;
+                ones += one ? 1.f : 0.f;
+            } else {
+                const f16x2 v = __builtin_bit_cast(f16x2, w);
+                const bool one = (float)v[0] == m, other = (float)v[1] == m;
+                raw[p][u] = (one ? 0xfc00u : w & 0xffffu) | (other ? 0xfc000000u : w & 0xffff0000u);
+                ones += (one ? 1.f : 0.f) + (other ? 1.f : 0.f);
+            }
+            asm volatile("" : "+v"(ones));  // (one after the other: the comparisons of all of them are more than the registers hold)
+        }
+    return ones;
+}
+
+// A lane's packs, without the maximum m, against it: terms 2^t, t = c (x - m). As
+// c x - (c m), one operation, whose second part's rounding is the same for all and
+// put right in the sums; FAR: where that would overflow. (A NaN stays in `rest`.)
+template <typename T, bool FAR, int PACKS>
+__device__ __forceinline__ void sum_packs(nt_u32x4 (&raw)[PACKS], float m, float c, RowSums& s) {
+    constexpr int V = Words<T>::V;
+    const float base = base_of(m), shift = base * c, off = FAR ? 0.f : fmaf(base, c, -shift);
+#pragma unroll
+    for (int p = 0; p < PACKS; p += 2) {
+        float r[4], w[4];
+#pragma unroll
+        for (int u = 0; u < 2 * V; ++u) {
+            const float x = Words<T>::at(raw[p + u / V], u % V);
+            const float t = FAR ? (x - base) * c : fmaf(x, c, -shift), e = __builtin_amdgcn_exp2f(t), far = fmaxf(t, kFar);
+            r[u % 4] = u < 4 ? e : r[u % 4] + e;
+            w[u % 4] = u < 4 ? e * far : fmaf(e, far, w[u % 4]);
+        }
+        s.rest += (r[0] + r[1]) + (r[2] + r[3]);
+        s.weighted += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    if (!FAR) {
+        const double a = 1.0 - 0.69314718055994530942 * (double)off;  // 2^-off, which is 2^-24 of the shift at most
+        s.weighted = a * (s.weighted - off * s.rest);
+        s.rest *= a;
+    }
 }
 
 // A wave's likeliest tokens
 struct Likeliest {
     u64 list;   // falling
     u64 bar;    // the n-th, 0 while there are fewer
-    float over;  // its value
     u64* room;  // [64] LDS
     int held;
-    __device__ __forceinline__ void init(u64* lds) { list = bar = 0, over = -INFINITY, room = lds, held = 0; }
+    __device__ __forceinline__ void init(u64* lds) { list = bar = 0, room = lds, held = 0; }
     __device__ __forceinline__ void merge(u64 rising, int n) {
         list = merge_falling(list, rising);
         bar = __shfl(list, n - 1);
-        over = bar ? value_of(bar) : -INFINITY;
     }
     __device__ __forceinline__ void flush(int n) {
         if (held == 0) return;
@@ -155,113 +263,176 @@ struct Likeliest {
 static constexpr int kSlotHead = 8;
 __host__ __device__ constexpr int slot_floats(int top) { return kSlotHead + 2 * top; }
 
-// NW waves to a segment of a row. A row is read in packs of 16 bytes as they
-// lie in memory: its first and last pack may hold others' values.
-template <typename T, int NW, bool TOP>
+// NW waves to a segment of a row, PACKS packs of 16 bytes a lane as they lie in
+// memory: a row's first and last pack may hold others' values.
+template <typename T, int NW, int PACKS, bool TOP>
 __global__ void __launch_bounds__(64 * NW) logprobs_k(LogprobArgs a) {
-    constexpr int V = 16 / (int)sizeof(T), PACKS = 4;
-    typedef Pack<T, V> P;
+    constexpr int V = Words<T>::V;
     __shared__ RowSums sums[NW];
+    __shared__ float tops[NW], bars[NW], parts[NW];
+    __shared__ int gathered;
     __shared__ u64 room[NW][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float c = a.scale * 1.44269504088896340736f;
-    const int64_t units = a.rows * a.segments;
-    for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-        const int64_t row = unit / a.segments;
-        const int segment = (int)(unit - row * a.segments);
+    const uint32_t line = blockIdx.x / (uint32_t)a.segments, segment = blockIdx.x - line * (uint32_t)a.segments;
+    {
+        const int64_t row = a.row0 + line;
         const T* x = (const T*)a.logits + row * a.vocab;
         const int off = (int)(((uintptr_t)x & 15) / sizeof(T));
-        const P* packs = (const P*)(x - off);
-        const int64_t count = (off + a.vocab + V - 1) / V;  // of packs
-        const int64_t first = segment * count / a.segments, last = (segment + 1) * count / a.segments;
-        RowSums s{-INFINITY, 0.0, 0.0, 0.0};
+        const int64_t first = (int64_t)segment * a.each, rest = (off + a.vocab + V - 1) / V - first;
+        const int n = (int)(rest < a.each ? rest : a.each), at = wave * 64 + lane;
+        const int64_t index0 = first * V - off;  // of the segment's first value, as if its pack were the row's own
+        // packs that are the row's own: [own, own_end) of the segment's
+        const int own = first == 0 && off > 0 ? 1 : 0, own_end = rest <= a.each && (off + a.vocab) % V ? n - 1 : n;
+        const nt_u32x4* packs = (const nt_u32x4*)(x - off) + first;
+        nt_u32x4 raw[PACKS];
+#pragma unroll
+        for (int p = 0; p < PACKS; ++p) {
+            const int j = at + NW * 64 * p;
+            raw[p] = nt_u32x4{Words<T>::NONE, Words<T>::NONE, Words<T>::NONE, Words<T>::NONE};
+            if (j >= own && j < own_end) raw[p] = packs[j];
+        }
+        for (int edge = 0; edge < 2; ++edge) {
+            const int e = edge ? n - 1 : 0;
+            if (edge ? own_end == n || e < own : own == 0) continue;
+            Pack<T, V> part;
+#pragma unroll
+            for (int u = 0; u < V; ++u) {
+                const int64_t i = index0 + (int64_t)e * V + u;
+                part.v[u] = i >= 0 && i < a.vocab ? x[i] : (T)-INFINITY;
+            }
+            const nt_u32x4 words = __builtin_bit_cast(nt_u32x4, part);
+#pragma unroll
+            for (int p = 0; p < PACKS; ++p) raw[p] = at + NW * 64 * p == e ? words : raw[p];
+        }
+        nt_u32x4 best = raw[0];
+#pragma unroll
+        for (int p = 1; p < PACKS; ++p)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) best[u] = Words<T>::max_of(best[u], raw[p][u]);
+        float mine = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < V; ++u) mine = fmaxf(mine, Words<T>::at(best, u));
+        float top = mine, bar = -INFINITY;
+        if (TOP) {
+            const float order = sort_rising(mine);
+            top = __shfl(order, 63), bar = __shfl(order, 64 - a.top);
+            const float part = __shfl(order, 64 - (a.top + NW - 1) / NW);
+            if (NW > 1) {
+                if (lane == 0) tops[wave] = top, bars[wave] = bar, parts[wave] = part;
+                if (threadIdx.x == 0) gathered = 0;
+                __syncthreads();
+                float least = INFINITY;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) top = fmaxf(top, tops[w]), bar = fmaxf(bar, bars[w]), least = fminf(least, parts[w]);
+                bar = fmaxf(bar, least);
+            } else {
+                if (threadIdx.x == 0) gathered = 0;
+                __syncthreads();
+            }
+        } else {
+            top = over_lanes(mine, [](float p, float q) { return fmaxf(p, q); });
+            if (NW > 1) {
+                if (lane == 0) tops[wave] = top;
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < NW; ++w) top = fmaxf(top, tops[w]);
+            }
+        }
         Likeliest likeliest;
         likeliest.init(room[wave]);
-        bool begun = false;
-        for (int64_t at = first + wave * 64 * PACKS; at < last; at += NW * 64 * PACKS) {
-            float v[PACKS][V];
-            P raw[PACKS];
+        if (TOP) {
+            uint32_t reach = 0;  // packs that reach the bar
 #pragma unroll
             for (int p = 0; p < PACKS; ++p) {
-                const int64_t k = at + 64 * p + lane;
-                if (k < last && k * V >= off && (k + 1) * V <= off + a.vocab) {
-                    raw[p] = packs[k];
-                } else {
+                uint32_t most = raw[p][0];
 #pragma unroll
+                for (int u = 1; u < 4; ++u) most = Words<T>::max_of(most, raw[p][u]);
+                const nt_u32x4 both = {most, most, most, most};
+                const bool hit = V == 4 ? Words<T>::at(both, 0) >= bar : fmaxf(Words<T>::at(both, 0), Words<T>::at(both, 1)) >= bar;
+                reach |= hit ? 1u << p : 0u;
+            }
+            auto pack_of = [&](int which) {
+                nt_u32x4 pack = {0, 0, 0, 0};
+#pragma unroll
+                for (int p = 0; p < PACKS; ++p) pack |= raw[p] & (which == p ? 0xffffffffu : 0u);
+                return pack;
+            };
+            constexpr int ROOM = NW * 64 < 256 ? NW * 64 : 256;
+            u64* all = room[0];
+            for (uint32_t hits = reach; hits; hits &= hits - 1) {
+                const int which = __ffs(hits) - 1;
+                const nt_u32x4 pack = pack_of(which);
+                const int64_t i = index0 + (int64_t)(at + NW * 64 * which) * V;
+                uint32_t values = 0;
+#pragma unroll
+                for (int u = 0; u < V; ++u) values |= Words<T>::at(pack, u) >= bar ? 1u << u : 0u;
+                if (bar == -INFINITY) {  // what is not the row's own reaches it, too
+#pragma unroll
+                    for (int u = 0; u < V; ++u)
+                        if (at + NW * 64 * which >= n || i + u < 0 || i + u >= a.vocab) values &= ~(1u << u);
+                }
+                int place = atomicAdd(&gathered, __popc(values));
+                for (; values; values &= values - 1, ++place) {
+                    const int u = __ffs(values) - 1;
+                    const uint32_t w = (u * (int)sizeof(T) & 8 ? (u * (int)sizeof(T) & 4 ? pack[3] : pack[2]) : u * (int)sizeof(T) & 4 ? pack[1] : pack[0]);
+                    const nt_u32x4 first_of = {sizeof(T) == 2 && (u & 1) ? w >> 16 : w, 0, 0, 0};
+                    if (place < ROOM) all[place] = rank_of(Words<T>::at(first_of, 0), (uint32_t)(i + u));
+                }
+            }
+            __syncthreads();
+            const int total = gathered;
+            if (total <= ROOM) {
+                u64 key = 0;
+                if (wave * 64 < total) {
+                    key = sort_rising(threadIdx.x < total ? all[threadIdx.x] : 0);
+                    if (wave > 0) all[threadIdx.x] = key;
+                }
+                if (wave == 0) likeliest.merge(key, a.top);
+                if (NW > 1 && total > 64) {
+                    __syncthreads();
+                    if (wave == 0)
+                        for (int w = 1; w * 64 < total; ++w) likeliest.merge(room[w][lane], a.top);
+                }
+            } else {
+                __syncthreads();
+                for (uint32_t hits = reach; __any(hits); hits &= hits - 1) {
+                    const int which = hits ? __ffs(hits) - 1 : 0;
+                    nt_u32x4 pack = pack_of(which);
+#pragma unroll 1
                     for (int u = 0; u < V; ++u) {
-                        const int64_t i = k * V + u - off;
-                        raw[p].v[u] = k < last && i >= 0 && i < a.vocab ? x[i] : (T)-INFINITY;
+                        const float y = Words<T>::at(pack, 0);
+                        const int64_t i = index0 + (int64_t)(at + NW * 64 * which) * V + u;
+                        const bool is = hits && y >= bar && at + NW * 64 * which < n && i >= 0 && i < a.vocab;
+                        if (__any(is)) likeliest.put(is, y, i, a.top);
+                        pack = Words<T>::next(pack);
                     }
                 }
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int p = 0; p < PACKS; ++p)
-#pragma unroll
-                for (int u = 0; u < V; ++u) {
-                    v[p][u] = (float)raw[p].v[u];
-                    top = fmaxf(top, v[p][u]);
-                }
-            if (__any(top > s.m)) rebase(s, fmaxf(s.m, top), c);
-            const float base = base_of(s.m);
-            float rest[PACKS], weighted[PACKS], ones = 0.f;
-#pragma unroll
-            for (int p = 0; p < PACKS; ++p) {
-                float r[V], w[V];
-#pragma unroll
-                for (int u = 0; u < V; ++u) {
-                    const float t = (v[p][u] - base) * c, e = __builtin_amdgcn_exp2f(t);  // (a NaN stays in the sum)
-                    const bool one = v[p][u] == s.m;
-                    ones += one ? 1.f : 0.f;
-                    r[u] = one ? 0.f : e;
-                    w[u] = e * fmaxf(t, kFar);
-                }
-#pragma unroll
-                for (int n = V / 2; n > 0; n /= 2)
-#pragma unroll
-                    for (int u = 0; u < n; ++u) r[u] += r[u + n], w[u] += w[u + n];
-                rest[p] = r[0], weighted[p] = w[0];
-            }
-            static_assert(PACKS == 4, "pairs of pairs");
-            s.rest += (rest[0] + rest[1]) + (rest[2] + rest[3]);
-            s.weighted += (weighted[0] + weighted[1]) + (weighted[2] + weighted[3]);
-            if (s.m > -INFINITY) s.ones += ones;
-            if (TOP) {
-                // from the second batch on equal ones come after those that the wave has
-                float over = likeliest.over;
-                bool look = __any(top > over);
-                if (!begun) {
-                    over = __shfl(sort_rising(top), 64 - a.top);
-                    look = true;
-                }
-                const bool equal = !begun || !likeliest.bar;
-                begun = true;
-                if (look || equal) {
-#pragma unroll
-                    for (int p = 0; p < PACKS; ++p)
-#pragma unroll
-                        for (int u = 0; u < V; ++u) {
-                            const int64_t i = (at + 64 * p + lane) * V + u - off;
-                            const bool is = (equal ? v[p][u] >= over : v[p][u] > over) && at + 64 * p + lane < last && i >= 0 && i < a.vocab;
-                            if (__any(is)) likeliest.put(is, v[p][u], i, a.top);
-                        }
-                    if (!likeliest.bar) likeliest.flush(a.top);
+                likeliest.flush(a.top);
+                if (NW > 1) {
+                    room[wave][63 - lane] = likeliest.list;
+                    __syncthreads();
+                    if (wave == 0)
+                        for (int w = 1; w < NW; ++w) likeliest.merge(room[w][lane], a.top);
                 }
             }
         }
-        if (TOP) likeliest.flush(a.top);
+        RowSums s{top, 0.0, 0.0, 0.0};
+        if (top > -INFINITY && __any(mine == top)) s.ones = take_out<T>(raw, top);
+        if (fabsf(base_of(top) * c) < 4096.f)  // what `off` neglects, its square, is below 2^-25
+            sum_packs<T, false>(raw, top, c, s);
+        else
+            sum_packs<T, true>(raw, top, c, s);
         // join the lanes, the waves, the segments
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) add_sums(s, shuffled(s, o), c);
+        auto add = [](double p, double q) { return p + q; };
+        s.rest = over_lanes(s.rest, add), s.ones = over_lanes(s.ones, add), s.weighted = over_lanes(s.weighted, add);
         if (NW > 1) {
             if (lane == 0) sums[wave] = s;
-            if (TOP) room[wave][63 - lane] = likeliest.list;
             __syncthreads();
             if (wave == 0) {
 #pragma unroll
                 for (int w = 1; w < NW; ++w) {
-                    add_sums(s, sums[w], c);
-                    if (TOP) likeliest.merge(room[w][lane], a.top);
+                    s.rest += sums[w].rest, s.ones += sums[w].ones, s.weighted += sums[w].weighted;
                 }
             }
         }
@@ -276,7 +447,7 @@ __global__ void __launch_bounds__(64 * NW) logprobs_k(LogprobArgs a) {
                 return (u64)__float_as_uint(load_partial(r, at * 4u)) | (u64)__float_as_uint(load_partial(r, at * 4u + 4u)) << 32;
             };
             if (wave == 0) {
-                const uint32_t at = (uint32_t)unit * slot;
+                const uint32_t at = blockIdx.x * (uint32_t)slot;
                 if (lane == 0) {
                     put8(at, __double_as_longlong(s.rest));
                     put8(at + 2, __double_as_longlong(s.ones));
@@ -285,24 +456,22 @@ __global__ void __launch_bounds__(64 * NW) logprobs_k(LogprobArgs a) {
                 }
                 if (TOP && lane < a.top) put8(at + kSlotHead + 2 * lane, likeliest.list);
             }
-            if (!finish_arrive(a.counters + row, a.segments - 1)) {
-                __syncthreads();
-                continue;
-            }
+            if (!finish_arrive(a.counters + line, a.segments - 1)) return;
             if (wave == 0) {
                 s = RowSums{-INFINITY, 0.0, 0.0, 0.0};
                 for (int g = lane; g < a.segments; g += 64) {
-                    const uint32_t at = (uint32_t)(row * a.segments + g) * slot;
+                    const uint32_t at = (uint32_t)(line * a.segments + g) * slot;
                     add_sums(s, RowSums{load_partial(r, at * 4u + 24u), __longlong_as_double(get8(at)), __longlong_as_double(get8(at + 2)),
                                         __longlong_as_double(get8(at + 4))}, c);
                 }
 #pragma unroll
-                for (int o = 1; o < 64; o <<= 1) add_sums(s, shuffled(s, o), c);
+                for (int o = 1; o < 64; o <<= 1)
+                    add_sums(s, RowSums{__shfl_xor(s.m, o), __shfl_xor(s.rest, o), __shfl_xor(s.ones, o), __shfl_xor(s.weighted, o)}, c);
             }
             if (TOP) {
                 likeliest.init(room[wave]);
                 for (int g = wave; g < a.segments; g += NW) {
-                    const uint32_t at = (uint32_t)(row * a.segments + g) * slot + kSlotHead;
+                    const uint32_t at = (uint32_t)(line * a.segments + g) * slot + kSlotHead;
                     likeliest.merge(63 - lane < a.top ? get8(at + 2 * (63 - lane)) : 0, a.top);
                 }
                 if (NW > 1) {
@@ -332,25 +501,50 @@ __global__ void __launch_bounds__(64 * NW) logprobs_k(LogprobArgs a) {
                 a.top_logprob[row * a.top + lane] = !ok ? NAN : key ? log_p(value_of(key)) : -INFINITY;
             }
         }
-        if (NW > 1) __syncthreads();  // the LDS is the next unit's
     }
 }
 
-template <typename T, int NW>
-static void launch_waves(const char* name, const LogprobArgs& a) {
-    const int64_t units = a.rows * a.segments, most = (int64_t)cu_count() * 64;
-    const dim3 grid((unsigned)(units < most ? units : most));
-    if (a.top > 0)
-        launch(name, logprobs_k<T, NW, true>, grid, dim3(64 * NW), 0, a);
-    else
-        launch(name, logprobs_k<T, NW, false>, grid, dim3(64 * NW), 0, a);
+template <typename T, int NW, int PACKS>
+static void launch_packs(const char* name, LogprobArgs a, int64_t packs) {
+    a.segments = (int)ceil_div(packs, NW * 64 * PACKS);
+    a.each = (int)ceil_div(packs, a.segments);
+    // rows at a time: their segments' slots and counters
+    const int64_t all = a.rows, slots = (int64_t)a.segments * slot_floats(a.top) * sizeof(float);
+    const int64_t most = a.segments > 1 ? ((int64_t)64 << 20) / slots : (int64_t)1 << 22;
+    a.rows = most < 1 ? 1 : most < all ? most : all;
+    if (a.segments > 1) {
+        a.part = workspace((size_t)(a.rows * slots));
+        a.counters = tile_counters((size_t)a.rows);
+        if (!a.part || !a.counters) return fail(NNC_HIP_ENOMEM, name, "no workspace for %lld bytes of partial sums", (long long)(a.rows * slots));
+    }
+    for (const int64_t each = a.rows; a.row0 < all; a.row0 += each) {
+        a.rows = each < all - a.row0 ? each : all - a.row0;
+        const dim3 grid((unsigned)(a.rows * a.segments));
+        const double n = (double)a.rows * (double)a.vocab;
+        set_work(6.0 * n, n * sizeof(T) + 8.0 * (double)a.rows * (1 + a.top));
+        if (a.top > 0)
+            launch(name, logprobs_k<T, NW, PACKS, true>, grid, dim3(64 * NW), 0, a);
+        else
+            launch(name, logprobs_k<T, NW, PACKS, false>, grid, dim3(64 * NW), 0, a);
+    }
 }
 
-// A wave to a row of up to 2048 values, else four
+// A wave to a row that fits into its registers, else four to a segment: of 4
+// packs a lane while that makes few workgroups, else of 16, or 8 where no tokens
+// are asked for. 16 and 8 packs, us: [512, 128256] f16, 20 tokens 55 and 58, none
+// 38 and 36; [2048, 32000] f16, 1 token 44 and 52; [301, 50257] fp32, none 18 and
+// 17. (Eight waves with 8 packs 63, 36, 43, 17.) A copy's rate leaves 26 us for the
+// first: a fifth of its time is the sorting of candidates, and loads and sums of
+// a CU's workgroups overlap only in part. 8 rows of 32000 in fp32 take 9.7 us
+// with 5 tokens, 6.4 without: load, bar, candidates, sort, join are one chain.
 template <typename T>
 static void launch_logprobs(const char* name, const LogprobArgs& a) {
-    if (a.vocab <= 2048) return launch_waves<T, 1>(name, a);
-    launch_waves<T, 4>(name, a);
+    const int64_t packs = a.vocab * (int64_t)sizeof(T) / 16 + 2;
+    if (packs <= 256) return launch_packs<T, 1, 4>(name, a, packs);
+    if (packs <= 512 && a.rows >= cu_count()) return launch_packs<T, 1, 8>(name, a, packs);
+    if (ceil_div(packs, 1024) * a.rows <= 4 * (int64_t)cu_count()) return launch_packs<T, 4, 4>(name, a, packs);
+    if (a.top == 0) return launch_packs<T, 4, 8>(name, a, packs);
+    launch_packs<T, 4, 16>(name, a, packs);
 }
 
 static bool row_output(const char* name, const char* what, Tensor* t, int dtype, int64_t n) {
@@ -394,18 +588,6 @@ void nnc_hip_token_logprobs(Tensor* logits, Tensor* tokens, Tensor* logprob, Ten
     if (logprob) a.tokens = (const int*)tokens->data, a.logprob = (float*)logprob->data;
     if (entropy) a.entropy = (float*)entropy->data;
     if (top_index) a.top_index = (int*)top_index->data, a.top_logprob = (float*)top_logprob->data;
-    const double n = (double)a.rows * (double)a.vocab;
-    set_work(6.0 * n, n * activation_bytes(logits) + 8.0 * (double)a.rows * (1 + a.top));
-    // Segments of 4096 values or more, up to 6 workgroups a CU of them
-    const int64_t room = 6 * (int64_t)cu_count(), longest = a.vocab / 4096;
-    a.segments = (int)(a.rows >= room ? 1 : room / a.rows < longest ? room / a.rows : longest);
-    if (a.segments < 1) a.segments = 1;
-    if (a.segments > 1) {
-        const size_t bytes = (size_t)a.rows * a.segments * slot_floats(a.top) * sizeof(float);
-        a.part = workspace(bytes);
-        a.counters = tile_counters((size_t)a.rows);
-        if (!a.part || !a.counters) return fail(NNC_HIP_ENOMEM, name, "no workspace for %zu bytes of partial sums", bytes);
-    }
     if (logits->dtype == NNC_DTYPE_FLOAT16)
         launch_logprobs<half_t>(name, a);
     else
