@@ -18,8 +18,8 @@
 // If more than 256 reach it (equal values, rows of -infinity), each wave keeps a
 // list of its best 64, one a lane, and merges 64 at a time into it. The last
 // segment to arrive joins a row's segments.
+#include "lanes.h"
 #include "mfma_tile.h"
-#include "quant8.h"
 
 namespace nnc {
 
@@ -40,7 +40,6 @@ struct LogprobArgs {
 // Whole numbers ordered as the values are, the earlier of equal ones first: a
 // value's bits, negative ones turned round, before the index's complement. 0 is
 // below all of them.
-typedef unsigned long long u64;
 __device__ __forceinline__ u64 rank_of(float x, uint32_t index) {
     const uint32_t bits = __float_as_uint(x + 0.f);  // (-0 becomes 0)
     return (u64)(bits ^ ((uint32_t)((int32_t)bits >> 31) | 0x80000000u)) << 32 | (0xffffffffu - index);
@@ -55,32 +54,6 @@ template <typename K>
 __device__ __forceinline__ K larger(K a, K b) { return a > b ? a : b; }
 template <typename K>
 __device__ __forceinline__ K smaller(K a, K b) { return a > b ? b : a; }
-
-// The word of lane ^ J, without a way through LDS: by DPP within 16 lanes, beyond
-// by exchanging rows of 16 and halves of 32.
-template <int J>
-__device__ __forceinline__ uint32_t lane_xor(uint32_t x) {
-    const int v = (int)x;
-    if constexpr (J == 1) return (uint32_t)__builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);  // quads 1 0 3 2
-    if constexpr (J == 2) return (uint32_t)__builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);  // quads 2 3 0 1
-    if constexpr (J == 4)  // 7 - i in eights, then 3 - i in quads
-        return (uint32_t)__builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true), 0x1b, 0xf, 0xf, true);
-    if constexpr (J == 8) return (uint32_t)__builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);  // turned by 8
-    if constexpr (J == 16) {
-        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-        return threadIdx.x & 16 ? r[0] : r[1];
-    }
-    if constexpr (J == 32) {
-        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-        return threadIdx.x & 32 ? r[0] : r[1];
-    }
-}
-template <int J>
-__device__ __forceinline__ float lane_xor(float x) { return __uint_as_float(lane_xor<J>(__float_as_uint(x))); }
-template <int J>
-__device__ __forceinline__ u64 lane_xor(u64 x) { return (u64)lane_xor<J>((uint32_t)(x >> 32)) << 32 | lane_xor<J>((uint32_t)x); }
-template <int J>
-__device__ __forceinline__ double lane_xor(double x) { return __longlong_as_double((long long)lane_xor<J>((u64)__double_as_longlong(x))); }
 
 // 64 keys, one a lane, in rising order
 template <int RUN, int J, typename K>
@@ -110,14 +83,6 @@ __device__ __forceinline__ u64 merge_step(u64 key) {
 }
 __device__ __forceinline__ u64 merge_falling(u64 falling, u64 rising) { return merge_step<32>(larger(falling, rising)); }
 
-// What `op` makes of all lanes' values
-template <int J = 32, typename K, class Op>
-__device__ __forceinline__ K over_lanes(K x, Op op) {
-    x = op(x, lane_xor<J>(x));
-    if constexpr (J > 1) return over_lanes<J / 2>(x, op);
-    return x;
-}
-
 // Sums of a part of a row: the terms e^(t (x - m)) that are less than 1, how
 // many are 1, and all of them times their exponents, in powers of two.
 struct RowSums {
@@ -142,33 +107,6 @@ __device__ __forceinline__ void add_sums(RowSums& s, RowSums t, float c) {
     rebase(s, m, c), rebase(t, m, c);
     s.rest += t.rest, s.ones += t.ones, s.weighted += t.weighted;
 }
-
-// 16 bytes of a row, kept as words
-template <typename T>
-struct Words {
-    static constexpr int V = 16 / (int)sizeof(T);
-    static constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xfc00fc00u;  // -infinity
-    __device__ __forceinline__ static float at(nt_u32x4 w, int u) {
-        if constexpr (sizeof(T) == 4) {
-            const uint32_t x = w[u];
-            return __uint_as_float(x);
-        } else {
-            const uint32_t x = w[u / 2];
-            return (float)__builtin_bit_cast(f16x2, x)[u % 2];
-        }
-    }
-    // the words with the next value first
-    __device__ __forceinline__ static nt_u32x4 next(nt_u32x4 w) {
-        if constexpr (sizeof(T) == 4) return nt_u32x4{w[1], w[2], w[3], w[0]};
-        return nt_u32x4{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16};
-    }
-    __device__ __forceinline__ static uint32_t max_of(uint32_t x, uint32_t y) {
-        if constexpr (sizeof(T) == 4)
-            return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
-        else
-            return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(f16x2, x), __builtin_bit_cast(f16x2, y)));
-    }
-};
 
 // Takes the values that are the maximum out of a lane's packs; how many.
 template <typename T, int PACKS>

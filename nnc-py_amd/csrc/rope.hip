@@ -11,6 +11,7 @@
 // result that depended on the order of a sum would be another whole number now
 // and then. A float64 operation takes no longer than a float32 one here.
 #include "kvcache.h"
+#include "lanes.h"
 
 namespace nnc {
 
@@ -25,7 +26,7 @@ struct RopeArgs {
     int64_t rows, places;
     int col, out_col, heads, dim, rot;
     bool interleaved, weight_each;
-    double eps;
+    double eps, inverse_dim;
 };
 
 // The sequence that a row belongs to, -1 if it is none's: the first whose rows
@@ -61,19 +62,19 @@ __device__ __forceinline__ int64_t rope_place(const RopeArgs& a, int64_t row) {
     return at < 0 ? 0 : at < a.places ? at : a.places - 1;
 }
 
-// To float32, then to the activations' type. (The compiler would make one
-// conversion of the two, which takes twenty operations for float16.)
-template <typename T>
-__device__ __forceinline__ T rounded(double y) {
-    float f = (float)y;
-    asm("" : "+v"(f));
-    return (T)f;
-}
-
 __device__ __forceinline__ double wave_add(double v) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
     return v;
+}
+
+// 1 / sqrt(m) by the hardware's approximation (2^-26 and better) and two of
+// Newton's steps
+__device__ __forceinline__ double inverse_root(double m) {
+    double y = __builtin_amdgcn_rsq(m);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y *= fma(-0.5 * m * y, y, 1.5);
+    return m == INFINITY ? 0.0 : y;
 }
 
 // Any sizes: a wave to a head of a row, a pair or an unpaired dim a lane.
@@ -93,30 +94,146 @@ __global__ void __launch_bounds__(256) rope_k(RopeArgs a) {
         if (a.weight) {
             double sum = 0.0;
             for (int d = lane; d < a.dim; d += 64) sum += (double)(float)x[d] * (double)(float)x[d];
-            r = 1.0 / sqrt(wave_add(sum) / a.dim + a.eps);
+            r = inverse_root(wave_add(sum) * a.inverse_dim + a.eps);
         }
         auto normed = [&](int d) { return a.weight ? (double)(float)x[d] * r * (double)(float)w[d] : (double)(float)x[d]; };
         for (int u = lane; u < a.dim - half; u += 64) {
             if (u >= half) {
-                y[u + half] = rounded<T>(normed(u + half));
+                y[u + half] = (T)Words<T>::narrow(normed(u + half));
                 continue;
             }
             const int one = a.interleaved ? 2 * u : u, other = a.interleaved ? 2 * u + 1 : u + half;
             const double c = a.angles[place * a.rot + u], s = a.angles[place * a.rot + half + u];
             const double p = normed(one), q = normed(other);
-            y[one] = rounded<T>(p * c - q * s);
-            y[other] = rounded<T>(q * c + p * s);
+            y[one] = (T)Words<T>::narrow(p * c - q * s);
+            y[other] = (T)Words<T>::narrow(q * c + p * s);
         }
     }
 }
 
-static void launch_rope(const char* name, bool f16, const RopeArgs& a) {
+// Heads of whole packs of 16 bytes: a lane takes two, whose values are each
+// other's pairs - dims i .. and i + rot / 2 .., or 2 V neighbours - or two packs
+// that stay; 2^bits lanes side by side are a head, and a wave goes through `per`
+// heads of a row for each of them with the row's angles in registers.
+template <typename T, bool NORM>
+__global__ void __launch_bounds__(256) rope_packs_k(RopeArgs a, int bits, int per, int chunks) {
+    typedef Words<T> W;
+    constexpr int V = W::V;
+    const int lane = threadIdx.x & 63, unit = lane & ((1 << bits) - 1), groups = 64 >> bits, half = a.rot / 2;
+    const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t row = item / (uint32_t)chunks, chunk = item - row * (uint32_t)chunks;
+    if (row >= a.rows) return;
+    const bool turned = 2 * V * unit < a.rot, mine = 2 * V * unit < a.dim;
+    const int one = turned && !a.interleaved ? V * unit : 2 * V * unit;
+    const int other = turned && !a.interleaved ? one + half : one + V;
+    int head = chunk * per * groups + (lane >> bits);
+    const T* x = (const T*)a.in + row * a.in_ld + a.col;
+    T* y = (T*)a.out + row * a.out_ld + a.out_col;
+    const int end = min(head + per * groups, a.heads);
+    nt_u32x4 p{}, q{}, wp{}, wq{};
+    auto load = [&](int h) {
+        if (mine && h < end) {
+            p = *(const nt_u32x4*)(x + (int64_t)h * a.dim + one), q = *(const nt_u32x4*)(x + (int64_t)h * a.dim + other);
+            if (NORM && a.weight_each) {
+                const T* w = (const T*)a.weight + (int64_t)h * a.dim;
+                wp = *(const nt_u32x4*)(w + one), wq = *(const nt_u32x4*)(w + other);
+            }
+        }
+    };
+    load(head);
+    if (NORM && !a.weight_each && mine) wp = *(const nt_u32x4*)((const T*)a.weight + one), wq = *(const nt_u32x4*)((const T*)a.weight + other);
+    const int64_t place = rope_place(a, row);
+    if (place < 0) return;
+    float cs[V], sn[V];
+    if (turned) {
+        const float* t = a.angles + place * a.rot + V * unit;
+#pragma unroll
+        for (int u = 0; u < V; u += 4) {
+            *(float4*)(cs + u) = *(const float4*)(t + u);
+            *(float4*)(sn + u) = *(const float4*)(t + half + u);
+        }
+    }
+    for (; head - (lane >> bits) < end; head += groups) {
+        const nt_u32x4 xp = p, xq = q, vp = wp, vq = wq;
+        const bool live = mine && head < end;
+        const int h = head;
+        load(head + groups);
+        double f[V], g[V];
+#pragma unroll
+        for (int u = 0; u < V; ++u) f[u] = W::at(xp, u), g[u] = W::at(xq, u);
+        if (NORM) {
+            double sum = 0.0;
+#pragma unroll
+            for (int u = 0; u < V; ++u) sum = fma(f[u], f[u], sum), sum = fma(g[u], g[u], sum);
+            if (!live) sum = 0.0;
+            auto add = [](double s, double t) { return s + t; };
+            if (bits > 0) sum = add(sum, lane_xor<1>(sum));
+            if (bits > 1) sum = add(sum, lane_xor<2>(sum));
+            if (bits > 2) sum = add(sum, lane_xor<4>(sum));
+            if (bits > 3) sum = add(sum, lane_xor<8>(sum));
+            if (bits > 4) sum = add(sum, lane_xor<16>(sum));
+            if (bits > 5) sum = add(sum, lane_xor<32>(sum));
+            const double r = inverse_root(sum * a.inverse_dim + a.eps);
+#pragma unroll
+            for (int u = 0; u < V; ++u) f[u] *= r * (double)W::at(vp, u), g[u] *= r * (double)W::at(vq, u);
+        }
+        if (turned) {
+#pragma unroll
+            for (int u = 0; u < V; ++u) {
+                const double c = cs[u], s = sn[u];
+                if (a.interleaved) {  // pair u of the unit's 2 V values
+                    double& m = u < V / 2 ? f[2 * u % V] : g[2 * u % V];
+                    double& n = u < V / 2 ? f[2 * u % V + 1] : g[2 * u % V + 1];
+                    const double t = m;
+                    m = t * c - n * s, n = n * c + t * s;
+                } else {
+                    const double t = f[u];
+                    f[u] = t * c - g[u] * s, g[u] = g[u] * c + t * s;
+                }
+            }
+        }
+        if (live) {
+            *(nt_u32x4*)(y + (int64_t)h * a.dim + one) = W::of(f);
+            *(nt_u32x4*)(y + (int64_t)h * a.dim + other) = W::of(g);
+        }
+    }
+}
+
+template <typename T>
+static bool in_packs(const RopeArgs& a) {
+    constexpr int V = 16 / (int)sizeof(T);
+    return a.dim % (2 * V) == 0 && a.dim <= 128 * V && a.rot % (2 * V) == 0 && aligned16(a.in) && aligned16(a.out) && aligned16(a.angles) &&
+           aligned16(a.weight) && a.in_ld % V == 0 && a.out_ld % V == 0 && a.col % V == 0 && a.out_col % V == 0;
+}
+
+template <typename T>
+static void launch_rope_type(const char* name, const RopeArgs& a) {
+    if (in_packs<T>(a)) {
+        constexpr int V = 16 / (int)sizeof(T);
+        int bits = 0;
+        while ((2 * V << bits) < a.dim) ++bits;
+        const int groups = 64 >> bits, passes = (int)ceil_div(a.heads, groups);
+        // waves of a row's whole heads while they are many
+        int per = passes;
+        while (per > 1 && a.rows * ceil_div(passes, per) < 16 * (int64_t)cu_count()) per = (per + 1) / 2;
+        const int chunks = (int)ceil_div(passes, per);
+        const int64_t blocks = ceil_div(a.rows * chunks, 4);
+        if (blocks * 256 <= UINT32_MAX) {
+            const dim3 grid((unsigned)blocks);
+            return a.weight ? launch(name, rope_packs_k<T, true>, grid, dim3(256), 0, a, bits, per, chunks)
+                            : launch(name, rope_packs_k<T, false>, grid, dim3(256), 0, a, bits, per, chunks);
+        }
+    }
     const int64_t blocks = ceil_div(a.rows * a.heads, 4), most = (int64_t)cu_count() * 32;
-    const dim3 grid((unsigned)(blocks < most ? blocks : most));
+    launch(name, rope_k<T>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, a);
+}
+
+static void launch_rope(const char* name, bool f16, RopeArgs a) {
+    a.inverse_dim = 1.0 / a.dim;
     if (f16)
-        launch(name, rope_k<half_t>, grid, dim3(256), 0, a);
+        launch_rope_type<half_t>(name, a);
     else
-        launch(name, rope_k<float>, grid, dim3(256), 0, a);
+        launch_rope_type<float>(name, a);
 }
 
 // ---------------------------------------------------------------------------
