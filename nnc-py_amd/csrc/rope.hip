@@ -111,17 +111,58 @@ __global__ void __launch_bounds__(256) rope_k(RopeArgs a) {
     }
 }
 
+// A unit's cosines and sines: its V pairs are the same rows' V in both layouts.
+template <int V>
+__device__ __forceinline__ void angles_of(const RopeArgs& a, int64_t place, int unit, float (&cs)[V], float (&sn)[V]) {
+    const float* t = a.angles + place * a.rot + V * unit;
+#pragma unroll
+    for (int u = 0; u < V; u += 4) {
+        *(float4*)(cs + u) = *(const float4*)(t + u);
+        *(float4*)(sn + u) = *(const float4*)(t + a.rot / 2 + u);
+    }
+}
+// The pairs of a unit's two packs: each other's values, or neighbours.
+template <int V>
+__device__ __forceinline__ void turn(double (&f)[V], double (&g)[V], const float (&cs)[V], const float (&sn)[V], bool interleaved) {
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+        const double c = cs[u], s = sn[u];
+        if (interleaved) {
+            double& m = u < V / 2 ? f[2 * u % V] : g[2 * u % V];
+            double& n = u < V / 2 ? f[2 * u % V + 1] : g[2 * u % V + 1];
+            const double t = m;
+            m = t * c - n * s, n = n * c + t * s;
+        } else {
+            const double t = f[u];
+            f[u] = t * c - g[u] * s, g[u] = g[u] * c + t * s;
+        }
+    }
+}
+// The sum over the 2^bits lanes of a head
+__device__ __forceinline__ double over_head(double sum, int bits) {
+    if (bits > 0) sum += lane_xor<1>(sum);
+    if (bits > 1) sum += lane_xor<2>(sum);
+    if (bits > 2) sum += lane_xor<4>(sum);
+    if (bits > 3) sum += lane_xor<8>(sum);
+    if (bits > 4) sum += lane_xor<16>(sum);
+    if (bits > 5) sum += lane_xor<32>(sum);
+    return sum;
+}
+
 // Heads of whole packs of 16 bytes: a lane takes two, whose values are each
 // other's pairs - dims i .. and i + rot / 2 .., or 2 V neighbours - or two packs
 // that stay; 2^bits lanes side by side are a head, and a wave goes through `per`
 // heads of a row for each of them with the row's angles in registers.
+struct RopeWaves {
+    int bits, per, chunks;  // chunks of heads for each row
+};
 template <typename T, bool NORM>
-__global__ void __launch_bounds__(256) rope_packs_k(RopeArgs a, int bits, int per, int chunks) {
+__device__ __forceinline__ void rope_heads(const RopeArgs& a, RopeWaves shape, uint32_t item) {
     typedef Words<T> W;
     constexpr int V = W::V;
+    const int bits = shape.bits, per = shape.per;
     const int lane = threadIdx.x & 63, unit = lane & ((1 << bits) - 1), groups = 64 >> bits, half = a.rot / 2;
-    const uint32_t item = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t row = item / (uint32_t)chunks, chunk = item - row * (uint32_t)chunks;
+    const uint32_t row = item / (uint32_t)shape.chunks, chunk = item - row * (uint32_t)shape.chunks;
     if (row >= a.rows) return;
     const bool turned = 2 * V * unit < a.rot, mine = 2 * V * unit < a.dim;
     const int one = turned && !a.interleaved ? V * unit : 2 * V * unit;
@@ -145,14 +186,7 @@ __global__ void __launch_bounds__(256) rope_packs_k(RopeArgs a, int bits, int pe
     const int64_t place = rope_place(a, row);
     if (place < 0) return;
     float cs[V], sn[V];
-    if (turned) {
-        const float* t = a.angles + place * a.rot + V * unit;
-#pragma unroll
-        for (int u = 0; u < V; u += 4) {
-            *(float4*)(cs + u) = *(const float4*)(t + u);
-            *(float4*)(sn + u) = *(const float4*)(t + half + u);
-        }
-    }
+    if (turned) angles_of<V>(a, place, unit, cs, sn);
     for (; head - (lane >> bits) < end; head += groups) {
         const nt_u32x4 xp = p, xq = q, vp = wp, vq = wq;
         const bool live = mine && head < end;
@@ -165,38 +199,22 @@ __global__ void __launch_bounds__(256) rope_packs_k(RopeArgs a, int bits, int pe
             double sum = 0.0;
 #pragma unroll
             for (int u = 0; u < V; ++u) sum = fma(f[u], f[u], sum), sum = fma(g[u], g[u], sum);
-            if (!live) sum = 0.0;
-            auto add = [](double s, double t) { return s + t; };
-            if (bits > 0) sum = add(sum, lane_xor<1>(sum));
-            if (bits > 1) sum = add(sum, lane_xor<2>(sum));
-            if (bits > 2) sum = add(sum, lane_xor<4>(sum));
-            if (bits > 3) sum = add(sum, lane_xor<8>(sum));
-            if (bits > 4) sum = add(sum, lane_xor<16>(sum));
-            if (bits > 5) sum = add(sum, lane_xor<32>(sum));
+            sum = over_head(live ? sum : 0.0, bits);
             const double r = inverse_root(sum * a.inverse_dim + a.eps);
 #pragma unroll
             for (int u = 0; u < V; ++u) f[u] *= r * (double)W::at(vp, u), g[u] *= r * (double)W::at(vq, u);
         }
-        if (turned) {
-#pragma unroll
-            for (int u = 0; u < V; ++u) {
-                const double c = cs[u], s = sn[u];
-                if (a.interleaved) {  // pair u of the unit's 2 V values
-                    double& m = u < V / 2 ? f[2 * u % V] : g[2 * u % V];
-                    double& n = u < V / 2 ? f[2 * u % V + 1] : g[2 * u % V + 1];
-                    const double t = m;
-                    m = t * c - n * s, n = n * c + t * s;
-                } else {
-                    const double t = f[u];
-                    f[u] = t * c - g[u] * s, g[u] = g[u] * c + t * s;
-                }
-            }
-        }
+        if (turned) turn<V>(f, g, cs, sn, a.interleaved);
         if (live) {
             *(nt_u32x4*)(y + (int64_t)h * a.dim + one) = W::of(f);
             *(nt_u32x4*)(y + (int64_t)h * a.dim + other) = W::of(g);
         }
     }
+}
+
+template <typename T, bool NORM>
+__global__ void __launch_bounds__(256) rope_packs_k(RopeArgs a, RopeWaves shape) {
+    rope_heads<T, NORM>(a, shape, blockIdx.x * 4 + (threadIdx.x >> 6));
 }
 
 template <typename T>
@@ -206,34 +224,206 @@ static bool in_packs(const RopeArgs& a) {
            aligned16(a.weight) && a.in_ld % V == 0 && a.out_ld % V == 0 && a.col % V == 0 && a.out_col % V == 0;
 }
 
+// A wave takes all of a row's heads, 64 >> bits at once, while rows are many
+static RopeWaves rope_waves(const RopeArgs& a, int v) {
+    RopeWaves s{};
+    while ((2 * v << s.bits) < a.dim) ++s.bits;
+    const int passes = (int)ceil_div(a.heads, 64 >> s.bits);
+    s.per = passes;
+    while (s.per > 1 && a.rows * ceil_div(passes, s.per) < 16 * (int64_t)cu_count()) s.per = (s.per + 1) / 2;
+    s.chunks = (int)ceil_div(passes, s.per);
+    return s;
+}
+
 template <typename T>
 static void launch_rope_type(const char* name, const RopeArgs& a) {
     if (in_packs<T>(a)) {
         constexpr int V = 16 / (int)sizeof(T);
-        int bits = 0;
-        while ((2 * V << bits) < a.dim) ++bits;
-        const int groups = 64 >> bits, passes = (int)ceil_div(a.heads, groups);
-        // waves of a row's whole heads while they are many
-        int per = passes;
-        while (per > 1 && a.rows * ceil_div(passes, per) < 16 * (int64_t)cu_count()) per = (per + 1) / 2;
-        const int chunks = (int)ceil_div(passes, per);
-        const int64_t blocks = ceil_div(a.rows * chunks, 4);
+        const RopeWaves shape = rope_waves(a, V);
+        const int64_t blocks = ceil_div(a.rows * shape.chunks, 4);
         if (blocks * 256 <= UINT32_MAX) {
             const dim3 grid((unsigned)blocks);
-            return a.weight ? launch(name, rope_packs_k<T, true>, grid, dim3(256), 0, a, bits, per, chunks)
-                            : launch(name, rope_packs_k<T, false>, grid, dim3(256), 0, a, bits, per, chunks);
+            return a.weight ? launch(name, rope_packs_k<T, true>, grid, dim3(256), 0, a, shape)
+                            : launch(name, rope_packs_k<T, false>, grid, dim3(256), 0, a, shape);
         }
     }
     const int64_t blocks = ceil_div(a.rows * a.heads, 4), most = (int64_t)cu_count() * 32;
     launch(name, rope_k<T>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, a);
 }
 
-static void launch_rope(const char* name, bool f16, RopeArgs a) {
-    a.inverse_dim = 1.0 / a.dim;
+static void launch_rope(const char* name, bool f16, const RopeArgs& a) {
     if (f16)
         launch_rope_type<half_t>(name, a);
     else
         launch_rope_type<float>(name, a);
+}
+
+// ---------------------------------------------------------------------------
+// Into the cache: a group of TPG threads takes a page's V of a head in quads
+// (kvcache.h), or its K in units of two packs, 2 QPER of them a thread, which
+// are turned in registers, rounded to the rows' type, and then scaled and cut as
+// nnc_hip_kv_write does. The workgroups behind those of the pages turn the queries,
+// a wave for a row's heads.
+// ---------------------------------------------------------------------------
+struct RopeKvArgs {
+    KvArgs w;
+    RopeArgs q, k;
+    RopeWaves shape;     // of the queries
+    uint32_t shares, kv_blocks;  // pages that can be touched; workgroups of pages
+};
+
+template <typename T, int TPG, int QPER>
+__device__ __forceinline__ void rope_page(const KvArgs& w, const RopeArgs& a, const Quads<T, TPG>& z, const PageShare& p, int head, float* part) {
+    typedef Words<T> W;
+    typedef Quads<T, TPG> Q;
+    constexpr int V = W::V, PER = 2 * QPER;
+    int bits = 0;
+    while ((2 * V << bits) < z.dim) ++bits;
+    const int unit = z.thread & ((1 << bits) - 1), half = a.rot / 2;
+    const bool turned = 2 * V * unit < a.rot;
+    const int one = turned && !a.interleaved ? V * unit : 2 * V * unit;
+    const int other = turned && !a.interleaved ? one + half : one + V;
+    const int64_t at = (int64_t)p.page_no * w.kv_heads + head;
+    const T* rows = (const T*)w.k_rows + w.k_col + head * z.dim;
+    int8_t* held = w.k + at * z.page * z.dim;
+    float* scale = w.k_scale + at;
+    const float before = *scale;
+    const int lo = p.fresh - p.begin, hi = p.stop - p.begin;
+    nt_u32x4 x[PER][2];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int t = (z.thread + TPG * i) >> bits;
+        const bool in = t >= lo && t < hi;
+        const T* row = rows + (int64_t)p.span.row(in ? p.begin + t : p.fresh) * w.k_ld;
+        x[i][0] = in ? *(const nt_u32x4*)(row + one) : nt_u32x4{0, 0, 0, 0};
+        x[i][1] = in ? *(const nt_u32x4*)(row + other) : nt_u32x4{0, 0, 0, 0};
+    }
+    nt_u32x4 wp{}, wq{};
+    if (a.weight) {
+        const T* weight = (const T*)a.weight + (a.weight_each ? head * z.dim : 0);
+        wp = *(const nt_u32x4*)(weight + one), wq = *(const nt_u32x4*)(weight + other);
+    }
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int t = (z.thread + TPG * i) >> bits;
+        const bool in = t >= lo && t < hi;
+        if (!__any(in)) continue;
+        double f[V], g[V];
+#pragma unroll
+        for (int u = 0; u < V; ++u) f[u] = W::at(x[i][0], u), g[u] = W::at(x[i][1], u);
+        if (a.weight) {
+            double sum = 0.0;
+#pragma unroll
+            for (int u = 0; u < V; ++u) sum = fma(f[u], f[u], sum), sum = fma(g[u], g[u], sum);
+            const double r = inverse_root(over_head(sum, bits) * a.inverse_dim + a.eps);
+#pragma unroll
+            for (int u = 0; u < V; ++u) f[u] *= r * (double)W::at(wp, u), g[u] *= r * (double)W::at(wq, u);
+        }
+        if (turned && in) {
+            int64_t place = p.begin + t;
+            if (a.positions) place = a.positions[p.span.row(p.begin + t)];
+            float cs[V], sn[V];
+            angles_of<V>(a, place < 0 ? 0 : place < a.places ? place : a.places - 1, unit, cs, sn);
+            turn<V>(f, g, cs, sn, a.interleaved);
+        }
+        x[i][0] = W::of(f), x[i][1] = W::of(g);
+        if (in)
+#pragma unroll
+            for (int u = 0; u < V; ++u) big = max(big, max(abs_bits(W::at(x[i][0], u)), abs_bits(W::at(x[i][1], u))));
+    }
+    float top = __uint_as_float(over_lanes(big, [](uint32_t s, uint32_t t) { return max(s, t); }));
+    if constexpr (TPG > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+        __syncthreads();  // everybody has read the scale, too
+        top = part[0];
+#pragma unroll
+        for (int i = 1; i < TPG / 64; ++i) top = max_nan(top, part[i]);
+    }
+    float step = unit8(top);
+    if (lo > 0) step = max_nan(before, step);
+    if (z.thread == 0) *scale = step;
+    if (lo > 0 && !(step == before)) {
+        for (int i = z.thread; i < lo * z.dim; i += TPG) held[i] = step > 0.f ? (int8_t)rint((double)held[i] * (double)before / (double)step) : 0;
+    }
+    const float inverse = inverse8(step);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int t = (z.thread + TPG * i) >> bits;
+        if (!(t >= lo && t < hi)) continue;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            float y[V];
+            typename Q::Held whole;
+#pragma unroll
+            for (int u = 0; u < V; ++u) y[u] = W::at(x[i][s], u);
+            whole8_run<V>(y, step, inverse, whole.v);
+            *(typename Q::Held*)(held + t * z.dim + (s ? other : one)) = whole;
+        }
+    }
+}
+
+template <typename T, int TPG, int QPER>
+__global__ void __launch_bounds__((Quads<T, TPG>::THREADS)) rope_kv_write_k(RopeKvArgs a) {
+    typedef Quads<T, TPG> Q;
+    extern __shared__ __align__(16) char rope_lds[];
+    __shared__ float part[Q::THREADS / 64];
+    if (blockIdx.x >= a.kv_blocks) {
+        const uint32_t item = (blockIdx.x - a.kv_blocks) * (Q::THREADS / 64) + (threadIdx.x >> 6);
+        if (a.q.weight)
+            rope_heads<T, true>(a.q, a.shape, item);
+        else
+            rope_heads<T, false>(a.q, a.shape, item);
+        return;
+    }
+    const Q z(a.w);
+    const uint32_t block = blockIdx.x / a.shares;
+    const int pair = block * Q::GROUPS + threadIdx.x / TPG, which = pair & 1, head = pair >> 1;
+    int share = blockIdx.x - block * a.shares;
+    const int b = find_share(share, a.w.g.batch, [&](int i) { return touched_pages(a.w.g, i); });
+    if (b < 0 || head >= a.w.kv_heads) return;  // (a workgroup of one group has one head)
+    const PageShare p(a.w.g, b, share);
+    if (p.page_no < 0) return;
+    if (which)
+        write_quads<T, TPG, QPER>(a.w, z, p, 1, head, rope_lds, part);
+    else
+        rope_page<T, TPG, QPER>(a.w, a.k, z, p, head, part);
+}
+
+template <typename T, int TPG, int QPER>
+static bool launch_rope_quads(const char* name, RopeKvArgs& a) {
+    typedef Quads<T, TPG> Q;
+    auto kernel = rope_kv_write_k<T, TPG, QPER>;
+    const size_t lds = (size_t)Q::GROUPS * a.w.dim * (a.w.g.page + 4);
+    if constexpr (TPG == 1024) {  // the largest pages: 66560 bytes
+        static const bool ok = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 256 * 260) == hipSuccess;
+        if (!ok) return fail(NNC_HIP_EDEVICE, name, "hipFuncSetAttribute failed"), true;
+    }
+    const int64_t shares = touched_bound(a.w.g.rows, a.w.g.batch, a.w.g.page), pairs = ceil_div(2 * a.w.kv_heads, Q::GROUPS);
+    const int64_t q_blocks = a.q.in ? ceil_div(a.q.rows * a.shape.chunks, Q::THREADS / 64) : 0;
+    if ((shares * pairs + q_blocks) * Q::THREADS > UINT32_MAX) return false;
+    a.shares = (uint32_t)shares, a.kv_blocks = (uint32_t)(shares * pairs);
+    launch(name, kernel, dim3((unsigned)(shares * pairs + q_blocks)), dim3(Q::THREADS), lds, a);
+    return true;
+}
+
+// In one launch, if rows, angles and weights lie in packs; false if not
+template <typename T>
+static bool launch_rope_kv(const char* name, RopeKvArgs& a) {
+    constexpr int V = 16 / (int)sizeof(T);
+    RopeArgs k = a.k;
+    k.out = a.w.k, k.out_ld = 0, k.out_col = 0;  // (the cache is aligned)
+    if (!quads<T>(a.w) || !in_packs<T>(k) || (a.q.in && !in_packs<T>(a.q))) return false;
+    if (a.q.in) a.shape = rope_waves(a.q, V);
+    const int n = a.w.g.page * a.w.dim * (int)sizeof(T) / 64;
+    if (n <= 64) return launch_rope_quads<T, 64, 1>(name, a);
+    if (n <= 256) return launch_rope_quads<T, 256, 1>(name, a);
+    if (n <= 512) return launch_rope_quads<T, 256, 2>(name, a);
+    if (n <= 1024) return launch_rope_quads<T, 256, 4>(name, a);
+    if constexpr (sizeof(T) == 4) {
+        if (n > 2048) return launch_rope_quads<T, 1024, 4>(name, a);
+    }
+    return launch_rope_quads<T, 1024, 2>(name, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -322,7 +512,7 @@ void nnc_hip_rope(Tensor* in, Tensor* weight, Tensor* angles, Tensor* positions,
     if (!rope_weight(name, "weight", in, weight, heads, dim, eps, &a) || !rope_angles(name, angles, positions, a.rows, dim, true, &a) ||
         !rope_out(name, in, out, col, out_col, width, a.rows, a.in_ld, &a))
         return;
-    a.in = in->data, a.col = col, a.heads = heads, a.dim = dim, a.interleaved = interleaved != 0;
+    a.in = in->data, a.col = col, a.heads = heads, a.dim = dim, a.inverse_dim = 1.0 / dim, a.interleaved = interleaved != 0;
     if (a.rows == 0) return;
     if (!ready(name)) return;
     const double n = (double)a.rows * (double)width;
@@ -340,7 +530,7 @@ void nnc_hip_rope_kv_write(Tensor* q, Tensor* k, Tensor* v, Tensor* q_weight, Te
     RopeArgs ka{}, qa{};
     if (!rope_weight(name, "k_weight", k, k_weight, w.kv_heads, w.dim, eps, &ka) || !rope_angles(name, angles, positions, rows, w.dim, false, &ka)) return;
     ka.in = k->data, ka.in_ld = w.k_ld, ka.col = k_col, ka.heads = w.kv_heads;
-    ka.rows = rows, ka.dim = w.dim, ka.interleaved = interleaved != 0, ka.g = w.g;
+    ka.rows = rows, ka.dim = w.dim, ka.inverse_dim = 1.0 / w.dim, ka.interleaved = interleaved != 0, ka.g = w.g;
     if (q) {
         qa = ka;
         if (heads < 1 || heads > 65535) return fail(NNC_HIP_EINVAL, name, "%d heads", heads);
@@ -361,13 +551,17 @@ void nnc_hip_rope_kv_write(Tensor* q, Tensor* k, Tensor* v, Tensor* q_weight, Te
     if (rows == 0 || w.g.batch == 0 || w.g.width == 0) return;
     if (!ready(name)) return;
     const bool f16 = k->dtype == NNC_DTYPE_FLOAT16;
+    const double n = (double)rows * activation_bytes(k);
+    RopeKvArgs all{};
+    all.w = w, all.q = qa, all.k = ka;
+    set_work(8.0 * rows * (q ? heads * w.dim : 0) + 20.0 * rows * kv_width, 2.0 * n * (q ? heads * w.dim : 0) + 2.0 * (n + rows) * kv_width);
+    if (f16 ? launch_rope_kv<half_t>(name, all) : launch_rope_kv<float>(name, all)) return;
     // the rotated keys pass through scratch
     const size_t bytes = (size_t)rows * kv_width * activation_bytes(k);
     ka.out = workspace(bytes);
     if (!ka.out) return fail(NNC_HIP_ENOMEM, name, "no workspace for %zu bytes of rotated keys", bytes);
     ka.out_ld = kv_width, ka.out_col = 0;
     w.k_rows = ka.out, w.k_ld = kv_width, w.k_col = 0;
-    const double n = (double)rows * activation_bytes(k);
     if (q) {
         set_work(8.0 * rows * heads * w.dim, 2.0 * n * heads * w.dim);
         launch_rope("nnc_hip_rope_kv_write_q", f16, qa);
