@@ -121,21 +121,19 @@ __device__ __forceinline__ void angles_of(const RopeArgs& a, int64_t place, int 
         *(float4*)(sn + u) = *(const float4*)(t + a.rot / 2 + u);
     }
 }
-// The pairs of a unit's two packs: each other's values, or neighbours.
-template <int V>
-__device__ __forceinline__ void turn(double (&f)[V], double (&g)[V], const float (&cs)[V], const float (&sn)[V], bool interleaved) {
+// The pairs of a unit's two packs: neighbours, or each other's values.
+template <bool INTER, int V>
+__device__ __forceinline__ void turn(double (&f)[V], double (&g)[V], const float (&cs)[V], const float (&sn)[V]) {
+    auto pair = [](double& p, double& q, double c, double s) {
+        const double t = p;
+        p = t * c - q * s, q = q * c + t * s;
+    };
+    if constexpr (INTER) {
 #pragma unroll
-    for (int u = 0; u < V; ++u) {
-        const double c = cs[u], s = sn[u];
-        if (interleaved) {
-            double& m = u < V / 2 ? f[2 * u % V] : g[2 * u % V];
-            double& n = u < V / 2 ? f[2 * u % V + 1] : g[2 * u % V + 1];
-            const double t = m;
-            m = t * c - n * s, n = n * c + t * s;
-        } else {
-            const double t = f[u];
-            f[u] = t * c - g[u] * s, g[u] = g[u] * c + t * s;
-        }
+        for (int u = 0; u < V / 2; ++u) pair(f[2 * u], f[2 * u + 1], cs[u], sn[u]), pair(g[2 * u], g[2 * u + 1], cs[V / 2 + u], sn[V / 2 + u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < V; ++u) pair(f[u], g[u], cs[u], sn[u]);
     }
 }
 // The sum over the 2^bits lanes of a head
@@ -156,7 +154,7 @@ __device__ __forceinline__ double over_head(double sum, int bits) {
 struct RopeWaves {
     int bits, per, chunks;  // chunks of heads for each row
 };
-template <typename T, bool NORM>
+template <typename T, bool NORM, bool INTER>
 __device__ __forceinline__ void rope_heads(const RopeArgs& a, RopeWaves shape, uint32_t item) {
     typedef Words<T> W;
     constexpr int V = W::V;
@@ -165,8 +163,8 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& a, RopeWaves shape, u
     const uint32_t row = item / (uint32_t)shape.chunks, chunk = item - row * (uint32_t)shape.chunks;
     if (row >= a.rows) return;
     const bool turned = 2 * V * unit < a.rot, mine = 2 * V * unit < a.dim;
-    const int one = turned && !a.interleaved ? V * unit : 2 * V * unit;
-    const int other = turned && !a.interleaved ? one + half : one + V;
+    const int one = turned && !INTER ? V * unit : 2 * V * unit;
+    const int other = turned && !INTER ? one + half : one + V;
     int head = chunk * per * groups + (lane >> bits);
     const T* x = (const T*)a.in + row * a.in_ld + a.col;
     T* y = (T*)a.out + row * a.out_ld + a.out_col;
@@ -204,7 +202,7 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& a, RopeWaves shape, u
 #pragma unroll
             for (int u = 0; u < V; ++u) f[u] *= r * (double)W::at(vp, u), g[u] *= r * (double)W::at(vq, u);
         }
-        if (turned) turn<V>(f, g, cs, sn, a.interleaved);
+        if (turned) turn<INTER>(f, g, cs, sn);
         if (live) {
             *(nt_u32x4*)(y + (int64_t)h * a.dim + one) = W::of(f);
             *(nt_u32x4*)(y + (int64_t)h * a.dim + other) = W::of(g);
@@ -212,9 +210,9 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& a, RopeWaves shape, u
     }
 }
 
-template <typename T, bool NORM>
+template <typename T, bool NORM, bool INTER>
 __global__ void __launch_bounds__(256) rope_packs_k(RopeArgs a, RopeWaves shape) {
-    rope_heads<T, NORM>(a, shape, blockIdx.x * 4 + (threadIdx.x >> 6));
+    rope_heads<T, NORM, INTER>(a, shape, blockIdx.x * 4 + (threadIdx.x >> 6));
 }
 
 template <typename T>
@@ -243,8 +241,9 @@ static void launch_rope_type(const char* name, const RopeArgs& a) {
         const int64_t blocks = ceil_div(a.rows * shape.chunks, 4);
         if (blocks * 256 <= UINT32_MAX) {
             const dim3 grid((unsigned)blocks);
-            return a.weight ? launch(name, rope_packs_k<T, true>, grid, dim3(256), 0, a, shape)
-                            : launch(name, rope_packs_k<T, false>, grid, dim3(256), 0, a, shape);
+            auto kernel = a.weight ? (a.interleaved ? rope_packs_k<T, true, true> : rope_packs_k<T, true, false>)
+                                   : (a.interleaved ? rope_packs_k<T, false, true> : rope_packs_k<T, false, false>);
+            return launch(name, kernel, grid, dim3(256), 0, a, shape);
         }
     }
     const int64_t blocks = ceil_div(a.rows * a.heads, 4), most = (int64_t)cu_count() * 32;
@@ -272,7 +271,7 @@ struct RopeKvArgs {
     uint32_t shares, kv_blocks;  // pages that can be touched; workgroups of pages
 };
 
-template <typename T, int TPG, int QPER>
+template <typename T, int TPG, int QPER, bool INTER>
 __device__ __forceinline__ void rope_page(const KvArgs& w, const RopeArgs& a, const Quads<T, TPG>& z, const PageShare& p, int head, float* part) {
     typedef Words<T> W;
     typedef Quads<T, TPG> Q;
@@ -281,8 +280,8 @@ __device__ __forceinline__ void rope_page(const KvArgs& w, const RopeArgs& a, co
     while ((2 * V << bits) < z.dim) ++bits;
     const int unit = z.thread & ((1 << bits) - 1), half = a.rot / 2;
     const bool turned = 2 * V * unit < a.rot;
-    const int one = turned && !a.interleaved ? V * unit : 2 * V * unit;
-    const int other = turned && !a.interleaved ? one + half : one + V;
+    const int one = turned && !INTER ? V * unit : 2 * V * unit;
+    const int other = turned && !INTER ? one + half : one + V;
     const int64_t at = (int64_t)p.page_no * w.kv_heads + head;
     const T* rows = (const T*)w.k_rows + w.k_col + head * z.dim;
     int8_t* held = w.k + at * z.page * z.dim;
@@ -325,7 +324,7 @@ __device__ __forceinline__ void rope_page(const KvArgs& w, const RopeArgs& a, co
             if (a.positions) place = a.positions[p.span.row(p.begin + t)];
             float cs[V], sn[V];
             angles_of<V>(a, place < 0 ? 0 : place < a.places ? place : a.places - 1, unit, cs, sn);
-            turn<V>(f, g, cs, sn, a.interleaved);
+            turn<INTER>(f, g, cs, sn);
         }
         x[i][0] = W::of(f), x[i][1] = W::of(g);
         if (in)
@@ -363,7 +362,7 @@ __device__ __forceinline__ void rope_page(const KvArgs& w, const RopeArgs& a, co
     }
 }
 
-template <typename T, int TPG, int QPER>
+template <typename T, int TPG, int QPER, bool INTER>
 __global__ void __launch_bounds__((Quads<T, TPG>::THREADS)) rope_kv_write_k(RopeKvArgs a) {
     typedef Quads<T, TPG> Q;
     extern __shared__ __align__(16) char rope_lds[];
@@ -371,9 +370,9 @@ __global__ void __launch_bounds__((Quads<T, TPG>::THREADS)) rope_kv_write_k(Rope
     if (blockIdx.x >= a.kv_blocks) {
         const uint32_t item = (blockIdx.x - a.kv_blocks) * (Q::THREADS / 64) + (threadIdx.x >> 6);
         if (a.q.weight)
-            rope_heads<T, true>(a.q, a.shape, item);
+            rope_heads<T, true, INTER>(a.q, a.shape, item);
         else
-            rope_heads<T, false>(a.q, a.shape, item);
+            rope_heads<T, false, INTER>(a.q, a.shape, item);
         return;
     }
     const Q z(a.w);
@@ -387,13 +386,13 @@ __global__ void __launch_bounds__((Quads<T, TPG>::THREADS)) rope_kv_write_k(Rope
     if (which)
         write_quads<T, TPG, QPER>(a.w, z, p, 1, head, rope_lds, part);
     else
-        rope_page<T, TPG, QPER>(a.w, a.k, z, p, head, part);
+        rope_page<T, TPG, QPER, INTER>(a.w, a.k, z, p, head, part);
 }
 
-template <typename T, int TPG, int QPER>
-static bool launch_rope_quads(const char* name, RopeKvArgs& a) {
+template <typename T, int TPG, int QPER, bool INTER>
+static bool launch_rope_pairs(const char* name, RopeKvArgs& a) {
     typedef Quads<T, TPG> Q;
-    auto kernel = rope_kv_write_k<T, TPG, QPER>;
+    auto kernel = rope_kv_write_k<T, TPG, QPER, INTER>;
     const size_t lds = (size_t)Q::GROUPS * a.w.dim * (a.w.g.page + 4);
     if constexpr (TPG == 1024) {  // the largest pages: 66560 bytes
         static const bool ok = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 256 * 260) == hipSuccess;
@@ -405,6 +404,11 @@ static bool launch_rope_quads(const char* name, RopeKvArgs& a) {
     a.shares = (uint32_t)shares, a.kv_blocks = (uint32_t)(shares * pairs);
     launch(name, kernel, dim3((unsigned)(shares * pairs + q_blocks)), dim3(Q::THREADS), lds, a);
     return true;
+}
+
+template <typename T, int TPG, int QPER>
+static bool launch_rope_quads(const char* name, RopeKvArgs& a) {
+    return a.k.interleaved ? launch_rope_pairs<T, TPG, QPER, true>(name, a) : launch_rope_pairs<T, TPG, QPER, false>(name, a);
 }
 
 // In one launch, if rows, angles and weights lie in packs; false if not
