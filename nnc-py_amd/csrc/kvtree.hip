@@ -21,6 +21,7 @@
 #include <limits.h>
 
 #include "kvattn.h"
+#include "lanes.h"
 
 namespace nnc {
 
@@ -46,7 +47,7 @@ struct TreeArgs {
 struct TreeSpan {
     Span span;
     int lo, tiles, units;
-    __device__ __forceinline__ TreeSpan(const TreeArgs& a, int b, int tile, int stride) : span(span_of(a.g, b)) {
+    __device__ __forceinline__ void set(const TreeArgs& a, int tile, int stride) {
         tiles = query_tiles(span, a.group, tile);
         // a row's position is first - 1 at least
         const int first = span.first();
@@ -55,51 +56,87 @@ struct TreeSpan {
     }
 };
 
-// Unit u of one cached head's: the sequence, u's place in it, and the tiles
-// before; how many units there are if u is -1. Every wave for itself, 64 sequences at a time.
+// Unit u of one cached head's: its sequence and tile, its place among the tile's
+// units, and the tiles of the sequences before.
 struct TreePlace {
-    int b;
-    int64_t u;
+    TreeSpan s;
+    int b, tile, unit;
     int64_t tiles;
 };
-__device__ __forceinline__ TreePlace locate(const TreeArgs& a, int64_t u, int tile, int stride) {
-    const int lane = threadIdx.x & 63;
-    int64_t units = 0, tiles = 0;
-    for (int base = 0; base < a.g.batch; base += 64) {
-        int64_t mine = 0, units_each = 0;
-        int t = 0;
+
+// The units of one cached head, found by 64 sequences at a time. The first 64
+// stay in registers, a sequence a lane.
+template <int TILE, int STRIDE>
+struct TreeIndex {
+    const TreeArgs& a;
+    TreeSpan mine;       // the lane's sequence
+    int tiles, upto_t;   // its tiles, with those of the lanes before
+    int64_t upto;        // units likewise
+    __device__ __forceinline__ void load(int base, int64_t tiles_before) {
+        const int lane = threadIdx.x & 63;
+        mine = TreeSpan{};
+        tiles = 0;
         if (base + lane < a.g.batch) {
-            const TreeSpan s(a, base + lane, tile, stride);
-            units_each = s.units, t = s.tiles;
-            mine = t * units_each;
+            mine.span = span_of(a.g, base + lane);
+            mine.set(a, TILE, STRIDE);
+            tiles = mine.tiles;
         }
         // (starts that decrease would make more tiles than there are counters for)
-        int upto_t = t;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int below = __shfl_up(upto_t, o);
-            if (lane >= o) upto_t += below;
-        }
-        const int before_t = upto_t - t;
-        const int64_t room = a.tiles - tiles - before_t;
-        if (room < t) t = room > 0 ? (int)room : 0, mine = t * units_each;
-        int64_t upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t below = __shfl_up((long long)upto, o);
-            if (lane >= o) upto += below;
-        }
-        const int64_t all = __shfl((long long)upto, 63);
-        if (u >= 0 && u - units < all) {
-            const int at = __ffsll((unsigned long long)__ballot(upto > u - units)) - 1;
-            return TreePlace{base + at, u - units - __shfl((long long)(upto - mine), at), tiles + __shfl(before_t, at)};
-        }
-        units += all;
-        tiles += __shfl(upto_t, 63);
-        if (tiles >= a.tiles) break;
+        upto_t = sum_before(tiles);
+        const int64_t room = a.tiles - tiles_before - (upto_t - tiles);
+        if (room < tiles) tiles = room > 0 ? (int)room : 0;
+        upto = (int64_t)sum_before((u64)tiles * (u64)mine.units);
     }
-    return TreePlace{-1, units, a.tiles};
-}
+    __device__ __forceinline__ explicit TreeIndex(const TreeArgs& args) : a(args) { load(0, 0); }
+    __device__ __forceinline__ int64_t total() {
+        int64_t units = 0, before = 0;
+        for (int base = 0;;) {
+            units += last(upto), before += last(upto_t);
+            base += 64;
+            if (base >= a.g.batch || before >= a.tiles) break;
+            load(base, before);
+        }
+        if (a.g.batch > 64) load(0, 0);
+        return units;
+    }
+    __device__ __forceinline__ static int64_t last(int64_t x) {
+        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, 63));
+    }
+    __device__ __forceinline__ static int last(int x) { return __builtin_amdgcn_readlane(x, 63); }
+    // u below total()
+    __device__ __forceinline__ TreePlace find(int64_t u) {
+        TreePlace p;
+        p.tiles = 0;
+        bool moved = false;
+        for (int base = 0;; base += 64, moved = true) {
+            if (base > 0) load(base, p.tiles);
+            const uint64_t past = __ballot(upto > u);
+            if (past || base + 64 >= a.g.batch) {
+                const int at = past ? __ffsll((unsigned long long)past) - 1 : 63;
+                auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+                p.b = base + at;
+                p.s.span.end = of(mine.span.end), p.s.span.length = of(mine.span.length), p.s.span.rows = of(mine.span.rows);
+                p.s.lo = of(mine.lo), p.s.tiles = of(tiles), p.s.units = of(mine.units);
+                const int64_t whole = (int64_t)((uint64_t)(uint32_t)of((int)(upto >> 32)) << 32 | (uint32_t)of((int)upto));
+                u -= whole - (int64_t)p.s.tiles * p.s.units;
+                p.tiles += of(upto_t) - of(mine.tiles);
+                break;
+            }
+            u -= last(upto), p.tiles += last(upto_t);
+        }
+        if (moved) load(0, 0);
+        if (u < p.s.units) {
+            p.tile = 0, p.unit = (int)u;
+        } else {
+            p.tile = (int)(u / p.s.units), p.unit = (int)(u - (int64_t)p.tile * p.s.units);
+        }
+        return p;
+    }
+};
+
+// Items of so many units or fewer are left whole: a unit takes a workgroup less
+// than storing and joining two shares do.
+static constexpr int kShort = 4;
 
 // A run's share of an item: units [unit, unit + n) of a tile and cached head.
 struct TreeShare {
@@ -514,24 +551,32 @@ template <typename T, int D, int RB, int NW, int OCC>
 __global__ void __launch_bounds__(64 * NW, OCC) kv_tree_k(TreeArgs a) {
     constexpr int STRIDE = 64 * NW, R = 16 * RB;
     extern __shared__ __align__(16) float tree_lds[];
-    const TreePlace sum = locate(a, -1, R, STRIDE);
-    const int64_t total = sum.u * a.kv_heads;
+    TreeIndex<R, STRIDE> index(a);
+    const int64_t each = index.total(), total = each * a.kv_heads;
     // runs of `least` units or more
     const int64_t useful = (total + a.least - 1) / a.least;
     const int runs = __builtin_amdgcn_readfirstlane((int)(useful < gridDim.x ? useful : gridDim.x));
     if ((int)blockIdx.x >= runs) return;
     const int run = xcd_remap(blockIdx.x, runs);
-    const int64_t end = run_begin(run + 1, total, runs);
-    for (int64_t at = run_begin(run, total, runs); at < end;) {
-        const int head_kv = (int)(at / sum.u);
-        const TreePlace p = locate(a, at - head_kv * sum.u, R, STRIDE);
-        const int b = __builtin_amdgcn_readfirstlane(p.b);
-        const TreeSpan s(a, b, R, STRIDE);
+    auto find = [&](int64_t u, int& head_kv) {
+        head_kv = u < each ? 0 : (int)(u / each);
+        return index.find(u - head_kv * each);
+    };
+    // a short item is not cut, but its first run's
+    auto begin_of = [&](int r) {
+        const int64_t u = run_begin(r, total, runs);
+        int head_kv;
+        if (u == 0 || u == total) return u;
+        const TreePlace p = find(u, head_kv);
+        return p.s.units <= kShort ? u - p.unit : u;
+    };
+    const int64_t end = begin_of(run + 1);
+    for (int64_t at = begin_of(run); at < end;) {
         TreeShare w;
-        w.span = s.span, w.b = b, w.head_kv = __builtin_amdgcn_readfirstlane(head_kv), w.lo = s.lo;
-        w.tile = __builtin_amdgcn_readfirstlane((int)(p.u / s.units));
-        w.unit = __builtin_amdgcn_readfirstlane((int)(p.u - (int64_t)w.tile * s.units));
-        w.n = __builtin_amdgcn_readfirstlane((int)(end - at < s.units - w.unit ? end - at : s.units - w.unit));
+        const TreePlace p = find(at, w.head_kv);
+        const TreeSpan& s = p.s;
+        w.span = s.span, w.b = p.b, w.lo = s.lo, w.tile = p.tile, w.unit = p.unit;
+        w.n = (int)(end - at < s.units - w.unit ? end - at : s.units - w.unit);
         w.whole = w.n == s.units;
         const int64_t begin = at - w.unit;  // of the item
         const int place = share_place(run, begin, total, runs);
@@ -545,7 +590,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) kv_tree_k(TreeArgs a) {
             tree_share<T, D, R, 1, NW>(a, w, place, tree_lds);
         if (!w.whole) {
             const int run0 = run_of(begin, total, runs), shares = run_of(begin + s.units - 1, total, runs) - run0 + 1;
-            if (finish_arrive(a.counters + (int64_t)head_kv * a.tiles + p.tiles + w.tile, shares - 1)) {
+            if (finish_arrive(a.counters + (int64_t)w.head_kv * a.tiles + p.tiles + w.tile, shares - 1)) {
                 const TreePlaces<D, R> places(a);
                 join_shares<T, D, R, 64 * NW>(
                     places, (int)min((int64_t)R, left), shares, [&](int sh) { return share_place(run0 + sh, begin, total, runs); },

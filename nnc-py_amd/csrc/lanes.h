@@ -34,6 +34,26 @@ __device__ __forceinline__ u64 lane_xor(u64 x) { return (u64)lane_xor<J>((uint32
 template <int J>
 __device__ __forceinline__ double lane_xor(double x) { return __longlong_as_double((long long)lane_xor<J>((u64)__double_as_longlong(x))); }
 
+// The sum of a lane's value and those of the lanes before it
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lanes_before(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 lanes_before(u64 x) {
+    return (u64)lanes_before<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | lanes_before<CTRL, ROWS>((uint32_t)x);
+}
+template <typename K>
+__device__ __forceinline__ K sum_before_unsigned(K x) {
+    x += lanes_before<0x111, 0xf>(x);  // 1, 2, 4, 8 lanes up in rows of 16
+    x += lanes_before<0x112, 0xf>(x);
+    x += lanes_before<0x114, 0xf>(x);
+    x += lanes_before<0x118, 0xf>(x);
+    x += lanes_before<0x142, 0xa>(x);  // a row's last to the next row, rows 1 and 3
+    x += lanes_before<0x143, 0xc>(x);  // lane 31 to rows 2 and 3
+    return x;
+}
+__device__ __forceinline__ u64 sum_before(u64 x) { return sum_before_unsigned(x); }
+__device__ __forceinline__ int sum_before(int x) { return (int)sum_before_unsigned((uint32_t)x); }
+
 // What `op` makes of the values of 2 J lanes side by side
 template <int J = 32, typename K, class Op>
 __device__ __forceinline__ K over_lanes(K x, Op op) {
