@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(64 * NW, OCC) kv_tree_k(TreeArgs a) {
     extern __shared__ __align__(16) float tree_lds[];
     TreeIndex<R, STRIDE> index(a);
     const int64_t each = index.total(), total = each * a.kv_heads;
-    // runs of `least` units or more
+    // runs of `least` units or more: two, or one where no item is cut
     const int64_t useful = (total + a.least - 1) / a.least;
     const int runs = __builtin_amdgcn_readfirstlane((int)(useful < gridDim.x ? useful : gridDim.x));
     if ((int)blockIdx.x >= runs) return;
@@ -676,7 +676,7 @@ void nnc_hip_kv_tree_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tens
     const int capacity = c.ragged.width * c.page;
     const int longest = max_length > 0 && max_length < capacity ? max_length : capacity;
     TreeArgs a{c.ragged, c.k, c.v, c.k_scale, c.v_scale, (const int*)tree->data, q->data, out->data, nullptr, nullptr, ld, 0, q_col, heads,
-               c.kv_heads, group, window_of(window, capacity), (int)tree->shape[1], 2, slot_magic(c.page / 16),
+               c.kv_heads, group, window_of(window, capacity), (int)tree->shape[1], longest <= 256 * kShort ? 1 : 2, slot_magic(c.page / 16),
                aligned16(q->data) && ld * activation_bytes(q) % 16 == 0 && q_col * activation_bytes(q) % 16 == 0,
                scale * 1.44269504088896340736f};
     a.g.rows = (int)rows;
