@@ -619,7 +619,9 @@ static void launch_blocks(const char* name, TreeArgs& a, int64_t rows) {
     constexpr int lds = tree_lds_bytes<T, D, RB, NW>();
     static const bool ok = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) == hipSuccess;
     if (!ok) return fail(NNC_HIP_EDEVICE, name, "hipFuncSetAttribute failed");
-    const int runs = cu_count() * OCC;
+    // (whole items on 16 rows, two workgroups a CU: 64 trees of 4 behind up to 1024 30 -> 26 us, 256 of 2 behind up to
+    // 500 87 -> 62)
+    const int runs = cu_count() * (OCC > 1 || (RB == 1 && D <= 128 && a.least == 1) ? 2 : 1);
     a.tiles = query_tiles_bound(rows, a.g.batch, a.group, 16 * RB);
     const int64_t items = a.tiles * a.kv_heads;
     const size_t bytes = (size_t)runs * 2 * 16 * RB * (D + 4) * sizeof(float);
