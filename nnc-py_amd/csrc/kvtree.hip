@@ -11,13 +11,19 @@
 //
 // Drafts are many rows for one cached head - tokens times the heads of a group -
 // but not enough to hide that the cache has to be read, and the keys are many.
-// So a wave takes up to 64 query rows (4 blocks of 16) with 64 keys at a time:
-// a key's whole numbers are made f16 once for all of them and stay in
-// registers, and waves need no barrier until their rows are joined. The keys of
-// all sequences and heads, in units of 64 for each wave, are one line that is cut
-// into as many runs as there are CUs, so that ragged lengths leave none idle:
-// what a run has of a sequence that others share is stored, and the last to
-// arrive joins the shares in their order.
+// So a wave takes 16 or 32 query rows with 64 keys at a time: a key's whole
+// numbers are made f16 in registers, once for all of them, and the four waves of
+// a workgroup need no barrier until their rows are joined. The keys of all
+// sequences and heads, in units of 64 for each wave, are one line that is cut
+// into a run for each workgroup that the CUs hold, so that ragged lengths leave
+// none idle: what a run has of a sequence that others share is stored, and the
+// last to arrive joins the shares in their order.
+//
+// Few rows are bound by the cache's bytes: 32 sequences of 4 behind 4096, 32
+// heads over 8 of 128 in f16, 53 us, 5.1 TB/s, the rate of a copy. Many by the
+// vector units, which widen the keys and make masks, maxima and exponentials: 32
+// sequences of 16 behind up to 8192 77 us, 2.7 TB/s, one of 64 behind 65536 122
+// us, 560 TFLOP/s of 1170.
 #include <limits.h>
 
 #include "kvattn.h"
@@ -581,11 +587,8 @@ __global__ void __launch_bounds__(64 * NW, OCC) kv_tree_k(TreeArgs a) {
         const int64_t begin = at - w.unit;  // of the item
         const int place = share_place(run, begin, total, runs);
         const int64_t left = (int64_t)s.span.rows * a.group - (int64_t)w.tile * R;
-        const int blocks = left >= R ? RB : (int)((left + 15) / 16);
-        if (RB > 2 && blocks > 2)
+        if (RB > 1 && left > 16)
             tree_share<T, D, R, RB, NW>(a, w, place, tree_lds);
-        else if (RB > 1 && blocks > 1)
-            tree_share<T, D, R, 2, NW>(a, w, place, tree_lds);
         else
             tree_share<T, D, R, 1, NW>(a, w, place, tree_lds);
         if (!w.whole) {
@@ -632,12 +635,19 @@ static void launch_blocks(const char* name, TreeArgs& a, int64_t rows) {
     launch(name, kernel, dim3((unsigned)runs), dim3(64 * NW), lds, a);
 }
 
-// Blocks of 16 query rows of a tile
+// Query rows of a tile: 16 while a sequence has no more for a cached head; 32 with
+// the registers of a SIMD for one wave while it has no more, else for two, of
+// which one has its exponentials while the other has its products. 32 rows, one
+// and two waves, us, of 32 heads over 8 of 128: 32 sequences of 8 behind 4096 56 and
+// 67, of 16 behind up to 8192 101 and 77, one of 64 behind 65536 147 and 122. (64
+// rows, whose sums leave no second wave: 93 and 148 for the last two.) Of dim 256,
+// 16 heads over 4, 16 rows and 32, us: 8 sequences of 16 behind 4096 40 and 44, of
+// 8 30 and 41, one of 64 behind 16384 61 and 60: 16 there.
 template <typename T, int D>
 static void launch_tree(const char* name, TreeArgs& a, int64_t rows) {
     const int64_t holders = rows < a.g.batch ? rows : a.g.batch, each = ceil_div(rows * a.group, holders);
-    if (D <= 128 && each > 32) return launch_blocks<T, D, 2, 4, D <= 128 ? 2 : 1>(name, a, rows);
-    if (D <= 128 || sizeof(T) == 2) {
+    if constexpr (D <= 128) {
+        if (each > 32) return launch_blocks<T, D, 2, 4, 2>(name, a, rows);
         if (each > 16) return launch_blocks<T, D, 2, 4, 1>(name, a, rows);
     }
     launch_blocks<T, D, 1, 4, 1>(name, a, rows);

@@ -213,231 +213,229 @@ __global__ void __launch_bounds__(64 * NW) logprobs_k(LogprobArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float c = a.scale * 1.44269504088896340736f;
     const uint32_t line = blockIdx.x / (uint32_t)a.segments, segment = blockIdx.x - line * (uint32_t)a.segments;
-    {
-        const int64_t row = a.row0 + line;
-        const T* x = (const T*)a.logits + row * a.vocab;
-        const int off = (int)(((uintptr_t)x & 15) / sizeof(T));
-        const int64_t first = (int64_t)segment * a.each, rest = (off + a.vocab + V - 1) / V - first;
-        const int n = (int)(rest < a.each ? rest : a.each), at = wave * 64 + lane;
-        const int64_t index0 = first * V - off;  // of the segment's first value, as if its pack were the row's own
-        // packs that are the row's own: [own, own_end) of the segment's
-        const int own = first == 0 && off > 0 ? 1 : 0, own_end = rest <= a.each && (off + a.vocab) % V ? n - 1 : n;
-        const nt_u32x4* packs = (const nt_u32x4*)(x - off) + first;
-        nt_u32x4 raw[PACKS];
+    const int64_t row = a.row0 + line;
+    const T* x = (const T*)a.logits + row * a.vocab;
+    const int off = (int)(((uintptr_t)x & 15) / sizeof(T));
+    const int64_t first = (int64_t)segment * a.each, rest = (off + a.vocab + V - 1) / V - first;
+    const int n = (int)(rest < a.each ? rest : a.each), at = wave * 64 + lane;
+    const int64_t index0 = first * V - off;  // of the segment's first value, as if its pack were the row's own
+    // packs that are the row's own: [own, own_end) of the segment's
+    const int own = first == 0 && off > 0 ? 1 : 0, own_end = rest <= a.each && (off + a.vocab) % V ? n - 1 : n;
+    const nt_u32x4* packs = (const nt_u32x4*)(x - off) + first;
+    nt_u32x4 raw[PACKS];
+#pragma unroll
+    for (int p = 0; p < PACKS; ++p) {
+        const int j = at + NW * 64 * p;
+        raw[p] = nt_u32x4{Words<T>::NONE, Words<T>::NONE, Words<T>::NONE, Words<T>::NONE};
+        if (j >= own && j < own_end) raw[p] = packs[j];
+    }
+    for (int edge = 0; edge < 2; ++edge) {
+        const int e = edge ? n - 1 : 0;
+        if (edge ? own_end == n || e < own : own == 0) continue;
+        Pack<T, V> part;
+#pragma unroll
+        for (int u = 0; u < V; ++u) {
+            const int64_t i = index0 + (int64_t)e * V + u;
+            part.v[u] = i >= 0 && i < a.vocab ? x[i] : (T)-INFINITY;
+        }
+        const nt_u32x4 words = __builtin_bit_cast(nt_u32x4, part);
+#pragma unroll
+        for (int p = 0; p < PACKS; ++p) raw[p] = at + NW * 64 * p == e ? words : raw[p];
+    }
+    nt_u32x4 best = raw[0];
+#pragma unroll
+    for (int p = 1; p < PACKS; ++p)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) best[u] = Words<T>::max_of(best[u], raw[p][u]);
+    float mine = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < V; ++u) mine = fmaxf(mine, Words<T>::at(best, u));
+    float top = mine, bar = -INFINITY;
+    if (TOP) {
+        const float order = sort_rising(mine);
+        top = __shfl(order, 63), bar = __shfl(order, 64 - a.top);
+        const float part = __shfl(order, 64 - (a.top + NW - 1) / NW);
+        if (NW > 1) {
+            if (lane == 0) tops[wave] = top, bars[wave] = bar, parts[wave] = part;
+            if (threadIdx.x == 0) gathered = 0;
+            __syncthreads();
+            float least = INFINITY;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) top = fmaxf(top, tops[w]), bar = fmaxf(bar, bars[w]), least = fminf(least, parts[w]);
+            bar = fmaxf(bar, least);
+        } else {
+            if (threadIdx.x == 0) gathered = 0;
+            __syncthreads();
+        }
+    } else {
+        top = over_lanes(mine, [](float p, float q) { return fmaxf(p, q); });
+        if (NW > 1) {
+            if (lane == 0) tops[wave] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; ++w) top = fmaxf(top, tops[w]);
+        }
+    }
+    Likeliest likeliest;
+    likeliest.init(room[wave]);
+    if (TOP) {
+        uint32_t reach = 0;  // packs that reach the bar
 #pragma unroll
         for (int p = 0; p < PACKS; ++p) {
-            const int j = at + NW * 64 * p;
-            raw[p] = nt_u32x4{Words<T>::NONE, Words<T>::NONE, Words<T>::NONE, Words<T>::NONE};
-            if (j >= own && j < own_end) raw[p] = packs[j];
-        }
-        for (int edge = 0; edge < 2; ++edge) {
-            const int e = edge ? n - 1 : 0;
-            if (edge ? own_end == n || e < own : own == 0) continue;
-            Pack<T, V> part;
+            uint32_t most = raw[p][0];
 #pragma unroll
-            for (int u = 0; u < V; ++u) {
-                const int64_t i = index0 + (int64_t)e * V + u;
-                part.v[u] = i >= 0 && i < a.vocab ? x[i] : (T)-INFINITY;
+            for (int u = 1; u < 4; ++u) most = Words<T>::max_of(most, raw[p][u]);
+            const nt_u32x4 both = {most, most, most, most};
+            const bool hit = V == 4 ? Words<T>::at(both, 0) >= bar : fmaxf(Words<T>::at(both, 0), Words<T>::at(both, 1)) >= bar;
+            reach |= hit ? 1u << p : 0u;
+        }
+        auto pack_of = [&](int which) {
+            nt_u32x4 pack = {0, 0, 0, 0};
+#pragma unroll
+            for (int p = 0; p < PACKS; ++p) pack |= raw[p] & (which == p ? 0xffffffffu : 0u);
+            return pack;
+        };
+        constexpr int ROOM = NW * 64 < 256 ? NW * 64 : 256;
+        u64* all = room[0];
+        for (uint32_t hits = reach; hits; hits &= hits - 1) {
+            const int which = __ffs(hits) - 1;
+            const nt_u32x4 pack = pack_of(which);
+            const int64_t i = index0 + (int64_t)(at + NW * 64 * which) * V;
+            uint32_t values = 0;
+#pragma unroll
+            for (int u = 0; u < V; ++u) values |= Words<T>::at(pack, u) >= bar ? 1u << u : 0u;
+            if (bar == -INFINITY) {  // what is not the row's own reaches it, too
+#pragma unroll
+                for (int u = 0; u < V; ++u)
+                    if (at + NW * 64 * which >= n || i + u < 0 || i + u >= a.vocab) values &= ~(1u << u);
             }
-            const nt_u32x4 words = __builtin_bit_cast(nt_u32x4, part);
-#pragma unroll
-            for (int p = 0; p < PACKS; ++p) raw[p] = at + NW * 64 * p == e ? words : raw[p];
+            int place = atomicAdd(&gathered, __popc(values));
+            for (; values; values &= values - 1, ++place) {
+                const int u = __ffs(values) - 1;
+                const uint32_t w = (u * (int)sizeof(T) & 8 ? (u * (int)sizeof(T) & 4 ? pack[3] : pack[2]) : u * (int)sizeof(T) & 4 ? pack[1] : pack[0]);
+                const nt_u32x4 first_of = {sizeof(T) == 2 && (u & 1) ? w >> 16 : w, 0, 0, 0};
+                if (place < ROOM) all[place] = rank_of(Words<T>::at(first_of, 0), (uint32_t)(i + u));
+            }
         }
-        nt_u32x4 best = raw[0];
-#pragma unroll
-        for (int p = 1; p < PACKS; ++p)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) best[u] = Words<T>::max_of(best[u], raw[p][u]);
-        float mine = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < V; ++u) mine = fmaxf(mine, Words<T>::at(best, u));
-        float top = mine, bar = -INFINITY;
-        if (TOP) {
-            const float order = sort_rising(mine);
-            top = __shfl(order, 63), bar = __shfl(order, 64 - a.top);
-            const float part = __shfl(order, 64 - (a.top + NW - 1) / NW);
-            if (NW > 1) {
-                if (lane == 0) tops[wave] = top, bars[wave] = bar, parts[wave] = part;
-                if (threadIdx.x == 0) gathered = 0;
+        __syncthreads();
+        const int total = gathered;
+        if (total <= ROOM) {
+            u64 key = 0;
+            if (wave * 64 < total) {
+                key = sort_rising(threadIdx.x < total ? all[threadIdx.x] : 0);
+                if (wave > 0) all[threadIdx.x] = key;
+            }
+            if (wave == 0) likeliest.merge(key, a.top);
+            if (NW > 1 && total > 64) {
                 __syncthreads();
-                float least = INFINITY;
-#pragma unroll
-                for (int w = 0; w < NW; ++w) top = fmaxf(top, tops[w]), bar = fmaxf(bar, bars[w]), least = fminf(least, parts[w]);
-                bar = fmaxf(bar, least);
-            } else {
-                if (threadIdx.x == 0) gathered = 0;
-                __syncthreads();
+                if (wave == 0)
+                    for (int w = 1; w * 64 < total; ++w) likeliest.merge(room[w][lane], a.top);
             }
         } else {
-            top = over_lanes(mine, [](float p, float q) { return fmaxf(p, q); });
-            if (NW > 1) {
-                if (lane == 0) tops[wave] = top;
-                __syncthreads();
-#pragma unroll
-                for (int w = 0; w < NW; ++w) top = fmaxf(top, tops[w]);
-            }
-        }
-        Likeliest likeliest;
-        likeliest.init(room[wave]);
-        if (TOP) {
-            uint32_t reach = 0;  // packs that reach the bar
-#pragma unroll
-            for (int p = 0; p < PACKS; ++p) {
-                uint32_t most = raw[p][0];
-#pragma unroll
-                for (int u = 1; u < 4; ++u) most = Words<T>::max_of(most, raw[p][u]);
-                const nt_u32x4 both = {most, most, most, most};
-                const bool hit = V == 4 ? Words<T>::at(both, 0) >= bar : fmaxf(Words<T>::at(both, 0), Words<T>::at(both, 1)) >= bar;
-                reach |= hit ? 1u << p : 0u;
-            }
-            auto pack_of = [&](int which) {
-                nt_u32x4 pack = {0, 0, 0, 0};
-#pragma unroll
-                for (int p = 0; p < PACKS; ++p) pack |= raw[p] & (which == p ? 0xffffffffu : 0u);
-                return pack;
-            };
-            constexpr int ROOM = NW * 64 < 256 ? NW * 64 : 256;
-            u64* all = room[0];
-            for (uint32_t hits = reach; hits; hits &= hits - 1) {
-                const int which = __ffs(hits) - 1;
-                const nt_u32x4 pack = pack_of(which);
-                const int64_t i = index0 + (int64_t)(at + NW * 64 * which) * V;
-                uint32_t values = 0;
-#pragma unroll
-                for (int u = 0; u < V; ++u) values |= Words<T>::at(pack, u) >= bar ? 1u << u : 0u;
-                if (bar == -INFINITY) {  // what is not the row's own reaches it, too
-#pragma unroll
-                    for (int u = 0; u < V; ++u)
-                        if (at + NW * 64 * which >= n || i + u < 0 || i + u >= a.vocab) values &= ~(1u << u);
-                }
-                int place = atomicAdd(&gathered, __popc(values));
-                for (; values; values &= values - 1, ++place) {
-                    const int u = __ffs(values) - 1;
-                    const uint32_t w = (u * (int)sizeof(T) & 8 ? (u * (int)sizeof(T) & 4 ? pack[3] : pack[2]) : u * (int)sizeof(T) & 4 ? pack[1] : pack[0]);
-                    const nt_u32x4 first_of = {sizeof(T) == 2 && (u & 1) ? w >> 16 : w, 0, 0, 0};
-                    if (place < ROOM) all[place] = rank_of(Words<T>::at(first_of, 0), (uint32_t)(i + u));
-                }
-            }
             __syncthreads();
-            const int total = gathered;
-            if (total <= ROOM) {
-                u64 key = 0;
-                if (wave * 64 < total) {
-                    key = sort_rising(threadIdx.x < total ? all[threadIdx.x] : 0);
-                    if (wave > 0) all[threadIdx.x] = key;
-                }
-                if (wave == 0) likeliest.merge(key, a.top);
-                if (NW > 1 && total > 64) {
-                    __syncthreads();
-                    if (wave == 0)
-                        for (int w = 1; w * 64 < total; ++w) likeliest.merge(room[w][lane], a.top);
-                }
-            } else {
-                __syncthreads();
-                for (uint32_t hits = reach; __any(hits); hits &= hits - 1) {
-                    const int which = hits ? __ffs(hits) - 1 : 0;
-                    nt_u32x4 pack = pack_of(which);
+            for (uint32_t hits = reach; __any(hits); hits &= hits - 1) {
+                const int which = hits ? __ffs(hits) - 1 : 0;
+                nt_u32x4 pack = pack_of(which);
 #pragma unroll 1
-                    for (int u = 0; u < V; ++u) {
-                        const float y = Words<T>::at(pack, 0);
-                        const int64_t i = index0 + (int64_t)(at + NW * 64 * which) * V + u;
-                        const bool is = hits && y >= bar && at + NW * 64 * which < n && i >= 0 && i < a.vocab;
-                        if (__any(is)) likeliest.put(is, y, i, a.top);
-                        pack = Words<T>::next(pack);
-                    }
+                for (int u = 0; u < V; ++u) {
+                    const float y = Words<T>::at(pack, 0);
+                    const int64_t i = index0 + (int64_t)(at + NW * 64 * which) * V + u;
+                    const bool is = hits && y >= bar && at + NW * 64 * which < n && i >= 0 && i < a.vocab;
+                    if (__any(is)) likeliest.put(is, y, i, a.top);
+                    pack = Words<T>::next(pack);
                 }
-                likeliest.flush(a.top);
-                if (NW > 1) {
-                    room[wave][63 - lane] = likeliest.list;
-                    __syncthreads();
-                    if (wave == 0)
-                        for (int w = 1; w < NW; ++w) likeliest.merge(room[w][lane], a.top);
-                }
+            }
+            likeliest.flush(a.top);
+            if (NW > 1) {
+                room[wave][63 - lane] = likeliest.list;
+                __syncthreads();
+                if (wave == 0)
+                    for (int w = 1; w < NW; ++w) likeliest.merge(room[w][lane], a.top);
             }
         }
-        RowSums s{top, 0.0, 0.0, 0.0};
-        if (top > -INFINITY && __any(mine == top)) s.ones = take_out<T>(raw, top);
-        if (fabsf(base_of(top) * c) < 4096.f)  // what `off` neglects, its square, is below 2^-25
-            sum_packs<T, false>(raw, top, c, s);
-        else
-            sum_packs<T, true>(raw, top, c, s);
-        // join the lanes, the waves, the segments
-        auto add = [](double p, double q) { return p + q; };
-        s.rest = over_lanes(s.rest, add), s.ones = over_lanes(s.ones, add), s.weighted = over_lanes(s.weighted, add);
-        if (NW > 1) {
-            if (lane == 0) sums[wave] = s;
-            __syncthreads();
-            if (wave == 0) {
-#pragma unroll
-                for (int w = 1; w < NW; ++w) {
-                    s.rest += sums[w].rest, s.ones += sums[w].ones, s.weighted += sums[w].weighted;
-                }
-            }
-        }
-        if (a.segments > 1) {
-            const int slot = slot_floats(a.top);
-            const __amdgpu_buffer_rsrc_t r = make_rsrc(a.part);
-            auto put8 = [&](uint32_t at, u64 x) {
-                store_partial(r, at * 4u, __uint_as_float((uint32_t)x));
-                store_partial(r, at * 4u + 4u, __uint_as_float((uint32_t)(x >> 32)));
-            };
-            auto get8 = [&](uint32_t at) {
-                return (u64)__float_as_uint(load_partial(r, at * 4u)) | (u64)__float_as_uint(load_partial(r, at * 4u + 4u)) << 32;
-            };
-            if (wave == 0) {
-                const uint32_t at = blockIdx.x * (uint32_t)slot;
-                if (lane == 0) {
-                    put8(at, __double_as_longlong(s.rest));
-                    put8(at + 2, __double_as_longlong(s.ones));
-                    put8(at + 4, __double_as_longlong(s.weighted));
-                    store_partial(r, at * 4u + 24u, s.m);
-                }
-                if (TOP && lane < a.top) put8(at + kSlotHead + 2 * lane, likeliest.list);
-            }
-            if (!finish_arrive(a.counters + line, a.segments - 1)) return;
-            if (wave == 0) {
-                s = RowSums{-INFINITY, 0.0, 0.0, 0.0};
-                for (int g = lane; g < a.segments; g += 64) {
-                    const uint32_t at = (uint32_t)(line * a.segments + g) * slot;
-                    add_sums(s, RowSums{load_partial(r, at * 4u + 24u), __longlong_as_double(get8(at)), __longlong_as_double(get8(at + 2)),
-                                        __longlong_as_double(get8(at + 4))}, c);
-                }
-#pragma unroll
-                for (int o = 1; o < 64; o <<= 1)
-                    add_sums(s, RowSums{__shfl_xor(s.m, o), __shfl_xor(s.rest, o), __shfl_xor(s.ones, o), __shfl_xor(s.weighted, o)}, c);
-            }
-            if (TOP) {
-                likeliest.init(room[wave]);
-                for (int g = wave; g < a.segments; g += NW) {
-                    const uint32_t at = (uint32_t)(line * a.segments + g) * slot + kSlotHead;
-                    likeliest.merge(63 - lane < a.top ? get8(at + 2 * (63 - lane)) : 0, a.top);
-                }
-                if (NW > 1) {
-                    room[wave][63 - lane] = likeliest.list;
-                    __syncthreads();
-                    if (wave == 0)
-#pragma unroll
-                        for (int w = 1; w < NW; ++w) likeliest.merge(room[w][lane], a.top);
-                }
-            }
-        }
+    }
+    RowSums s{top, 0.0, 0.0, 0.0};
+    if (top > -INFINITY && __any(mine == top)) s.ones = take_out<T>(raw, top);
+    if (fabsf(base_of(top) * c) < 4096.f)  // what `off` neglects, its square, is below 2^-25
+        sum_packs<T, false>(raw, top, c, s);
+    else
+        sum_packs<T, true>(raw, top, c, s);
+    // join the lanes, the waves, the segments
+    auto add = [](double p, double q) { return p + q; };
+    s.rest = over_lanes(s.rest, add), s.ones = over_lanes(s.ones, add), s.weighted = over_lanes(s.weighted, add);
+    if (NW > 1) {
+        if (lane == 0) sums[wave] = s;
+        __syncthreads();
         if (wave == 0) {
-            const double sum = s.rest + s.ones;
-            const bool ok = fabsf(s.m) < INFINITY && sum == sum;
-            const double log_sum = s.ones == 1.0 ? log1p(s.rest) : log(sum);
-            auto log_p = [&](float y) { return (float)((double)a.scale * ((double)y - (double)s.m) - log_sum); };
+#pragma unroll
+            for (int w = 1; w < NW; ++w) {
+                s.rest += sums[w].rest, s.ones += sums[w].ones, s.weighted += sums[w].weighted;
+            }
+        }
+    }
+    if (a.segments > 1) {
+        const int slot = slot_floats(a.top);
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(a.part);
+        auto put8 = [&](uint32_t at, u64 x) {
+            store_partial(r, at * 4u, __uint_as_float((uint32_t)x));
+            store_partial(r, at * 4u + 4u, __uint_as_float((uint32_t)(x >> 32)));
+        };
+        auto get8 = [&](uint32_t at) {
+            return (u64)__float_as_uint(load_partial(r, at * 4u)) | (u64)__float_as_uint(load_partial(r, at * 4u + 4u)) << 32;
+        };
+        if (wave == 0) {
+            const uint32_t at = blockIdx.x * (uint32_t)slot;
             if (lane == 0) {
-                if (a.entropy) a.entropy[row] = ok ? (float)(log_sum - s.weighted / sum * 0.69314718055994530942) : NAN;
-                if (a.logprob) {
-                    const int t = a.tokens[row];
-                    a.logprob[row] = ok && t >= 0 && t < a.vocab ? log_p((float)x[t]) : NAN;
-                }
+                put8(at, __double_as_longlong(s.rest));
+                put8(at + 2, __double_as_longlong(s.ones));
+                put8(at + 4, __double_as_longlong(s.weighted));
+                store_partial(r, at * 4u + 24u, s.m);
             }
-            if (TOP && lane < a.top) {
-                const u64 key = likeliest.list;
-                a.top_index[row * a.top + lane] = ok && key ? index_of(key) : -1;
-                a.top_logprob[row * a.top + lane] = !ok ? NAN : key ? log_p(value_of(key)) : -INFINITY;
+            if (TOP && lane < a.top) put8(at + kSlotHead + 2 * lane, likeliest.list);
+        }
+        if (!finish_arrive(a.counters + line, a.segments - 1)) return;
+        if (wave == 0) {
+            s = RowSums{-INFINITY, 0.0, 0.0, 0.0};
+            for (int g = lane; g < a.segments; g += 64) {
+                const uint32_t at = (uint32_t)(line * a.segments + g) * slot;
+                add_sums(s, RowSums{load_partial(r, at * 4u + 24u), __longlong_as_double(get8(at)), __longlong_as_double(get8(at + 2)),
+                                    __longlong_as_double(get8(at + 4))}, c);
             }
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1)
+                add_sums(s, RowSums{__shfl_xor(s.m, o), __shfl_xor(s.rest, o), __shfl_xor(s.ones, o), __shfl_xor(s.weighted, o)}, c);
+        }
+        if (TOP) {
+            likeliest.init(room[wave]);
+            for (int g = wave; g < a.segments; g += NW) {
+                const uint32_t at = (uint32_t)(line * a.segments + g) * slot + kSlotHead;
+                likeliest.merge(63 - lane < a.top ? get8(at + 2 * (63 - lane)) : 0, a.top);
+            }
+            if (NW > 1) {
+                room[wave][63 - lane] = likeliest.list;
+                __syncthreads();
+                if (wave == 0)
+#pragma unroll
+                    for (int w = 1; w < NW; ++w) likeliest.merge(room[w][lane], a.top);
+            }
+        }
+    }
+    if (wave == 0) {
+        const double sum = s.rest + s.ones;
+        const bool ok = fabsf(s.m) < INFINITY && sum == sum;
+        const double log_sum = s.ones == 1.0 ? log1p(s.rest) : log(sum);
+        auto log_p = [&](float y) { return (float)((double)a.scale * ((double)y - (double)s.m) - log_sum); };
+        if (lane == 0) {
+            if (a.entropy) a.entropy[row] = ok ? (float)(log_sum - s.weighted / sum * 0.69314718055994530942) : NAN;
+            if (a.logprob) {
+                const int t = a.tokens[row];
+                a.logprob[row] = ok && t >= 0 && t < a.vocab ? log_p((float)x[t]) : NAN;
+            }
+        }
+        if (TOP && lane < a.top) {
+            const u64 key = likeliest.list;
+            a.top_index[row * a.top + lane] = ok && key ? index_of(key) : -1;
+            a.top_logprob[row * a.top + lane] = !ok ? NAN : key ? log_p(value_of(key)) : -INFINITY;
         }
     }
 }

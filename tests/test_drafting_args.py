@@ -9,9 +9,19 @@ from pathlib import Path
 import numpy as np
 import pytest
 
-from test_serving8_args import EINVAL, ESTATE, EUNSUPP, F16, F32, I8, I32, I64, cache, cache_changes, check, lib  # noqa: F401
+from test_serving8_args import EINVAL, ESTATE, EUNSUPP, F16, F32, I8, I32, I64, Lib, cache, cache_changes, check
 
 ROOT = Path(__file__).resolve().parent.parent
+
+
+@pytest.fixture
+def lib(abi, pkg):
+    # the calls in order name memory that is not there: none may run where the
+    # library could have been initialised, whatever another runtime says
+    if Path("/dev/kfd").exists():
+        pytest.skip("a GPU is there: these calls would run")
+    from nnc_py_amd import runtime
+    return Lib(abi, runtime)
 
 
 def test_index_arithmetic_of_masks(tmp_path):
@@ -23,7 +33,7 @@ def test_index_arithmetic_of_masks(tmp_path):
     assert res.returncode == 0 and res.stdout == "ok\n", res.stdout + res.stderr
 
 
-def test_rope_refusals(lib):  # noqa: F811
+def test_rope_refusals(lib):
     t = lib.t
     far = 1 << 20
     good = {"in": t(F16, 7, 300), "weight": t(F16, 64), "angles": t(F32, 50, 32), "positions": t(I32, 7), "out": t(F16, 7, 256, data=far),
@@ -50,7 +60,7 @@ def test_rope_refusals(lib):  # noqa: F811
     assert lib.code("nnc_hip_rope", t(F16, 0, 300), None, None, None, t(F16, 0, 256), 0, 0, 4, 64, 0, 1e-6) == 0
 
 
-def rope_kv_write(lib, **change):  # noqa: F811
+def rope_kv_write(lib, **change):
     t = lib.t
     x = t(F16, 7, 512)
     good = {"q": x, "k": x, "v": x, "q_weight": t(F16, 64), "k_weight": t(F16, 64), "angles": t(F32, 50, 32), "positions": t(I32, 7),
@@ -58,7 +68,7 @@ def rope_kv_write(lib, **change):  # noqa: F811
     return {**good, **change}
 
 
-def test_rope_kv_write_refusals(lib):  # noqa: F811
+def test_rope_kv_write_refusals(lib):
     t = lib.t
     check(lib, "nnc_hip_rope_kv_write", rope_kv_write(lib), cache_changes(t) + [
         ("no keys", {"k": None}, EINVAL), ("no values", {"v": None}, EINVAL), ("integers", {"k": t(I8, 7, 512)}, EUNSUPP),
@@ -77,7 +87,7 @@ def test_rope_kv_write_refusals(lib):  # noqa: F811
         assert lib.code("nnc_hip_rope_kv_write", *rope_kv_write(lib, **change).values()) == ESTATE, change
 
 
-def test_kv_tree_attention_refusals(lib):  # noqa: F811
+def test_kv_tree_attention_refusals(lib):
     t = lib.t
     good = {"q": t(F32, 7, 300), **cache(lib), "tree": t(I32, 7, 2), "out": t(F32, 7, 256), "q_col": 44, "heads": 4, "scale": 0.125, "window": 0,
             "max_length": 0}
@@ -90,7 +100,7 @@ def test_kv_tree_attention_refusals(lib):  # noqa: F811
         ("flat tree", {"tree": t(I32, 14)}, EINVAL), ("int64 tree", {"tree": t(I64, 7, 1)}, EUNSUPP)])
 
 
-def test_token_logprobs_refusals(lib):  # noqa: F811
+def test_token_logprobs_refusals(lib):
     t = lib.t
     good = {"logits": t(F16, 2, 3, 1000), "tokens": t(I32, 6), "logprob": t(F32, 6), "entropy": t(F32, 2, 3), "top_index": t(I32, 2, 3, 5),
             "top_logprob": t(F32, 6, 5), "scale": 1.0}
