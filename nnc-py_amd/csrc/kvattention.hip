@@ -445,14 +445,6 @@ __global__ void __launch_bounds__(64 * NW, D == 32 ? 4 : 1) kv_attention_k(KvAtt
 // rows hit all 64 banks. Two stages: chunk t + 1 is widened and stored, and
 // the loads of t + 2 go out, before t is used, with one barrier for each.
 // ---------------------------------------------------------------------------
-typedef float fx16 __attribute__((ext_vector_type(16)));
-
-template <int RB>
-__device__ __forceinline__ int lds_chunk(int row, int chunk) {  // byte offset; rows of RB bytes
-    const int key = RB >= 256 ? row & 15 : RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
-    return row * RB + (chunk ^ key) * 16;
-}
-
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(64 * NW, D <= 128 || NW == 8 ? 2 : 1) kv_prompt_k(KvAttnArgs a) {
     constexpr bool F32 = sizeof(T) == 4;

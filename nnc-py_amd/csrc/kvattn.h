@@ -1,5 +1,5 @@
 // What the kernels that attend over the paged 8-bit cache share
-// (kvattention.hip, kvtree.hip): whole numbers as MFMA operands, and a softmax
+// (kvattention.hip, kvtree.hip, kvtree_rows.hip): whole numbers as MFMA operands, and a softmax
 // whose weights carry the scales of the values' pages. kvattention.hip has the
 // formulas.
 #pragma once
@@ -58,5 +58,15 @@ __device__ __forceinline__ float exponent(float m, float largest) { return floor
 __device__ __forceinline__ float rescale(float m, float e, float to_m, float to_e) { return __builtin_amdgcn_exp2f((m - to_m) + (to_e - e)); }
 // e before anything was seen
 static constexpr float kUnseen = 400.f - kPLog;
+
+typedef float fx16 __attribute__((ext_vector_type(16)));
+
+// Where a 16-byte chunk of a row of RB bytes is in LDS: permuted, so that 16 lanes
+// reading a chunk of 16 rows hit all 64 banks
+template <int RB>
+__device__ __forceinline__ int lds_chunk(int row, int chunk) {
+    const int key = RB >= 256 ? row & 15 : RB == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+    return row * RB + (chunk ^ key) * 16;
+}
 
 }  // namespace nnc

@@ -22,225 +22,11 @@
 // Few rows are bound by the cache's bytes: 32 sequences of 4 behind 4096, 32
 // heads over 8 of 128 in f16, 53 us, 5.1 TB/s, the rate of a copy. Many by the
 // vector units, which widen the keys and make masks, maxima and exponentials: 32
-// sequences of 16 behind up to 8192 77 us, 2.7 TB/s, one of 64 behind 65536 122
-// us, 560 TFLOP/s of 1170.
-#include <limits.h>
-
-#include "kvattn.h"
-#include "lanes.h"
+// sequences of 16 behind up to 8192 77 us, 2.7 TB/s, where a copy's rate leaves 41
+// (kvtree_rows.hip has the kernel for the longest lines of them).
+#include "kvtree.h"
 
 namespace nnc {
-
-struct TreeArgs {
-    Ragged g;
-    const int8_t *k, *v;
-    const float *k_scale, *v_scale;
-    const int* tree;  // [rows][words]
-    const void* q;
-    void* out;
-    float* part;    // [run][2][row of the tile][dim + 4]: sums, m, l, e
-    int* counters;  // [cached head][tile], zero
-    int64_t ld;
-    int64_t tiles;  // for each cached head, at most
-    int q_col, heads, kv_heads, group, window, words, least;
-    uint32_t slot_magic;
-    bool q_vec;   // query rows start on 16 bytes
-    float scale;  // with log2(e)
-};
-
-// The keys that rows of a sequence see, [lo, hi), and the tiles and units that
-// they make for each cached head.
-struct TreeSpan {
-    Span span;
-    int lo, tiles, units;
-    __device__ __forceinline__ void set(const TreeArgs& a, int tile, int stride) {
-        tiles = query_tiles(span, a.group, tile);
-        // a row's position is first - 1 at least
-        const int first = span.first();
-        lo = a.window > 0 && first > a.window ? (first - a.window) & ~63 : 0;
-        units = max(1, (span.length - lo + stride - 1) / stride);
-    }
-};
-
-// Unit u of one cached head's: its sequence and tile, its place among the tile's
-// units, and the tiles of the sequences before.
-struct TreePlace {
-    TreeSpan s;
-    int b, tile, unit;
-    int64_t tiles;
-};
-
-// The units of one cached head, found by 64 sequences at a time. The first 64
-// stay in registers, a sequence a lane.
-template <int TILE, int STRIDE>
-struct TreeIndex {
-    const TreeArgs& a;
-    TreeSpan mine;       // the lane's sequence
-    int tiles, upto_t;   // its tiles, with those of the lanes before
-    int64_t upto;        // units likewise
-    __device__ __forceinline__ void load(int base, int64_t tiles_before) {
-        const int lane = threadIdx.x & 63;
-        mine = TreeSpan{};
-        tiles = 0;
-        if (base + lane < a.g.batch) {
-            mine.span = span_of(a.g, base + lane);
-            mine.set(a, TILE, STRIDE);
-            tiles = mine.tiles;
-        }
-        // (starts that decrease would make more tiles than there are counters for)
-        upto_t = sum_before(tiles);
-        const int64_t room = a.tiles - tiles_before - (upto_t - tiles);
-        if (room < tiles) tiles = room > 0 ? (int)room : 0;
-        upto = (int64_t)sum_before((u64)tiles * (u64)mine.units);
-    }
-    __device__ __forceinline__ explicit TreeIndex(const TreeArgs& args) : a(args) { load(0, 0); }
-    __device__ __forceinline__ int64_t total() {
-        int64_t units = 0, before = 0;
-        for (int base = 0;;) {
-            units += last(upto), before += last(upto_t);
-            base += 64;
-            if (base >= a.g.batch || before >= a.tiles) break;
-            load(base, before);
-        }
-        if (a.g.batch > 64) load(0, 0);
-        return units;
-    }
-    __device__ __forceinline__ static int64_t last(int64_t x) {
-        return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, 63));
-    }
-    __device__ __forceinline__ static int last(int x) { return __builtin_amdgcn_readlane(x, 63); }
-    // u below total()
-    __device__ __forceinline__ TreePlace find(int64_t u) {
-        TreePlace p;
-        p.tiles = 0;
-        bool moved = false;
-        for (int base = 0;; base += 64, moved = true) {
-            if (base > 0) load(base, p.tiles);
-            const uint64_t past = __ballot(upto > u);
-            if (past || base + 64 >= a.g.batch) {
-                const int at = past ? __ffsll((unsigned long long)past) - 1 : 63;
-                auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
-                p.b = base + at;
-                p.s.span.end = of(mine.span.end), p.s.span.length = of(mine.span.length), p.s.span.rows = of(mine.span.rows);
-                p.s.lo = of(mine.lo), p.s.tiles = of(tiles), p.s.units = of(mine.units);
-                const int64_t whole = (int64_t)((uint64_t)(uint32_t)of((int)(upto >> 32)) << 32 | (uint32_t)of((int)upto));
-                u -= whole - (int64_t)p.s.tiles * p.s.units;
-                p.tiles += of(upto_t) - of(mine.tiles);
-                break;
-            }
-            u -= last(upto), p.tiles += last(upto_t);
-        }
-        if (moved) load(0, 0);
-        if (u < p.s.units) {
-            p.tile = 0, p.unit = (int)u;
-        } else {
-            p.tile = (int)(u / p.s.units), p.unit = (int)(u - (int64_t)p.tile * p.s.units);
-        }
-        return p;
-    }
-};
-
-// Items of so many units or fewer are left whole: a unit takes a workgroup less
-// than storing and joining two shares do.
-static constexpr int kShort = 4;
-
-// A run's share of an item: units [unit, unit + n) of a tile and cached head.
-struct TreeShare {
-    Span span;
-    int b, tile, head_kv, lo, unit, n;
-    bool whole;
-};
-
-template <int D, int R>
-struct TreePlaces {
-    static constexpr int ROW = D + 4;
-    __amdgpu_buffer_rsrc_t r;
-    __device__ __forceinline__ explicit TreePlaces(const TreeArgs& a) : r(make_rsrc(a.part)) {}
-    __device__ __forceinline__ uint32_t at(int place, int row, int col) const { return (uint32_t)((place * R + row) * ROW + col) * 4u; }
-    __device__ __forceinline__ void put4(int place, int row, int col, float x, float y, float z, float w) const {
-        typedef unsigned ux4 __attribute__((ext_vector_type(4)));
-        __builtin_amdgcn_raw_buffer_store_b128(ux4{__float_as_uint(x), __float_as_uint(y), __float_as_uint(z), __float_as_uint(w)}, r,
-                                               (int)at(place, row, col), 0, kDeviceScope);
-    }
-};
-
-// The shares of an item, joined by the workgroup that arrives last: kJoin of
-// them at a time, each row's maxima and divisors first, then 4 dims of a row a
-// thread. place(s) is where share s is; out(row) the row's output.
-static constexpr int kJoin = 32;
-template <typename T, int D, int R, int THREADS, class Place, class Out>
-__device__ __forceinline__ void join_shares(const TreePlaces<D, R>& from, int rows, int shares, Place place, Out out, float* lds) {
-    constexpr int QUADS = D / 4, PER = (R * QUADS + THREADS - 1) / THREADS, AHEAD = PER >= 8 ? 4 : 8;
-    static_assert(R <= THREADS && kJoin <= THREADS, "a thread each");
-    float (*ms)[R] = reinterpret_cast<float (*)[R]>(lds);             // [kJoin][R]
-    float (*ls)[R] = reinterpret_cast<float (*)[R]>(lds + kJoin * R), (*es)[R] = reinterpret_cast<float (*)[R]>(lds + 2 * kJoin * R);
-    float* scale = lds + 3 * kJoin * R;  // [R]
-    float* exps = scale + R;             // [R]
-    int* places = reinterpret_cast<int*>(exps + R);  // [kJoin]
-    const int tid = threadIdx.x;
-    auto row_of = [&](int q) { return min((tid + THREADS * q) / QUADS, R - 1); };
-    float top = kNone, e = kUnseen, sum = 0.f;  // of row tid
-    f32x4 o[PER];
-#pragma unroll
-    for (int q = 0; q < PER; ++q) o[q] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < shares; s0 += kJoin) {
-        const int n = min(kJoin, shares - s0);
-        __syncthreads();
-        if (tid < n) places[tid] = place(s0 + tid);
-        __syncthreads();
-        for (int k = tid; k < n * R; k += THREADS) {
-            const int sh = k / R, row = k % R;
-            const f32x4 x = load_partial4(from.r, from.at(places[sh], min(row, rows - 1), D));
-            ms[sh][row] = x[0], ls[sh][row] = x[1], es[sh][row] = x[2];
-        }
-        __syncthreads();
-        if (tid < R) {
-            float m = top, far = reference(top, e);
-            for (int sh = 0; sh < n; ++sh) m = fmaxf(m, ms[sh][tid]), far = fmaxf(far, reference(ms[sh][tid], es[sh][tid]));
-            const float en = exponent(m, far);
-            sum *= rescale(top, e, m, en);
-            for (int sh = 0; sh < n; ++sh) {
-                sum = fmaf(rescale(ms[sh][tid], es[sh][tid], m, en), ls[sh][tid], sum);
-                ms[sh][tid] = __builtin_amdgcn_exp2f(ms[sh][tid] - m);
-            }
-            scale[tid] = __builtin_amdgcn_exp2f(top - m);
-            top = m, e = en;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < PER; ++q) o[q] *= scale[row_of(q)];
-        for (int t = 0; t < n; t += AHEAD) {
-            f32x4 v[AHEAD][PER];
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-                for (int q = 0; q < PER; ++q)
-                    v[u][q] = load_partial4(from.r, from.at(places[min(t + u, n - 1)], min(row_of(q), rows - 1), (tid + THREADS * q) % QUADS * 4));
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-                for (int q = 0; q < PER; ++q) {
-                    const float w = t + u < n ? ms[min(t + u, n - 1)][row_of(q)] : 0.f;
-                    o[q] += v[u][q] * w;
-                }
-        }
-    }
-    __syncthreads();
-    if (tid < R) scale[tid] = sum == 0.f ? 0.f : 1.0f / sum, exps[tid] = e;
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < PER; ++q) {
-        const int row = row_of(q), d = (tid + THREADS * q) % QUADS * 4;
-        if (row >= rows || tid + THREADS * q >= R * QUADS) continue;
-        T v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float y = o[q][r];
-            v[r] = (T)ldexpf(y * scale[row], (int)exps[row]);
-        }
-        __builtin_memcpy(__builtin_assume_aligned(out(row) + d, 4 * sizeof(T)), v, sizeof v);
-    }
-}
 
 // NB blocks of 16 query rows of a tile of R against a share's keys: to the
 // output if the share is whole, else to its place.
@@ -557,57 +343,18 @@ template <typename T, int D, int RB, int NW, int OCC>
 __global__ void __launch_bounds__(64 * NW, OCC) kv_tree_k(TreeArgs a) {
     constexpr int STRIDE = 64 * NW, R = 16 * RB;
     extern __shared__ __align__(16) float tree_lds[];
-    TreeIndex<R, STRIDE> index(a);
-    const int64_t each = index.total(), total = each * a.kv_heads;
-    // runs of `least` units or more: two, or one where no item is cut
-    const int64_t useful = (total + a.least - 1) / a.least;
-    const int runs = __builtin_amdgcn_readfirstlane((int)(useful < gridDim.x ? useful : gridDim.x));
-    if ((int)blockIdx.x >= runs) return;
-    const int run = xcd_remap(blockIdx.x, runs);
-    auto find = [&](int64_t u, int& head_kv) {
-        head_kv = u < each ? 0 : (int)(u / each);
-        return index.find(u - head_kv * each);
-    };
-    // a short item is not cut, but its first run's
-    auto begin_of = [&](int r) {
-        const int64_t u = run_begin(r, total, runs);
-        int head_kv;
-        if (u == 0 || u == total) return u;
-        const TreePlace p = find(u, head_kv);
-        return p.s.units <= kShort ? u - p.unit : u;
-    };
-    const int64_t end = begin_of(run + 1);
-    for (int64_t at = begin_of(run); at < end;) {
-        TreeShare w;
-        const TreePlace p = find(at, w.head_kv);
-        const TreeSpan& s = p.s;
-        w.span = s.span, w.b = p.b, w.lo = s.lo, w.tile = p.tile, w.unit = p.unit;
-        w.n = (int)(end - at < s.units - w.unit ? end - at : s.units - w.unit);
-        w.whole = w.n == s.units;
-        const int64_t begin = at - w.unit;  // of the item
-        const int place = share_place(run, begin, total, runs);
-        const int64_t left = (int64_t)s.span.rows * a.group - (int64_t)w.tile * R;
-        if (RB > 1 && left > 16)
-            tree_share<T, D, R, RB, NW>(a, w, place, tree_lds);
-        else
-            tree_share<T, D, R, 1, NW>(a, w, place, tree_lds);
-        if (!w.whole) {
-            const int run0 = run_of(begin, total, runs), shares = run_of(begin + s.units - 1, total, runs) - run0 + 1;
-            if (finish_arrive(a.counters + (int64_t)w.head_kv * a.tiles + p.tiles + w.tile, shares - 1)) {
-                const TreePlaces<D, R> places(a);
-                join_shares<T, D, R, 64 * NW>(
-                    places, (int)min((int64_t)R, left), shares, [&](int sh) { return share_place(run0 + sh, begin, total, runs); },
-                    [&](int r) {
-                        const int64_t f = (int64_t)w.tile * R + r;
-                        const int t = (int)(f / a.group), head = w.head_kv * a.group + (int)(f - (int64_t)t * a.group);
-                        return (T*)a.out + ((int64_t)(s.span.end - s.span.rows + t) * a.heads + head) * D;
-                    },
-                    tree_lds);
-            }
-        }
-        at += w.n;
-        __syncthreads();  // the LDS is the next share's
-    }
+    walk_run<R, STRIDE, kShortKeys / STRIDE>(
+        a,
+        [&](const TreeShare& w, int place) {
+            if (RB > 1 && w.rows > 16)
+                tree_share<T, D, R, RB, NW>(a, w, place, tree_lds);
+            else
+                tree_share<T, D, R, 1, NW>(a, w, place, tree_lds);
+        },
+        [&](const TreeShare& w, int64_t tile, int shares, auto place) {
+            if (!finish_arrive(a.counters + w.head_kv * a.tiles + tile, shares - 1)) return;
+            join_shares<T, D, R, R, 64 * NW>(TreePlaces<D, R>(a), 0, w.rows, shares, place, [&](int r) { return tree_row<T, D, R>(a, w, r); }, tree_lds);
+        });
 }
 
 template <typename T, int D, int RB, int NW>
@@ -624,15 +371,11 @@ static void launch_blocks(const char* name, TreeArgs& a, int64_t rows) {
     if (!ok) return fail(NNC_HIP_EDEVICE, name, "hipFuncSetAttribute failed");
     // (whole items on 16 rows, two workgroups a CU: 64 trees of 4 behind up to 1024 30 -> 26 us, 256 of 2 behind up to
     // 500 87 -> 62)
-    const int runs = cu_count() * (OCC > 1 || (RB == 1 && D <= 128 && a.least == 1) ? 2 : 1);
-    a.tiles = query_tiles_bound(rows, a.g.batch, a.group, 16 * RB);
-    const int64_t items = a.tiles * a.kv_heads;
-    const size_t bytes = (size_t)runs * 2 * 16 * RB * (D + 4) * sizeof(float);
-    if (items > INT32_MAX) return fail(NNC_HIP_EUNSUPP, name, "%lld rows of %d heads", (long long)rows, a.heads);
-    a.part = workspace(bytes);
-    a.counters = tile_counters((size_t)items);
-    if (!a.part || !a.counters) return fail(NNC_HIP_ENOMEM, name, "no workspace for %zu bytes of partial sums", bytes);
-    launch(name, kernel, dim3((unsigned)runs), dim3(64 * NW), lds, a);
+    a.runs = cu_count() * (OCC > 1 || (RB == 1 && D <= 128 && a.least == 1) ? 2 : 1);
+    if (!tree_scratch(name, a, rows, 16 * RB, D)) return;
+    a.counters = tile_counters((size_t)(a.tiles * a.kv_heads));
+    if (!a.counters) return fail(NNC_HIP_ENOMEM, name, "no workspace for counters");
+    launch(name, kernel, dim3((unsigned)a.runs), dim3(64 * NW), lds, a);
 }
 
 // Query rows of a tile: 16 while a sequence has no more for a cached head; 32 with
@@ -644,8 +387,7 @@ static void launch_blocks(const char* name, TreeArgs& a, int64_t rows) {
 // 16 heads over 4, 16 rows and 32, us: 8 sequences of 16 behind 4096 40 and 44, of
 // 8 30 and 41, one of 64 behind 16384 61 and 60: 16 there.
 template <typename T, int D>
-static void launch_tree(const char* name, TreeArgs& a, int64_t rows) {
-    const int64_t holders = rows < a.g.batch ? rows : a.g.batch, each = ceil_div(rows * a.group, holders);
+static void launch_tree(const char* name, TreeArgs& a, int64_t rows, int64_t each) {
     if constexpr (D <= 128) {
         if (each > 32) return launch_blocks<T, D, 2, 4, 2>(name, a, rows);
         if (each > 16) return launch_blocks<T, D, 2, 4, 1>(name, a, rows);
@@ -688,18 +430,20 @@ void nnc_hip_kv_tree_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tens
     const int capacity = c.ragged.width * c.page;
     const int longest = max_length > 0 && max_length < capacity ? max_length : capacity;
     TreeArgs a{c.ragged, c.k, c.v, c.k_scale, c.v_scale, (const int*)tree->data, q->data, out->data, nullptr, nullptr, ld, 0, q_col, heads,
-               c.kv_heads, group, window_of(window, capacity), (int)tree->shape[1], longest <= 256 * kShort ? 1 : 2, slot_magic(c.page / 16),
+               c.kv_heads, group, window_of(window, capacity), (int)tree->shape[1], longest <= kShortKeys ? 1 : 2, 0, slot_magic(c.page / 16),
                aligned16(q->data) && ld * activation_bytes(q) % 16 == 0 && q_col * activation_bytes(q) % 16 == 0,
                scale * 1.44269504088896340736f};
     a.g.rows = (int)rows;
     const int64_t reach = a.window > 0 ? (int64_t)a.window - 1 + ceil_div(rows, c.ragged.batch) : longest;
     set_work(0.0, 2.0 * c.kv_heads * c.dim * (double)(reach < longest ? reach : longest) * c.ragged.batch);
     const bool f16 = q->dtype == NNC_DTYPE_FLOAT16;
+    const int64_t holders = rows < a.g.batch ? rows : a.g.batch, each = ceil_div(rows * a.group, holders);
+    if (launch_tree_rows(name, f16, c.dim, a, rows, each, longest)) return;
     switch (c.dim) {
-        case 32: return f16 ? launch_tree<half_t, 32>(name, a, rows) : launch_tree<float, 32>(name, a, rows);
-        case 64: return f16 ? launch_tree<half_t, 64>(name, a, rows) : launch_tree<float, 64>(name, a, rows);
-        case 128: return f16 ? launch_tree<half_t, 128>(name, a, rows) : launch_tree<float, 128>(name, a, rows);
-        default: return f16 ? launch_tree<half_t, 256>(name, a, rows) : launch_tree<float, 256>(name, a, rows);
+        case 32: return f16 ? launch_tree<half_t, 32>(name, a, rows, each) : launch_tree<float, 32>(name, a, rows, each);
+        case 64: return f16 ? launch_tree<half_t, 64>(name, a, rows, each) : launch_tree<float, 64>(name, a, rows, each);
+        case 128: return f16 ? launch_tree<half_t, 128>(name, a, rows, each) : launch_tree<float, 128>(name, a, rows, each);
+        default: return f16 ? launch_tree<half_t, 256>(name, a, rows, each) : launch_tree<float, 256>(name, a, rows, each);
     }
 }
 

@@ -472,6 +472,103 @@ def test_tree_attention_hidden_drafts_that_are_not_finite(dev):
     assert np.isfinite(got[:16]).all() and np.isnan(got[16:32]).all()
 
 
+# Many rows for a cached head behind contexts that are cut, some with few in
+# their last tile; tables that could hold more than the kernel for 256 rows asks
+# for
+MANY = [([1500, 1200, 4000, 3000, 2047, 40], [16, 1, 40, 0, 3, 9]), ([1500, 1200, 4000, 64, 2047, 70], [130, 64, 70, 65, 33, 5]),
+        ([1700, 1, 4000, 2048, 1025, 260], [300, 1, 64, 0, 2, 257])]
+
+
+def wide(batch, kv, page):
+    return 1 + 24 * 256 * 64 // (batch * kv * page)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("heads,kv,dim,page", [(8, 2, 128, 16), (4, 1, 64, 64), (16, 1, 32, 48), (6, 2, 128, 256)])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_tree_attention_many_rows_of_long_contexts(which, heads, kv, dim, page, t, dev):
+    rng = np.random.default_rng(dim + which)
+    lengths, rows = MANY[which]
+    run_tree(dev, rng, lengths, rows, heads, kv, dim, page, t, q_col=4 if which == 1 else 3, width=wide(6, kv, page))
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("rows", [9, 16, 17, 31, 32, 33, 63, 64, 65, 130])
+def test_tree_attention_many_rows_of_one_long_context(rows, t, dev):
+    rng = np.random.default_rng(rows)
+    run_tree(dev, rng, [9000 + rows], [rows], 4, 1, 128, 64, t, pad=0, width=wide(1, 1, 64))
+    run_tree(dev, rng, [1025], [rows], 8, 2, 64, 16, t, pad=3, width=wide(1, 2, 16), max_length=1030 if rows % 2 else 0)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("window", [1, 64, 700, 1500, 3999])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_tree_attention_many_rows_window(which, window, t, dev):
+    rng = np.random.default_rng(window + which)
+    run_tree(dev, rng, *MANY[which], 4, 1, 64, 32, t, window=window, garbage=False, width=wide(6, 1, 32))
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("batch,most", [(70, 30), (70, 200), (140, 160)])
+def test_tree_attention_many_rows_of_many_sequences(batch, most, t, dev):
+    rng = np.random.default_rng(batch)
+    lengths = [int(n) for n in rng.integers(0, 1800, batch)]
+    rows = [int(r) for r in rng.integers(0, most, batch)]
+    lengths[:4], rows[:4] = [2500, 0, 1, 300], [9, 0, 1, 200]
+    run_tree(dev, rng, lengths, rows, 4, 2, 32, 16, t, width=wide(batch, 2, 16) + 200)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("rows", [40, 100, 300])
+def test_tree_attention_many_rows_pages_of_different_size(rows, t, dev):
+    rng = np.random.default_rng(rows)
+    lengths, all_rows = [2700, 1300], [rows, 30]
+    width = wide(2, 1, 16)
+    run_tree(dev, rng, lengths, all_rows, 2, 1, 64, 16, t, garbage=False, spread=9 if t == F16 else 60, width=width)
+    run_tree(dev, rng, lengths, all_rows, 2, 1, 64, 16, t, sharp=200.0, width=width)
+    run_tree(dev, rng, lengths, all_rows, 2, 1, 64, 16, t, sharp=0.0, width=width)
+
+
+@pytest.mark.parametrize("t", [F32, F16])
+@pytest.mark.parametrize("rows", [[40, 20], [100, 90], [300, 90]])
+def test_tree_attention_many_rows_that_see_little(rows, t, dev):
+    """Masks of nothing, pages that cannot be read, drafts that are not finite
+    and that the others do not see, lengths and starts that cannot be."""
+    rng = np.random.default_rng(4)
+    lengths, kv, dim = [3000, 1290], 1, 64
+    starts, total = ragged(rows)
+    table, pages = tables(rng, lengths, 16, width=wide(2, kv, 16))
+    cache = s8.Cache(rng, pages, kv, 16, dim, table)
+    cache.table[0, 3], cache.table[0, 111], cache.table[1, :35] = -1, pages, [2 ** 31 - 1, -2 ** 31, pages + 5, -1, -7] * 7
+    lines = dr.trees(rng, rows)
+    lines[0][7] = []
+    tree = dr.masks(lines, -(-max(rows) // 32), total)
+    q = rng.standard_normal((total, 2 * dim)).astype(t)
+    d = dev({"q": q, **cache_arrays(cache, starts, lengths), "tree": tree, "out": np.full((total, 2 * dim), 7, t)})
+
+    def run():
+        d.call("nnc_hip_kv_tree_attention", "q", *CACHE, "starts", "lengths", "tree", "out", 0, 2, 0.125, 0, 0)
+        return d.get("out")
+    want = run()
+    dr.check_tree(want, q.reshape(total, 2, dim), cache, starts, lengths, tree, F32(0.125), 0)
+    d.set("table", np.full_like(cache.table, -1))
+    assert not run()[:starts[-1]].any()
+    for s, n in (([0, 20, 1000], [10 ** 9, -4]), ([0, -5, 7], [200, 90]), ([50, 20, 10], [3, 3000]), ([0, 10 ** 9, 5], [3000, 3000]), ([0, 30, 2 ** 31 - 1], [3000, 1290])):
+        d.set("starts", np.array(s, I32))
+        d.set("lengths", np.array(n, I32))
+        assert np.isfinite(run()).all()
+    # the last 8 drafts, those of the last page, are not finite, and the others do not see them
+    cache.table[0, 3], cache.table[0, 111] = table[0, 3], table[0, 111]
+    last = cache.page_of(0, 2999)
+    cache.ks[last], cache.vs[last] = np.nan, np.nan
+    d.set("starts", starts), d.set("lengths", np.array(lengths, I32)), d.set("table", cache.table)
+    d.set("k_scale", cache.ks), d.set("v_scale", cache.vs)
+    alone = [[[j for j in line if j < n - 9] if i < n - 9 else line for i, line in enumerate(own)] for own, n in zip(lines, rows)]
+    d.set("tree", dr.masks(alone, -(-max(rows) // 32), total))
+    got = run()
+    assert np.isfinite(got[:rows[0] - 9]).all() and np.isnan(got[rows[0] - 1]).all()
+
+
 # ---------------------------------------------------------------------------
 # log probabilities
 # ---------------------------------------------------------------------------
