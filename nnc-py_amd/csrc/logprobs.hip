@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(64 * NW) logprobs_k(LogprobArgs a) {
             }
         }
     }
-    if (a.segments > 1) {
+    if (NW > 1 && a.segments > 1) {  // (a wave has whole rows)
         const int slot = slot_floats(a.top);
         const __amdgpu_buffer_rsrc_t r = make_rsrc(a.part);
         auto put8 = [&](uint32_t at, u64 x) {
