@@ -411,13 +411,11 @@ __global__ void __launch_bounds__(64 * NW) logprobs_k(LogprobArgs a) {
                 const uint32_t at = (uint32_t)(line * a.segments + g) * slot + kSlotHead;
                 likeliest.merge(63 - lane < a.top ? get8(at + 2 * (63 - lane)) : 0, a.top);
             }
-            if (NW > 1) {
-                room[wave][63 - lane] = likeliest.list;
-                __syncthreads();
-                if (wave == 0)
+            room[wave][63 - lane] = likeliest.list;
+            __syncthreads();
+            if (wave == 0)
 #pragma unroll
-                    for (int w = 1; w < NW; ++w) likeliest.merge(room[w][lane], a.top);
-            }
+                for (int w = 1; w < NW; ++w) likeliest.merge(room[w][lane], a.top);
         }
     }
     if (wave == 0) {
