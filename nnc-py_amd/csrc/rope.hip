@@ -564,12 +564,16 @@ void nnc_hip_rope_kv_write(Tensor* q, Tensor* k, Tensor* v, Tensor* q_weight, Te
     } else if (q_weight || q_out) {
         return fail(NNC_HIP_EINVAL, name, "q_weight or q_out without q");
     }
-    if (rows == 0 || w.g.batch == 0 || w.g.width == 0) return;
+    if (rows == 0 || w.g.batch == 0 || (w.g.width == 0 && !q)) return;
     if (!ready(name)) return;
     const bool f16 = k->dtype == NNC_DTYPE_FLOAT16;
     const double n = (double)rows * activation_bytes(k);
     RopeKvArgs all{};
     all.w = w, all.q = qa, all.k = ka;
+    if (w.g.width == 0) {  // no pages to write to
+        set_work(8.0 * rows * heads * w.dim, 2.0 * n * heads * w.dim);
+        return launch_rope("nnc_hip_rope_kv_write_q", f16, qa);
+    }
     set_work(8.0 * rows * (q ? heads * w.dim : 0) + 20.0 * rows * kv_width, 2.0 * n * (q ? heads * w.dim : 0) + 2.0 * (n + rows) * kv_width);
     if (f16 ? launch_rope_kv<half_t>(name, all) : launch_rope_kv<float>(name, all)) return;
     // the rotated keys pass through scratch

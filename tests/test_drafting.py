@@ -310,6 +310,23 @@ def test_rope_kv_write_with_bad_tables_and_lengths(dev):
         d.get(n)  # nothing written outside
 
 
+def test_rope_kv_write_without_pages(dev):
+    """A table of no columns: nothing is cached, the queries are turned all the same."""
+    rng = np.random.default_rng(12)
+    starts, total = ragged([3, 4], 2)
+    cache = s8.Cache(rng, 2, 1, 16, 64, np.zeros((2, 0), I32))
+    x = rng.standard_normal((total, 4, 64)).astype(F16)
+    angles = turn_table(rng, 40, 64)
+    at = rng.integers(0, 40, total).astype(I32)
+    d = dev({"x": x.reshape(total, -1), **cache_arrays(cache, starts, [0, 0]), "angles": angles, "at": at, "q": np.full((total, 128), 7, F16)})
+    d.call("nnc_hip_rope_kv_write", "x", "x", "x", None, None, "angles", "at", "q", *CACHE, "starts", "lengths", 0, 2, 128, 192, 0, 0.0)
+    want, _ = dr.rope(x[:7, :2], None, angles, at[:7], False, 0.0)
+    got = d.get("q").reshape(total, 2, 64)
+    np.testing.assert_array_equal(got[:7], want.astype(F32).astype(F16))
+    assert (got[7:] == 7).all()
+    check_cache(d, cache)
+
+
 # ---------------------------------------------------------------------------
 # attention of drafts
 # ---------------------------------------------------------------------------
