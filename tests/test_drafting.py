@@ -862,3 +862,127 @@ def test_two_threads_and_the_second_stream(dev, hip):
     runtime.sync()
     same()
     assert runtime.last_error()[0] == 0
+
+
+def test_many_rows_captured_and_replayed(dev, hip):
+    """The kernel for 256 rows in a graph: lengths, trees and queries change
+    between the replays, an eager call of another shape uses the same scratch."""
+    from nnc_py_amd import runtime
+    rng = np.random.default_rng(21)
+    heads, kv, dim, page, rows = 8, 2, 64, 32, [90, 70]
+    starts, total = ragged(rows)
+    table, pages = tables(rng, [2600, 2000], page, width=wide(2, kv, page))
+    cache = s8.Cache(rng, pages, kv, page, dim, table)
+    d = dev({"q": np.zeros((total, heads * dim), F16), **cache_arrays(cache, starts, [0, 0]), "tree": np.zeros((total, 3), I32),
+             "out": np.zeros((total, heads * dim), F16), "other": np.zeros((total, heads * dim), F16)})
+    T = lambda *names: [d.t(n) for n in names]  # noqa: E731
+
+    def call(out, longest=0):
+        hip.nnc_hip_kv_tree_attention(*T("q", *CACHE, "starts", "lengths", "tree", out), 0, heads, 0.125, 0, longest)
+    call("out")
+    runtime.sync()
+    runtime.check(hip.nnc_hip_graph_begin(), "begin")
+    call("out")
+    runtime.check(hip.nnc_hip_graph_end(), "end")
+    for lengths in ([2600, 2000], [90, 1999], [0, 71], [1500, 1300], [1500, 1300]):
+        q = rng.standard_normal((total, heads * dim)).astype(F16)
+        tree = dr.masks(dr.trees(rng, rows), 3, total)
+        for name, a in (("q", q), ("tree", tree), ("lengths", np.array(lengths, I32))):
+            d.set(name, a)
+        call("other", 2600)  # by the other kernel
+        runtime.check(hip.nnc_hip_graph_launch(), "launch")
+        runtime.sync()
+        got, other = d.get("out"), d.get("other")
+        for x in got, other:
+            dr.check_tree(x, q.reshape(total, heads, dim), cache, starts, lengths, tree, F32(0.125), 0)
+        call("out")
+        runtime.sync()
+        np.testing.assert_array_equal(d.get("out"), got)
+    hip.nnc_hip_graph_destroy()
+
+
+@pytest.mark.parametrize("dim", [64, 18])
+def test_rope_behind_four_gib(dim, hip, dev):
+    """Rows at the far end of a matrix of more than 4 GiB, in place."""
+    from nnc_py_amd import runtime
+    rows, ld, heads, col = 1100000, 2048, 2, 1800
+    assert rows * ld * 2 > 2 ** 32
+    rng = np.random.default_rng(dim)
+    big = runtime.DeviceBuffer.empty((rows, ld), F16)
+    try:
+        some = [0, 5, rows // 2, rows - 2, rows - 1]
+        x = rng.standard_normal((len(some), ld)).astype(F16)
+        for i, r in enumerate(some):
+            runtime.check(hip.nnc_hip_memcpy_h2d(big.ptr + r * ld * 2, np.ascontiguousarray(x[i]).ctypes.data, ld * 2), "upload")
+        at = rng.integers(0, 99, rows).astype(I32)
+        angles = turn_table(rng, 99, dim)
+        d = dev({"at": at, "angles": angles})
+        d.desc["x"], shape = big.tensor()
+        d.kept.append(shape)
+        d.call("nnc_hip_rope", "x", None, "angles", "at", "x", col, col, heads, dim, 1, 0.0)
+        want = x.copy()
+        y, _ = dr.rope(x[:, col:col + heads * dim].reshape(-1, heads, dim), None, angles, at[some], True, 0.0)
+        want[:, col:col + heads * dim] = y.astype(F32).astype(F16).reshape(len(some), -1)
+        for i, r in enumerate(some):
+            got = np.empty(ld, F16)
+            runtime.check(hip.nnc_hip_memcpy_d2h(got.ctypes.data, big.ptr + r * ld * 2, ld * 2), "download")
+            np.testing.assert_array_equal(got, want[i])
+    finally:
+        big.free()
+
+
+def test_cache_behind_four_gib(hip, dev):
+    """Pages at the far end of caches of more than 4 GiB each: written, and
+    attended by few rows and by many."""
+    from nnc_py_amd import runtime
+    rng = np.random.default_rng(5)
+    page, kv, dim, heads, pages = 128, 4, 128, 8, 70000
+    assert pages * kv * page * dim > 2 ** 32
+    lengths, rows = [300, 700], [40, 150]
+    starts, total = ragged(rows)
+    table, held = tables(rng, lengths, page)
+    cache = s8.Cache(rng, held, kv, page, dim, table)
+    far = pages - held
+    scales = np.zeros((2, pages, kv), F32)
+    scales[0, far:], scales[1, far:] = cache.ks, cache.vs
+    big = [runtime.DeviceBuffer.empty((pages, kv, page, dim), np.int8), runtime.DeviceBuffer.empty((pages, kv, dim, page), np.int8)]
+    try:
+        bytes_of = page * kv * dim
+        for buf, a in zip(big, (cache.k, cache.v)):
+            runtime.check(hip.nnc_hip_memcpy_h2d(buf.ptr + far * bytes_of, np.ascontiguousarray(a).ctypes.data, a.nbytes), "upload")
+        x = rng.standard_normal((total, heads + 2 * kv, dim)).astype(F16)
+        angles = turn_table(rng, 900, dim)
+        tree = dr.masks(dr.trees(rng, rows), 5, total)
+        wide_table = np.full((2, wide(2, kv, page)), -1, I32)
+        wide_table[:, :table.shape[1]] = np.where(table < held, table + far, -1)
+        d = dev({"x": x.reshape(total, -1), "k_scale": scales[0], "v_scale": scales[1], "table": wide_table, "starts": starts, "lengths": np.array(lengths, I32),
+                 "angles": angles, "q": np.zeros((total, heads * dim), F16), "tree": tree, "out": np.zeros((total, heads * dim), F16)})
+        for name, buf in zip(("k_cache", "v_cache"), big):
+            d.desc[name], shape = buf.tensor()
+            d.kept.append(shape)
+        d.call("nnc_hip_rope_kv_write", "x", "x", "x", None, None, "angles", None, "q", *CACHE, "starts", "lengths", 0, heads, heads * dim, (heads + kv) * dim, 0, 0.0)
+        place = np.concatenate([np.arange(n - r, n) for n, r in zip(lengths, rows)])
+        own = slice(starts[0], starts[-1])
+        k, _ = dr.rope(x[own, heads:heads + kv], None, angles, place, False, 0.0)
+        keys = np.zeros((total, kv, dim), F16)
+        keys[own] = k.astype(F32).astype(F16)
+        cache.write(keys, x[:, heads + kv:], starts, lengths)
+        for buf, a in zip(big, (cache.k, cache.v)):
+            got = np.empty_like(a)
+            runtime.check(hip.nnc_hip_memcpy_d2h(got.ctypes.data, buf.ptr + far * bytes_of, a.nbytes), "download")
+            np.testing.assert_array_equal(got, a)
+        np.testing.assert_array_equal(d.get("k_scale")[far:], cache.ks)
+        q = d.get("q").reshape(total, heads, dim)
+        for longest in (0, 700):  # by the kernel for 256 rows, and by the other
+            d.call("nnc_hip_kv_tree_attention", "q", *CACHE, "starts", "lengths", "tree", "out", 0, heads, 0.09, 0, longest)
+            dr.check_tree(d.get("out"), q, cache, starts, lengths, tree, F32(0.09), 0)
+    finally:
+        for buf in big:
+            buf.free()
+
+
+def test_token_logprobs_of_many_rows_and_of_one_long(dev):
+    """More rows than one launch takes; a row of several hundred segments."""
+    rng = np.random.default_rng(8)
+    run_logprobs(dev, rng.standard_normal(((1 << 22) + 3, 3)).astype(F16), top=1, rng=rng)
+    run_logprobs(dev, logits(rng, 1, 3000017, F32), top=64, rng=rng)
