@@ -108,12 +108,24 @@ __device__ __forceinline__ void add_sums(RowSums& s, RowSums t, float c) {
     s.rest += t.rest, s.ones += t.ones, s.weighted += t.weighted;
 }
 
-// Takes the values that are the maximum out of a lane's packs; how many.
+// A pack's largest value
+template <typename T>
+__device__ __forceinline__ float largest_of(nt_u32x4 pack) {
+    uint32_t most = pack[0];
+#pragma unroll
+    for (int u = 1; u < 4; ++u) most = Words<T>::max_of(most, pack[u]);
+    const nt_u32x4 both = {most, most, most, most};
+    return sizeof(T) == 4 ? Words<T>::at(both, 0) : fmaxf(Words<T>::at(both, 0), Words<T>::at(both, 1));
+}
+
+// Takes the values that are the maximum out of a lane's packs; how many. (Few of
+// a wave's packs have one: the others are passed over together.)
 template <typename T, int PACKS>
 __device__ __forceinline__ float take_out(nt_u32x4 (&raw)[PACKS], float m) {
     float ones = 0.f;
 #pragma unroll
-    for (int p = 0; p < PACKS; ++p)
+    for (int p = 0; p < PACKS; ++p) {
+        if (!__any(largest_of<T>(raw[p]) == m)) continue;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const uint32_t w = raw[p][u];
@@ -129,6 +141,7 @@ __device__ __forceinline__ float take_out(nt_u32x4 (&raw)[PACKS], float m) {
             }
             asm volatile("" : "+v"(ones));  // (one after the other: the comparisons of all of them are more than the registers hold)
         }
+    }
     return ones;
 }
 
@@ -282,11 +295,7 @@ __global__ void __launch_bounds__(64 * NW) logprobs_k(LogprobArgs a) {
         uint32_t reach = 0;  // packs that reach the bar
 #pragma unroll
         for (int p = 0; p < PACKS; ++p) {
-            uint32_t most = raw[p][0];
-#pragma unroll
-            for (int u = 1; u < 4; ++u) most = Words<T>::max_of(most, raw[p][u]);
-            const nt_u32x4 both = {most, most, most, most};
-            const bool hit = V == 4 ? Words<T>::at(both, 0) >= bar : fmaxf(Words<T>::at(both, 0), Words<T>::at(both, 1)) >= bar;
+            const bool hit = largest_of<T>(raw[p]) >= bar;
             reach |= hit ? 1u << p : 0u;
         }
         auto pack_of = [&](int which) {
