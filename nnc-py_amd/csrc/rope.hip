@@ -185,10 +185,12 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& a, RopeWaves shape, u
             }
         }
     };
-    load(head);
+    const bool all_rows = a.g.batch == 0;  // else a row may be no sequence's, and those are not read
+    if (all_rows) load(head);
     if (NORM && !a.weight_each && mine) wp = *(const nt_u32x4*)((const T*)a.weight + one), wq = *(const nt_u32x4*)((const T*)a.weight + other);
     const int64_t place = rope_place(a, row);
     if (place < 0) return;
+    if (!all_rows) load(head);
     float cs[V], sn[V];
     if (turned) angles_of<V>(a, place, unit, cs, sn);
     for (; head - (lane >> bits) < end; head += groups) {
