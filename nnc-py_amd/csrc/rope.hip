@@ -13,6 +13,8 @@
 #include "kvcache.h"
 #include "lanes.h"
 
+#include "heads.h"
+
 namespace nnc {
 
 struct RopeArgs {
@@ -155,26 +157,23 @@ __device__ __forceinline__ double over_head(double sum, int bits) {
 // heads of a row for each of them with the row's angles in registers, the next
 // head's values on their way. Bound by the bytes: [16384, 32 + 8 heads of 128] f16
 // 67 us for its 336 MB, a copy's 5.0 TB/s; a decoding step's [16, 40 x 128] is a
-// launch, 3.6 us. The pairing is the kernel's, not a register's: the
+// launch, 3.1 us. The pairing is the kernel's, not a register's: the
 // selection of partners takes a fourth of the instructions otherwise (72 us).
-struct RopeWaves {
-    int bits, per, chunks;  // chunks of heads for each row
-};
 template <typename T, bool NORM, bool INTER>
 __device__ __forceinline__ void rope_heads(const RopeArgs& a, RopeWaves shape, uint32_t item) {
     typedef Words<T> W;
     constexpr int V = W::V;
-    const int bits = shape.bits, per = shape.per;
-    const int lane = threadIdx.x & 63, unit = lane & ((1 << bits) - 1), groups = 64 >> bits, half = a.rot / 2;
+    const int bits = shape.bits;
+    const int lane = threadIdx.x & 63, unit = lane & ((1 << bits) - 1), groups = shape.groups(), half = a.rot / 2;
     const uint32_t row = item / (uint32_t)shape.chunks, chunk = item - row * (uint32_t)shape.chunks;
     if (row >= a.rows) return;
     const bool turned = 2 * V * unit < a.rot, mine = 2 * V * unit < a.dim;
     const int one = turned && !INTER ? V * unit : 2 * V * unit;
     const int other = turned && !INTER ? one + half : one + V;
-    int head = chunk * per * groups + (lane >> bits);
     const T* x = (const T*)a.in + row * a.in_ld + a.col;
     T* y = (T*)a.out + row * a.out_ld + a.out_col;
-    const int end = min(head + per * groups, a.heads);
+    int head = shape.begin(chunk) + (lane >> bits);
+    const int end = shape.end(chunk, a.heads);
     nt_u32x4 p{}, q{}, wp{}, wq{};
     auto load = [&](int h) {
         if (mine && h < end) {
@@ -193,7 +192,7 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& a, RopeWaves shape, u
     if (!all_rows) load(head);
     float cs[V], sn[V];
     if (turned) angles_of<V>(a, place, unit, cs, sn);
-    for (; head - (lane >> bits) < end; head += groups) {
+    for (int first = shape.begin(chunk); first < end; first += groups, head += groups) {
         const nt_u32x4 xp = p, xq = q, vp = wp, vq = wq;
         const bool live = mine && head < end;
         const int h = head;
@@ -230,22 +229,11 @@ static bool in_packs(const RopeArgs& a) {
            aligned16(a.weight) && a.in_ld % V == 0 && a.out_ld % V == 0 && a.col % V == 0 && a.out_col % V == 0;
 }
 
-// A wave takes all of a row's heads, 64 >> bits at once, while rows are many
-static RopeWaves rope_waves(const RopeArgs& a, int v) {
-    RopeWaves s{};
-    while ((2 * v << s.bits) < a.dim) ++s.bits;
-    const int passes = (int)ceil_div(a.heads, 64 >> s.bits);
-    s.per = passes;
-    while (s.per > 1 && a.rows * ceil_div(passes, s.per) < 16 * (int64_t)cu_count()) s.per = (s.per + 1) / 2;
-    s.chunks = (int)ceil_div(passes, s.per);
-    return s;
-}
-
 template <typename T>
 static void launch_rope_type(const char* name, const RopeArgs& a) {
     if (in_packs<T>(a)) {
         constexpr int V = 16 / (int)sizeof(T);
-        const RopeWaves shape = rope_waves(a, V);
+        const RopeWaves shape = rope_waves(a.rows, a.heads, a.dim, V, cu_count());
         const int64_t blocks = ceil_div(a.rows * shape.chunks, 4);
         if (blocks * 256 <= UINT32_MAX) {
             const dim3 grid((unsigned)blocks);
@@ -432,7 +420,7 @@ static bool launch_rope_kv(const char* name, RopeKvArgs& a) {
     RopeArgs k = a.k;
     k.out = a.w.k, k.out_ld = 0, k.out_col = 0;  // (the cache is aligned)
     if (!quads<T>(a.w) || !in_packs<T>(k) || (a.q.in && !in_packs<T>(a.q))) return false;
-    if (a.q.in) a.shape = rope_waves(a.q, V);
+    if (a.q.in) a.shape = rope_waves(a.q.rows, a.q.heads, a.q.dim, V, cu_count());
     const int n = a.w.g.page * a.w.dim * (int)sizeof(T) / 64;
     if (n <= 64) return launch_rope_quads<T, 64, 1>(name, a);
     if (n <= 256) return launch_rope_quads<T, 256, 1>(name, a);
