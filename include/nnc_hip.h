@@ -449,7 +449,7 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
  * window, p = the first row's position + the row's set bits - 1, which is its
  * position if its mask names the drafts that lead to it and itself. Drafts that
  * a mask names are seen whatever the window. Everything else as for
- * nnc_hip_kv_attention.
+ * nnc_hip_kv_attention; window and rows, too, decide how the work is divided.
  *
  * nnc_hip_token_logprobs: of rows of logits [rows][vocab], p = softmax(scale *
  * logits): logprob float32 [rows] = log p[tokens[row]] (tokens int32 [rows]);

@@ -35,9 +35,7 @@ struct TreeSpan {
     int lo, tiles, units;
     __device__ __forceinline__ void set(const TreeArgs& a, int tile, int stride) {
         tiles = query_tiles(span, a.group, tile);
-        // a row's position is first - 1 at least
-        const int first = span.first();
-        lo = a.window > 0 && first > a.window ? (first - a.window) & ~63 : 0;
+        lo = tree_low(span.first(), a.window);
         units = max(1, (span.length - lo + stride - 1) / stride);
     }
 };
@@ -313,7 +311,7 @@ inline bool tree_scratch(const char* name, TreeArgs& a, int64_t rows, int tile, 
 }
 
 // Many rows of long contexts (kvtree_rows.hip): false if its kernels are not for
-// these
-bool launch_tree_rows(const char* name, bool f16, int dim, const TreeArgs& a, int64_t rows, int64_t each, int64_t longest);
+// these; reach: the keys of a sequence, at most
+bool launch_tree_rows(const char* name, bool f16, int dim, const TreeArgs& a, int64_t rows, int64_t each, int64_t reach);
 
 }  // namespace nnc

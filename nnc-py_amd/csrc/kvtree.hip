@@ -428,17 +428,18 @@ void nnc_hip_kv_tree_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tens
         return fail(NNC_HIP_EUNSUPP, name, "%lld rows of %d heads", (long long)rows, heads);
     if (!ready(name)) return;
     const int capacity = c.ragged.width * c.page;
-    const int longest = max_length > 0 && max_length < capacity ? max_length : capacity;
+    const int longest = max_length > 0 && max_length < capacity ? max_length : capacity, seen = window_of(window, capacity);
+    const int64_t holders = rows < c.ragged.batch ? rows : c.ragged.batch, each = ceil_div(rows * group, holders);
+    const int64_t reach = tree_reach(seen, ceil_div(rows, holders), longest);
     TreeArgs a{c.ragged, c.k, c.v, c.k_scale, c.v_scale, (const int*)tree->data, q->data, out->data, nullptr, nullptr, ld, 0, q_col, heads,
-               c.kv_heads, group, window_of(window, capacity), (int)tree->shape[1], longest <= kShortKeys ? 1 : 2, 0, slot_magic(c.page / 16),
+               c.kv_heads, group, seen, (int)tree->shape[1], reach <= kShortKeys ? 1 : 2, 0, slot_magic(c.page / 16),
                aligned16(q->data) && ld * activation_bytes(q) % 16 == 0 && q_col * activation_bytes(q) % 16 == 0,
                scale * 1.44269504088896340736f};
     a.g.rows = (int)rows;
-    const int64_t reach = a.window > 0 ? (int64_t)a.window - 1 + ceil_div(rows, c.ragged.batch) : longest;
-    set_work(0.0, 2.0 * c.kv_heads * c.dim * (double)(reach < longest ? reach : longest) * c.ragged.batch);
+    const int64_t once = seen > 0 ? (int64_t)seen - 1 + ceil_div(rows, holders) : longest;  // the keys of a sequence that a row sees
+    set_work(0.0, 2.0 * c.kv_heads * c.dim * (double)(once < longest ? once : longest) * c.ragged.batch);
     const bool f16 = q->dtype == NNC_DTYPE_FLOAT16;
-    const int64_t holders = rows < a.g.batch ? rows : a.g.batch, each = ceil_div(rows * a.group, holders);
-    if (launch_tree_rows(name, f16, c.dim, a, rows, each, longest)) return;
+    if (launch_tree_rows(name, f16, c.dim, a, rows, each, reach)) return;
     switch (c.dim) {
         case 32: return f16 ? launch_tree<half_t, 32>(name, a, rows, each) : launch_tree<float, 32>(name, a, rows, each);
         case 64: return f16 ? launch_tree<half_t, 64>(name, a, rows, each) : launch_tree<float, 64>(name, a, rows, each);

@@ -333,16 +333,18 @@ static void launch_rows(const char* name, TreeArgs a, int64_t rows) {
 }
 
 // For more than 128 rows of f16 behind so many keys that a CU has 24 times 64 of
-// a tile, were all sequences the longest. us, 32 heads over 8 of 128, this and
-// 32 rows a wave: 16 sequences behind 4096 of 36 drafts 98 and 119, of 64 115 and 128,
-// of 128 180 and 248; with 16 times 64 keys 8 of 64 behind 4096 71 and 63, with 8 4
-// of 64 50 and 44. Tiles of 128 rows in two workgroups a CU: 18 drafts 69 and 84, but 32 82 and
-// 70; of 64 rows, two waves to a row's keys: 16 behind up to 8192 96 and 77. fp32
-// of 64 162 and 169, of 40 139 and 135 (dim 256 has no registers for it).
-bool launch_tree_rows(const char* name, bool f16, int dim, const TreeArgs& a, int64_t rows, int64_t each, int64_t longest) {
+// a tile, were all sequences the longest, or as long as a window leaves them. us,
+// 32 heads over 8 of 128, this and 32 rows a wave: 16 sequences behind 4096 of 36
+// drafts 98 and 119, of 64 115 and 128, of 128 180 and 248; with 16 times 64 keys 8
+// of 64 behind 4096 71 and 63, with 8 4 of 64 50 and 44; 2 of 100 behind 16384 under
+// a window of 4096 51 and 52, of 1024 44 and 32, of 100 24 and 13. Tiles of 128 rows
+// in two workgroups a CU: 18 drafts 69 and 84, but 32 82 and 70; of 64 rows, two
+// waves to a row's keys: 16 behind up to 8192 96 and 77. fp32 of 64 162 and 169, of
+// 40 139 and 135 (dim 256 has no registers for it).
+bool launch_tree_rows(const char* name, bool f16, int dim, const TreeArgs& a, int64_t rows, int64_t each, int64_t reach) {
     if (!f16 || dim > 128 || each <= kRows / 2) return false;
     const int64_t holders = rows < a.g.batch ? rows : a.g.batch;
-    if (ceil_div(each, kRows) * holders * a.kv_heads * ceil_div(longest, 64) < 24 * (int64_t)cu_count()) return false;
+    if (ceil_div(each, kRows) * holders * a.kv_heads * ceil_div(reach, 64) < 24 * (int64_t)cu_count()) return false;
     // (the join's grid: whole tiles for each sequence)
     if ((rows * a.group + kRows * holders) / kJoinRows * a.kv_heads * 256 > UINT32_MAX) return false;
     switch (dim) {

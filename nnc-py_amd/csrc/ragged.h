@@ -133,6 +133,15 @@ RAGGED_HD int tree_depth(const int* mask, int words, int rows) {
     return n;
 }
 
+// The first key, a multiple of 64, that drafts from position `first` on go
+// through: a row's position is first - 1 at least. And how many keys a sequence of
+// `rows` drafts has from there on, at most, if it is no longer than `longest`.
+RAGGED_HD int tree_low(int first, int window) { return window > 0 && first > window ? (first - window) & ~63 : 0; }
+RAGGED_HD int64_t tree_reach(int window, int64_t rows, int64_t longest) {
+    const int64_t some = (int64_t)window + rows + 63;
+    return window > 0 && some < longest ? some : longest;
+}
+
 // `total` units of work, one after the other, in `parts` runs of equal length:
 // run p has [run_begin(p), run_begin(p + 1)), and unit i is in run_of(i). An
 // item, a range of units, that several runs have a share of is put together
