@@ -448,7 +448,9 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
  * sequence's first row; with window > 0 those of them that are later than p -
  * window, p = the first row's position + the row's set bits - 1, which is its
  * position if its mask names the drafts that lead to it and itself. Drafts that
- * a mask names are seen whatever the window. Everything else as for
+ * a mask names are seen whatever the window; a mask of the last `window` drafts
+ * that lead to a row gives it what nnc_hip_kv_attention gives to a run of tokens,
+ * and no context where they are that many. Everything else as for
  * nnc_hip_kv_attention; window and rows, too, decide how the work is divided.
  *
  * nnc_hip_token_logprobs: of rows of logits [rows][vocab], p = softmax(scale *
