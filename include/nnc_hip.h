@@ -461,7 +461,11 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
  * logprob). Logits of -infinity have probability 0; a row whose largest is not
  * finite (a NaN or +infinity in it, or nothing but -infinity) has NaN for
  * results and -1 for tokens. A token outside [0, vocab): NaN. Where there are
- * fewer than n tokens: -1, -infinity. Sums are float64. */
+ * fewer than n tokens: -1, -infinity. Terms are float32's; up to 16 of them are
+ * summed in float32, these sums in float64, and the largest is counted: a log
+ * probability is off by less than 2^-21 + 2^-22 D before it is rounded to float32,
+ * or 2^-18 + 2^-22 D where several workgroups have a row (of up to ten million
+ * logits), D being the mean, by p, of scale times the distance to the largest. */
 void nnc_hip_rope(Tensor* in, Tensor* weight, Tensor* angles, Tensor* positions, Tensor* out, int col, int out_col,
                   int heads, int dim, int interleaved, float eps);
 void nnc_hip_rope_kv_write(Tensor* q, Tensor* k, Tensor* v, Tensor* q_weight, Tensor* k_weight, Tensor* angles,

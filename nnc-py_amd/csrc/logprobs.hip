@@ -15,9 +15,9 @@
 // maxima, and the least of the waves' (n / waves)-th largest; the highest of these
 // bars is what few more than n reach. Those gather in LDS, are sorted, 64 to a
 // wave, as whole numbers that compare as (value, earlier index) do, and merged.
-// If more than 256 reach it (equal values, rows of -infinity), each wave keeps a
-// list of its best 64, one a lane, and merges 64 at a time into it. The last
-// segment to arrive joins a row's segments.
+// If more than 256 reach it, or 64 where a wave has whole rows (equal values, rows
+// of -infinity), each wave keeps a list of its best 64, one a lane, and merges 64 at
+// a time into it. The last segment to arrive joins a row's segments.
 #include "lanes.h"
 #include "mfma_tile.h"
 
