@@ -178,7 +178,7 @@ struct TreePlaces {
 static constexpr int kJoin = 32;
 template <typename T, int D, int TILE, int R, int THREADS, class Place, class Out>
 __device__ __forceinline__ void join_shares(const TreePlaces<D, TILE>& from, int row0, int rows, int shares, Place place, Out out, float* lds) {
-    constexpr int QUADS = D / 4, PER = (R * QUADS + THREADS - 1) / THREADS, AHEAD = PER >= 8 ? 4 : 8;
+    constexpr int QUADS = D / 4, PER = (R * QUADS + THREADS - 1) / THREADS, AHEAD = 8;
     static_assert(R <= THREADS && kJoin <= THREADS, "a thread each");
     float (*ms)[R] = reinterpret_cast<float (*)[R]>(lds);             // [kJoin][R]
     float (*ls)[R] = reinterpret_cast<float (*)[R]>(lds + kJoin * R), (*es)[R] = reinterpret_cast<float (*)[R]>(lds + 2 * kJoin * R);

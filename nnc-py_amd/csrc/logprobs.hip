@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(64 * NW) logprobs_k(LogprobArgs a) {
     }
 }
 
-template <typename T, int NW, int PACKS>
+template <typename T, int NW, int PACKS, bool TOP>
 static void launch_packs(const char* name, LogprobArgs a, int64_t packs) {
     a.segments = (int)ceil_div(packs, NW * 64 * PACKS);
     a.each = (int)ceil_div(packs, a.segments);
@@ -465,10 +465,7 @@ static void launch_packs(const char* name, LogprobArgs a, int64_t packs) {
         const dim3 grid((unsigned)(a.rows * a.segments));
         const double n = (double)a.rows * (double)a.vocab;
         set_work(6.0 * n, n * sizeof(T) + 8.0 * (double)a.rows * (1 + a.top));
-        if (a.top > 0)
-            launch(name, logprobs_k<T, NW, PACKS, true>, grid, dim3(64 * NW), 0, a);
-        else
-            launch(name, logprobs_k<T, NW, PACKS, false>, grid, dim3(64 * NW), 0, a);
+        launch(name, logprobs_k<T, NW, PACKS, TOP>, grid, dim3(64 * NW), 0, a);
     }
 }
 
@@ -481,14 +478,13 @@ static void launch_packs(const char* name, LogprobArgs a, int64_t packs) {
 // sorting of candidates, and loads and sums of a CU's workgroups overlap only in
 // part. 8 rows of 32000 in fp32 take 9.7 us with 5 tokens, 6.0 without: load, bar,
 // candidates, sort, join are one chain.
-template <typename T>
+template <typename T, bool TOP>
 static void launch_logprobs(const char* name, const LogprobArgs& a) {
     const int64_t packs = a.vocab * (int64_t)sizeof(T) / 16 + 2;
-    if (packs <= 256) return launch_packs<T, 1, 4>(name, a, packs);
-    if (packs <= 512 && a.rows >= cu_count()) return launch_packs<T, 1, 8>(name, a, packs);
-    if (ceil_div(packs, 1024) * a.rows <= 4 * (int64_t)cu_count()) return launch_packs<T, 4, 4>(name, a, packs);
-    if (a.top == 0) return launch_packs<T, 4, 8>(name, a, packs);
-    launch_packs<T, 4, 16>(name, a, packs);
+    if (packs <= 256) return launch_packs<T, 1, 4, TOP>(name, a, packs);
+    if (packs <= 512 && a.rows >= cu_count()) return launch_packs<T, 1, 8, TOP>(name, a, packs);
+    if (ceil_div(packs, 1024) * a.rows <= 4 * (int64_t)cu_count()) return launch_packs<T, 4, 4, TOP>(name, a, packs);
+    launch_packs<T, 4, TOP ? 16 : 8, TOP>(name, a, packs);
 }
 
 static bool row_output(const char* name, const char* what, Tensor* t, int dtype, int64_t n) {
@@ -533,9 +529,9 @@ void nnc_hip_token_logprobs(Tensor* logits, Tensor* tokens, Tensor* logprob, Ten
     if (entropy) a.entropy = (float*)entropy->data;
     if (top_index) a.top_index = (int*)top_index->data, a.top_logprob = (float*)top_logprob->data;
     if (logits->dtype == NNC_DTYPE_FLOAT16)
-        launch_logprobs<half_t>(name, a);
+        a.top ? launch_logprobs<half_t, true>(name, a) : launch_logprobs<half_t, false>(name, a);
     else
-        launch_logprobs<float>(name, a);
+        a.top ? launch_logprobs<float, true>(name, a) : launch_logprobs<float, false>(name, a);
 }
 
 }  // extern "C"

@@ -3,6 +3,8 @@ bounds for rows that one workgroup has and for rows that several share."""
 
 from __future__ import annotations
 
+import re
+
 import numpy as np
 import pytest
 
@@ -155,3 +157,14 @@ def test_the_bound_holds_for_the_roundings_and_not_for_more(vocab, t):
     for i, row in enumerate(x):
         log_sum, _ = kernel_like(row, 1.0, 2.0 ** -20)
         assert abs(-log_sum - p[i].max()) > off[i]
+
+
+def test_the_library_has_the_kernels_that_calls_reach(pkg):
+    """(waves, packs a lane, with the likeliest tokens) of each type; without
+    tokens 8 packs, with them 16."""
+    from nnc_py_amd import runtime
+    if not runtime.LIB_PATH.exists():
+        pytest.fail("libnnc_hip.so is not built: run __graft_entry__.build()")
+    found = set(re.findall(rb"logprobs_kI(DF16_|f)Li(\d+)ELi(\d+)ELb(\d)EEE", runtime.LIB_PATH.read_bytes()))
+    each = [(1, 4, 0), (1, 4, 1), (1, 8, 0), (1, 8, 1), (4, 4, 0), (4, 4, 1), (4, 8, 0), (4, 16, 1)]
+    assert found == {(t, *(b"%d" % n for n in k)) for t in (b"DF16_", b"f") for k in each}
