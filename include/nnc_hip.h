@@ -431,7 +431,8 @@ void nnc_hip_kv_attention(Tensor* q, Tensor* k_cache, Tensor* v_cache, Tensor* k
  *
  * nnc_hip_rope_kv_write: nnc_hip_rope of a call's queries and keys, the keys
  * and the values going into the paged cache as by nnc_hip_kv_write; the
- * results are those of the three calls, bit for bit. q's columns from q_col:
+ * results are those of the three calls, bit for bit on rows and weights of the
+ * same alignment (the order of a sum of squares goes by it). q's columns from q_col:
  * heads * dim, to q_out ([rows][heads * dim]), or in place if that is NULL; no
  * queries if q is NULL. q, k and v may be one tensor, but rotated queries must
  * not lie over keys or values (NNC_HIP_EINVAL). q_weight [dim] or

@@ -20,10 +20,11 @@
 // last to arrive joins the shares in their order.
 //
 // Few rows are bound by the cache's bytes: 32 sequences of 4 behind 4096, 32
-// heads over 8 of 128 in f16, 53 us, 5.1 TB/s, the rate of a copy. Many by the
-// vector units, which widen the keys and make masks, maxima and exponentials: 32
-// sequences of 16 behind up to 8192 77 us, 2.7 TB/s, where a copy's rate leaves 41
-// (kvtree_rows.hip has the kernel for the longest lines of them).
+// heads over 8 of 128 in f16, 52 us, 5.1 TB/s, the rate of a copy. More by what
+// passes L2, as each 32 rows of a head read the keys for themselves: 32 sequences of
+// 16 behind up to 8192 77 us, 344 MB at 4.8 TB/s, of which the keys are 207, with the
+// vector units, which widen the keys and make masks, maxima and exponentials, 49%
+// busy (kvtree_rows.hip has the kernel for the longest lines of them).
 #include "kvtree.h"
 
 namespace nnc {

@@ -11,12 +11,12 @@
 // of so large a tile would keep the others waiting (32 shares of 256 rows are 4
 // MB), so that is a kernel of its own, 8 rows a workgroup.
 //
-// 64 drafts behind 65536, 32 heads over 8 of 128, f16: 105 us, 650 TFLOP/s of the
-// 1170 of a large f16 product, where 32 rows a wave without LDS take 123; 64
-// sequences of 64 behind 2048 215 and 350. 64 keys of a tile take a CU 2.5 us; the
-// matrix units work 31% of the time, the vector units 47%; storing the shares and
-// joining them takes 8 us, the first keys' way into LDS and the last sums' out of
-// registers 10.
+// 64 drafts behind 65536, 32 heads over 8 of 128, f16: 102 to 111 us from card to
+// card, 620 to 670 TFLOP/s of the 1170 of a large f16 product, where 32 rows a wave
+// without LDS take 123; 64 sequences of 64 behind 2048 215 and 350. 64 keys of a
+// tile take a CU 2.5 us; the matrix units work 32% of the time, the vector units 48%;
+// storing the shares and joining them takes 8 us, the first keys' way into LDS and
+// the last sums' out of registers 10.
 #include "kvtree.h"
 
 namespace nnc {

@@ -474,10 +474,11 @@ static void launch_packs(const char* name, LogprobArgs a, int64_t packs) {
 // are asked for. 16 and 8 packs, us: [512, 128256] f16, 20 tokens 50 and 56, none
 // 37 and 33; [2048, 32000] f16, 1 token 37 and 49; [301, 50257] fp32, none 18 and
 // 16. (12 packs with 20 tokens 53; eight waves with 8 packs were slower by a
-// tenth.) A copy's rate leaves 26 us for the first: a third of its time is the
-// sorting of candidates, and loads and sums of a CU's workgroups overlap only in
-// part. 8 rows of 32000 in fp32 take 9.7 us with 5 tokens, 6.0 without: load, bar,
-// candidates, sort, join are one chain.
+// tenth.) A copy's rate leaves 26 us for the first two. With tokens a third of the
+// time is the sorting of candidates, and 150 registers leave 3 waves a SIMD to cover
+// it; without, the sums keep the vector units busy for 82% of the time. 8 rows of
+// 32000 in fp32 take 9.7 us with 5 tokens, 6.0 without: load, bar, candidates, sort,
+// join are one chain.
 template <typename T, bool TOP>
 static void launch_logprobs(const char* name, const LogprobArgs& a) {
     const int64_t packs = a.vocab * (int64_t)sizeof(T) / 16 + 2;
