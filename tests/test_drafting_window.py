@@ -23,9 +23,9 @@ JOIN = "nnc_hip_kv_tree_attention_join"  # of the kernel for 256 rows alone
 
 
 def test_keys_that_a_window_leaves(tmp_path):
-    exe = tmp_path / "window_check"
+    exe = tmp_path / "draft_window_check"
     subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-fsanitize=undefined,address", "-fno-sanitize-recover=all",
-                    f"-I{ROOT / 'nnc-py_amd' / 'csrc'}", str(ROOT / "tests" / "native" / "window_check.cpp"), "-o", str(exe)],
+                    f"-I{ROOT / 'nnc-py_amd' / 'csrc'}", str(ROOT / "tests" / "native" / "draft_window_check.cpp"), "-o", str(exe)],
                    check=True)
     res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
     assert res.returncode == 0 and res.stdout == "ok\n", res.stdout + res.stderr
